@@ -32,8 +32,8 @@ _i64 = ctypes.c_int64
 _i = ctypes.c_int
 _f = ctypes.c_float
 
-# name -> (restype, argtypes); must mirror include/theria_sdpa.h and
-# include/theria_ln.h exactly.
+# name -> (restype, argtypes); must mirror include/theria_sdpa.h,
+# include/theria_ln.h and include/theria_lm.h exactly.
 SIGNATURES = {
     "theria_status_string": (ctypes.c_char_p, [_i]),
     "theria_version": (ctypes.c_char_p, []),
@@ -64,6 +64,20 @@ SIGNATURES = {
                            _i64, _i64, _i64, _f, _vp]),
     "theria_ln_bwd2": (_i, [_vp, _vp, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp,
                             _vp, _i64, _i64, _i64, _i64, _f, _vp]),
+    "theria_embed_fwd": (_i, [_vp, _i, _vp, _vp, _i64, _i64, _i64, _i, _f, _i64, _vp]),
+    "theria_embed_bwd_workspace_bytes": (_i64, [_i64] * 3),
+    "theria_embed_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i, _f, _i64,
+                              _vp]),
+    "theria_norm_fwd": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _i64, _i64, _i, _f, _vp]),
+    "theria_norm_bwd_workspace_bytes": (_i64, [_i64] * 2),
+    "theria_norm_bwd": (_i, [_vp, _vp, _i] + [_vp] * 6 + [_i64, _i64, _i64, _i, _vp]),
+    "theria_norm_bwd2": (_i, [_vp, _vp, _i] + [_vp] * 9 + [_i64, _i64, _i64, _i, _vp]),
+    "theria_xent_fwd_workspace_bytes": (_i64, [_i64] * 3 + [_i]),
+    "theria_xent_fwd": (_i, [_vp, _vp, _vp, _i, _i64, _i, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
+                             _i64, _i, _vp]),
+    "theria_xent_bwd_workspace_bytes": (_i64, [_i64] * 3 + [_i]),
+    "theria_xent_bwd": (_i, [_vp, _vp, _vp, _i, _i64, _i] + [_vp] * 6 + [_i64, _i64, _i64, _i64,
+                                                                        _i, _vp]),
     "theria_get_device_error": (_i, [ctypes.POINTER(ctypes.c_int), _vp]),
     "theria_clear_device_error": (_i, [_vp]),
     "theria_diag_bounded_wait": (_i, [_i, _vp, _vp]),

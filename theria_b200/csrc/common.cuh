@@ -11,6 +11,8 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/theria_sdpa.h"
 
@@ -86,8 +88,9 @@ inline int launch_status() {
 inline int64_t elem_size(int dtype) { return dtype == THERIA_F32 ? 4 : 2; }
 
 // Device-side error word (one per device that loads the library); a kernel
-// whose bounded wait runs out sets it instead of spinning forever.  The
-// library is one translation unit, so a plain __device__ variable serves.
-__device__ int g_device_error = 0;
+// whose bounded wait runs out sets it instead of spinning forever, as does one
+// that meets a token id outside the vocabulary.  Each of the library's two
+// translation units has its own; theria_get_device_error reads both.
+static __device__ int g_device_error = 0;
 
 }  // namespace theria

@@ -1,0 +1,295 @@
+// Linear layer to the vocabulary fused with its softmax cross entropy.
+//
+//   z = h w^T,  lse_i = log sum_v exp z_iv,  loss_i = lse_i - z_{i, t_i}
+//   dz_iv = c_i (exp(z_iv - lse_i) - [v == t_i]),  dh = dz w,  dw = dz^T h
+//
+// The scores z [N, V] are never stored: the forward makes them tile by tile
+// and keeps each tile's row maximum and row sum of exponentials; the backward
+// makes them again, a piece of the vocabulary at a time, as dz.  Rows whose
+// target is ignored are left out from the start: the rows that count are
+// numbered 0 .. n_live - 1 in order (`prep_kernel`) and only those are
+// computed, so neither their scores nor what their hidden states hold (NaN
+// included) reaches a result.
+#pragma once
+
+#include "common.cuh"
+
+namespace theria {
+namespace xent {
+
+// pos[i] = the number of row i among the rows that count, or -1; row_of and
+// tgt by that number; *n_live.  One CTA.  loss / lse rows that do not count
+// are zeroed here (either may be NULL).
+__global__ void __launch_bounds__(1024)
+prep_kernel(const void* __restrict__ target, int wide, int64_t ignore_index, int64_t N, int64_t V,
+            int* __restrict__ pos, int* __restrict__ row_of, int* __restrict__ tgt,
+            int* __restrict__ n_live, float* __restrict__ count, float* __restrict__ loss,
+            float* __restrict__ lse) {
+  __shared__ int part[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = (N + 1023) / 1024;
+  const int64_t b = threadIdx.x * per, e = b + per < N ? b + per : N;
+  auto live = [&](int64_t i, int64_t& t) {
+    t = wide ? static_cast<const int64_t*>(target)[i]
+             : (int64_t) static_cast<const int32_t*>(target)[i];
+    if (t == ignore_index) return false;
+    if (t >= 0 && t < V) return true;
+    atomicExch(&g_device_error, THERIA_ERR_INVALID_ARG);
+    return false;
+  };
+  int mine = 0;
+  int64_t t;
+  for (int64_t i = b; i < e; ++i) mine += live(i, t) ? 1 : 0;
+  int run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) part[warp] = run;
+  __syncthreads();
+  if (warp == 0) {
+    int p = part[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) p += up;
+    }
+    part[lane] = p;
+  }
+  __syncthreads();
+  int at = run - mine + (warp ? part[warp - 1] : 0);
+  for (int64_t i = b; i < e; ++i) {
+    if (live(i, t)) {
+      pos[i] = at;
+      row_of[at] = (int)i;
+      tgt[at] = (int)t;
+      ++at;
+    } else {
+      pos[i] = -1;
+      if (loss) loss[i] = 0.f;
+      if (lse) lse[i] = 0.f;
+    }
+  }
+  if (threadIdx.x == 0) {
+    *n_live = part[31];
+    if (count) *count = (float)part[31];
+  }
+}
+
+// ------------------------------------------------------------- CUDA cores
+// out(m, n) = sum_k a(m, k) b(n, k): 64 x 64 tiles, 16 x 16 threads of 4 x 4.
+constexpr int TM = 64, TN = 64, TK = 16;
+
+template <typename FA, typename FB>
+__device__ __forceinline__ void tile_product(FA a, FB b, int64_t K, float (&acc)[4][4]) {
+  __shared__ float sa[TK][TM + 4], sb[TK][TN + 4];
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  for (int64_t k0 = 0; k0 < K; k0 += TK) {
+#pragma unroll
+    for (int i = 0; i < TM * TK / 256; ++i) {
+      const int e = threadIdx.x + i * 256;
+      a.load(sa, e, k0);
+      b.load(sb, e, k0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < TK; ++k) {
+      float ra[4], rb[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ra[i] = sa[k][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rb[j] = sb[k][tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(ra[i], rb[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+}
+
+// Operands of tile_product.  Rows: element (r, k) of a matrix with k
+// contiguous, rows through an index list or not; Cols: the r axis contiguous.
+template <typename T>
+struct Rows {
+  const T* p;
+  const int* list;
+  int64_t r0, n, ld, K;
+  __device__ void load(float (&s)[TK][TM + 4], int e, int64_t k0) const {
+    const int k = e % TK, r = e / TK;
+    const int64_t i = r0 + r;
+    s[k][r] = i < n && k0 + k < K ? to_f32(p[(list ? list[i] : i) * ld + k0 + k]) : 0.f;
+  }
+};
+template <typename T>
+struct Cols {
+  const T* p;
+  const int* list;  // of the k axis
+  int64_t r0, n, ld, K;
+  __device__ void load(float (&s)[TK][TM + 4], int e, int64_t k0) const {
+    const int r = e % TM, k = e / TM;
+    const int64_t i = r0 + r, kk = k0 + k;
+    s[k][r] = i < n && kk < K ? to_f32(p[(list ? list[kk] : kk) * ld + i]) : 0.f;
+  }
+};
+
+// part[m][tile] = (max, sum exp(z - max)) of the tile's columns; zt[m] the
+// target's score.  Grid (vocabulary tiles, row tiles).
+template <typename T>
+__global__ void __launch_bounds__(256)
+score_kernel(const T* __restrict__ h, const T* __restrict__ w, const int* __restrict__ row_of,
+             const int* __restrict__ tgt, const int* __restrict__ n_live,
+             float2* __restrict__ part, float* __restrict__ zt, int64_t V, int64_t D) {
+  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, v0 = (int64_t)blockIdx.x * TN;
+  if (m0 >= n) return;
+  float z[4][4];
+  tile_product(Rows<T>{h, row_of, m0, n, D, D}, Rows<T>{w, nullptr, v0, V, D, D}, D, z);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + ty * 4 + i;
+    const int t = m < n ? tgt[m] : -1;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t v = v0 + tx * 4 + j;
+      if (v >= V) continue;
+      top = fmaxf(top, z[i][j]);
+      if (v == t) zt[m] = z[i][j];
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v0 + tx * 4 + j < V) sum += expf(z[i][j] - top);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (tx == 0 && m < n) part[m * gridDim.x + blockIdx.x] = make_float2(top, sum);
+  }
+}
+
+// lse and loss of each row that counts, from its tiles' (max, sum).  A warp
+// per row.
+__global__ void __launch_bounds__(256)
+join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
+            const int* __restrict__ row_of, const int* __restrict__ n_live, int tiles,
+            float* __restrict__ loss, float* __restrict__ lse) {
+  const int lane = threadIdx.x & 31;
+  const int n = *n_live;
+  for (int m = blockIdx.x * 8 + (threadIdx.x >> 5); m < n; m += gridDim.x * 8) {
+    const float2* p = part + (int64_t)m * tiles;
+    float top = -INFINITY, sum = 0.f;
+    for (int j = lane; j < tiles; j += 32) top = fmaxf(top, p[j].x);
+    top = warp_max(top);
+    for (int j = lane; j < tiles; j += 32) sum += p[j].y * expf(p[j].x - top);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      const int64_t i = row_of[m];
+      lse[i] = top + logf(sum);
+      loss[i] = lse[i] - zt[m];
+    }
+  }
+}
+
+// out[0] = the sum of x [n] (mean: over *count), one CTA, fixed order.
+__global__ void __launch_bounds__(1024)
+total_kernel(const float* __restrict__ x, int64_t n, const float* __restrict__ count, int mean,
+             float* __restrict__ out) {
+  __shared__ float part[32];
+  float s = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += x[i];
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    s = warp_sum(part[threadIdx.x]);
+    if (threadIdx.x == 0) out[0] = mean ? s / *count : s;
+  }
+}
+
+// dz[m][c] of the vocabulary piece [c0, c0 + C), float32.
+template <typename T>
+__global__ void __launch_bounds__(256)
+dz_kernel(const T* __restrict__ h, const T* __restrict__ w, const int* __restrict__ row_of,
+          const int* __restrict__ tgt, const int* __restrict__ n_live,
+          const float* __restrict__ lse, const float* __restrict__ gloss, int per_row,
+          const float* __restrict__ count, float* __restrict__ dz, int64_t c0, int64_t C,
+          int64_t V, int64_t D) {
+  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, v0 = c0 + (int64_t)blockIdx.x * TN;
+  if (m0 >= n) return;
+  float z[4][4];
+  tile_product(Rows<T>{h, row_of, m0, n, D, D}, Rows<T>{w, nullptr, v0, V, D, D}, D, z);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + ty * 4 + i;
+    if (m >= n) continue;
+    const int64_t row = row_of[m];
+    const float l = lse[row], g = gloss[per_row ? row : 0] / (count ? *count : 1.f);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t v = v0 + tx * 4 + j;
+      if (v < V && v < c0 + C)
+        dz[m * C + v - c0] = g * (expf(z[i][j] - l) - (v == tgt[m] ? 1.f : 0.f));
+    }
+  }
+}
+
+// acc[m][d] (+)= sum_c dz[m][c] w[c0 + c][d]
+template <typename T>
+__global__ void __launch_bounds__(256)
+dh_kernel(const float* __restrict__ dz, const T* __restrict__ w, const int* __restrict__ n_live,
+          float* __restrict__ acc, int64_t c0, int64_t C, int64_t Cn, int64_t D, int first) {
+  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, d0 = (int64_t)blockIdx.x * TN;
+  if (m0 >= n) return;
+  float o[4][4];
+  tile_product(Rows<float>{dz, nullptr, m0, n, C, Cn}, Cols<T>{w + c0 * D, nullptr, d0, D, D, Cn},
+               Cn, o);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t m = m0 + ty * 4 + i, d = d0 + tx * 4 + j;
+      if (m < n && d < D) acc[m * D + d] = first ? o[i][j] : acc[m * D + d] + o[i][j];
+    }
+}
+
+// dw[c0 + c][d] = sum_m dz[m][c] h[m][d]
+template <typename T>
+__global__ void __launch_bounds__(256)
+dw_kernel(const float* __restrict__ dz, const T* __restrict__ h, const int* __restrict__ row_of,
+          const int* __restrict__ n_live, T* __restrict__ dw, int64_t c0, int64_t C, int64_t Cn,
+          int64_t D) {
+  const int64_t n = *n_live, r0 = (int64_t)blockIdx.y * TM, d0 = (int64_t)blockIdx.x * TN;
+  float o[4][4];
+  tile_product(Cols<float>{dz, nullptr, r0, Cn, C, n}, Cols<T>{h, row_of, d0, D, D, n}, n, o);
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t r = r0 + ty * 4 + i, d = d0 + tx * 4 + j;
+      if (r < Cn && d < D) dw[(c0 + r) * D + d] = from_f32<T>(o[i][j]);
+    }
+}
+
+// dh[i] = acc[pos[i]], or zeros where row i does not count.
+template <typename T>
+__global__ void dh_finish_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
+                                 T* __restrict__ dh, int64_t N, int64_t D) {
+  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * D;
+       e += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t i = e / D, d = e - i * D;
+    const int m = pos[i];
+    dh[e] = from_f32<T>(m < 0 ? 0.f : acc[m * D + d]);
+  }
+}
+
+}  // namespace xent
+}  // namespace theria

@@ -1,6 +1,7 @@
 // libtheria_sm100.so: the C ABI declared in include/theria_sdpa.h.
 //
-// The whole library is one translation unit (no relocatable device code):
+// The library is two translation units without relocatable device code: the
+// language-model operators of include/theria_lm.h are in theria_lm.cu, and
 // this file includes the kernel headers and implements argument checking,
 // workspace carving and kernel selection for each entry point.
 #include <algorithm>
@@ -23,6 +24,11 @@
 #include "tc_host.cuh"
 
 namespace theria {
+
+// The device error word of theria_lm.cu's kernels.
+int lm_read_device_error(int* out, cudaStream_t st);
+int lm_clear_device_error(cudaStream_t st);
+
 namespace {
 
 constexpr int64_t kAlign = 256;
@@ -831,18 +837,22 @@ int theria_diag_bounded_wait(int max_polls, int* out, void* stream) {
 int theria_get_device_error(int* out_flag, void* stream) {
   if (!out_flag) return THERIA_ERR_INVALID_ARG;
   cudaStream_t st = (cudaStream_t)stream;
+  int lm_flag = 0;  // the word of the other translation unit's kernels
   if (cudaMemcpyFromSymbolAsync(out_flag, g_device_error, sizeof(int), 0,
-                                cudaMemcpyDeviceToHost, st) != cudaSuccess)
+                                cudaMemcpyDeviceToHost, st) != cudaSuccess ||
+      theria::lm_read_device_error(&lm_flag, st) != THERIA_OK ||
+      cudaStreamSynchronize(st) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
-  return cudaStreamSynchronize(st) == cudaSuccess ? THERIA_OK : THERIA_ERR_LAUNCH;
+  if (*out_flag == THERIA_OK) *out_flag = lm_flag;
+  return THERIA_OK;
 }
 
 int theria_clear_device_error(void* stream) {
   static const int zero = 0;
-  return cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice,
-                                 (cudaStream_t)stream) == cudaSuccess
-             ? THERIA_OK
-             : THERIA_ERR_LAUNCH;
+  if (cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice,
+                              (cudaStream_t)stream) != cudaSuccess)
+    return THERIA_ERR_LAUNCH;
+  return theria::lm_clear_device_error((cudaStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------

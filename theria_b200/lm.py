@@ -1,0 +1,346 @@
+"""Language-model operators around the attention: what stands before, between
+and after the blocks of a pre-LN decoder.
+
+    embedding(ids, weight, scale)                 scale * weight[ids]
+    layer_norm(x, weight, bias)                   over the last axis, any width
+    linear_cross_entropy(hidden, weight, target)  cross entropy of hidden @ weight.T
+
+Each runs hand-written kernels of libtheria_sm100.so (``include/theria_lm.h``)
+on float32, float16 and bfloat16 CUDA tensors, on torch's current stream, and
+each has its gradient.  Sums, softmax statistics and weight gradients are
+float32 whatever the type, every result is rounded once, and the same inputs
+give the same bits: no result depends on the order of atomics.  There is no
+CPU path.
+
+A token id or target outside the vocabulary is found on the device, where it
+cannot raise: it counts as a row of zeros (an ignored row in the loss), and
+``theria_b200.check_device_error()`` then raises.
+
+The reference library has no such operators; its decoder example composes them
+from torch modules (``examples/minimal_decoder_transformer.py:82-263``).
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from theria_b200 import _lib
+
+IGNORE_INDEX = -100
+EPS = 1e-5
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_opaque = torch.compiler.disable
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(name, like, *args):
+    """One library call on `like`'s device and torch's current stream there."""
+    fn = getattr(_lib.load(), name)
+    with torch.cuda.device(like.device):
+        st = fn(*args, torch.cuda.current_stream(like.device).cuda_stream)
+    _lib.check(st, name)
+
+
+def _workspace(name, like, *sizes):
+    n = getattr(_lib.load(), name)(*sizes)
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=like.device), n
+
+
+def _check(what, **tensors):
+    ref = None
+    for name, t in tensors.items():
+        if not t.is_cuda:
+            raise AssertionError(f"{what} requires CUDA tensors")
+        if t.dtype not in _DTYPES:
+            raise AssertionError(f"Unsupported dtype for {name}: {t.dtype}")
+        ref = t if ref is None else ref
+        if t.device != ref.device:
+            raise AssertionError(f"{what}: {name} is on {t.device}, not {ref.device}")
+
+
+def _check_ids(what, name, ids, like):
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise AssertionError(f"{what}: {name} must be int64 or int32, got {ids.dtype}")
+    if ids.device != like.device:
+        raise AssertionError(f"{what}: {name} is on {ids.device}, not {like.device}")
+
+
+def _wide(ids):
+    return int(ids.dtype == torch.int64)
+
+
+# Each operator's backward is a Function of its own, entered only while a graph
+# of the gradients is being made (create_graph=True), so that a second
+# derivative is either right or refused, never silently cut.
+
+# ------------------------------------------------------------------ embedding
+def _embed(ids, weight, scale, zero_idx):
+    V, D = weight.shape
+    out = torch.empty(*ids.shape, D, dtype=weight.dtype, device=weight.device)
+    _call("theria_embed_fwd", weight, ids.data_ptr(), _wide(ids), weight.data_ptr(),
+          out.data_ptr(), ids.numel(), V, D, _DTYPES[weight.dtype], scale, zero_idx)
+    return out
+
+
+def _embed_grad(gy, ids, V, scale, padding):
+    gy = gy.contiguous()
+    D, n = gy.shape[-1], ids.numel()
+    gw = torch.empty(V, D, dtype=gy.dtype, device=gy.device)
+    ws, size = _workspace("theria_embed_bwd_workspace_bytes", gy, n, V, D)
+    _call("theria_embed_bwd", gy, ids.data_ptr(), _wide(ids), gy.data_ptr(), gw.data_ptr(),
+          ws.data_ptr(), size, n, V, D, _DTYPES[gy.dtype], scale, padding)
+    return gw
+
+
+class _EmbeddingBackward(torch.autograd.Function):
+    """gy -> gw, linear: its backward is the lookup of the cotangent's rows
+    (zeros at the padding tokens, which gw leaves out)."""
+
+    @staticmethod
+    def forward(ctx, gy, ids, V, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.padding = scale, padding
+        return _embed_grad(gy, ids, V, scale, padding)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, u):
+        (ids,) = ctx.saved_tensors
+        return _embed(ids, u.contiguous(), ctx.scale, ctx.padding), None, None, None, None
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding):
+        ctx.save_for_backward(ids)
+        ctx.V, ctx.scale, ctx.padding = weight.shape[0], scale, padding
+        return _embed(ids, weight, scale, -1)
+
+    @staticmethod
+    def backward(ctx, gy):
+        (ids,) = ctx.saved_tensors
+        grad = _EmbeddingBackward.apply if torch.is_grad_enabled() else _embed_grad
+        return grad(gy, ids, ctx.V, ctx.scale, ctx.padding), None, None, None
+
+
+@_opaque
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """``scale * weight[ids]`` for ids of any shape (int64 or int32), weight
+    [V, D]; differentiable twice in weight.
+
+    The weight's gradient (dense) sums each token's rows in token order; the
+    row ``padding_idx`` (negative: from the end) gets none.
+    """
+    _check("theria embedding", weight=weight)
+    _check_ids("theria embedding", "ids", ids, weight)
+    if weight.ndim != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise AssertionError("weight must have shape (V,D)")
+    V = weight.shape[0]
+    padding = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise AssertionError(f"padding_idx must be within the {V} rows of weight")
+        padding = padding_idx % V
+    ids, weight, scale = ids.contiguous(), weight.contiguous(), float(scale)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(weight, ids, scale, padding)
+    return _embed(ids, weight, scale, -1)
+
+
+# ----------------------------------------------------------------- layer norm
+def _norm(x, w, b, eps, need_stats):
+    D = x.shape[-1]
+    N = x.numel() // D
+    y = torch.empty_like(x)
+    stats = torch.empty(2, N, dtype=torch.float32, device=x.device) if need_stats else None
+    _call("theria_norm_fwd", x, x.data_ptr(), _ptr(w), _ptr(b), _affine_dtype(x, w, b),
+          y.data_ptr(), _ptr(stats), N, D, _DTYPES[x.dtype], eps)
+    return y, stats
+
+
+def _affine_dtype(x, w, b):
+    return _DTYPES[(w if w is not None else b if b is not None else x).dtype]
+
+
+def _norm_grad(x, w, b, stats, gy, need):
+    gy = gy.contiguous()
+    D = x.shape[-1]
+    N = x.numel() // D
+    gx = torch.empty_like(x) if need[0] else None
+    gw = gb = ws = None
+    size = 0
+    if need[1] or need[2]:
+        gw, gb = torch.empty(2, D, dtype=(w if w is not None else b).dtype,
+                             device=x.device).unbind(0)
+        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x, N, D)
+    _call("theria_norm_bwd", x, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b), gy.data_ptr(),
+          stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), size, N, D,
+          _DTYPES[x.dtype])
+    return gx, gw if need[1] else None, gb if need[2] else None
+
+
+class _LayerNormBackward(torch.autograd.Function):
+    """(x, w, gy) -> (gx, gw, gb); its backward is the second derivative.
+    The statistics are functions of x, differentiated through there."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, gy, stats, need):
+        gy = gy.contiguous()
+        ctx.save_for_backward(x, w, b, gy, stats)
+        return _norm_grad(x, w, b, stats, gy, need)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, u, a, c):
+        x, w, b, gy, stats = ctx.saved_tensors
+        D = x.shape[-1]
+        N = x.numel() // D
+        u, a, c = (None if t is None else t.contiguous() for t in (u, a, c))
+        dx, dgy = torch.empty_like(x), torch.empty_like(x)
+        dw = None if w is None else torch.empty_like(w)
+        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x, N, D)
+        _call("theria_norm_bwd2", x, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
+              gy.data_ptr(), stats.data_ptr(), _ptr(u), _ptr(a), _ptr(c), dx.data_ptr(),
+              _ptr(dw), dgy.data_ptr(), ws.data_ptr(), size, N, D, _DTYPES[x.dtype])
+        return dx, dw, None, dgy, None, None
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps):
+        y, stats = _norm(x, w, b, eps, True)
+        ctx.save_for_backward(x, w, b, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, w, b, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad[:3]
+        if torch.is_grad_enabled():
+            grads = _LayerNormBackward.apply(x, w, b, gy, stats, need)
+        else:
+            grads = _norm_grad(x, w, b, stats, gy, need)
+        return (*grads, None)
+
+
+@_opaque
+def layer_norm(x, weight=None, bias=None, eps=EPS):
+    """Layer norm over the last axis of x [..., D]; weight, bias [D] (either
+    may be None) of x's type or float32.  Differentiable twice."""
+    _check("theria layer_norm", x=x, **{n: t for n, t in (("weight", weight), ("bias", bias))
+                                        if t is not None})
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise AssertionError("x must have shape (...,D)")
+    kinds = set()
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (x.shape[-1],):
+            raise AssertionError(f"{name} must have shape ({x.shape[-1]},)")
+        if t.dtype not in (x.dtype, torch.float32):
+            raise AssertionError(f"{name} dtype must be {x.dtype} or float32")
+        kinds.add(t.dtype)
+    if len(kinds) > 1:
+        raise AssertionError("weight and bias must share one dtype")
+    x = x.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _norm(x, weight, bias, float(eps), False)[0]
+
+
+# ------------------------------------------------------- linear cross entropy
+def _loss(h, w, target, ignore_index, reduction):
+    (N, D), V = h.shape, w.shape[0]
+    loss = torch.empty(N if reduction == 0 else 1, dtype=torch.float32, device=h.device)
+    lse = torch.empty(N, dtype=torch.float32, device=h.device)
+    count = torch.empty(1, dtype=torch.float32, device=h.device)
+    ws, size = _workspace("theria_xent_fwd_workspace_bytes", h, N, V, D, _DTYPES[h.dtype])
+    _call("theria_xent_fwd", h, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
+          ignore_index, reduction, loss.data_ptr(), lse.data_ptr(), count.data_ptr(),
+          ws.data_ptr(), size, N, V, D, _DTYPES[h.dtype])
+    return loss, lse, count
+
+
+def _loss_grad(h, w, g, target, lse, count, ignore_index, reduction, need):
+    (N, D), V = h.shape, w.shape[0]
+    g = g.to(torch.float32).contiguous()
+    dh = torch.empty_like(h) if need[0] else None
+    dw = torch.empty_like(w) if need[1] else None
+    ws, size = _workspace("theria_xent_bwd_workspace_bytes", h, N, V, D, _DTYPES[h.dtype])
+    _call("theria_xent_bwd", h, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
+          ignore_index, reduction, g.data_ptr(), lse.data_ptr(), count.data_ptr(), _ptr(dh),
+          _ptr(dw), ws.data_ptr(), size, N, V, D, _DTYPES[h.dtype])
+    return dh, dw
+
+
+class _LinearCrossEntropyBackward(torch.autograd.Function):
+    """(h, w, g) -> (dh, dw); a second derivative is refused."""
+
+    @staticmethod
+    def forward(ctx, h, w, g, *rest):
+        return _loss_grad(h, w, g, *rest)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("theria linear_cross_entropy is differentiable once: its gradients "
+                           "have no second derivative here")
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, w, target, ignore_index, reduction):
+        loss, lse, count = _loss(h, w, target, ignore_index, reduction)
+        ctx.save_for_backward(h, w, target, lse, count)
+        ctx.rest = ignore_index, reduction
+        return loss
+
+    @staticmethod
+    def backward(ctx, g):
+        h, w, target, lse, count = ctx.saved_tensors
+        grad = _LinearCrossEntropyBackward.apply if torch.is_grad_enabled() else _loss_grad
+        dh, dw = grad(h, w, g, target, lse, count, *ctx.rest, ctx.needs_input_grad[:2])
+        return dh, dw, None, None, None
+
+
+@_opaque
+def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, reduction="mean"):
+    """Softmax cross entropy of the scores ``hidden @ weight.T`` without
+    keeping them: hidden [..., D], weight [V, D] of one type, target [...]
+    (int64 or int32).  Differentiable once, in hidden and weight.
+
+    Rows whose target is ``ignore_index`` are left out: loss 0, no gradient,
+    and nothing that their hidden states hold reaches a result.  The loss is
+    float32: one per row for ``reduction="none"`` (target's shape), else a
+    scalar; the mean over no row at all is NaN, with zero gradients.
+    """
+    what = "theria linear_cross_entropy"
+    _check(what, hidden=hidden, weight=weight)
+    _check_ids(what, "target", target, hidden)
+    if weight.dtype != hidden.dtype:
+        raise AssertionError("hidden and weight must share one dtype")
+    if weight.ndim != 2 or 0 in weight.shape:
+        raise AssertionError("weight must have shape (V,D)")
+    if hidden.ndim == 0 or hidden.shape[-1] != weight.shape[1]:
+        raise AssertionError("hidden must have shape (...,D) with D matching weight")
+    if target.shape != hidden.shape[:-1]:
+        raise AssertionError(f"target shape must be {tuple(hidden.shape[:-1])}")
+    if reduction not in _REDUCTIONS:
+        raise AssertionError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    h, w = hidden.reshape(-1, hidden.shape[-1]).contiguous(), weight.contiguous()
+    t, red = target.reshape(-1).contiguous(), _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(h, w, t, int(ignore_index), red)
+    else:
+        loss = _loss(h, w, t, int(ignore_index), red)[0]
+    return loss.view(target.shape) if red == 0 else loss.view(())
+
+
+__all__ = ["embedding", "layer_norm", "linear_cross_entropy"]
