@@ -1,0 +1,554 @@
+// The tensor-core products of the linear cross entropy: one persistent kernel
+// with four epilogues.
+//
+//   kScore  z  = h w^T    -> per row and 128 columns (max, sum exp), target score
+//   kDz     z  = h w^T    -> dz = rowscale * (exp(z - lse) - onehot), stored
+//   kDh     dh = dz w     -> float32 partial sums, per split of the vocabulary
+//   kDw     dw = dz^T h   -> the result, scaled and rounded once
+//
+// A cluster of two CTAs (two SMs of one TPC) makes 256 x 256 tiles with
+// tcgen05.mma.cta_group::2: each CTA stages 128 rows of A and 128 of B by TMA,
+// 32 KB for a contraction step of 64, so a tile reads half the shared memory
+// and half the L2 bytes per product that two single-SM tiles would; those
+// bytes, not the tensor pipe, would otherwise set the pace (a 128 x 256 tile
+// needs 96 bytes a cycle from L2 per SM).  The accumulator (256 columns of
+// TMEM in each CTA) is double-buffered: eight warps read one while the next
+// tile is being multiplied.
+//
+// float32 operands come as three bfloat16 planes (x = hi + mid + lo exactly,
+// 8 bits each) and the contraction runs over six of the nine plane pairs,
+// smallest products first; what is left out is below 2^-24 of a product.
+#pragma once
+
+#include "common.cuh"
+#include "tc_common.cuh"
+
+namespace theria {
+namespace xent {
+
+enum Epi { kScore = 0, kDz = 1, kDh = 2, kDw = 3 };
+
+constexpr int BM = 256, BN = 256, BK = 64;  // of a CTA pair
+constexpr int HALF = 128;                   // rows of A and of B per CTA
+constexpr int SUB = 128;                    // columns per score partial
+constexpr int STAGES = 6;
+constexpr int OPERAND = HALF * BK * 2;      // bytes of one operand's stage
+constexpr int EPI_WARPS = 8;
+constexpr int TC_THREADS = 128 + EPI_WARPS * 32;
+constexpr uint32_t ACC_COLS = 256;
+constexpr uint32_t POLLS = 1u << 20;  // bound of one wait; a poll suspends the thread for a while
+
+struct TcArgs {
+  const int* n_live;
+  int V, D;
+  int c0, Cn;           // piece of the vocabulary (kDz, kDh, kDw): start, columns
+  int pairs;            // plane pairs: 1 (16-bit operands) or 6 (float32)
+  int plane_a, plane_b; // elements between planes of one row
+  int splits, split_kb; // kDh: splits of the contraction, k blocks in each
+  int add;              // kDh: add to what the partials hold (a later piece)
+  const int* tgt;       // kScore, kDz
+  float2* part;         // kScore: [row][sub_tiles]
+  int sub_tiles;
+  float* zt;
+  const float* lse;     // kDz, by packed row
+  const float* rowscale;
+  void* dz;             // kDz: [row][planes][ld_dz]
+  int ld_dz;
+  float* acc;           // kDh: [split][acc_rows][ld_acc]
+  int64_t acc_rows;
+  int ld_acc;
+  void* out;            // kDw: [V][D]
+  int out_vec;
+  const float* post;    // kDw: the factor of the result
+};
+
+// Planes (of a, of b) of the i-th of six pairs, smallest products first.
+__device__ __forceinline__ int pair_a(int i) { return (0x001102 >> (4 * i)) & 15; }
+__device__ __forceinline__ int pair_b(int i) { return (0x010120 >> (4 * i)) & 15; }
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
+               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The shared::cluster address of `p` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc::smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
+               : "memory");
+}
+// Box at (x, y) of `map` into this CTA's shared memory; the bytes count on a
+// barrier that may be the pair's other CTA's.
+__device__ __forceinline__ void load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int x,
+                                        int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile"
+      ".mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on this barrier of both CTAs when all earlier products are done.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(tc::smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+struct TcSmem {
+  static constexpr int oA = 0;
+  static constexpr int oB = STAGES * OPERAND;
+  static constexpr int oBar = 2 * STAGES * OPERAND;  // full, empty, acc_full, acc_empty
+  static constexpr int kBars = 2 * STAGES + 4;
+  static constexpr int oTmem = oBar + kBars * 8;
+  static constexpr int oAbort = oTmem + 4;
+  static constexpr int kBytes = oAbort + 4;
+  static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024
+};
+
+// What one cluster works on next.
+struct Unit {
+  int m0, n0;   // tile origin
+  int kb0, kbs; // k blocks of each plane pair
+  int split;
+};
+
+template <int EPI>
+struct Sched {
+  int mt, nt, kb, units, splits, split_kb;
+  __device__ explicit Sched(const TcArgs& a) {
+    const int live = *a.n_live;
+    const int rows = (live + BM - 1) / BM > 0 ? (live + BM - 1) / BM : 1;
+    splits = 1;
+    if (EPI == kScore || EPI == kDz) {
+      mt = rows;
+      nt = ((EPI == kScore ? a.V : a.Cn) + BN - 1) / BN;
+      kb = (a.D + BK - 1) / BK;
+    } else if (EPI == kDh) {
+      mt = rows;
+      nt = (a.D + BN - 1) / BN;
+      kb = (a.Cn + BK - 1) / BK;
+      splits = a.splits;
+    } else {
+      mt = (a.Cn + BM - 1) / BM;
+      nt = (a.D + BN - 1) / BN;
+      kb = live > 0 ? (live + BK - 1) / BK : 1;
+    }
+    split_kb = EPI == kDh ? a.split_kb : kb;
+    units = mt * nt * splits;
+  }
+  // Tiles in groups of 8 rows of tiles, so that the clusters at work at one
+  // time share both operands' tiles in L2.
+  __device__ Unit at(int u) const {
+    Unit r;
+    r.split = u / (mt * nt);
+    const int t = u - r.split * (mt * nt);
+    const int g = t / (8 * nt), in = t - g * 8 * nt;
+    const int gm = mt - g * 8 < 8 ? mt - g * 8 : 8;
+    r.m0 = (g * 8 + in % gm) * BM;
+    r.n0 = (in / gm) * BN;
+    r.kb0 = r.split * split_kb;
+    r.kbs = kb - r.kb0 < split_kb ? kb - r.kb0 : split_kb;
+    return r;
+  }
+};
+
+// 32 consecutive values of one row, converted and stored.
+template <typename O>
+__device__ __forceinline__ void store32(O* dst, const float (&v)[32], int valid, bool vec) {
+  if (vec && valid >= 32) {
+    if constexpr (sizeof(O) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<float4*>(dst)[i] =
+            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* e = v + 8 * i;
+        reinterpret_cast<uint4*>(dst)[i] =
+            make_uint4(tc::pack2<O>(e[0], e[1]), tc::pack2<O>(e[2], e[3]),
+                       tc::pack2<O>(e[4], e[5]), tc::pack2<O>(e[6], e[7]));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (i < valid) dst[i] = from_f32<O>(v[i]);
+  }
+}
+
+// x = hi + mid + lo, each the leading 8 bits of what the ones before leave.
+__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
+  p[0] = __float2bfloat16_rz(x);
+  const float r1 = isfinite(x) ? x - __bfloat162float(p[0]) : 0.f;
+  p[1] = __float2bfloat16_rz(r1);
+  p[2] = __float2bfloat16_rz(r1 - __bfloat162float(p[1]));
+}
+
+// T: the operands' type.  O: the type of the user's tensors (float32 with T =
+// bfloat16 planes, else T).
+template <typename T, typename O, int EPI>
+__global__ void __launch_bounds__(TC_THREADS, 1) __cluster_dims__(2, 1, 1)
+tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+          const __grid_constant__ TcArgs args) {
+  constexpr bool A_MN = EPI == kDw, B_MN = EPI == kDh || EPI == kDw;
+  using L = TcSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::oBar);
+  uint64_t* empty = full + STAGES;
+  uint64_t* acc_full = empty + STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oTmem);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::oAbort);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(full + i, 1);
+      tc::mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(acc_full + i, 1);
+      tc::mbar_init(acc_empty + i, 2 * EPI_WARPS);
+    }
+    *abort = 0;
+    tc::fence_barrier_init();
+    tc::prefetch_tmap(&map_a);
+    tc::prefetch_tmap(&map_b);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     tc::smem_u32(tmem_slot)),
+                 "r"(2 * ACC_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Sched<EPI> sched(args);
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------ loads, in both CTAs
+    uint32_t it = 0;
+    bool ok = true;
+    for (int u = cluster; ok && u < sched.units; u += clusters) {
+      const Unit un = sched.at(u);
+      const int m0 = un.m0 + rank * HALF, n0 = un.n0 + rank * HALF;
+      for (int i = 0, n = args.pairs * un.kbs; i < n; ++i, ++it) {
+        const int slot = it % STAGES;
+        if (!tc::mbar_wait(empty + slot, ((it / STAGES) & 1) ^ 1, abort, POLLS)) {
+          ok = false;
+          break;
+        }
+        const int pr = i / un.kbs, k = (un.kb0 + i - pr * un.kbs) * BK;
+        const int xa = args.pairs > 1 ? pair_a(pr) * args.plane_a : 0;
+        const int xb = args.pairs > 1 ? pair_b(pr) * args.plane_b : 0;
+        uint8_t* a = smem + L::oA + slot * OPERAND;
+        uint8_t* b = smem + L::oB + slot * OPERAND;
+        if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
+        const uint32_t bar = map_rank(full + slot, 0);
+        if constexpr (A_MN) {
+          load_2d(a, &map_a, bar, xa + m0, k);
+          load_2d(a + OPERAND / 2, &map_a, bar, xa + m0 + 64, k);
+        } else {
+          load_2d(a, &map_a, bar, xa + k, m0);
+        }
+        if constexpr (B_MN) {
+          const int y = (EPI == kDh ? args.c0 : 0) + k;
+          load_2d(b, &map_b, bar, xb + n0, y);
+          load_2d(b + OPERAND / 2, &map_b, bar, xb + n0 + 64, y);
+        } else {
+          load_2d(b, &map_b, bar, xb + k, (EPI == kDz ? args.c0 : 0) + n0);
+        }
+      }
+    }
+    // every stage used is given back before the CTA may end
+    for (int s = 0; ok && s < STAGES && s < (int)it; ++s) {
+      const uint32_t last = it - 1 - s;
+      ok = tc::mbar_wait(empty + last % STAGES, (last / STAGES) & 1, abort, POLLS);
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // --------------------------------------- products, in the leading CTA
+    constexpr uint32_t id = tc::idesc_f16(BM, BN, tc::AbFmt<T>::v, A_MN, B_MN);
+    constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;
+    const uint64_t da = tc::sw128_desc(tc::smem_u32(smem + L::oA), A_MN ? OPERAND / 2 : 16, 1024);
+    const uint64_t db = tc::sw128_desc(tc::smem_u32(smem + L::oB), B_MN ? OPERAND / 2 : 16, 1024);
+    uint32_t it = 0, n_unit = 0;
+    bool ok = true;
+    for (int u = cluster; ok && u < sched.units; u += clusters, ++n_unit) {
+      const Unit un = sched.at(u);
+      const uint32_t buf = n_unit & 1;
+      if (!tc::mbar_wait(acc_empty + buf, ((n_unit >> 1) & 1) ^ 1, abort, POLLS)) break;
+      tc::tc_fence_after();
+      const uint32_t d = tmem + buf * ACC_COLS;
+      for (int i = 0, n = args.pairs * un.kbs; i < n; ++i, ++it) {
+        const int slot = it % STAGES;
+        if (!tc::mbar_wait(full + slot, (it / STAGES) & 1, abort, POLLS)) {
+          ok = false;
+          break;
+        }
+        tc::tc_fence_after();
+        const uint64_t a = tc::desc_at(da, slot * OPERAND), b = tc::desc_at(db, slot * OPERAND);
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k)
+          mma_pair(d, tc::desc_at(a, k * step_a), tc::desc_at(b, k * step_b), id,
+                   (i > 0 || k > 0) ? 1u : 0u);
+        commit_pair(empty + slot);
+      }
+      if (ok) commit_pair(acc_full + buf);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------- epilogue, in both CTAs
+    const int quarter = warp & 3, side = (warp - 4) >> 2;  // TMEM lanes, column half
+    const int r = quarter * 32 + lane;
+    const int live = *args.n_live;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint32_t n_unit = 0;
+    for (int u = cluster; u < sched.units; u += clusters, ++n_unit) {
+      const Unit un = sched.at(u);
+      const uint32_t buf = n_unit & 1;
+      const int m = un.m0 + rank * HALF + r, n0 = un.n0 + side * SUB;
+      // what the row needs, fetched while the product is still running
+      int t = -1;
+      float l = 0.f, rs = 0.f, post = 1.f;
+      if (EPI == kScore || EPI == kDz) t = m < live ? args.tgt[m] - (EPI == kDz ? args.c0 : 0) : -1;
+      if (EPI == kDz && m < live) {
+        l = args.lse[m];
+        rs = args.rowscale[m];
+      }
+      if (EPI == kDw) post = *args.post;
+      const bool got = __all_sync(0xffffffffu,
+                                  tc::mbar_wait(acc_full + buf, (n_unit >> 1) & 1, abort, POLLS));
+      if (!got) break;
+      tc::tc_fence_after();
+      const uint32_t src = tmem + buf * ACC_COLS + lanes + side * SUB;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < SUB; c += 32) {
+        float v[32];
+        tc::tmem_ld32(src + c, v);  // warp-collective
+        const int n = n0 + c;
+        if constexpr (EPI == kScore) {
+          const int valid = args.V - n;
+          if (valid <= 0) continue;
+          if (valid < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= valid) v[i] = -INFINITY;
+          }
+          if (t >= n && t < n + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (n + i == t) args.zt[m] = v[i];
+          }
+          float most = v[0];
+#pragma unroll
+          for (int i = 1; i < 32; ++i) most = fmaxf(most, v[i]);
+          const float now = fmaxf(top, most);
+          const float base = now == -INFINITY ? 0.f : now * 1.4426950408889634f;
+          sum *= tc::ex2(fmaf(top, 1.4426950408889634f, -base));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            sum += tc::ex2(fmaf(v[i], 1.4426950408889634f, -base));
+          top = now;
+        } else if constexpr (EPI == kDz) {
+          const int valid = args.Cn - n;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float p;
+            if constexpr (sizeof(O) == 4) p = expf(v[i] - l);
+            else p = tc::ex2((v[i] - l) * 1.4426950408889634f);
+            if (n + i == t) p -= 1.f;
+            v[i] = (m < live && i < valid) ? rs * p : 0.f;
+          }
+          if constexpr (sizeof(O) == 4) {
+            __nv_bfloat16* row = (__nv_bfloat16*)args.dz + (int64_t)m * 3 * args.ld_dz + n;
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) {
+              uint32_t w[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                __nv_bfloat16 x[3], y[3];
+                split3(v[2 * i], x);
+                split3(v[2 * i + 1], y);
+                const __nv_bfloat162 q = __halves2bfloat162(x[pl], y[pl]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&q);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                reinterpret_cast<uint4*>(row + pl * args.ld_dz)[i] =
+                    make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            }
+          } else {
+            store32<T>((T*)args.dz + (int64_t)m * args.ld_dz + n, v, 32, true);
+          }
+        } else if constexpr (EPI == kDh) {
+          if (m < live && n < args.ld_acc) {
+            float* dst = args.acc + (un.split * args.acc_rows + m) * args.ld_acc + n;
+            if (args.add) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 o = reinterpret_cast<const float4*>(dst)[i];
+                v[4 * i] += o.x;
+                v[4 * i + 1] += o.y;
+                v[4 * i + 2] += o.z;
+                v[4 * i + 3] += o.w;
+              }
+            }
+            store32<float>(dst, v, 32, true);
+          }
+        } else {
+          if (m < args.Cn && n < args.D) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= post;
+            store32<O>((O*)args.out + (int64_t)(args.c0 + m) * args.D + n, v, args.D - n,
+                       args.out_vec);
+          }
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(map_rank(acc_empty + buf, 0));
+      if (EPI == kScore && m < live && n0 < args.V)
+        args.part[(int64_t)m * args.sub_tiles + n0 / SUB] = make_float2(top, sum);
+    }
+  }
+
+  // Copies in flight after a wait that gave up land before the CTA ends.
+  __syncwarp();
+  __syncthreads();
+  if (*abort) {
+    for (int i = 0; i < 1000; ++i) __nanosleep(2000);
+  }
+  tc::tc_fence_before();
+  cluster_sync();
+  tc::tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(2 * ACC_COLS)
+                 : "memory");
+  }
+}
+
+// dst[m][plane][Kp] = the rows of src (by `row_of`, or all), packed: zeros
+// past D and in the rows n_live .. up to a multiple of BM.  T: the operands'
+// type; O float: three planes.
+template <typename T, typename O>
+__global__ void __launch_bounds__(256)
+pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
+            const int* __restrict__ n_live, int64_t rows, T* __restrict__ dst, int64_t D,
+            int64_t Kp, int vec) {
+  const int64_t live = n_live ? *n_live : rows;
+  const int64_t end = n_live ? (live > 0 ? (live + BM - 1) / BM * BM : BM) : rows;
+  constexpr int planes = sizeof(O) == 4 ? 3 : 1;
+  const int64_t units = Kp / 8;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < end * units;
+       e += (int64_t)gridDim.x * 256) {
+    const int64_t m = e / units, k = (e - m * units) * 8;
+    const O* s = src + (m < live ? (row_of ? row_of[m] : m) : 0) * D + k;
+    __align__(16) O x[8];
+    if (m < live && vec && k + 8 <= D) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(O) / 2; ++i)
+        reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(s)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = m < live && k + i < D ? s[i] : from_f32<O>(0.f);
+    }
+    T* d = dst + m * planes * Kp + k;
+    if constexpr (sizeof(O) == 4) {
+      __nv_bfloat16 p[8][3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) split3(x[i], p[i]);
+#pragma unroll
+      for (int pl = 0; pl < 3; ++pl) {
+        __align__(16) __nv_bfloat16 o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = p[i][pl];
+        *reinterpret_cast<uint4*>(d + pl * Kp) = *reinterpret_cast<const uint4*>(o);
+      }
+    } else {
+      *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(x);
+    }
+  }
+}
+
+// By packed row: lse, and the row's factor of dz.  *post: the factor of the
+// results.  float16 holds dz in [2^-29, 2^15] (units of 1 / 32768 of the
+// largest row's factor): probabilities of 1e-9 stay normal numbers.
+constexpr float HALF_SCALE = 32768.f;
+__global__ void __launch_bounds__(1024)
+scale_kernel(const int* __restrict__ row_of, const int* __restrict__ n_live,
+             const float* __restrict__ gloss, int per_row, const float* __restrict__ count,
+             const float* __restrict__ lse, int half, float* __restrict__ lse_p,
+             float* __restrict__ rowscale, float* __restrict__ post) {
+  __shared__ float part[32];
+  const int n = *n_live;
+  const float unit = half ? HALF_SCALE : 1.f;
+  float most = 0.f;
+  if (per_row && half) {
+    for (int m = threadIdx.x; m < n; m += 1024) {
+      const float g = fabsf(gloss[row_of[m]]);
+      if (isfinite(g)) most = fmaxf(most, g);
+    }
+    most = warp_max(most);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+    __syncthreads();
+    most = warp_max(part[threadIdx.x & 31]);
+  }
+  if (most == 0.f) most = 1.f;
+  for (int m = threadIdx.x; m < n; m += 1024) {
+    const int row = row_of[m];
+    lse_p[m] = lse[row];
+    rowscale[m] = unit * (per_row ? gloss[row] / most : 1.f);
+  }
+  if (threadIdx.x == 0)
+    *post = (per_row ? most : count ? (n > 0 ? gloss[0] / *count : 0.f) : gloss[0]) / unit;
+}
+
+// dh[i] = post * the sum of the splits' partials of row pos[i], or zeros.
+template <typename O>
+__global__ void __launch_bounds__(256)
+dh_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
+              const float* __restrict__ post, int splits, int64_t acc_rows, int ld_acc,
+              O* __restrict__ dh, int64_t N, int64_t D) {
+  const float f = *post;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < N * D;
+       e += (int64_t)gridDim.x * 256) {
+    const int64_t i = e / D, d = e - i * D;
+    const int m = pos[i];
+    float s = 0.f;
+    if (m >= 0)
+      for (int k = 0; k < splits; ++k) s += acc[(k * acc_rows + m) * ld_acc + d];
+    dh[e] = from_f32<O>(s * f);
+  }
+}
+
+}  // namespace xent
+}  // namespace theria

@@ -6,6 +6,8 @@
 #include "lm_embed.cuh"
 #include "lm_norm.cuh"
 #include "lm_xent.cuh"
+#include "lm_xent_tc.cuh"
+#include "tc_host.cuh"
 #include "../../include/theria_lm.h"
 
 namespace theria {
@@ -359,6 +361,7 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.n_live = c.take<int>(1);
   return r;
 }
+// --------------------------------------------------------- CUDA-core path
 struct XentFwdWs {
   XentRows rows;
   float2* part;
@@ -392,16 +395,238 @@ XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V, int64_t D) {
   return w;
 }
 
+// ------------------------------------------------------- tensor-core path
+constexpr int kClusters = kSMs / 2;
+
+// Problems this small run on CUDA cores in fewer launches.
+bool xent_small(int64_t N, int64_t V, int64_t D) { return N * V * D <= (1ll << 24); }
+
+struct TcSizes {
+  int64_t Mp, Kp;          // packed rows, elements of a packed row (one plane)
+  int planes;
+  bool pack_w;             // w needs a packed copy
+  int64_t piece;           // of the vocabulary, backward
+  int64_t ld_acc, split_kb, splits;
+};
+TcSizes tc_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
+  TcSizes z;
+  z.Mp = up(N, xent::BM);
+  z.Kp = up(D, xent::BK);
+  z.planes = dtype == THERIA_F32 ? 3 : 1;
+  z.pack_w = z.planes > 1 || D % 8 != 0;
+  // dz of a piece within 512 MB
+  const int64_t fit = (512ll << 20) / (z.Mp * 2 * z.planes) / xent::BN * xent::BN;
+  z.piece = std::min(up(V, xent::BN), std::max<int64_t>(xent::BN, fit));
+  z.ld_acc = up(D, 32);
+  // dh: the contraction over the piece is split where whole tiles would leave
+  // clusters idle.  Cost in k blocks (0.28 us): the longest cluster's share
+  // with 8 for each unit's start and end, and the partials' traffic.
+  const int64_t tiles = z.Mp / xent::BM * cdiv(D, xent::BN), kb = cdiv(z.piece, xent::BK);
+  const int pairs = z.planes > 1 ? 6 : 1;
+  double best = 1e30;
+  z.splits = 1;
+  z.split_kb = kb;
+  for (int64_t s = 1; s <= std::min<int64_t>(kClusters, kb); ++s) {
+    const int64_t per = cdiv(kb, s), n = cdiv(kb, per);
+    const double cost = (double)cdiv(tiles * n, kClusters) * (per * pairs + 8) +
+                        (double)n * z.Mp * z.ld_acc * 8 / 6.5e12 / 0.28e-6;
+    if (cost < best) {
+      best = cost;
+      z.splits = n;
+      z.split_kb = per;
+    }
+  }
+  return z;
+}
+
+struct TcFwdWs {
+  XentRows rows;
+  void *hp, *wp;
+  float2* part;
+  float *zt, *each;
+  int64_t bytes;
+};
+TcFwdWs tc_fwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z) {
+  Carver c{(char*)base};
+  TcFwdWs w;
+  w.rows = xent_rows(c, N);
+  w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
+  w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
+  w.part = c.take<float2>(z.Mp * cdiv(V, xent::SUB));
+  w.zt = c.take<float>(z.Mp);
+  w.each = c.take<float>(N);
+  w.bytes = c.used;
+  return w;
+}
+struct TcBwdWs {
+  XentRows rows;
+  void *hp, *wp, *dz;
+  float *acc, *lse, *rowscale, *post;
+  int64_t bytes;
+};
+TcBwdWs tc_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z) {
+  Carver c{(char*)base};
+  TcBwdWs w;
+  w.rows = xent_rows(c, N);
+  w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
+  w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
+  w.dz = c.take<uint16_t>(z.Mp * z.piece * z.planes);
+  w.acc = c.take<float>(z.splits * z.Mp * z.ld_acc);
+  w.lse = c.take<float>(N);
+  w.rowscale = c.take<float>(N);
+  w.post = c.take<float>(1);
+  w.bytes = c.used;
+  return w;
+}
+
+// 2-D map of 16-bit rows [rows][inner] at ld elements, box {64, box_rows}.
+bool map_2d(CUtensorMap* map, const void* base, bool bf16, int64_t inner, int64_t rows, int64_t ld,
+            int box_rows) {
+  tc::EncodeTiledFn fn = tc::encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename O, int EPI>
+int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const xent::TcArgs& args, int64_t units,
+              cudaStream_t st) {
+  auto kern = xent::tc_kernel<T, O, EPI>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           xent::TcSmem::kAlloc) != cudaSuccess)
+    return THERIA_ERR_LAUNCH;
+  const unsigned grid = 2 * (unsigned)std::min<int64_t>(units, kClusters);
+  kern<<<grid, xent::TC_THREADS, xent::TcSmem::kAlloc, st>>>(a, b, args);
+  return launch_status();
+}
+
+template <typename T, typename O>
+int tc_pack(const void* src, const int* row_of, const int* n_live, int64_t rows, void* dst,
+            int64_t D, int64_t Kp, cudaStream_t st) {
+  const int dtype = std::is_same<O, float>::value ? THERIA_F32 : THERIA_F16;
+  const int64_t threads = (n_live ? up(rows, xent::BM) : rows) * (Kp / 8);
+  xent::pack_kernel<T, O><<<(unsigned)std::min<int64_t>(cdiv(threads, 256), kSMs * 32), 256, 0,
+                            st>>>((const O*)src, row_of, n_live, rows, (T*)dst, D, Kp,
+                                  vec_rows(D, dtype, {src}));
+  return launch_status();
+}
+
+// T: the operands' type; O: the tensors'.
+template <typename T, typename O>
+struct Tc {
+  static constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+
+  static int fwd(const void* h, const void* w, const TcFwdWs& ws, const TcSizes& z, float* each,
+                 float* lse, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
+    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, st)) return e;
+    if (z.pack_w)
+      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, st)) return e;
+    CUtensorMap ma, mb;
+    if (!map_2d(&ma, ws.hp, bf16, z.Kp * z.planes, z.Mp, z.Kp * z.planes, xent::HALF) ||
+        !(z.pack_w ? map_2d(&mb, ws.wp, bf16, z.Kp * z.planes, V, z.Kp * z.planes, xent::HALF)
+                   : map_2d(&mb, w, bf16, D, V, D, xent::HALF)))
+      return THERIA_ERR_LAUNCH;
+    xent::TcArgs a{};
+    a.n_live = ws.rows.n_live;
+    a.V = (int)V;
+    a.D = (int)D;
+    a.pairs = z.planes > 1 ? 6 : 1;
+    a.plane_a = a.plane_b = (int)z.Kp;
+    a.tgt = ws.rows.tgt;
+    a.part = ws.part;
+    a.sub_tiles = (int)cdiv(V, xent::SUB);
+    a.zt = ws.zt;
+    if (int e = tc_launch<T, O, xent::kScore>(ma, mb, a, z.Mp / xent::BM * cdiv(V, xent::BN), st))
+      return e;
+    xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
+        ws.part, ws.zt, ws.rows.row_of, ws.rows.n_live, a.sub_tiles, each, lse);
+    return launch_status();
+  }
+
+  static int bwd(const void* h, const void* w, const TcBwdWs& ws, const TcSizes& z, void* dh,
+                 void* dw, int64_t N, int64_t V, int64_t D, int dtype, cudaStream_t st) {
+    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, st)) return e;
+    if (z.pack_w)
+      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, st)) return e;
+    const int64_t row = z.Kp * z.planes, zrow = z.piece * z.planes;
+    const void* wsrc = z.pack_w ? ws.wp : w;
+    const int64_t wrow = z.pack_w ? row : D;
+    CUtensorMap hk, hm, wk, wm, zk, zm;  // contraction along the row (k) or across rows (m)
+    if (!map_2d(&hk, ws.hp, bf16, row, z.Mp, row, xent::HALF) ||
+        !map_2d(&hm, ws.hp, bf16, row, z.Mp, row, xent::BK) ||
+        !map_2d(&wk, wsrc, bf16, wrow, V, wrow, xent::HALF) ||
+        !map_2d(&wm, wsrc, bf16, wrow, V, wrow, xent::BK) ||
+        !map_2d(&zk, ws.dz, bf16, zrow, z.Mp, zrow, xent::HALF) ||
+        !map_2d(&zm, ws.dz, bf16, zrow, z.Mp, zrow, xent::BK))
+      return THERIA_ERR_LAUNCH;
+    const int64_t mt = z.Mp / xent::BM, dt = cdiv(D, xent::BN);
+    for (int64_t c0 = 0; c0 < V; c0 += z.piece) {
+      const int64_t C = std::min(z.piece, V - c0), ct = cdiv(C, xent::BN);
+      xent::TcArgs a{};
+      a.n_live = ws.rows.n_live;
+      a.V = (int)V;
+      a.D = (int)D;
+      a.c0 = (int)c0;
+      a.Cn = (int)C;
+      a.pairs = z.planes > 1 ? 6 : 1;
+      a.plane_a = a.plane_b = (int)z.Kp;
+      a.tgt = ws.rows.tgt;
+      a.lse = ws.lse;
+      a.rowscale = ws.rowscale;
+      a.dz = ws.dz;
+      a.ld_dz = (int)z.piece;
+      a.acc = ws.acc;
+      a.acc_rows = z.Mp;
+      a.ld_acc = (int)z.ld_acc;
+      a.out = dw;
+      a.out_vec = vec_rows(D, dtype, {dw});
+      a.post = ws.post;
+      a.split_kb = (int)z.split_kb;
+      a.splits = (int)cdiv(cdiv(C, xent::BK), z.split_kb);
+      a.add = c0 > 0;
+      if (int e = tc_launch<T, O, xent::kDz>(hk, wk, a, mt * ct, st)) return e;
+      a.plane_a = (int)z.piece;
+      if (dh)
+        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, a, mt * dt * a.splits, st)) return e;
+      if (dw)
+        if (int e = tc_launch<T, O, xent::kDw>(zm, hm, a, ct * dt, st)) return e;
+    }
+    if (!dh) return THERIA_OK;
+    xent::dh_sum_kernel<O><<<(unsigned)std::min<int64_t>(cdiv(N * D, 256), kSMs * 16), 256, 0,
+                             st>>>(ws.acc, ws.rows.pos, ws.post, (int)z.splits, z.Mp,
+                                   (int)z.ld_acc, (O*)dh, N, D);
+    return launch_status();
+  }
+};
+
+// Whether this call runs on the tensor cores.
+bool use_tc(int64_t N, int64_t V, int64_t D, int dtype, const void* w) {
+  return !xent_small(N, V, D) && tc::encode_fn() != nullptr &&
+         (dtype == THERIA_F32 || D % 8 != 0 || tc::aligned16(w));
+}
+
 }  // namespace
 }  // namespace theria
 
 extern "C" {
 
 int64_t theria_xent_fwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
-  return N <= 0 || V <= 0 || D <= 0 ? 0 : xent_fwd_ws(nullptr, N, V).bytes;
+  if (N <= 0 || V <= 0 || D <= 0) return 0;
+  const int64_t b = xent_fwd_ws(nullptr, N, V).bytes;
+  if (xent_small(N, V, D)) return b;
+  return std::max(b, tc_fwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes);
 }
 int64_t theria_xent_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
-  return N <= 0 || V <= 0 || D <= 0 ? 0 : xent_bwd_ws(nullptr, N, V, D).bytes;
+  if (N <= 0 || V <= 0 || D <= 0) return 0;
+  const int64_t b = xent_bwd_ws(nullptr, N, V, D).bytes;
+  if (xent_small(N, V, D)) return b;
+  return std::max(b, tc_bwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes);
 }
 
 int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
@@ -415,28 +640,47 @@ int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
   if (N > 0 && (!h || !w || !target)) return THERIA_ERR_INVALID_ARG;
   if (N > 0 && (!workspace || workspace_bytes < theria_xent_fwd_workspace_bytes(N, V, D, dtype)))
     return THERIA_ERR_WORKSPACE;
-  const XentFwdWs ws = xent_fwd_ws(workspace, N > 0 ? N : 1, V);
-  float* each = reduction == THERIA_LOSS_NONE ? loss : ws.each;
+  const float* each = loss;
   if (N == 0) {
     cudaMemsetAsync(count, 0, sizeof(float), st);
     if (reduction == THERIA_LOSS_NONE) return THERIA_OK;
   } else {
-    const int tiles = (int)cdiv(V, xent::TN);
-    xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, ws.rows.pos,
-                                          ws.rows.row_of, ws.rows.tgt, ws.rows.n_live, count, each,
-                                          lse);
-    if (int e = launch_status()) return e;
-    int e = by_type(dtype, [&](auto t) {
-      using T = decltype(t);
-      xent::score_kernel<T><<<dim3((unsigned)tiles, (unsigned)cdiv(N, xent::TM)), 256, 0, st>>>(
-          (const T*)h, (const T*)w, ws.rows.row_of, ws.rows.tgt, ws.rows.n_live, ws.part, ws.zt, V,
-          D);
+    auto prep = [&](const XentRows& r, float* out) {
+      xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, r.pos, r.row_of,
+                                            r.tgt, r.n_live, count, out, lse);
       return launch_status();
-    });
-    if (e) return e;
-    xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
-        ws.part, ws.zt, ws.rows.row_of, ws.rows.n_live, tiles, each, lse);
-    if (int e2 = launch_status()) return e2;
+    };
+    if (use_tc(N, V, D, dtype, w)) {
+      const TcSizes z = tc_sizes(N, V, D, dtype);
+      const TcFwdWs ws = tc_fwd_ws(workspace, N, V, D, z);
+      float* out = reduction == THERIA_LOSS_NONE ? loss : ws.each;
+      each = out;
+      if (int e = prep(ws.rows, out)) return e;
+      const int e =
+          dtype == THERIA_F32  ? Tc<__nv_bfloat16, float>::fwd(h, w, ws, z, out, lse, N, V, D, st)
+          : dtype == THERIA_F16 ? Tc<__half, __half>::fwd(h, w, ws, z, out, lse, N, V, D, st)
+                                : Tc<__nv_bfloat16, __nv_bfloat16>::fwd(h, w, ws, z, out, lse, N,
+                                                                        V, D, st);
+      if (e) return e;
+    } else {
+      const XentFwdWs ws = xent_fwd_ws(workspace, N, V);
+      float* out = reduction == THERIA_LOSS_NONE ? loss : ws.each;
+      each = out;
+      if (int e = prep(ws.rows, out)) return e;
+      const int tiles = (int)cdiv(V, xent::TN);
+      const int e = by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        xent::score_kernel<T>
+            <<<dim3((unsigned)tiles, (unsigned)cdiv(N, xent::TM)), 256, 0, st>>>(
+                (const T*)h, (const T*)w, ws.rows.row_of, ws.rows.tgt, ws.rows.n_live, ws.part,
+                ws.zt, V, D);
+        return launch_status();
+      });
+      if (e) return e;
+      xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
+          ws.part, ws.zt, ws.rows.row_of, ws.rows.n_live, tiles, out, lse);
+      if (int e2 = launch_status()) return e2;
+    }
     if (reduction == THERIA_LOSS_NONE) return THERIA_OK;
   }
   xent::total_kernel<<<1, 1024, 0, st>>>(each, N, count, reduction == THERIA_LOSS_MEAN, loss);
@@ -459,11 +703,29 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   if (!dh && !dw) return THERIA_OK;
   if (!workspace || workspace_bytes < theria_xent_bwd_workspace_bytes(N, V, D, dtype))
     return THERIA_ERR_WORKSPACE;
+  const float* mean_of = reduction == THERIA_LOSS_MEAN ? count : nullptr;
+  auto prep = [&](const XentRows& r) {
+    xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, r.pos, r.row_of,
+                                          r.tgt, r.n_live, nullptr, nullptr, nullptr);
+    return launch_status();
+  };
+  if (use_tc(N, V, D, dtype, w)) {
+    const TcSizes z = tc_sizes(N, V, D, dtype);
+    const TcBwdWs ws = tc_bwd_ws(workspace, N, V, D, z);
+    if (int e = prep(ws.rows)) return e;
+    xent::scale_kernel<<<1, 1024, 0, st>>>(ws.rows.row_of, ws.rows.n_live, gloss,
+                                           reduction == THERIA_LOSS_NONE, mean_of, lse,
+                                           dtype == THERIA_F16, ws.lse, ws.rowscale, ws.post);
+    if (int e = launch_status()) return e;
+    return dtype == THERIA_F32
+               ? Tc<__nv_bfloat16, float>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
+           : dtype == THERIA_F16
+               ? Tc<__half, __half>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
+               : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st);
+  }
   const XentBwdWs ws = xent_bwd_ws(workspace, N, V, D);
   const XentRows& r = ws.rows;
-  xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, r.pos, r.row_of, r.tgt,
-                                        r.n_live, nullptr, nullptr, nullptr);
-  if (int e = launch_status()) return e;
+  if (int e = prep(r)) return e;
   const unsigned mt = (unsigned)cdiv(N, xent::TM), dt = (unsigned)cdiv(D, xent::TN);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -472,8 +734,7 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
       const unsigned ct = (unsigned)cdiv(C, xent::TN);
       xent::dz_kernel<T><<<dim3(ct, mt), 256, 0, st>>>(
           (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, lse, gloss,
-          reduction == THERIA_LOSS_NONE, reduction == THERIA_LOSS_MEAN ? count : nullptr, ws.dz,
-          c0, C, V, D);
+          reduction == THERIA_LOSS_NONE, mean_of, ws.dz, c0, C, V, D);
       if (int e = launch_status()) return e;
       if (dh) {
         xent::dh_kernel<T><<<dim3(dt, mt), 256, 0, st>>>(ws.dz, (const T*)w, r.n_live, ws.acc, c0,
