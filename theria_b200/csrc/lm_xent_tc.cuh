@@ -21,6 +21,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "lm_embed.cuh"
 #include "tc_common.cuh"
 
 namespace theria {
@@ -34,6 +35,7 @@ constexpr int SUB = 128;                    // columns per score partial
 constexpr int STAGES = 6;
 constexpr int OPERAND = HALF * BK * 2;      // bytes of one operand's stage
 constexpr int EPI_WARPS = 8;
+constexpr int STAGE_OUT = 4096;             // a warp's stage of results: 32 rows of 128 bytes
 constexpr int TC_THREADS = 128 + EPI_WARPS * 32;
 constexpr uint32_t ACC_COLS = 256;
 constexpr uint32_t POLLS = 1u << 20;  // bound of one wait; a poll suspends the thread for a while
@@ -46,19 +48,18 @@ struct TcArgs {
   int plane_a, plane_b; // elements between planes of one row
   int splits, split_kb; // kDh: splits of the contraction, k blocks in each
   int add;              // kDh: add to what the partials hold (a later piece)
+  int rows;             // all rows; if every one counts, A (B for kDw) is h itself, unpacked
+  int h_plain;          // ... where h can be read as it is
   const int* tgt;       // kScore, kDz
   float2* part;         // kScore: [row][sub_tiles]
   int sub_tiles;
   float* zt;
   const float* lse;     // kDz, by packed row
   const float* rowscale;
-  void* dz;             // kDz: [row][planes][ld_dz]
-  int ld_dz;
-  float* acc;           // kDh: [split][acc_rows][ld_acc]
-  int64_t acc_rows;
+  int ld_dz;            // kDz: dz is [row][planes][ld_dz]
+  int acc_rows;         // kDh: [split][acc_rows][ld_acc] partial sums
   int ld_acc;
-  void* out;            // kDw: [V][D]
-  int out_vec;
+  void* out;            // kDw: [V][D], where it cannot be stored by TMA
   const float* post;    // kDw: the factor of the result
 };
 
@@ -84,6 +85,23 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                : "memory");
+}
+// A warp's staged 32 x 128-byte tile to (x, y) of `map`, or added to it
+// (float32); one bulk group of this thread.
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(tc::smem_u32(src)), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void add_2d(const CUtensorMap* map, const void* src, int x, int y) {
+  asm volatile(
+      "cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}],"
+      " [%1];\n\t"
+      "cp.async.bulk.commit_group;" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(tc::smem_u32(src)), "r"(x), "r"(y)
+      : "memory");
 }
 // Box at (x, y) of `map` into this CTA's shared memory; the bytes count on a
 // barrier that may be the pair's other CTA's.
@@ -116,12 +134,14 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
 struct TcSmem {
   static constexpr int oA = 0;
   static constexpr int oB = STAGES * OPERAND;
-  static constexpr int oBar = 2 * STAGES * OPERAND;  // full, empty, acc_full, acc_empty
+  static constexpr int oOut = 2 * STAGES * OPERAND;
+  static constexpr int oBar = oOut + EPI_WARPS * STAGE_OUT;  // full, empty, acc_full, acc_empty
   static constexpr int kBars = 2 * STAGES + 4;
   static constexpr int oTmem = oBar + kBars * 8;
   static constexpr int oAbort = oTmem + 4;
   static constexpr int kBytes = oAbort + 4;
   static constexpr int kAlloc = kBytes + 1024;  // the base is aligned to 1024
+  static_assert(kAlloc <= 232448, "shared memory of one CTA");
 };
 
 // What one cluster works on next.
@@ -171,28 +191,24 @@ struct Sched {
   }
 };
 
-// 32 consecutive values of one row, converted and stored.
+// 32 consecutive values of one row: into a 128-byte row of a warp's stage, as
+// its 16-byte chunks c0 .. (128-byte swizzle).
 template <typename O>
-__device__ __forceinline__ void store32(O* dst, const float (&v)[32], int valid, bool vec) {
-  if (vec && valid >= 32) {
-    if constexpr (sizeof(O) == 4) {
+__device__ __forceinline__ void stage32(uint32_t row, int lane, const float (&v)[32], int c0) {
+  if constexpr (sizeof(O) == 4) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        reinterpret_cast<float4*>(dst)[i] =
-            make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float* e = v + 8 * i;
-        reinterpret_cast<uint4*>(dst)[i] =
-            make_uint4(tc::pack2<O>(e[0], e[1]), tc::pack2<O>(e[2], e[3]),
-                       tc::pack2<O>(e[4], e[5]), tc::pack2<O>(e[6], e[7]));
-      }
-    }
+    for (int i = 0; i < 8; ++i)
+      tc::st_shared_v4(row + ((i ^ (lane & 7)) << 4), __float_as_uint(v[4 * i]),
+                       __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]),
+                       __float_as_uint(v[4 * i + 3]));
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (i < valid) dst[i] = from_f32<O>(v[i]);
+    for (int i = 0; i < 4; ++i) {
+      const float* e = v + 8 * i;
+      tc::st_shared_v4(row + (((c0 + i) ^ (lane & 7)) << 4), tc::pack2<O>(e[0], e[1]),
+                       tc::pack2<O>(e[2], e[3]), tc::pack2<O>(e[4], e[5]),
+                       tc::pack2<O>(e[6], e[7]));
+    }
   }
 }
 
@@ -204,13 +220,21 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   p[2] = __float2bfloat16_rz(r1 - __bfloat162float(p[1]));
 }
 
+// k blocks that one accumulation in TMEM runs over for float32.  The tensor
+// core cuts each sum to the accumulator's precision instead of rounding it,
+// which over a long contraction leaves a bias of about one unit in the last
+// place per step; the sums of short chunks are added in registers instead.
+constexpr int F32_CHUNK = 4;
+
 // T: the operands' type.  O: the type of the user's tensors (float32 with T =
 // bfloat16 planes, else T).
 template <typename T, typename O, int EPI>
 __global__ void __launch_bounds__(TC_THREADS, 1) __cluster_dims__(2, 1, 1)
 tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+          const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_o,
           const __grid_constant__ TcArgs args) {
   constexpr bool A_MN = EPI == kDw, B_MN = EPI == kDh || EPI == kDw;
+  constexpr bool F32 = sizeof(O) == 4;
   using L = TcSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -236,8 +260,6 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     }
     *abort = 0;
     tc::fence_barrier_init();
-    tc::prefetch_tmap(&map_a);
-    tc::prefetch_tmap(&map_b);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -252,39 +274,47 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const Sched<EPI> sched(args);
+  // k blocks per accumulation
+  const auto chunk = [](const Unit& un) { return F32 ? F32_CHUNK : un.kbs; };
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------ loads, in both CTAs
+    const bool plain = args.h_plain && *args.n_live == args.rows;
+    const CUtensorMap* pa = EPI <= kDz && plain ? &map_h : &map_a;
+    const CUtensorMap* pb = EPI == kDw && plain ? &map_h : &map_b;
     uint32_t it = 0;
     bool ok = true;
     for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = sched.at(u);
       const int m0 = un.m0 + rank * HALF, n0 = un.n0 + rank * HALF;
-      for (int i = 0, n = args.pairs * un.kbs; i < n; ++i, ++it) {
-        const int slot = it % STAGES;
-        if (!tc::mbar_wait(empty + slot, ((it / STAGES) & 1) ^ 1, abort, POLLS)) {
-          ok = false;
-          break;
-        }
-        const int pr = i / un.kbs, k = (un.kb0 + i - pr * un.kbs) * BK;
-        const int xa = args.pairs > 1 ? pair_a(pr) * args.plane_a : 0;
-        const int xb = args.pairs > 1 ? pair_b(pr) * args.plane_b : 0;
-        uint8_t* a = smem + L::oA + slot * OPERAND;
-        uint8_t* b = smem + L::oB + slot * OPERAND;
-        if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
-        const uint32_t bar = map_rank(full + slot, 0);
-        if constexpr (A_MN) {
-          load_2d(a, &map_a, bar, xa + m0, k);
-          load_2d(a + OPERAND / 2, &map_a, bar, xa + m0 + 64, k);
-        } else {
-          load_2d(a, &map_a, bar, xa + k, m0);
-        }
-        if constexpr (B_MN) {
-          const int y = (EPI == kDh ? args.c0 : 0) + k;
-          load_2d(b, &map_b, bar, xb + n0, y);
-          load_2d(b + OPERAND / 2, &map_b, bar, xb + n0 + 64, y);
-        } else {
-          load_2d(b, &map_b, bar, xb + k, (EPI == kDz ? args.c0 : 0) + n0);
+      for (int kc = 0; ok && kc < un.kbs; kc += chunk(un)) {
+        const int len = min(chunk(un), un.kbs - kc);
+        for (int i = 0, n = args.pairs * len; i < n; ++i, ++it) {
+          const int slot = it % STAGES;
+          if (!tc::mbar_wait(empty + slot, ((it / STAGES) & 1) ^ 1, abort, POLLS)) {
+            ok = false;
+            break;
+          }
+          const int pr = i / len, k = (un.kb0 + kc + i - pr * len) * BK;
+          const int xa = F32 ? pair_a(pr) * args.plane_a : 0;
+          const int xb = F32 ? pair_b(pr) * args.plane_b : 0;
+          uint8_t* a = smem + L::oA + slot * OPERAND;
+          uint8_t* b = smem + L::oB + slot * OPERAND;
+          if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
+          const uint32_t bar = map_rank(full + slot, 0);
+          if constexpr (A_MN) {
+            load_2d(a, pa, bar, xa + m0, k);
+            load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, k);
+          } else {
+            load_2d(a, pa, bar, xa + k, m0);
+          }
+          if constexpr (B_MN) {
+            const int y = (EPI == kDh ? args.c0 : 0) + k;
+            load_2d(b, pb, bar, xb + n0, y);
+            load_2d(b + OPERAND / 2, pb, bar, xb + n0 + 64, y);
+          } else {
+            load_2d(b, pb, bar, xb + k, (EPI == kDz ? args.c0 : 0) + n0);
+          }
         }
       }
     }
@@ -299,64 +329,78 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;
     const uint64_t da = tc::sw128_desc(tc::smem_u32(smem + L::oA), A_MN ? OPERAND / 2 : 16, 1024);
     const uint64_t db = tc::sw128_desc(tc::smem_u32(smem + L::oB), B_MN ? OPERAND / 2 : 16, 1024);
-    uint32_t it = 0, n_unit = 0;
+    uint32_t it = 0, n_acc = 0;
     bool ok = true;
-    for (int u = cluster; ok && u < sched.units; u += clusters, ++n_unit) {
+    for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = sched.at(u);
-      const uint32_t buf = n_unit & 1;
-      if (!tc::mbar_wait(acc_empty + buf, ((n_unit >> 1) & 1) ^ 1, abort, POLLS)) break;
-      tc::tc_fence_after();
-      const uint32_t d = tmem + buf * ACC_COLS;
-      for (int i = 0, n = args.pairs * un.kbs; i < n; ++i, ++it) {
-        const int slot = it % STAGES;
-        if (!tc::mbar_wait(full + slot, (it / STAGES) & 1, abort, POLLS)) {
+      for (int kc = 0; ok && kc < un.kbs; kc += chunk(un), ++n_acc) {
+        const uint32_t buf = n_acc & 1;
+        if (!tc::mbar_wait(acc_empty + buf, ((n_acc >> 1) & 1) ^ 1, abort, POLLS)) {
           ok = false;
           break;
         }
         tc::tc_fence_after();
-        const uint64_t a = tc::desc_at(da, slot * OPERAND), b = tc::desc_at(db, slot * OPERAND);
+        const uint32_t d = tmem + buf * ACC_COLS;
+        const int len = min(chunk(un), un.kbs - kc);
+        for (int i = 0, n = args.pairs * len; i < n; ++i, ++it) {
+          const int slot = it % STAGES;
+          if (!tc::mbar_wait(full + slot, (it / STAGES) & 1, abort, POLLS)) {
+            ok = false;
+            break;
+          }
+          tc::tc_fence_after();
+          const uint64_t a = tc::desc_at(da, slot * OPERAND), b = tc::desc_at(db, slot * OPERAND);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          mma_pair(d, tc::desc_at(a, k * step_a), tc::desc_at(b, k * step_b), id,
-                   (i > 0 || k > 0) ? 1u : 0u);
-        commit_pair(empty + slot);
+          for (int k = 0; k < BK / 16; ++k)
+            mma_pair(d, tc::desc_at(a, k * step_a), tc::desc_at(b, k * step_b), id,
+                     (i > 0 || k > 0) ? 1u : 0u);
+          commit_pair(empty + slot);
+        }
+        if (ok) commit_pair(acc_full + buf);
       }
-      if (ok) commit_pair(acc_full + buf);
     }
   } else if (warp >= 4) {
     // ------------------------------------------- epilogue, in both CTAs
     const int quarter = warp & 3, side = (warp - 4) >> 2;  // TMEM lanes, column half
-    const int r = quarter * 32 + lane;
     const int live = *args.n_live;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    uint32_t n_unit = 0;
-    for (int u = cluster; u < sched.units; u += clusters, ++n_unit) {
+    const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + side * SUB;
+    uint8_t* out = smem + L::oOut + (warp - 4) * STAGE_OUT;
+    const uint32_t out_row = tc::smem_u32(out) + lane * 128;
+    const float post = EPI == kDw ? *args.post : 1.f;
+    // The stage may be written again once the store before has read it.
+    auto stage_free = [&] {
+      if (lane == 0) tc::bulk_wait_read_all();
+      __syncwarp();
+    };
+    auto stage_full = [&](int x, int y) {
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (EPI == kDh && args.add) add_2d(&map_o, out, x, y);
+        else store_2d(&map_o, out, x, y);
+      }
+    };
+    uint32_t n_acc = 0;
+    bool ok = true;
+    for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = sched.at(u);
-      const uint32_t buf = n_unit & 1;
-      const int m = un.m0 + rank * HALF + r, n0 = un.n0 + side * SUB;
+      const int m_warp = un.m0 + rank * HALF + quarter * 32, m = m_warp + lane;
+      const int n0 = un.n0 + side * SUB;
       // what the row needs, fetched while the product is still running
       int t = -1;
-      float l = 0.f, rs = 0.f, post = 1.f;
-      if (EPI == kScore || EPI == kDz) t = m < live ? args.tgt[m] - (EPI == kDz ? args.c0 : 0) : -1;
+      float l = 0.f, rs = 0.f, top = -INFINITY, sum = 0.f;
+      if (EPI <= kDz && m < live) t = args.tgt[m] - (EPI == kDz ? args.c0 : 0);
       if (EPI == kDz && m < live) {
         l = args.lse[m];
         rs = args.rowscale[m];
       }
-      if (EPI == kDw) post = *args.post;
-      const bool got = __all_sync(0xffffffffu,
-                                  tc::mbar_wait(acc_full + buf, (n_unit >> 1) & 1, abort, POLLS));
-      if (!got) break;
-      tc::tc_fence_after();
-      const uint32_t src = tmem + buf * ACC_COLS + lanes + side * SUB;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < SUB; c += 32) {
-        float v[32];
-        tc::tmem_ld32(src + c, v);  // warp-collective
+
+      // columns n .. n + 31 of this thread's row; c: their place in the half
+      auto take = [&](float (&v)[32], int c) {
         const int n = n0 + c;
         if constexpr (EPI == kScore) {
           const int valid = args.V - n;
-          if (valid <= 0) continue;
+          if (valid <= 0) return;
           if (valid < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -374,70 +418,122 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           const float base = now == -INFINITY ? 0.f : now * 1.4426950408889634f;
           sum *= tc::ex2(fmaf(top, 1.4426950408889634f, -base));
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            sum += tc::ex2(fmaf(v[i], 1.4426950408889634f, -base));
+          for (int i = 0; i < 32; ++i) sum += tc::ex2(fmaf(v[i], 1.4426950408889634f, -base));
           top = now;
         } else if constexpr (EPI == kDz) {
           const int valid = args.Cn - n;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             float p;
-            if constexpr (sizeof(O) == 4) p = expf(v[i] - l);
+            if constexpr (F32) p = expf(v[i] - l);
             else p = tc::ex2((v[i] - l) * 1.4426950408889634f);
             if (n + i == t) p -= 1.f;
             v[i] = (m < live && i < valid) ? rs * p : 0.f;
           }
-          if constexpr (sizeof(O) == 4) {
-            __nv_bfloat16* row = (__nv_bfloat16*)args.dz + (int64_t)m * 3 * args.ld_dz + n;
+          if constexpr (F32) {
+            // 32 columns of the three planes: planes 0, 1 side by side in one
+            // stage would split a box, so each is staged on its own
 #pragma unroll
             for (int pl = 0; pl < 3; ++pl) {
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                __nv_bfloat16 x[3], y[3];
-                split3(v[2 * i], x);
-                split3(v[2 * i + 1], y);
-                const __nv_bfloat162 q = __halves2bfloat162(x[pl], y[pl]);
+                const __nv_bfloat16 x = __float2bfloat16_rz(v[2 * i]);
+                const __nv_bfloat16 y = __float2bfloat16_rz(v[2 * i + 1]);
+                const __nv_bfloat162 q = __halves2bfloat162(x, y);
                 w[i] = *reinterpret_cast<const uint32_t*>(&q);
+                v[2 * i] -= __bfloat162float(x);
+                v[2 * i + 1] -= __bfloat162float(y);
               }
+              stage_free();
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                reinterpret_cast<uint4*>(row + pl * args.ld_dz)[i] =
-                    make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                tc::st_shared_v4(tc::smem_u32(out) + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4),
+                                 w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              stage_full(pl * args.ld_dz + n, m_warp);
             }
           } else {
-            store32<T>((T*)args.dz + (int64_t)m * args.ld_dz + n, v, 32, true);
+            if (c % 64 == 0) stage_free();
+            stage32<T>(out_row, lane, v, c % 64 / 8);
+            if (c % 64 == 32) stage_full(n - 32, m_warp);
           }
         } else if constexpr (EPI == kDh) {
-          if (m < live && n < args.ld_acc) {
-            float* dst = args.acc + (un.split * args.acc_rows + m) * args.ld_acc + n;
-            if (args.add) {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 o = reinterpret_cast<const float4*>(dst)[i];
-                v[4 * i] += o.x;
-                v[4 * i + 1] += o.y;
-                v[4 * i + 2] += o.z;
-                v[4 * i + 3] += o.w;
-              }
-            }
-            store32<float>(dst, v, 32, true);
-          }
+          if (n >= args.ld_acc) return;
+          stage_free();
+          stage32<float>(out_row, lane, v, 0);
+          stage_full(n, un.split * args.acc_rows + m_warp);
         } else {
-          if (m < args.Cn && n < args.D) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= post;
-            store32<O>((O*)args.out + (int64_t)(args.c0 + m) * args.D + n, v, args.D - n,
-                       args.out_vec);
+          for (int i = 0; i < 32; ++i) v[i] *= post;
+          if (args.out) {
+            if (m < args.Cn) {
+              O* dst = (O*)args.out + (int64_t)(args.c0 + m) * args.D + n;
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (n + i < args.D) dst[i] = from_f32<O>(v[i]);
+            }
+          } else if constexpr (F32) {
+            stage_free();
+            stage32<float>(out_row, lane, v, 0);
+            if (n < args.D && m_warp < args.Cn) stage_full(n, args.c0 + m_warp);
+          } else {
+            if (c % 64 == 0) stage_free();
+            stage32<O>(out_row, lane, v, c % 64 / 8);
+            if (c % 64 == 32 && n - 32 < args.D && m_warp < args.Cn)
+              stage_full(n - 32, args.c0 + m_warp);
           }
         }
+      };
+      // the buffer is read: the leading CTA may multiply into it again
+      auto give_back = [&](uint32_t buf) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(map_rank(acc_empty + buf, 0));
+      };
+
+      if constexpr (F32) {
+        float acc[SUB / 32][32];
+#pragma unroll
+        for (int c = 0; c < SUB / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
+        for (int kc = 0; kc < un.kbs; kc += F32_CHUNK, ++n_acc) {
+          const uint32_t buf = n_acc & 1;
+          ok = __all_sync(0xffffffffu,
+                          tc::mbar_wait(acc_full + buf, (n_acc >> 1) & 1, abort, POLLS));
+          if (!ok) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < SUB / 32; ++c) {
+            float v[32];
+            tc::tmem_ld32(src + buf * ACC_COLS + c * 32, v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[c][i] += v[i];
+          }
+          give_back(buf);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < SUB / 32; ++c) take(acc[c], c * 32);
+      } else {
+        const uint32_t buf = n_acc & 1;
+        ok = __all_sync(0xffffffffu,
+                        tc::mbar_wait(acc_full + buf, (n_acc >> 1) & 1, abort, POLLS));
+        if (!ok) break;
+        ++n_acc;
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < SUB; c += 32) {
+          float v[32];
+          tc::tmem_ld32(src + buf * ACC_COLS + c, v);  // warp-collective
+          if (c == SUB - 32) give_back(buf);
+          take(v, c);
+        }
       }
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_cluster(map_rank(acc_empty + buf, 0));
       if (EPI == kScore && m < live && n0 < args.V)
         args.part[(int64_t)m * args.sub_tiles + n0 / SUB] = make_float2(top, sum);
     }
+    if (lane == 0) tc::bulk_wait_all();
   }
 
   // Copies in flight after a wait that gave up land before the CTA ends.
@@ -463,8 +559,9 @@ template <typename T, typename O>
 __global__ void __launch_bounds__(256)
 pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
             const int* __restrict__ n_live, int64_t rows, T* __restrict__ dst, int64_t D,
-            int64_t Kp, int vec) {
+            int64_t Kp, int vec, int plain) {
   const int64_t live = n_live ? *n_live : rows;
+  if (plain && live == rows) return;  // the products read src itself
   const int64_t end = n_live ? (live > 0 ? (live + BM - 1) / BM * BM : BM) : rows;
   constexpr int planes = sizeof(O) == 4 ? 3 : 1;
   const int64_t units = Kp / 8;
@@ -499,54 +596,43 @@ pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
   }
 }
 
-// By packed row: lse, and the row's factor of dz.  *post: the factor of the
-// results.  float16 holds dz in [2^-29, 2^15] (units of 1 / 32768 of the
-// largest row's factor): probabilities of 1e-9 stay normal numbers.
-constexpr float HALF_SCALE = 32768.f;
-__global__ void __launch_bounds__(1024)
-scale_kernel(const int* __restrict__ row_of, const int* __restrict__ n_live,
-             const float* __restrict__ gloss, int per_row, const float* __restrict__ count,
-             const float* __restrict__ lse, int half, float* __restrict__ lse_p,
-             float* __restrict__ rowscale, float* __restrict__ post) {
-  __shared__ float part[32];
-  const int n = *n_live;
-  const float unit = half ? HALF_SCALE : 1.f;
-  float most = 0.f;
-  if (per_row && half) {
-    for (int m = threadIdx.x; m < n; m += 1024) {
-      const float g = fabsf(gloss[row_of[m]]);
-      if (isfinite(g)) most = fmaxf(most, g);
-    }
-    most = warp_max(most);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
-    __syncthreads();
-    most = warp_max(part[threadIdx.x & 31]);
-  }
-  if (most == 0.f) most = 1.f;
-  for (int m = threadIdx.x; m < n; m += 1024) {
-    const int row = row_of[m];
-    lse_p[m] = lse[row];
-    rowscale[m] = unit * (per_row ? gloss[row] / most : 1.f);
-  }
-  if (threadIdx.x == 0)
-    *post = (per_row ? most : count ? (n > 0 ? gloss[0] / *count : 0.f) : gloss[0]) / unit;
-}
-
 // dh[i] = post * the sum of the splits' partials of row pos[i], or zeros.
-template <typename O>
+// VEC values a thread.
+template <typename O, int VEC>
 __global__ void __launch_bounds__(256)
 dh_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
               const float* __restrict__ post, int splits, int64_t acc_rows, int ld_acc,
-              O* __restrict__ dh, int64_t N, int64_t D) {
+              O* __restrict__ dh, int64_t N, int D) {
   const float f = *post;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < N * D;
-       e += (int64_t)gridDim.x * 256) {
-    const int64_t i = e / D, d = e - i * D;
+  const int units = D / VEC;
+  for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
     const int m = pos[i];
-    float s = 0.f;
-    if (m >= 0)
-      for (int k = 0; k < splits; ++k) s += acc[(k * acc_rows + m) * ld_acc + d];
-    dh[e] = from_f32<O>(s * f);
+    for (int u = threadIdx.x; u < units; u += 256) {
+      float s[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s[k] = 0.f;
+      if (m >= 0) {
+#pragma unroll 4
+        for (int k = 0; k < splits; ++k) {
+          const float* p = acc + (k * acc_rows + m) * ld_acc + u * VEC;
+          if constexpr (VEC == 1) {
+            s[0] += p[0];
+          } else {
+#pragma unroll
+            for (int q = 0; q < VEC / 4; ++q) {
+              const float4 x = reinterpret_cast<const float4*>(p)[q];
+              s[4 * q] += x.x;
+              s[4 * q + 1] += x.y;
+              s[4 * q + 2] += x.z;
+              s[4 * q + 3] += x.w;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s[k] *= f;
+      embed::store_vec<O, VEC>(dh + i * D + u * VEC, s);
+    }
   }
 }
 

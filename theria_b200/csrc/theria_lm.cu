@@ -352,14 +352,46 @@ int xent_check(int64_t N, int64_t V, int64_t D, int dtype, int reduction) {
 
 struct XentRows {  // filled by prep_kernel
   int *pos, *row_of, *tgt, *n_live;
+  unsigned* done;
+  float *lse, *rowscale, *post;  // backward
 };
 XentRows xent_rows(Carver& c, int64_t N) {
   XentRows r;
   r.pos = c.take<int>(N);
   r.row_of = c.take<int>(N);
   r.tgt = c.take<int>(N);
-  r.n_live = c.take<int>(1);
+  r.lse = c.take<float>(N);
+  r.rowscale = c.take<float>(N);
+  r.n_live = c.take<int>(64);  // and what else is one value
+  r.done = (unsigned*)r.n_live + 1;
+  r.post = (float*)r.n_live + 2;
   return r;
+}
+xent::Prep xent_prep(const XentRows& r, const void* target, int wide, int64_t ignore_index,
+                     int64_t N, int64_t V) {
+  xent::Prep p{};
+  p.target = target;
+  p.wide = wide;
+  p.ignore_index = ignore_index;
+  p.N = N;
+  p.V = V;
+  p.pos = r.pos;
+  p.row_of = r.row_of;
+  p.tgt = r.tgt;
+  p.n_live = r.n_live;
+  p.done = r.done;
+  return p;
+}
+// Where the forward's loss goes: each row's, and their sum or mean (NULL: no).
+struct LossOut {
+  float *each, *lse, *out;
+  int mean;
+};
+int xent_join(const XentRows& r, const float2* part, const float* zt, int tiles,
+              const LossOut& o, int64_t N, cudaStream_t st) {
+  xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
+      part, zt, r.row_of, r.n_live, tiles, o.each, o.lse, r.done, o.out, o.mean, N);
+  return launch_status();
 }
 // --------------------------------------------------------- CUDA-core path
 struct XentFwdWs {
@@ -461,7 +493,7 @@ TcFwdWs tc_fwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z)
 struct TcBwdWs {
   XentRows rows;
   void *hp, *wp, *dz;
-  float *acc, *lse, *rowscale, *post;
+  float* acc;
   int64_t bytes;
 };
 TcBwdWs tc_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z) {
@@ -472,135 +504,159 @@ TcBwdWs tc_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z)
   w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
   w.dz = c.take<uint16_t>(z.Mp * z.piece * z.planes);
   w.acc = c.take<float>(z.splits * z.Mp * z.ld_acc);
-  w.lse = c.take<float>(N);
-  w.rowscale = c.take<float>(N);
-  w.post = c.take<float>(1);
   w.bytes = c.used;
   return w;
 }
 
-// 2-D map of 16-bit rows [rows][inner] at ld elements, box {64, box_rows}.
-bool map_2d(CUtensorMap* map, const void* base, bool bf16, int64_t inner, int64_t rows, int64_t ld,
-            int box_rows) {
+// 2-D map of rows [rows][inner] of `dtype`, `inner` apart, box {bytes / size,
+// box_rows}, swizzled by `bytes` (128 or 64).
+bool map_2d(CUtensorMap* map, const void* base, int dtype, int64_t inner, int64_t rows,
+            int box_rows, int bytes = 128) {
   tc::EncodeTiledFn fn = tc::encode_fn();
   if (fn == nullptr) return false;
+  const int64_t size = elem_size(dtype);
   cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
-  cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(inner * size)};
+  cuuint32_t box[2] = {(cuuint32_t)(bytes / size), (cuuint32_t)box_rows};
   cuuint32_t estr[2] = {1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(map,
+            dtype == THERIA_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+            : dtype == THERIA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                  : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, typename O, int EPI>
-int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const xent::TcArgs& args, int64_t units,
-              cudaStream_t st) {
+int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& h,
+              const CUtensorMap& o, const xent::TcArgs& args, int64_t units, cudaStream_t st) {
   auto kern = xent::tc_kernel<T, O, EPI>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            xent::TcSmem::kAlloc) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(units, kClusters);
-  kern<<<grid, xent::TC_THREADS, xent::TcSmem::kAlloc, st>>>(a, b, args);
+  kern<<<grid, xent::TC_THREADS, xent::TcSmem::kAlloc, st>>>(a, b, h, o, args);
   return launch_status();
 }
 
 template <typename T, typename O>
 int tc_pack(const void* src, const int* row_of, const int* n_live, int64_t rows, void* dst,
-            int64_t D, int64_t Kp, cudaStream_t st) {
+            int64_t D, int64_t Kp, bool plain, cudaStream_t st) {
   const int dtype = std::is_same<O, float>::value ? THERIA_F32 : THERIA_F16;
   const int64_t threads = (n_live ? up(rows, xent::BM) : rows) * (Kp / 8);
   xent::pack_kernel<T, O><<<(unsigned)std::min<int64_t>(cdiv(threads, 256), kSMs * 32), 256, 0,
                             st>>>((const O*)src, row_of, n_live, rows, (T*)dst, D, Kp,
-                                  vec_rows(D, dtype, {src}));
+                                  vec_rows(D, dtype, {src}), plain);
   return launch_status();
 }
 
 // T: the operands' type; O: the tensors'.
 template <typename T, typename O>
 struct Tc {
-  static constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int op = std::is_same<T, __half>::value ? THERIA_F16 : THERIA_BF16;
 
-  static int fwd(const void* h, const void* w, const TcFwdWs& ws, const TcSizes& z, float* each,
-                 float* lse, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
-    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, st)) return e;
-    if (z.pack_w)
-      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, st)) return e;
-    CUtensorMap ma, mb;
-    if (!map_2d(&ma, ws.hp, bf16, z.Kp * z.planes, z.Mp, z.Kp * z.planes, xent::HALF) ||
-        !(z.pack_w ? map_2d(&mb, ws.wp, bf16, z.Kp * z.planes, V, z.Kp * z.planes, xent::HALF)
-                   : map_2d(&mb, w, bf16, D, V, D, xent::HALF)))
-      return THERIA_ERR_LAUNCH;
+  // h can be read by TMA as it is (where every row counts)
+  static bool plain(const void* h, int64_t D, const TcSizes& z) {
+    return z.planes == 1 && D % 8 == 0 && tc::aligned16(h);
+  }
+  static xent::TcArgs common(const void* h, const XentRows& r, const TcSizes& z, int64_t N,
+                             int64_t V, int64_t D) {
     xent::TcArgs a{};
-    a.n_live = ws.rows.n_live;
+    a.n_live = r.n_live;
     a.V = (int)V;
     a.D = (int)D;
     a.pairs = z.planes > 1 ? 6 : 1;
     a.plane_a = a.plane_b = (int)z.Kp;
-    a.tgt = ws.rows.tgt;
+    a.tgt = r.tgt;
+    a.rows = (int)N;
+    a.h_plain = plain(h, D, z);
+    return a;
+  }
+
+  static int fwd(const void* h, const void* w, const TcFwdWs& ws, const TcSizes& z,
+                 const LossOut& out, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
+    xent::TcArgs a = common(h, ws.rows, z, N, V, D);
+    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, a.h_plain, st))
+      return e;
+    if (z.pack_w)
+      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, false, st)) return e;
+    const int64_t row = z.Kp * z.planes;
+    CUtensorMap ma, mb, mh;
+    if (!map_2d(&ma, ws.hp, op, row, z.Mp, xent::HALF) ||
+        !map_2d(&mb, z.pack_w ? ws.wp : w, op, z.pack_w ? row : D, V, xent::HALF))
+      return THERIA_ERR_LAUNCH;
+    mh = ma;
+    if (a.h_plain && !map_2d(&mh, h, op, D, N, xent::HALF)) return THERIA_ERR_LAUNCH;
     a.part = ws.part;
     a.sub_tiles = (int)cdiv(V, xent::SUB);
     a.zt = ws.zt;
-    if (int e = tc_launch<T, O, xent::kScore>(ma, mb, a, z.Mp / xent::BM * cdiv(V, xent::BN), st))
+    if (int e = tc_launch<T, O, xent::kScore>(ma, mb, mh, ma, a,
+                                              z.Mp / xent::BM * cdiv(V, xent::BN), st))
       return e;
-    xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
-        ws.part, ws.zt, ws.rows.row_of, ws.rows.n_live, a.sub_tiles, each, lse);
-    return launch_status();
+    return xent_join(ws.rows, ws.part, ws.zt, a.sub_tiles, out, N, st);
   }
 
   static int bwd(const void* h, const void* w, const TcBwdWs& ws, const TcSizes& z, void* dh,
                  void* dw, int64_t N, int64_t V, int64_t D, int dtype, cudaStream_t st) {
-    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, st)) return e;
+    const XentRows& r = ws.rows;
+    const xent::TcArgs base = common(h, r, z, N, V, D);
+    if (int e = tc_pack<T, O>(h, r.row_of, r.n_live, N, ws.hp, D, z.Kp, base.h_plain, st))
+      return e;
     if (z.pack_w)
-      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, st)) return e;
+      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, false, st)) return e;
     const int64_t row = z.Kp * z.planes, zrow = z.piece * z.planes;
     const void* wsrc = z.pack_w ? ws.wp : w;
     const int64_t wrow = z.pack_w ? row : D;
-    CUtensorMap hk, hm, wk, wm, zk, zm;  // contraction along the row (k) or across rows (m)
-    if (!map_2d(&hk, ws.hp, bf16, row, z.Mp, row, xent::HALF) ||
-        !map_2d(&hm, ws.hp, bf16, row, z.Mp, row, xent::BK) ||
-        !map_2d(&wk, wsrc, bf16, wrow, V, wrow, xent::HALF) ||
-        !map_2d(&wm, wsrc, bf16, wrow, V, wrow, xent::BK) ||
-        !map_2d(&zk, ws.dz, bf16, zrow, z.Mp, zrow, xent::HALF) ||
-        !map_2d(&zm, ws.dz, bf16, zrow, z.Mp, zrow, xent::BK))
+    const bool dw_tma = dw && vec_rows(D, dtype, {dw});
+    // contraction along the row (k) or across rows (m); outputs (o)
+    CUtensorMap hk, hm, hk1, hm1, wk, wm, zk, zm, zo, ho, wo;
+    if (!map_2d(&hk, ws.hp, op, row, z.Mp, xent::HALF) ||
+        !map_2d(&hm, ws.hp, op, row, z.Mp, xent::BK) ||
+        !map_2d(&wk, wsrc, op, wrow, V, xent::HALF) ||
+        !map_2d(&wm, wsrc, op, wrow, V, xent::BK) ||
+        !map_2d(&zk, ws.dz, op, zrow, z.Mp, xent::HALF) ||
+        !map_2d(&zm, ws.dz, op, zrow, z.Mp, xent::BK) ||
+        !map_2d(&zo, ws.dz, op, zrow, z.Mp, 32, z.planes > 1 ? 64 : 128) ||
+        !map_2d(&ho, ws.acc, THERIA_F32, z.ld_acc, z.splits * z.Mp, 32))
       return THERIA_ERR_LAUNCH;
+    hk1 = hk;
+    hm1 = hm;
+    wo = zo;
+    if (base.h_plain && (!map_2d(&hk1, h, op, D, N, xent::HALF) ||
+                         !map_2d(&hm1, h, op, D, N, xent::BK)))
+      return THERIA_ERR_LAUNCH;
+    if (dw_tma && !map_2d(&wo, dw, dtype, D, V, 32)) return THERIA_ERR_LAUNCH;
     const int64_t mt = z.Mp / xent::BM, dt = cdiv(D, xent::BN);
     for (int64_t c0 = 0; c0 < V; c0 += z.piece) {
       const int64_t C = std::min(z.piece, V - c0), ct = cdiv(C, xent::BN);
-      xent::TcArgs a{};
-      a.n_live = ws.rows.n_live;
-      a.V = (int)V;
-      a.D = (int)D;
+      xent::TcArgs a = base;
       a.c0 = (int)c0;
       a.Cn = (int)C;
-      a.pairs = z.planes > 1 ? 6 : 1;
-      a.plane_a = a.plane_b = (int)z.Kp;
-      a.tgt = ws.rows.tgt;
-      a.lse = ws.lse;
-      a.rowscale = ws.rowscale;
-      a.dz = ws.dz;
+      a.lse = r.lse;
+      a.rowscale = r.rowscale;
       a.ld_dz = (int)z.piece;
-      a.acc = ws.acc;
-      a.acc_rows = z.Mp;
+      a.acc_rows = (int)z.Mp;
       a.ld_acc = (int)z.ld_acc;
-      a.out = dw;
-      a.out_vec = vec_rows(D, dtype, {dw});
-      a.post = ws.post;
+      a.out = dw_tma ? nullptr : dw;
+      a.post = r.post;
       a.split_kb = (int)z.split_kb;
       a.splits = (int)cdiv(cdiv(C, xent::BK), z.split_kb);
       a.add = c0 > 0;
-      if (int e = tc_launch<T, O, xent::kDz>(hk, wk, a, mt * ct, st)) return e;
+      if (int e = tc_launch<T, O, xent::kDz>(hk, wk, hk1, zo, a, mt * ct, st)) return e;
       a.plane_a = (int)z.piece;
       if (dh)
-        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, a, mt * dt * a.splits, st)) return e;
+        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, a, mt * dt * a.splits, st))
+          return e;
       if (dw)
-        if (int e = tc_launch<T, O, xent::kDw>(zm, hm, a, ct * dt, st)) return e;
+        if (int e = tc_launch<T, O, xent::kDw>(zm, hm, hm1, wo, a, ct * dt, st)) return e;
     }
     if (!dh) return THERIA_OK;
-    xent::dh_sum_kernel<O><<<(unsigned)std::min<int64_t>(cdiv(N * D, 256), kSMs * 16), 256, 0,
-                             st>>>(ws.acc, ws.rows.pos, ws.post, (int)z.splits, z.Mp,
-                                   (int)z.ld_acc, (O*)dh, N, D);
+    constexpr int VEC = embed::Vec<O>::n;
+    auto kern = vec_rows(D, dtype, {dh}) ? xent::dh_sum_kernel<O, VEC> : xent::dh_sum_kernel<O, 1>;
+    kern<<<(unsigned)std::min<int64_t>(N, kSMs * 16), 256, 0, st>>>(
+        ws.acc, r.pos, r.post, (int)z.splits, z.Mp, (int)z.ld_acc, (O*)dh, N, (int)D);
     return launch_status();
   }
 };
@@ -640,51 +696,44 @@ int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
   if (N > 0 && (!h || !w || !target)) return THERIA_ERR_INVALID_ARG;
   if (N > 0 && (!workspace || workspace_bytes < theria_xent_fwd_workspace_bytes(N, V, D, dtype)))
     return THERIA_ERR_WORKSPACE;
-  const float* each = loss;
   if (N == 0) {
-    cudaMemsetAsync(count, 0, sizeof(float), st);
+    // the sum of no rows, and their mean
+    if (cudaMemsetAsync(count, 0, sizeof(float), st) != cudaSuccess) return THERIA_ERR_LAUNCH;
     if (reduction == THERIA_LOSS_NONE) return THERIA_OK;
-  } else {
-    auto prep = [&](const XentRows& r, float* out) {
-      xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, r.pos, r.row_of,
-                                            r.tgt, r.n_live, count, out, lse);
-      return launch_status();
-    };
-    if (use_tc(N, V, D, dtype, w)) {
-      const TcSizes z = tc_sizes(N, V, D, dtype);
-      const TcFwdWs ws = tc_fwd_ws(workspace, N, V, D, z);
-      float* out = reduction == THERIA_LOSS_NONE ? loss : ws.each;
-      each = out;
-      if (int e = prep(ws.rows, out)) return e;
-      const int e =
-          dtype == THERIA_F32  ? Tc<__nv_bfloat16, float>::fwd(h, w, ws, z, out, lse, N, V, D, st)
-          : dtype == THERIA_F16 ? Tc<__half, __half>::fwd(h, w, ws, z, out, lse, N, V, D, st)
-                                : Tc<__nv_bfloat16, __nv_bfloat16>::fwd(h, w, ws, z, out, lse, N,
-                                                                        V, D, st);
-      if (e) return e;
-    } else {
-      const XentFwdWs ws = xent_fwd_ws(workspace, N, V);
-      float* out = reduction == THERIA_LOSS_NONE ? loss : ws.each;
-      each = out;
-      if (int e = prep(ws.rows, out)) return e;
-      const int tiles = (int)cdiv(V, xent::TN);
-      const int e = by_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        xent::score_kernel<T>
-            <<<dim3((unsigned)tiles, (unsigned)cdiv(N, xent::TM)), 256, 0, st>>>(
-                (const T*)h, (const T*)w, ws.rows.row_of, ws.rows.tgt, ws.rows.n_live, ws.part,
-                ws.zt, V, D);
-        return launch_status();
-      });
-      if (e) return e;
-      xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
-          ws.part, ws.zt, ws.rows.row_of, ws.rows.n_live, tiles, out, lse);
-      if (int e2 = launch_status()) return e2;
-    }
-    if (reduction == THERIA_LOSS_NONE) return THERIA_OK;
+    return cudaMemsetAsync(loss, reduction == THERIA_LOSS_MEAN ? 0xff : 0, sizeof(float), st) ==
+                   cudaSuccess  // all bits set: NaN
+               ? THERIA_OK
+               : THERIA_ERR_LAUNCH;
   }
-  xent::total_kernel<<<1, 1024, 0, st>>>(each, N, count, reduction == THERIA_LOSS_MEAN, loss);
-  return launch_status();
+  const bool tensor = use_tc(N, V, D, dtype, w);
+  const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
+  TcFwdWs tw;
+  XentFwdWs sw;
+  if (tensor) tw = tc_fwd_ws(workspace, N, V, D, z);
+  else sw = xent_fwd_ws(workspace, N, V);
+  const XentRows& r = tensor ? tw.rows : sw.rows;
+  LossOut out{reduction == THERIA_LOSS_NONE ? loss : tensor ? tw.each : sw.each, lse,
+              reduction == THERIA_LOSS_NONE ? nullptr : loss, reduction == THERIA_LOSS_MEAN};
+  xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
+  p.count = count;
+  p.loss = out.each;
+  p.lse = lse;
+  xent::prep_kernel<<<1, 1024, 0, st>>>(p);
+  if (int e = launch_status()) return e;
+  if (tensor)
+    return dtype == THERIA_F32   ? Tc<__nv_bfloat16, float>::fwd(h, w, tw, z, out, N, V, D, st)
+           : dtype == THERIA_F16 ? Tc<__half, __half>::fwd(h, w, tw, z, out, N, V, D, st)
+                                 : Tc<__nv_bfloat16, __nv_bfloat16>::fwd(h, w, tw, z, out, N, V, D,
+                                                                         st);
+  const int tiles = (int)cdiv(V, xent::TN);
+  const int e = by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    xent::score_kernel<T><<<dim3((unsigned)tiles, (unsigned)cdiv(N, xent::TM)), 256, 0, st>>>(
+        (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, sw.part, sw.zt, V, D);
+    return launch_status();
+  });
+  if (e) return e;
+  return xent_join(r, sw.part, sw.zt, tiles, out, N, st);
 }
 
 int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
@@ -703,29 +752,30 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   if (!dh && !dw) return THERIA_OK;
   if (!workspace || workspace_bytes < theria_xent_bwd_workspace_bytes(N, V, D, dtype))
     return THERIA_ERR_WORKSPACE;
-  const float* mean_of = reduction == THERIA_LOSS_MEAN ? count : nullptr;
-  auto prep = [&](const XentRows& r) {
-    xent::prep_kernel<<<1, 1024, 0, st>>>(target, wide, ignore_index, N, V, r.pos, r.row_of,
-                                          r.tgt, r.n_live, nullptr, nullptr, nullptr);
-    return launch_status();
-  };
-  if (use_tc(N, V, D, dtype, w)) {
-    const TcSizes z = tc_sizes(N, V, D, dtype);
-    const TcBwdWs ws = tc_bwd_ws(workspace, N, V, D, z);
-    if (int e = prep(ws.rows)) return e;
-    xent::scale_kernel<<<1, 1024, 0, st>>>(ws.rows.row_of, ws.rows.n_live, gloss,
-                                           reduction == THERIA_LOSS_NONE, mean_of, lse,
-                                           dtype == THERIA_F16, ws.lse, ws.rowscale, ws.post);
-    if (int e = launch_status()) return e;
+  const bool tensor = use_tc(N, V, D, dtype, w);
+  const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
+  TcBwdWs tw;
+  XentBwdWs ws;
+  if (tensor) tw = tc_bwd_ws(workspace, N, V, D, z);
+  else ws = xent_bwd_ws(workspace, N, V, D);
+  const XentRows& r = tensor ? tw.rows : ws.rows;
+  xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
+  p.gloss = gloss;
+  p.lse_in = lse;
+  p.mean_of = reduction == THERIA_LOSS_MEAN ? count : nullptr;
+  p.per_row = reduction == THERIA_LOSS_NONE;
+  p.half = tensor && dtype == THERIA_F16;
+  p.lse_p = r.lse;
+  p.rowscale = r.rowscale;
+  p.post = r.post;
+  xent::prep_kernel<<<1, 1024, 0, st>>>(p);
+  if (int e = launch_status()) return e;
+  if (tensor)
     return dtype == THERIA_F32
-               ? Tc<__nv_bfloat16, float>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
+               ? Tc<__nv_bfloat16, float>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st)
            : dtype == THERIA_F16
-               ? Tc<__half, __half>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
-               : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st);
-  }
-  const XentBwdWs ws = xent_bwd_ws(workspace, N, V, D);
-  const XentRows& r = ws.rows;
-  if (int e = prep(r)) return e;
+               ? Tc<__half, __half>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st)
+               : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st);
   const unsigned mt = (unsigned)cdiv(N, xent::TM), dt = (unsigned)cdiv(D, xent::TN);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -733,8 +783,8 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
       const int64_t C = std::min(ws.piece, V - c0);
       const unsigned ct = (unsigned)cdiv(C, xent::TN);
       xent::dz_kernel<T><<<dim3(ct, mt), 256, 0, st>>>(
-          (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, lse, gloss,
-          reduction == THERIA_LOSS_NONE, mean_of, ws.dz, c0, C, V, D);
+          (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, r.lse, r.rowscale, ws.dz, c0, C, V,
+          D);
       if (int e = launch_status()) return e;
       if (dh) {
         xent::dh_kernel<T><<<dim3(dt, mt), 256, 0, st>>>(ws.dz, (const T*)w, r.n_live, ws.acc, c0,
@@ -743,13 +793,13 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
       }
       if (dw) {
         xent::dw_kernel<T><<<dim3(dt, ct), 256, 0, st>>>(ws.dz, (const T*)h, r.row_of, r.n_live,
-                                                         (T*)dw, c0, C, C, D);
+                                                         r.post, (T*)dw, c0, C, C, D);
         if (int e = launch_status()) return e;
       }
     }
     if (dh) {
       xent::dh_finish_kernel<T><<<(unsigned)std::min<int64_t>(cdiv(N * D, 256), kSMs * 16), 256, 0,
-                                  st>>>(ws.acc, r.pos, (T*)dh, N, D);
+                                  st>>>(ws.acc, r.pos, r.post, (T*)dh, N, D);
       return launch_status();
     }
     return THERIA_OK;
