@@ -162,7 +162,8 @@ __device__ __forceinline__ void tile_product(FA a, FB b, int64_t K, float (&acc)
 }
 
 // Operands of tile_product.  Rows: element (r, k) of a matrix with k
-// contiguous, rows through an index list or not; Cols: the r axis contiguous.
+// contiguous, rows through an index list (negative: zeros) or not; Cols: the r
+// axis contiguous.
 template <typename T>
 struct Rows {
   const T* p;
@@ -170,8 +171,8 @@ struct Rows {
   int64_t r0, n, ld, K;
   __device__ void load(float (&s)[TK][TM + 4], int e, int64_t k0) const {
     const int k = e % TK, r = e / TK;
-    const int64_t i = r0 + r;
-    s[k][r] = i < n && k0 + k < K ? to_f32(p[(list ? list[i] : i) * ld + k0 + k]) : 0.f;
+    const int64_t i = r0 + r, at = i < n ? (list ? list[i] : i) : -1;
+    s[k][r] = at >= 0 && k0 + k < K ? to_f32(p[at * ld + k0 + k]) : 0.f;
   }
 };
 template <typename T>
@@ -268,14 +269,14 @@ join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
   }
 }
 
-// dz[m][c] of the vocabulary piece [c0, c0 + C), float32.
+// dz[m][v], float32.
 template <typename T>
 __global__ void __launch_bounds__(256)
 dz_kernel(const T* __restrict__ h, const T* __restrict__ w, const int* __restrict__ row_of,
           const int* __restrict__ tgt, const int* __restrict__ n_live,
           const float* __restrict__ lse, const float* __restrict__ rowscale,
-          float* __restrict__ dz, int64_t c0, int64_t C, int64_t V, int64_t D) {
-  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, v0 = c0 + (int64_t)blockIdx.x * TN;
+          float* __restrict__ dz, int64_t V, int64_t D) {
+  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, v0 = (int64_t)blockIdx.x * TN;
   if (m0 >= n) return;
   float z[4][4];
   tile_product(Rows<T>{h, row_of, m0, n, D, D}, Rows<T>{w, nullptr, v0, V, D, D}, D, z);
@@ -288,62 +289,46 @@ dz_kernel(const T* __restrict__ h, const T* __restrict__ w, const int* __restric
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t v = v0 + tx * 4 + j;
-      if (v < V && v < c0 + C)
-        dz[m * C + v - c0] = g * (expf(z[i][j] - l) - (v == tgt[m] ? 1.f : 0.f));
+      if (v < V) dz[m * V + v] = g * (expf(z[i][j] - l) - (v == tgt[m] ? 1.f : 0.f));
     }
   }
 }
 
-// acc[m][d] (+)= sum_c dz[m][c] w[c0 + c][d]
+// dh[i][d] = sum_v dz[pos[i]][v] w[v][d]; zeros where row i does not count.
 template <typename T>
 __global__ void __launch_bounds__(256)
-dh_kernel(const float* __restrict__ dz, const T* __restrict__ w, const int* __restrict__ n_live,
-          float* __restrict__ acc, int64_t c0, int64_t C, int64_t Cn, int64_t D, int first) {
-  const int64_t n = *n_live, m0 = (int64_t)blockIdx.y * TM, d0 = (int64_t)blockIdx.x * TN;
-  if (m0 >= n) return;
+dh_kernel(const float* __restrict__ dz, const T* __restrict__ w, const int* __restrict__ pos,
+          const float* __restrict__ post, T* __restrict__ dh, int64_t N, int64_t V, int64_t D) {
+  const int64_t m0 = (int64_t)blockIdx.y * TM, d0 = (int64_t)blockIdx.x * TN;
   float o[4][4];
-  tile_product(Rows<float>{dz, nullptr, m0, n, C, Cn}, Cols<T>{w + c0 * D, nullptr, d0, D, D, Cn},
-               Cn, o);
+  tile_product(Rows<float>{dz, pos, m0, N, V, V}, Cols<T>{w, nullptr, d0, D, D, V}, V, o);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t m = m0 + ty * 4 + i, d = d0 + tx * 4 + j;
-      if (m < n && d < D) acc[m * D + d] = first ? o[i][j] : acc[m * D + d] + o[i][j];
+      if (m < N && d < D) dh[m * D + d] = from_f32<T>(pos[m] < 0 ? 0.f : *post * o[i][j]);
     }
 }
 
-// dw[c0 + c][d] = sum_m dz[m][c] h[m][d]
+// dw[v][d] = sum_m dz[m][v] h[m][d]
 template <typename T>
 __global__ void __launch_bounds__(256)
 dw_kernel(const float* __restrict__ dz, const T* __restrict__ h, const int* __restrict__ row_of,
           const int* __restrict__ n_live, const float* __restrict__ post, T* __restrict__ dw,
-          int64_t c0, int64_t C, int64_t Cn, int64_t D) {
+          int64_t V, int64_t D) {
   const int64_t n = *n_live, r0 = (int64_t)blockIdx.y * TM, d0 = (int64_t)blockIdx.x * TN;
   float o[4][4];
-  tile_product(Cols<float>{dz, nullptr, r0, Cn, C, n}, Cols<T>{h, row_of, d0, D, D, n}, n, o);
+  tile_product(Cols<float>{dz, nullptr, r0, V, V, n}, Cols<T>{h, row_of, d0, D, D, n}, n, o);
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t r = r0 + ty * 4 + i, d = d0 + tx * 4 + j;
-      if (r < Cn && d < D) dw[(c0 + r) * D + d] = from_f32<T>(*post * o[i][j]);
+      if (r < V && d < D) dw[r * D + d] = from_f32<T>(*post * o[i][j]);
     }
-}
-
-// dh[i] = acc[pos[i]], or zeros where row i does not count.
-template <typename T>
-__global__ void dh_finish_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
-                                 const float* __restrict__ post, T* __restrict__ dh, int64_t N,
-                                 int64_t D) {
-  for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < N * D;
-       e += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = e / D, d = e - i * D;
-    const int m = pos[i];
-    dh[e] = from_f32<T>(m < 0 ? 0.f : *post * acc[m * D + d]);
-  }
 }
 
 }  // namespace xent

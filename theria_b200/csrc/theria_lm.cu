@@ -412,17 +412,14 @@ XentFwdWs xent_fwd_ws(void* base, int64_t N, int64_t V) {
 }
 struct XentBwdWs {
   XentRows rows;
-  float *dz, *acc;
-  int64_t piece, bytes;
+  float* dz;
+  int64_t bytes;
 };
-XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V, int64_t D) {
+XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V) {
   Carver c{(char*)base};
   XentBwdWs w;
   w.rows = xent_rows(c, N);
-  w.piece = std::min<int64_t>(up(V, xent::TN),
-                              std::max<int64_t>(xent::TN, up((64ll << 20) / N, xent::TN)));
-  w.dz = c.take<float>(N * w.piece);
-  w.acc = c.take<float>(N * D);
+  w.dz = c.take<float>(N * V);
   w.bytes = c.used;
   return w;
 }
@@ -661,10 +658,10 @@ struct Tc {
   }
 };
 
-// Whether this call runs on the tensor cores.
-bool use_tc(int64_t N, int64_t V, int64_t D, int dtype, const void* w) {
-  return !xent_small(N, V, D) && tc::encode_fn() != nullptr &&
-         (dtype == THERIA_F32 || D % 8 != 0 || tc::aligned16(w));
+// Whether the tensor-core kernels can read w: 16 bytes at a time, where they
+// do not pack it first.
+bool w_readable(const void* w, int64_t D, int dtype) {
+  return dtype == THERIA_F32 || D % 8 != 0 || tc::aligned16(w);
 }
 
 }  // namespace
@@ -674,15 +671,13 @@ extern "C" {
 
 int64_t theria_xent_fwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
-  const int64_t b = xent_fwd_ws(nullptr, N, V).bytes;
-  if (xent_small(N, V, D)) return b;
-  return std::max(b, tc_fwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes);
+  return xent_small(N, V, D) ? xent_fwd_ws(nullptr, N, V).bytes
+                             : tc_fwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes;
 }
 int64_t theria_xent_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
-  const int64_t b = xent_bwd_ws(nullptr, N, V, D).bytes;
-  if (xent_small(N, V, D)) return b;
-  return std::max(b, tc_bwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes);
+  return xent_small(N, V, D) ? xent_bwd_ws(nullptr, N, V).bytes
+                             : tc_bwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes;
 }
 
 int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
@@ -705,7 +700,8 @@ int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
                ? THERIA_OK
                : THERIA_ERR_LAUNCH;
   }
-  const bool tensor = use_tc(N, V, D, dtype, w);
+  const bool tensor = !xent_small(N, V, D);
+  if (tensor && !w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
   const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
   TcFwdWs tw;
   XentFwdWs sw;
@@ -752,12 +748,13 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   if (!dh && !dw) return THERIA_OK;
   if (!workspace || workspace_bytes < theria_xent_bwd_workspace_bytes(N, V, D, dtype))
     return THERIA_ERR_WORKSPACE;
-  const bool tensor = use_tc(N, V, D, dtype, w);
+  const bool tensor = !xent_small(N, V, D);
+  if (tensor && !w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
   const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
   TcBwdWs tw;
   XentBwdWs ws;
   if (tensor) tw = tc_bwd_ws(workspace, N, V, D, z);
-  else ws = xent_bwd_ws(workspace, N, V, D);
+  else ws = xent_bwd_ws(workspace, N, V);
   const XentRows& r = tensor ? tw.rows : ws.rows;
   xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
   p.gloss = gloss;
@@ -776,33 +773,22 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
            : dtype == THERIA_F16
                ? Tc<__half, __half>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st)
                : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st);
-  const unsigned mt = (unsigned)cdiv(N, xent::TM), dt = (unsigned)cdiv(D, xent::TN);
+  const unsigned mt = (unsigned)cdiv(N, xent::TM), dt = (unsigned)cdiv(D, xent::TN),
+                 vt = (unsigned)cdiv(V, xent::TN);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    for (int64_t c0 = 0; c0 < V; c0 += ws.piece) {
-      const int64_t C = std::min(ws.piece, V - c0);
-      const unsigned ct = (unsigned)cdiv(C, xent::TN);
-      xent::dz_kernel<T><<<dim3(ct, mt), 256, 0, st>>>(
-          (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, r.lse, r.rowscale, ws.dz, c0, C, V,
-          D);
-      if (int e = launch_status()) return e;
-      if (dh) {
-        xent::dh_kernel<T><<<dim3(dt, mt), 256, 0, st>>>(ws.dz, (const T*)w, r.n_live, ws.acc, c0,
-                                                         C, C, D, c0 == 0);
-        if (int e = launch_status()) return e;
-      }
-      if (dw) {
-        xent::dw_kernel<T><<<dim3(dt, ct), 256, 0, st>>>(ws.dz, (const T*)h, r.row_of, r.n_live,
-                                                         r.post, (T*)dw, c0, C, C, D);
-        if (int e = launch_status()) return e;
-      }
-    }
+    xent::dz_kernel<T><<<dim3(vt, mt), 256, 0, st>>>((const T*)h, (const T*)w, r.row_of, r.tgt,
+                                                     r.n_live, r.lse, r.rowscale, ws.dz, V, D);
+    if (int e = launch_status()) return e;
     if (dh) {
-      xent::dh_finish_kernel<T><<<(unsigned)std::min<int64_t>(cdiv(N * D, 256), kSMs * 16), 256, 0,
-                                  st>>>(ws.acc, r.pos, r.post, (T*)dh, N, D);
-      return launch_status();
+      xent::dh_kernel<T><<<dim3(dt, mt), 256, 0, st>>>(ws.dz, (const T*)w, r.pos, r.post, (T*)dh,
+                                                       N, V, D);
+      if (int e = launch_status()) return e;
     }
-    return THERIA_OK;
+    if (dw)
+      xent::dw_kernel<T><<<dim3(dt, vt), 256, 0, st>>>(ws.dz, (const T*)h, r.row_of, r.n_live,
+                                                       r.post, (T*)dw, V, D);
+    return dw ? launch_status() : THERIA_OK;
   });
 }
 

@@ -34,40 +34,51 @@ _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _opaque = torch.compiler.disable
 
 
+_fns = {}
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _call(name, like, *args):
-    """One library call on `like`'s device and torch's current stream there."""
-    fn = getattr(_lib.load(), name)
-    with torch.cuda.device(like.device):
-        st = fn(*args, torch.cuda.current_stream(like.device).cuda_stream)
-    _lib.check(st, name)
+def _fn(name):
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.load(), name)
+    return fn
 
 
-def _workspace(name, like, *sizes):
-    n = getattr(_lib.load(), name)(*sizes)
-    return torch.empty(max(n, 1), dtype=torch.uint8, device=like.device), n
+def _call(name, device, *args):
+    """One library call on `device` and torch's current stream there."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        st = _fn(name)(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(device):
+            st = _fn(name)(*args, torch._C._cuda_getCurrentRawStream(i))
+    if st:
+        _lib.check(st, name)
 
 
-def _check(what, **tensors):
-    ref = None
-    for name, t in tensors.items():
-        if not t.is_cuda:
-            raise AssertionError(f"{what} requires CUDA tensors")
-        if t.dtype not in _DTYPES:
-            raise AssertionError(f"Unsupported dtype for {name}: {t.dtype}")
-        ref = t if ref is None else ref
-        if t.device != ref.device:
-            raise AssertionError(f"{what}: {name} is on {t.device}, not {ref.device}")
+def _workspace(name, device, *sizes):
+    n = _fn(name)(*sizes)
+    return torch.empty(n, dtype=torch.uint8, device=device), n
 
 
-def _check_ids(what, name, ids, like):
-    if ids.dtype not in (torch.int64, torch.int32):
+def _check(what, name, t, device=None):
+    if not t.is_cuda:
+        raise AssertionError(f"{what} requires CUDA tensors")
+    if t.dtype not in _DTYPES:
+        raise AssertionError(f"Unsupported dtype for {name}: {t.dtype}")
+    if device is not None and t.device != device:
+        raise AssertionError(f"{what}: {name} is on {t.device}, not {device}")
+
+
+def _check_ids(what, name, ids, device):
+    if ids.dtype is not torch.int64 and ids.dtype is not torch.int32:
         raise AssertionError(f"{what}: {name} must be int64 or int32, got {ids.dtype}")
-    if ids.device != like.device:
-        raise AssertionError(f"{what}: {name} is on {ids.device}, not {like.device}")
+    if ids.device != device:
+        raise AssertionError(f"{what}: {name} is on {ids.device}, not {device}")
 
 
 def _wide(ids):
@@ -81,8 +92,8 @@ def _wide(ids):
 # ------------------------------------------------------------------ embedding
 def _embed(ids, weight, scale, zero_idx):
     V, D = weight.shape
-    out = torch.empty(*ids.shape, D, dtype=weight.dtype, device=weight.device)
-    _call("theria_embed_fwd", weight, ids.data_ptr(), _wide(ids), weight.data_ptr(),
+    out = torch.empty((*ids.shape, D), dtype=weight.dtype, device=weight.device)
+    _call("theria_embed_fwd", weight.device, ids.data_ptr(), _wide(ids), weight.data_ptr(),
           out.data_ptr(), ids.numel(), V, D, _DTYPES[weight.dtype], scale, zero_idx)
     return out
 
@@ -91,8 +102,8 @@ def _embed_grad(gy, ids, V, scale, padding):
     gy = gy.contiguous()
     D, n = gy.shape[-1], ids.numel()
     gw = torch.empty(V, D, dtype=gy.dtype, device=gy.device)
-    ws, size = _workspace("theria_embed_bwd_workspace_bytes", gy, n, V, D)
-    _call("theria_embed_bwd", gy, ids.data_ptr(), _wide(ids), gy.data_ptr(), gw.data_ptr(),
+    ws, size = _workspace("theria_embed_bwd_workspace_bytes", gy.device, n, V, D)
+    _call("theria_embed_bwd", gy.device, ids.data_ptr(), _wide(ids), gy.data_ptr(), gw.data_ptr(),
           ws.data_ptr(), size, n, V, D, _DTYPES[gy.dtype], scale, padding)
     return gw
 
@@ -136,8 +147,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     The weight's gradient (dense) sums each token's rows in token order; the
     row ``padding_idx`` (negative: from the end) gets none.
     """
-    _check("theria embedding", weight=weight)
-    _check_ids("theria embedding", "ids", ids, weight)
+    _check("theria embedding", "weight", weight)
+    _check_ids("theria embedding", "ids", ids, weight.device)
     if weight.ndim != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise AssertionError("weight must have shape (V,D)")
     V = weight.shape[0]
@@ -158,7 +169,7 @@ def _norm(x, w, b, eps, need_stats):
     N = x.numel() // D
     y = torch.empty_like(x)
     stats = torch.empty(2, N, dtype=torch.float32, device=x.device) if need_stats else None
-    _call("theria_norm_fwd", x, x.data_ptr(), _ptr(w), _ptr(b), _affine_dtype(x, w, b),
+    _call("theria_norm_fwd", x.device, x.data_ptr(), _ptr(w), _ptr(b), _affine_dtype(x, w, b),
           y.data_ptr(), _ptr(stats), N, D, _DTYPES[x.dtype], eps)
     return y, stats
 
@@ -175,11 +186,11 @@ def _norm_grad(x, w, b, stats, gy, need):
     gw = gb = ws = None
     size = 0
     if need[1] or need[2]:
-        gw, gb = torch.empty(2, D, dtype=(w if w is not None else b).dtype,
-                             device=x.device).unbind(0)
-        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x, N, D)
-    _call("theria_norm_bwd", x, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b), gy.data_ptr(),
-          stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), size, N, D,
+        like = w if w is not None else b
+        gw, gb = torch.empty_like(like), torch.empty_like(like)
+        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x.device, N, D)
+    _call("theria_norm_bwd", x.device, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
+          gy.data_ptr(), stats.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), size, N, D,
           _DTYPES[x.dtype])
     return gx, gw if need[1] else None, gb if need[2] else None
 
@@ -203,8 +214,8 @@ class _LayerNormBackward(torch.autograd.Function):
         u, a, c = (None if t is None else t.contiguous() for t in (u, a, c))
         dx, dgy = torch.empty_like(x), torch.empty_like(x)
         dw = None if w is None else torch.empty_like(w)
-        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x, N, D)
-        _call("theria_norm_bwd2", x, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
+        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x.device, N, D)
+        _call("theria_norm_bwd2", x.device, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
               gy.data_ptr(), stats.data_ptr(), _ptr(u), _ptr(a), _ptr(c), dx.data_ptr(),
               _ptr(dw), dgy.data_ptr(), ws.data_ptr(), size, N, D, _DTYPES[x.dtype])
         return dx, dw, None, dgy, None, None
@@ -232,52 +243,55 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=EPS):
     """Layer norm over the last axis of x [..., D]; weight, bias [D] (either
     may be None) of x's type or float32.  Differentiable twice."""
-    _check("theria layer_norm", x=x, **{n: t for n, t in (("weight", weight), ("bias", bias))
-                                        if t is not None})
+    what = "theria layer_norm"
+    _check(what, "x", x)
     if x.ndim == 0 or x.shape[-1] == 0:
         raise AssertionError("x must have shape (...,D)")
-    kinds = set()
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        if tuple(t.shape) != (x.shape[-1],):
+        _check(what, name, t, x.device)
+        if t.ndim != 1 or t.shape[0] != x.shape[-1]:
             raise AssertionError(f"{name} must have shape ({x.shape[-1]},)")
-        if t.dtype not in (x.dtype, torch.float32):
+        if t.dtype is not x.dtype and t.dtype is not torch.float32:
             raise AssertionError(f"{name} dtype must be {x.dtype} or float32")
-        kinds.add(t.dtype)
-    if len(kinds) > 1:
+    if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise AssertionError("weight and bias must share one dtype")
     x = x.contiguous()
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or weight is not None and weight.requires_grad
+                                    or bias is not None and bias.requires_grad):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _norm(x, weight, bias, float(eps), False)[0]
 
 
 # ------------------------------------------------------- linear cross entropy
 def _loss(h, w, target, ignore_index, reduction):
-    (N, D), V = h.shape, w.shape[0]
-    loss = torch.empty(N if reduction == 0 else 1, dtype=torch.float32, device=h.device)
-    lse = torch.empty(N, dtype=torch.float32, device=h.device)
-    count = torch.empty(1, dtype=torch.float32, device=h.device)
-    ws, size = _workspace("theria_xent_fwd_workspace_bytes", h, N, V, D, _DTYPES[h.dtype])
-    _call("theria_xent_fwd", h, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
-          ignore_index, reduction, loss.data_ptr(), lse.data_ptr(), count.data_ptr(),
-          ws.data_ptr(), size, N, V, D, _DTYPES[h.dtype])
-    return loss, lse, count
+    V, D = w.shape
+    N, dt, dev = target.numel(), _DTYPES[h.dtype], h.device
+    loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
+    stats = torch.empty(N + 1, dtype=torch.float32, device=dev)  # lse, count
+    ws, size = _workspace("theria_xent_fwd_workspace_bytes", dev, N, V, D, dt)
+    lse = stats.data_ptr()
+    _call("theria_xent_fwd", dev, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
+          ignore_index, reduction, loss.data_ptr(), lse, lse + 4 * N, ws.data_ptr(), size, N, V,
+          D, dt)
+    return loss, stats
 
 
-def _loss_grad(h, w, g, target, lse, count, ignore_index, reduction, need):
-    (N, D), V = h.shape, w.shape[0]
+def _loss_grad(h, w, g, target, stats, ignore_index, reduction, need):
+    V, D = w.shape
+    N, dt, dev = target.numel(), _DTYPES[h.dtype], h.device
     g = g.to(torch.float32).contiguous()
     dh = torch.empty_like(h) if need[0] else None
     dw = torch.empty_like(w) if need[1] else None
-    ws, size = _workspace("theria_xent_bwd_workspace_bytes", h, N, V, D, _DTYPES[h.dtype])
-    _call("theria_xent_bwd", h, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
-          ignore_index, reduction, g.data_ptr(), lse.data_ptr(), count.data_ptr(), _ptr(dh),
-          _ptr(dw), ws.data_ptr(), size, N, V, D, _DTYPES[h.dtype])
+    ws, size = _workspace("theria_xent_bwd_workspace_bytes", dev, N, V, D, dt)
+    lse = stats.data_ptr()
+    _call("theria_xent_bwd", dev, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
+          ignore_index, reduction, g.data_ptr(), lse, lse + 4 * N, _ptr(dh), _ptr(dw),
+          ws.data_ptr(), size, N, V, D, dt)
     return dh, dw
 
 
@@ -297,17 +311,23 @@ class _LinearCrossEntropyBackward(torch.autograd.Function):
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h, w, target, ignore_index, reduction):
-        loss, lse, count = _loss(h, w, target, ignore_index, reduction)
-        ctx.save_for_backward(h, w, target, lse, count)
+        loss, stats = _loss(h, w, target, ignore_index, reduction)
+        ctx.save_for_backward(h, w, target, stats)
         ctx.rest = ignore_index, reduction
         return loss
 
     @staticmethod
     def backward(ctx, g):
-        h, w, target, lse, count = ctx.saved_tensors
+        h, w, target, stats = ctx.saved_tensors
         grad = _LinearCrossEntropyBackward.apply if torch.is_grad_enabled() else _loss_grad
-        dh, dw = grad(h, w, g, target, lse, count, *ctx.rest, ctx.needs_input_grad[:2])
+        dh, dw = grad(h, w, g, target, stats, *ctx.rest, ctx.needs_input_grad[:2])
         return dh, dw, None, None, None
+
+
+def _aligned(t):
+    # the tensor-core kernels read 16 bytes at a time
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 @_opaque
@@ -322,8 +342,9 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, redu
     scalar; the mean over no row at all is NaN, with zero gradients.
     """
     what = "theria linear_cross_entropy"
-    _check(what, hidden=hidden, weight=weight)
-    _check_ids(what, "target", target, hidden)
+    _check(what, "hidden", hidden)
+    _check(what, "weight", weight, hidden.device)
+    _check_ids(what, "target", target, hidden.device)
     if weight.dtype != hidden.dtype:
         raise AssertionError("hidden and weight must share one dtype")
     if weight.ndim != 2 or 0 in weight.shape:
@@ -334,13 +355,10 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, redu
         raise AssertionError(f"target shape must be {tuple(hidden.shape[:-1])}")
     if reduction not in _REDUCTIONS:
         raise AssertionError(f"reduction must be one of {sorted(_REDUCTIONS)}")
-    h, w = hidden.reshape(-1, hidden.shape[-1]).contiguous(), weight.contiguous()
-    t, red = target.reshape(-1).contiguous(), _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
-        loss = _LinearCrossEntropy.apply(h, w, t, int(ignore_index), red)
-    else:
-        loss = _loss(h, w, t, int(ignore_index), red)[0]
-    return loss.view(target.shape) if red == 0 else loss.view(())
+    h, w, t = hidden.contiguous(), _aligned(weight), target.contiguous()
+    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
+        return _LinearCrossEntropy.apply(h, w, t, int(ignore_index), _REDUCTIONS[reduction])
+    return _loss(h, w, t, int(ignore_index), _REDUCTIONS[reduction])[0]
 
 
 __all__ = ["embedding", "layer_norm", "linear_cross_entropy"]
