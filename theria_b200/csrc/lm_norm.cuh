@@ -12,11 +12,10 @@
 //
 // Both directions are bound by HBM: x read and y written once, then x and gy
 // read and gx written once.  A row stays in registers between its load and
-// its store (rows up to 256 threads x NV vectors); the variance is taken
-// around the mean already known, so it loses nothing to cancellation.
-// Statistics, sums and the weight gradients are float32; each result is
-// rounded once.  The sums over rows go through per-CTA partials added by a
-// second kernel in a fixed order: the same bits every time.
+// its store; the variance is taken around the mean already known, so it loses
+// nothing to cancellation.  Statistics, sums and the weight gradients are
+// float32; each result is rounded once.  The sums over rows go through per-CTA
+// partials added by a second kernel in a fixed order: the same bits every time.
 #pragma once
 
 #include "common.cuh"
@@ -30,56 +29,93 @@ using embed::store_vec;
 
 constexpr int SUMS = 7;  // the most values one reduction carries
 
-// NW warps (one, or the whole CTA) own a row; sums of NS values over it.
+// NW warps own a row (one of several in the CTA for NW == 1, else the whole
+// CTA); sums of NS values over it.  `red` alternates between two halves from
+// call to call, so one barrier per call is enough.
 template <int NW, int NS>
-__device__ __forceinline__ void row_sum(float (&s)[NS], float (*red)[SUMS]) {
+__device__ __forceinline__ void row_sum(float (&s)[NS], float (*red)[32][SUMS], int& turn) {
 #pragma unroll
   for (int i = 0; i < NS; ++i) s[i] = warp_sum(s[i]);
   if constexpr (NW > 1) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float (*r)[SUMS] = red[turn];
+    turn ^= 1;
     if (lane == 0) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) red[warp][i] = s[i];
+      for (int i = 0; i < NS; ++i) r[warp][i] = s[i];
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      s[i] = 0.f;
+      if constexpr (NW >= 8) {
+        s[i] = warp_sum(lane < NW ? r[lane][i] : 0.f);
+      } else {
+        s[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < NW; ++w) s[i] += red[w][i];
+        for (int w = 0; w < NW; ++w) s[i] += r[w][i];
+      }
     }
-    __syncthreads();
   }
 }
 
-// One affine value (w, b may be of float32 or of x's type; NULL: `none`).
+// VEC affine values from column c (float32 where f32, else x's type; NULL:
+// `none`).  VEC > 1: p is 16-byte aligned there.
+template <typename T, int VEC>
+__device__ __forceinline__ void affine_vec(const void* p, bool f32, int64_t c, float none,
+                                           float (&v)[VEC]) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = none;
+  } else if (sizeof(T) == 4 || !f32) {
+    load_vec<T, VEC>(static_cast<const T*>(p) + c, v);
+  } else if constexpr (VEC == 8) {
+    const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + c);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = static_cast<const float*>(p)[c + k];
+  }
+}
+// One affine value, for the kernels of wide rows.
 __device__ __forceinline__ float affine(const void* p, int dtype, int64_t i, float none) {
   return p ? load_any(p, i, dtype) : none;
 }
 
-// NW warps per row (1: each warp of the CTA has its own row; 8: the CTA has
-// one), NV vectors of VEC values per thread.
+// Threads and rows of a CTA whose rows belong to NW warps.
+template <int NW> struct Block {
+  static constexpr int threads = NW == 1 ? 256 : NW * 32;
+  static constexpr int G = NW * 32;        // threads of a row
+  static constexpr int rows = threads / G; // rows at a time
+};
+
+// NW warps per row, NV vectors of VEC values per thread.
 template <typename T, int VEC, int NV, int NW>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(Block<NW>::threads)
 fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
-           int wdtype, T* __restrict__ y, float* __restrict__ stats, int64_t N, int D, float eps) {
-  constexpr int G = NW * 32, ROWS = 256 / G;
-  __shared__ float red[8][SUMS];
+           int wf32, T* __restrict__ y, float* __restrict__ stats, int64_t N, int D, float eps) {
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   const int g = threadIdx.x % G;
+  const float inv = 1.f / (float)D;
   for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
        r += (int64_t)gridDim.x * ROWS) {
     float v[NV][VEC], s[1] = {0.f}, q[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
-      if (c < D) {
-        load_vec<T, VEC>(x + r * D + c, v[j]);
+      if (c < D) load_vec<T, VEC>(x + r * D + c, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if ((j * G + g) * VEC < D) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) s[0] += v[j][k];
       }
-    }
-    row_sum<NW>(s, red);
-    const float mean = s[0] / (float)D;
+    row_sum<NW>(s, red, turn);
+    const float mean = s[0] * inv;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
       if ((j * G + g) * VEC < D) {
@@ -90,18 +126,19 @@ fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __re
           q[1] += v[j][k];
         }
       }
-    row_sum<NW>(q, red);
+    row_sum<NW>(q, red, turn);
     // what the rounding of a large mean left in the deviations
-    const float left = q[1] / (float)D;
-    const float rstd = rsqrtf(fmaxf(q[0] / (float)D - left * left, 0.f) + eps);
+    const float left = q[1] * inv;
+    const float rstd = rsqrtf(fmaxf(q[0] * inv - left * left, 0.f) + eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c < D) {
+        float wv[VEC], bv[VEC];
+        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+        affine_vec<T, VEC>(b, wf32, c, 0.f, bv);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k)
-          v[j][k] = fmaf((v[j][k] - left) * rstd, affine(w, wdtype, c + k, 1.f),
-                         affine(b, wdtype, c + k, 0.f));
+        for (int k = 0; k < VEC; ++k) v[j][k] = fmaf((v[j][k] - left) * rstd, wv[k], bv[k]);
         store_vec<T, VEC>(y + r * D + c, v[j]);
       }
     }
@@ -117,7 +154,7 @@ fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __re
 template <int NW, int NV, int VEC>
 __device__ __forceinline__ void store_part(const float (&a)[NV][VEC], const float (&b)[NV][VEC],
                                            float* part, int D) {
-  constexpr int G = NW * 32, ROWS = 256 / G;
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
   extern __shared__ float cols[];
   const int g = threadIdx.x % G;
   float* mine = part + (int64_t)blockIdx.x * 2 * D;
@@ -143,51 +180,94 @@ __device__ __forceinline__ void store_part(const float (&a)[NV][VEC], const floa
   }
 }
 
-// part[cta][2][D]: this CTA's sums of gy * xhat and gy.
+// VEC values as they are in memory: what a prefetch keeps in registers.
+template <typename T, int VEC>
+struct Raw {
+  typename std::conditional<VEC == 1, T, uint4>::type v;
+  __device__ void load(const T* p) { v = *reinterpret_cast<const decltype(v)*>(p); }
+  __device__ void get(float (&f)[VEC]) const {
+    if constexpr (VEC == 1) {
+      f[0] = to_f32(v);
+    } else {
+      const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) f[k] = to_f32(e[k]);
+    }
+  }
+};
+
+// part[cta][2][D]: this CTA's sums of gy * xhat and gy.  Persistent CTAs; a
+// row's loads are issued before the sums of the one before it.
 template <typename T, int VEC, int NV, int NW>
-__global__ void __launch_bounds__(256)
-bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
+__global__ void __launch_bounds__(Block<NW>::threads)
+bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
            const T* __restrict__ gy, const float* __restrict__ stats, T* __restrict__ gx,
            float* __restrict__ part, int64_t N, int D) {
-  constexpr int G = NW * 32, ROWS = 256 / G;
-  __shared__ float red[8][SUMS];
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   const int g = threadIdx.x % G;
+  const float inv = 1.f / (float)D;
   float aw[NV][VEC], ab[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) aw[j][k] = ab[j][k] = 0.f;
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
-       r += (int64_t)gridDim.x * ROWS) {
-    const float mean = stats[r], rstd = stats[N + r];
-    float h[NV][VEC], u[NV][VEC], s[2] = {0.f, 0.f};
+  Raw<T, VEC> xr[NV], gr[NV];
+  float mean = 0.f, rstd = 0.f;
+  auto fetch = [&](int64_t r) {
+    if (r >= N) return;
+    mean = stats[r];
+    rstd = stats[N + r];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c < D) {
-        load_vec<T, VEC>(x + r * D + c, h[j]);
-        load_vec<T, VEC>(gy + r * D + c, u[j]);
+        xr[j].load(x + r * D + c);
+        gr[j].load(gy + r * D + c);
+      }
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
+  fetch(r);
+  for (; r < N; r += step) {
+    float h[NV][VEC], u[NV][VEC], s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if ((j * G + g) * VEC < D) {
+        xr[j].get(h[j]);
+        gr[j].get(u[j]);
+      }
+    const float m = mean, rs = rstd;
+    fetch(r + step);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + g) * VEC;
+      if (c < D) {
+        float wv[VEC];
+        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          h[j][k] = (h[j][k] - mean) * rstd;
+          h[j][k] = (h[j][k] - m) * rs;
           aw[j][k] = fmaf(u[j][k], h[j][k], aw[j][k]);
           ab[j][k] += u[j][k];
-          u[j][k] *= affine(w, wdtype, c + k, 1.f);
+          u[j][k] *= wv[k];
           s[0] += u[j][k];
           s[1] = fmaf(u[j][k], h[j][k], s[1]);
         }
       }
     }
     if (gx == nullptr) continue;
-    row_sum<NW>(s, red);
-    s[0] /= (float)D;
-    s[1] /= (float)D;
+    row_sum<NW>(s, red, turn);
+    s[0] *= inv;
+    s[1] *= inv;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c < D) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) u[j][k] = rstd * (u[j][k] - s[0] - h[j][k] * s[1]);
+        for (int k = 0; k < VEC; ++k) u[j][k] = rs * (u[j][k] - s[0] - h[j][k] * s[1]);
         store_vec<T, VEC>(gx + r * D + c, u[j]);
       }
     }
@@ -202,19 +282,20 @@ __global__ void __launch_bounds__(256)
 fwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
                 int wdtype, T* __restrict__ y, float* __restrict__ stats, int64_t N, int64_t D,
                 float eps) {
-  __shared__ float red[8][SUMS];
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
     const T* row = x + r * D;
     float s[1] = {0.f}, q[2] = {0.f, 0.f};
     for (int64_t c = threadIdx.x; c < D; c += 256) s[0] += to_f32(row[c]);
-    row_sum<8>(s, red);
+    row_sum<8>(s, red, turn);
     const float mean = s[0] / (float)D;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
       const float d = to_f32(row[c]) - mean;
       q[0] = fmaf(d, d, q[0]);
       q[1] += d;
     }
-    row_sum<8>(q, red);
+    row_sum<8>(q, red, turn);
     const float left = q[1] / (float)D;
     const float rstd = rsqrtf(fmaxf(q[0] / (float)D - left * left, 0.f) + eps);
     for (int64_t c = threadIdx.x; c < D; c += 256)
@@ -234,7 +315,8 @@ __global__ void __launch_bounds__(256)
 bwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
                 const T* __restrict__ gy, const float* __restrict__ stats, T* __restrict__ gx,
                 float* __restrict__ part, int64_t N, int64_t D) {
-  __shared__ float red[8][SUMS];
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   float* mine = part ? part + (int64_t)blockIdx.x * 2 * D : nullptr;
   if (mine)
     for (int64_t c = threadIdx.x; c < D; c += 256) mine[c] = mine[D + c] = 0.f;
@@ -252,7 +334,7 @@ bwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
       s[1] = fmaf(uw, h, s[1]);
     }
     if (gx == nullptr) continue;
-    row_sum<8>(s, red);
+    row_sum<8>(s, red, turn);
     s[0] /= (float)D;
     s[1] /= (float)D;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
@@ -299,13 +381,14 @@ __device__ __forceinline__ void second_terms(float (&s)[SUMS], float h, float u,
 // The backward's backward; u, a, c may be NULL (zero).  part[cta][2][D]: the
 // CTA's sums for dw (the second half is unused, zero).
 template <typename T, int VEC, int NV, int NW>
-__global__ void __launch_bounds__(256)
-bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
+__global__ void __launch_bounds__(Block<NW>::threads)
+bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
             const T* __restrict__ gy, const float* __restrict__ stats, const T* __restrict__ u,
             const void* __restrict__ a, const void* __restrict__ c, T* __restrict__ dx,
             T* __restrict__ dgy, float* __restrict__ part, int64_t N, int D) {
-  constexpr int G = NW * 32, ROWS = 256 / G;
-  __shared__ float red[8][SUMS];
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   const int lane = threadIdx.x % G;
   float aw[NV][VEC], none[NV][VEC];
 #pragma unroll
@@ -330,28 +413,32 @@ bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
 #pragma unroll
           for (int k = 0; k < VEC; ++k) v[j][k] = 0.f;
         }
+        float wv[VEC], av[VEC];
+        affine_vec<T, VEC>(w, wf32, col, 1.f, wv);
+        affine_vec<T, VEC>(a, wf32, col, 0.f, av);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           h[j][k] = (h[j][k] - mean) * rstd;
-          second_terms(s, h[j][k], v[j][k], g[j][k] * affine(w, wdtype, col + k, 1.f),
-                       g[j][k] * affine(a, wdtype, col + k, 0.f));
+          second_terms(s, h[j][k], v[j][k], g[j][k] * wv[k], g[j][k] * av[k]);
         }
       }
     }
-    row_sum<NW>(s, red);
+    row_sum<NW>(s, red, turn);
     const Second f(s, D, rstd);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int col = (j * G + lane) * VEC;
       if (col < D) {
-        float o[VEC];
+        float o[VEC], wv[VEC], av[VEC], cv[VEC];
+        affine_vec<T, VEC>(w, wf32, col, 1.f, wv);
+        affine_vec<T, VEC>(a, wf32, col, 0.f, av);
+        affine_vec<T, VEC>(c, wf32, col, 0.f, cv);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          const float wk = affine(w, wdtype, col + k, 1.f), ak = affine(a, wdtype, col + k, 0.f);
           const float pu = f.pu(v[j][k], h[j][k]);
           aw[j][k] = fmaf(rstd * g[j][k], pu, aw[j][k]);
-          o[k] = rstd * wk * pu + ak * h[j][k] + affine(c, wdtype, col + k, 0.f);
-          v[j][k] = f.dx(h[j][k], v[j][k], g[j][k] * wk, g[j][k] * ak);
+          o[k] = rstd * wv[k] * pu + av[k] * h[j][k] + cv[k];
+          v[j][k] = f.dx(h[j][k], v[j][k], g[j][k] * wv[k], g[j][k] * av[k]);
         }
         store_vec<T, VEC>(dgy + r * D + col, o);
         store_vec<T, VEC>(dx + r * D + col, v[j]);
@@ -368,7 +455,8 @@ bwd2_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype
                  const T* __restrict__ u, const void* __restrict__ a, const void* __restrict__ c,
                  T* __restrict__ dx, T* __restrict__ dgy, float* __restrict__ part, int64_t N,
                  int64_t D) {
-  __shared__ float red[8][SUMS];
+  __shared__ float red[2][32][SUMS];
+  int turn = 0;
   float* mine = part + (int64_t)blockIdx.x * 2 * D;
   for (int64_t e = threadIdx.x; e < D; e += 256) mine[e] = mine[D + e] = 0.f;
   for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
@@ -381,7 +469,7 @@ bwd2_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype
       second_terms(s, h, u ? to_f32(u[r * D + e]) : 0.f, g * affine(w, wdtype, e, 1.f),
                    g * affine(a, wdtype, e, 0.f));
     }
-    row_sum<8>(s, red);
+    row_sum<8>(s, red, turn);
     const Second f(s, D, rstd);
     for (int64_t e = threadIdx.x; e < D; e += 256) {
       const float h = (to_f32(x[r * D + e]) - mean) * rstd, g = to_f32(gy[r * D + e]);

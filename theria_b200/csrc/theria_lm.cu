@@ -184,23 +184,35 @@ int norm_check(int64_t N, int64_t D, int dtype, int wdtype) {
 }
 
 // Calls f(NV, NW) (integral constants) for rows of `units` vectors of VEC
-// values: a warp per row where a lane holds up to 8 values' worth of vectors,
-// else a CTA of 8 warps per row; false where the row does not fit the
-// registers (32 values a thread).
-template <int VEC, typename F>
+// values: the fewest warps per row that hold it in MOST values a thread (one
+// warp needs no barrier), and the fewest vectors a thread among MOST / VEC and
+// its half (a quarter and an eighth for one warp); false where even 32 warps
+// do not hold it.
+template <int VEC, int MOST, int NW, typename F>
+bool norm_vectors(int64_t units, F f) {
+  constexpr int NV = MOST / VEC;
+  constexpr int64_t G = 32 * NW;
+  using W = std::integral_constant<int, NW>;
+  if (units > G * NV) return false;
+  if constexpr (NW == 1 && NV >= 8)
+    if (units <= G * (NV / 8)) return f(std::integral_constant<int, NV / 8>{}, W{}), true;
+  if constexpr (NW == 1 && NV >= 4)
+    if (units <= G * (NV / 4)) return f(std::integral_constant<int, NV / 4>{}, W{}), true;
+  if constexpr (NV >= 2)
+    if (units <= G * (NV / 2)) return f(std::integral_constant<int, NV / 2>{}, W{}), true;
+  return f(std::integral_constant<int, NV>{}, W{}), true;
+}
+template <int VEC, int MOST, typename F>
 bool norm_shape(int64_t D, F f) {
   const int64_t units = cdiv(D, VEC);
-  constexpr int A = VEC == 1 ? 4 : 1, B = VEC == 1 ? 16 : VEC == 4 ? 4 : 2,
-                C = 32 / VEC;  // vectors per thread
-  if (units <= 32 * A) f(std::integral_constant<int, A>{}, std::integral_constant<int, 1>{});
-  else if (units <= 32 * B) f(std::integral_constant<int, B>{}, std::integral_constant<int, 1>{});
-  else if (units <= 256 * A) f(std::integral_constant<int, A>{}, std::integral_constant<int, 8>{});
-  else if (units <= 256 * C) f(std::integral_constant<int, C>{}, std::integral_constant<int, 8>{});
-  else return false;
-  return true;
+  return norm_vectors<VEC, MOST, 1>(units, f) || norm_vectors<VEC, MOST, 4>(units, f) ||
+         norm_vectors<VEC, MOST, 8>(units, f) || norm_vectors<VEC, MOST, 16>(units, f) ||
+         norm_vectors<VEC, MOST, 32>(units, f);
 }
+constexpr int kNormFwd = 32, kNormBwd = 16;  // values a thread: two rows at work in the backward
 
-int64_t norm_ctas(int64_t N) { return std::min<int64_t>(N, kSMs * 2); }
+// CTAs of the backward: what its column sums are split over.
+int64_t norm_ctas(int64_t N) { return std::min<int64_t>(N, kSMs * 4); }
 
 }  // namespace
 }  // namespace theria
@@ -213,17 +225,18 @@ int theria_norm_fwd(const void* x, const void* w, const void* b, int wdtype, voi
   if (N == 0) return THERIA_OK;
   if (!x || !y) return THERIA_ERR_INVALID_ARG;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = vec_rows(D, dtype, {x, y});
+  const bool vec = vec_rows(D, dtype, {x, y, w, b});
+  const int wf32 = wdtype == THERIA_F32;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC>(D, [&](auto nv, auto nw) {
+      return norm_shape<VEC, kNormFwd>(D, [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
-        const int64_t rows = 8 / NW;
+        using B = norm::Block<NW>;
         norm::fwd_kernel<T, VEC, NV, NW>
-            <<<(unsigned)std::min<int64_t>(cdiv(N, rows), kSMs * 32), 256, 0, st>>>(
-                (const T*)x, w, b, wdtype, (T*)y, stats, N, (int)D, eps);
+            <<<(unsigned)std::min<int64_t>(cdiv(N, B::rows), kSMs * 32), B::threads, 0, st>>>(
+                (const T*)x, w, b, wf32, (T*)y, stats, N, (int)D, eps);
       });
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
@@ -256,23 +269,24 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
   if (!gx && !gw) return THERIA_OK;
   if (gw && (!workspace || workspace_bytes < theria_norm_bwd_workspace_bytes(N, D)))
     return THERIA_ERR_WORKSPACE;
-  const bool vec = vec_rows(D, dtype, {x, gy, gx});
+  const bool vec = vec_rows(D, dtype, {x, gy, gx, w});
+  const int wf32 = wdtype == THERIA_F32;
   float* part = gw ? (float*)workspace : nullptr;
   int ctas = 0;
   int e = by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC>(D, [&](auto nv, auto nw) {
+      return norm_shape<VEC, kNormBwd>(D, [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
-        const int64_t rows = 8 / NW;
-        ctas = (int)std::min<int64_t>(cdiv(N, rows), norm_ctas(N));
+        using B = norm::Block<NW>;
         auto kern = norm::bwd_kernel<T, VEC, NV, NW>;
+        ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
         const size_t smem = NW == 1 && part ? 8 * 2 * D * sizeof(float) : 0;
         if (smem > 48 * 1024)
           cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        kern<<<(unsigned)ctas, 256, smem, st>>>((const T*)x, w, wdtype, (const T*)gy, stats,
-                                                (T*)gx, part, N, (int)D);
+        kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy, stats,
+                                                       (T*)gx, part, N, (int)D);
       });
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
@@ -302,21 +316,23 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
   if (!x || !gy || !stats || !dx || !dgy || (dw && !w)) return THERIA_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < theria_norm_bwd_workspace_bytes(N, D))
     return THERIA_ERR_WORKSPACE;
-  const bool vec = vec_rows(D, dtype, {x, gy, u, dx, dgy});
+  const bool vec = vec_rows(D, dtype, {x, gy, u, dx, dgy, w, a, c});
+  const int wf32 = wdtype == THERIA_F32;
   float* part = (float*)workspace;
   int ctas = 0;
   int e = by_type(dtype, [&](auto t) {
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC>(D, [&](auto nv, auto nw) {
+      return norm_shape<VEC, kNormBwd>(D, [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
-        ctas = (int)std::min<int64_t>(cdiv(N, 8 / NW), norm_ctas(N));
+        using B = norm::Block<NW>;
+        ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
         auto kern = norm::bwd2_kernel<T, VEC, NV, NW>;
         const size_t smem = NW == 1 ? 8 * 2 * D * sizeof(float) : 0;
         if (smem > 48 * 1024)
           cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        kern<<<(unsigned)ctas, 256, smem, st>>>((const T*)x, w, wdtype, (const T*)gy, stats,
+        kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy, stats,
                                                 (const T*)u, a, c, (T*)dx, (T*)dgy, part, N,
                                                 (int)D);
       });
