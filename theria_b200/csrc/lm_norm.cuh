@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "lm_embed.cuh"  // load_vec / store_vec
+#include "tc_common.cuh"
 
 namespace theria {
 namespace norm {
@@ -78,6 +79,89 @@ __device__ __forceinline__ void affine_vec(const void* p, bool f32, int64_t c, f
     for (int k = 0; k < VEC; ++k) v[k] = static_cast<const float*>(p)[c + k];
   }
 }
+// Vector arithmetic two values to an instruction (issue slots, not HBM, set the
+// pace of 16-bit rows otherwise: 20 instructions a value without).
+struct Pair {
+  float a = 0.f, b = 0.f;
+  __device__ __forceinline__ float total() const { return a + b; }
+};
+template <int VEC>
+__device__ __forceinline__ void vsum(Pair& p, const float (&v)[VEC]) {  // p += sum v
+  if constexpr (VEC == 1) {
+    p.a += v[0];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) tc::add2(p.a, p.b, p.a, p.b, v[k], v[k + 1]);
+  }
+}
+template <int VEC>  // p += sum u v
+__device__ __forceinline__ void vdot(Pair& p, const float (&u)[VEC], const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    p.a = fmaf(u[0], v[0], p.a);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2)
+      tc::fma2(p.a, p.b, u[k], u[k + 1], v[k], v[k + 1], p.a, p.b);
+  }
+}
+template <int VEC>  // d = a b + c
+__device__ __forceinline__ void vfma(float (&d)[VEC], const float (&a)[VEC],
+                                     const float (&b)[VEC], const float (&c)[VEC]) {
+  if constexpr (VEC == 1) {
+    d[0] = fmaf(a[0], b[0], c[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2)
+      tc::fma2(d[k], d[k + 1], a[k], a[k + 1], b[k], b[k + 1], c[k], c[k + 1]);
+  }
+}
+template <int VEC>  // d = a m + s
+__device__ __forceinline__ void vscale(float (&d)[VEC], const float (&a)[VEC], float m, float s) {
+  if constexpr (VEC == 1) {
+    d[0] = fmaf(a[0], m, s);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) tc::fma2(d[k], d[k + 1], a[k], a[k + 1], m, m, s, s);
+  }
+}
+template <int VEC>  // d += a m
+__device__ __forceinline__ void vaxpy(float (&d)[VEC], const float (&a)[VEC], float m) {
+  if constexpr (VEC == 1) {
+    d[0] = fmaf(a[0], m, d[0]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2)
+      tc::fma2(d[k], d[k + 1], a[k], a[k + 1], m, m, d[k], d[k + 1]);
+  }
+}
+template <int VEC>  // d += a
+__device__ __forceinline__ void vadd(float (&d)[VEC], const float (&a)[VEC]) {
+  if constexpr (VEC == 1) {
+    d[0] += a[0];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) tc::add2(d[k], d[k + 1], d[k], d[k + 1], a[k], a[k + 1]);
+  }
+}
+template <int VEC>  // d += s
+__device__ __forceinline__ void vshift(float (&d)[VEC], float s) {
+  if constexpr (VEC == 1) {
+    d[0] += s;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) tc::add2(d[k], d[k + 1], d[k], d[k + 1], s, s);
+  }
+}
+template <int VEC>  // d *= a
+__device__ __forceinline__ void vmul(float (&d)[VEC], const float (&a)[VEC]) {
+  if constexpr (VEC == 1) {
+    d[0] *= a[0];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 2) tc::mul2(d[k], d[k + 1], d[k], d[k + 1], a[k], a[k + 1]);
+  }
+}
+
 // One affine value, for the kernels of wide rows.
 __device__ __forceinline__ float affine(const void* p, int dtype, int64_t i, float none) {
   return p ? load_any(p, i, dtype) : none;
@@ -90,9 +174,55 @@ template <int NW> struct Block {
   static constexpr int rows = threads / G; // rows at a time
 };
 
-// NW warps per row, NV vectors of VEC values per thread.
+// One row of the forward in registers: x in v becomes y; the statistics to
+// `stats` (may be NULL).
 template <typename T, int VEC, int NV, int NW>
-__global__ void __launch_bounds__(Block<NW>::threads)
+__device__ __forceinline__ void fwd_row(float (&v)[NV][VEC], const void* w, const void* b,
+                                        int wf32, float* stats, int64_t N, int64_t r, int D,
+                                        float inv, float eps, float (*red)[32][SUMS], int& turn) {
+  constexpr int G = Block<NW>::G;
+  const int g = threadIdx.x % G;
+  Pair sum, dev, sq;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if ((j * G + g) * VEC < D) vsum(sum, v[j]);
+  float s[1] = {sum.total()};
+  row_sum<NW>(s, red, turn);
+  const float mean = s[0] * inv;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if ((j * G + g) * VEC < D) {
+      vshift(v[j], -mean);
+      vdot(sq, v[j], v[j]);
+      vsum(dev, v[j]);
+    }
+  float q[2] = {sq.total(), dev.total()};
+  row_sum<NW>(q, red, turn);
+  // what the rounding of a large mean left in the deviations
+  const float left = q[1] * inv;
+  const float rstd = rsqrtf(fmaxf(q[0] * inv - left * left, 0.f) + eps);
+  const float off = -left * rstd;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * G + g) * VEC;
+    if (c < D) {
+      float wv[VEC], bv[VEC];
+      affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+      affine_vec<T, VEC>(b, wf32, c, 0.f, bv);
+      vscale(v[j], v[j], rstd, off);
+      vfma(v[j], v[j], wv, bv);
+    }
+  }
+  if (stats && g == 0) {
+    stats[r] = mean + left;
+    stats[N + r] = rstd;
+  }
+}
+
+// NW warps per row, NV vectors of VEC values per thread; 1024 threads an SM
+// (64 registers), so that as many rows as possible are on their way.
+template <typename T, int VEC, int NV, int NW>
+__global__ void __launch_bounds__(Block<NW>::threads, 1024 / Block<NW>::threads)
 fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
            int wf32, T* __restrict__ y, float* __restrict__ stats, int64_t N, int D, float eps) {
   constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
@@ -102,49 +232,17 @@ fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __re
   const float inv = 1.f / (float)D;
   for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
        r += (int64_t)gridDim.x * ROWS) {
-    float v[NV][VEC], s[1] = {0.f}, q[2] = {0.f, 0.f};
+    float v[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c < D) load_vec<T, VEC>(x + r * D + c, v[j]);
     }
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if ((j * G + g) * VEC < D) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) s[0] += v[j][k];
-      }
-    row_sum<NW>(s, red, turn);
-    const float mean = s[0] * inv;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if ((j * G + g) * VEC < D) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          v[j][k] -= mean;
-          q[0] = fmaf(v[j][k], v[j][k], q[0]);
-          q[1] += v[j][k];
-        }
-      }
-    row_sum<NW>(q, red, turn);
-    // what the rounding of a large mean left in the deviations
-    const float left = q[1] * inv;
-    const float rstd = rsqrtf(fmaxf(q[0] * inv - left * left, 0.f) + eps);
+    fwd_row<T, VEC, NV, NW>(v, w, b, wf32, stats, N, r, D, inv, eps, red, turn);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
-      if (c < D) {
-        float wv[VEC], bv[VEC];
-        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
-        affine_vec<T, VEC>(b, wf32, c, 0.f, bv);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) v[j][k] = fmaf((v[j][k] - left) * rstd, wv[k], bv[k]);
-        store_vec<T, VEC>(y + r * D + c, v[j]);
-      }
-    }
-    if (stats && g == 0) {
-      stats[r] = mean + left;
-      stats[N + r] = rstd;
+      if (c < D) store_vec<T, VEC>(y + r * D + c, v[j]);
     }
   }
 }
@@ -180,24 +278,47 @@ __device__ __forceinline__ void store_part(const float (&a)[NV][VEC], const floa
   }
 }
 
-// VEC values as they are in memory: what a prefetch keeps in registers.
-template <typename T, int VEC>
-struct Raw {
-  typename std::conditional<VEC == 1, T, uint4>::type v;
-  __device__ void load(const T* p) { v = *reinterpret_cast<const decltype(v)*>(p); }
-  __device__ void get(float (&f)[VEC]) const {
-    if constexpr (VEC == 1) {
-      f[0] = to_f32(v);
-    } else {
-      const T* e = reinterpret_cast<const T*>(&v);
+// One row of the backward in registers: x in h and gy in u become xhat and gx;
+// the column sums aw, ab take the row in.
+template <typename T, int VEC, int NV, int NW>
+__device__ __forceinline__ void bwd_row(float (&h)[NV][VEC], float (&u)[NV][VEC],
+                                        float (&aw)[NV][VEC], float (&ab)[NV][VEC],
+                                        const void* w, int wf32, float mean, float rstd, int D,
+                                        float inv, float (*red)[32][SUMS], int& turn) {
+  constexpr int G = Block<NW>::G;
+  const int g = threadIdx.x % G;
+  Pair p, q;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) f[k] = to_f32(e[k]);
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * G + g) * VEC;
+    if (c < D) {
+      float wv[VEC];
+      affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+      vshift(h[j], -mean);  // in this order: a mean far above the deviations loses nothing
+      vscale(h[j], h[j], rstd, 0.f);
+      vfma(aw[j], u[j], h[j], aw[j]);
+      vadd(ab[j], u[j]);
+      vmul(u[j], wv);
+      vsum(p, u[j]);
+      vdot(q, u[j], h[j]);
     }
   }
-};
+  float s[2] = {p.total(), q.total()};
+  row_sum<NW>(s, red, turn);
+  // the means first: where they cancel u, they do so before rstd enlarges it
+  const float c0 = -s[0] * inv, c1 = -s[1] * inv;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if ((j * G + g) * VEC < D) {
+      vshift(u[j], c0);
+      vaxpy(u[j], h[j], c1);
+      vscale(u[j], u[j], rstd, 0.f);
+    }
+  }
+}
 
-// part[cta][2][D]: this CTA's sums of gy * xhat and gy.  Persistent CTAs; a
-// row's loads are issued before the sums of the one before it.
+// part[cta][2][D]: this CTA's sums of gy * xhat and gy.  Persistent CTAs, rows
+// read by each thread (rows that are not whole 16-byte vectors).
 template <typename T, int VEC, int NV, int NW>
 __global__ void __launch_bounds__(Block<NW>::threads)
 bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
@@ -213,65 +334,223 @@ bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) aw[j][k] = ab[j][k] = 0.f;
-  Raw<T, VEC> xr[NV], gr[NV];
-  float mean = 0.f, rstd = 0.f;
-  auto fetch = [&](int64_t r) {
-    if (r >= N) return;
-    mean = stats[r];
-    rstd = stats[N + r];
+  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
+       r += (int64_t)gridDim.x * ROWS) {
+    float h[NV][VEC], u[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c < D) {
-        xr[j].load(x + r * D + c);
-        gr[j].load(gy + r * D + c);
+        load_vec<T, VEC>(x + r * D + c, h[j]);
+        load_vec<T, VEC>(gy + r * D + c, u[j]);
       }
     }
-  };
-  const int64_t step = (int64_t)gridDim.x * ROWS;
-  int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G;
-  fetch(r);
-  for (; r < N; r += step) {
-    float h[NV][VEC], u[NV][VEC], s[2] = {0.f, 0.f};
+    bwd_row<T, VEC, NV, NW>(h, u, aw, ab, w, wf32, stats[r], stats[N + r], D, inv, red, turn);
+    if (gx) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if ((j * G + g) * VEC < D) {
-        xr[j].get(h[j]);
-        gr[j].get(u[j]);
-      }
-    const float m = mean, rs = rstd;
-    fetch(r + step);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * G + g) * VEC;
-      if (c < D) {
-        float wv[VEC];
-        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          h[j][k] = (h[j][k] - m) * rs;
-          aw[j][k] = fmaf(u[j][k], h[j][k], aw[j][k]);
-          ab[j][k] += u[j][k];
-          u[j][k] *= wv[k];
-          s[0] += u[j][k];
-          s[1] = fmaf(u[j][k], h[j][k], s[1]);
-        }
-      }
-    }
-    if (gx == nullptr) continue;
-    row_sum<NW>(s, red, turn);
-    s[0] *= inv;
-    s[1] *= inv;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * G + g) * VEC;
-      if (c < D) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) u[j][k] = rs * (u[j][k] - s[0] - h[j][k] * s[1]);
-        store_vec<T, VEC>(gx + r * D + c, u[j]);
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + g) * VEC;
+        if (c < D) store_vec<T, VEC>(gx + r * D + c, u[j]);
       }
     }
   }
+  if (part) store_part<NW, NV, VEC>(aw, ab, part, D);
+}
+
+// Sums of M values (a power of two) over NW warps.  Each step of the butterfly
+// halves the values a lane keeps, so M sums cost little more than one.
+template <int NW, int M>
+__device__ __forceinline__ void batch_sum(float (&s)[M], float (*red)[32][8], int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int LANES = 32 / M;  // lanes that end with the same value
+  float t[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) t[i] = s[i];
+#pragma unroll
+  for (int m = M, o = 16; o > 0; m >>= 1, o >>= 1) {
+    if (m > 1) {
+#pragma unroll
+      for (int i = 0; i < m / 2; ++i) {
+        const bool upper = lane & o;
+        const float give = upper ? t[i] : t[i + m / 2], keep = upper ? t[i + m / 2] : t[i];
+        t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    } else {
+      t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+    }
+  }
+  if constexpr (NW > 1) {
+    float (*r)[8] = red[turn];
+    turn ^= 1;
+    if (lane % LANES == 0) r[warp][lane / LANES] = t[0];
+    __syncthreads();
+    t[0] = 0.f;
+#pragma unroll
+    for (int w = 0; w < (NW + LANES - 1) / LANES; ++w)
+      if (w * LANES + lane % LANES < NW) t[0] += r[w * LANES + lane % LANES][lane / LANES];
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) s[i] = __shfl_sync(0xffffffffu, t[0], i * LANES);
+}
+
+// Blocks of consecutive rows, of x and of gy, in a ring of shared-memory
+// stages filled by bulk copies.  A wait that gives up sets the device error
+// word, and the kernel goes on with what the stage holds.
+constexpr int MAX_STAGES = 4;
+struct Ring {
+  uint64_t* full;
+  volatile int* abort;
+  uint8_t* mem;
+  const uint8_t *x, *gy;
+  int rows, stages, stage = 0;
+  uint32_t phase = 0;
+  int64_t N, row_bytes, blocks;
+  __device__ Ring(uint64_t* f, volatile int* a, uint8_t* m, const void* x_, const void* gy_,
+                  int rows_, int stages_, int64_t n, int64_t rb)
+      : full(f), abort(a), mem(m), x((const uint8_t*)x_), gy((const uint8_t*)gy_), rows(rows_),
+        stages(stages_), N(n), row_bytes(rb), blocks((n + rows_ - 1) / rows_) {
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < MAX_STAGES; ++i) tc::mbar_init(full + i, 1);
+      *abort = 0;
+      tc::fence_barrier_init();
+      for (int i = 0; i < stages; ++i) fetch(blockIdx.x + (int64_t)i * gridDim.x, i);
+    }
+    __syncthreads();
+  }
+  __device__ uint8_t* at(int s) const { return mem + (int64_t)s * 2 * rows * row_bytes; }
+  // block b into stage s, by one thread
+  __device__ void fetch(int64_t b, int s) {
+    if (b >= blocks) return;
+    const int64_t r0 = b * rows;
+    const uint32_t bytes = (uint32_t)((N - r0 < rows ? N - r0 : rows) * row_bytes);
+    tc::mbar_expect_tx(full + s, 2 * bytes);
+    tc::bulk_load(at(s), x + r0 * row_bytes, bytes, full + s);
+    tc::bulk_load(at(s) + rows * row_bytes, gy + r0 * row_bytes, bytes, full + s);
+  }
+  __device__ void wait() { tc::mbar_wait(full + stage, phase, abort); }
+  __device__ void next() {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  // copies in flight after a wait that gave up land before the CTA ends
+  __device__ void end() {
+    if (*abort)
+      for (int i = 0; i < 1000; ++i) __nanosleep(2000);
+    __syncthreads();
+  }
+};
+
+// bwd_kernel for rows of whole 16-byte vectors.  A batch of R rows per group of
+// NW warps goes through the reduction together: one barrier and one butterfly
+// for 2 R sums.  The rows are read from their stage twice (for the sums, and
+// for gx) instead of being held in registers, which the column sums need.
+template <typename T, int VEC, int NV, int NW, int R>
+__global__ void __launch_bounds__(Block<NW>::threads)
+bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
+                 const T* __restrict__ gy, const float* __restrict__ stats, T* __restrict__ gx,
+                 float* __restrict__ part, int64_t N, int D, int stages) {
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows * R;
+  extern __shared__ __align__(16) uint8_t ring_mem[];  // afterwards store_part's
+  __shared__ float red[2][32][8];
+  __shared__ __align__(8) uint64_t full[MAX_STAGES];
+  __shared__ volatile int abort;
+  int turn = 0;
+  const int g = threadIdx.x % G, q = threadIdx.x / G;
+  const float inv = 1.f / (float)D;
+  Ring ring(full, &abort, ring_mem, x, gy, ROWS, stages, N, (int64_t)D * sizeof(T));
+  float aw[NV][VEC], ab[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) aw[j][k] = ab[j][k] = 0.f;
+  // of the batch to come
+  float mean[R], rstd[R];
+  auto statistics = [&](int64_t blk) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = blk * ROWS + q * R + i;
+      mean[i] = r < N ? stats[r] : 0.f;
+      rstd[i] = r < N ? stats[N + r] : 0.f;
+    }
+  };
+  statistics(blockIdx.x);
+  int before = -1;  // the stage of the batch before, read by every thread at the next barrier
+  for (int64_t blk = blockIdx.x; blk < ring.blocks; blk += gridDim.x) {
+    ring.wait();
+    const T* sx = reinterpret_cast<const T*>(ring.at(ring.stage)) + (int64_t)q * R * D;
+    const T* sg = sx + (int64_t)ROWS * D;
+    const int64_t r0 = blk * ROWS + q * R;
+    float m[R], rs[R], s[2 * R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      m[i] = mean[i];
+      rs[i] = rstd[i];
+    }
+    statistics(blk + gridDim.x);
+    Pair su[R], sh[R];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + g) * VEC;
+      if (c >= D) continue;
+      float wv[VEC];
+      affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (r0 + i >= N) continue;
+        float h[VEC], u[VEC];
+        load_vec<T, VEC>(sx + (int64_t)i * D + c, h);
+        load_vec<T, VEC>(sg + (int64_t)i * D + c, u);
+        vshift(h, -m[i]);  // in this order: a mean far above the deviations loses nothing
+        vscale(h, h, rs[i], 0.f);
+        vfma(aw[j], u, h, aw[j]);
+        vadd(ab[j], u);
+        vmul(u, wv);
+        vsum(su[i], u);
+        vdot(sh[i], u, h);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      s[2 * i] = su[i].total();
+      s[2 * i + 1] = sh[i].total();
+    }
+    batch_sum<NW>(s, red, turn);
+    if (NW == 1) __syncthreads();
+    if (threadIdx.x == 0 && before >= 0)
+      ring.fetch(blk + (int64_t)(stages - 1) * gridDim.x, before);
+    before = ring.stage;
+    if (gx) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + g) * VEC;
+        if (c >= D) continue;
+        float wv[VEC];
+        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          if (r0 + i >= N) continue;
+          float h[VEC], u[VEC];
+          load_vec<T, VEC>(sx + (int64_t)i * D + c, h);
+          load_vec<T, VEC>(sg + (int64_t)i * D + c, u);
+          vshift(h, -m[i]);
+          vscale(h, h, rs[i], 0.f);
+          // the means first: where they cancel u, they do so before rstd
+          // enlarges it
+          vmul(u, wv);
+          vshift(u, -s[2 * i] * inv);
+          vaxpy(u, h, -s[2 * i + 1] * inv);
+          vscale(u, u, rs[i], 0.f);
+          store_vec<T, VEC>(gx + (r0 + i) * D + c, u);
+        }
+      }
+    }
+    ring.next();
+  }
+  ring.end();
   if (part) store_part<NW, NV, VEC>(aw, ab, part, D);
 }
 

@@ -133,6 +133,16 @@ __device__ __forceinline__ void bulk_wait_all() {
 }
 
 // ---------------------------------------------------------------- TMA
+// Untiled load of `bytes` into this CTA's shared memory, completing on `bar`;
+// both addresses and the size are multiples of 16.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
 // 3-D tiled load of box {64 elems, rows, 1} at (x, y, z) into smem,
 // completing on `bar` (transaction bytes).  x must be 16-byte aligned in
 // elements (a multiple of 8 for 16-bit types): every caller passes 0 or 64.

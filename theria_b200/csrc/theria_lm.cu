@@ -209,9 +209,13 @@ bool norm_shape(int64_t D, F f) {
          norm_vectors<VEC, MOST, 8>(units, f) || norm_vectors<VEC, MOST, 16>(units, f) ||
          norm_vectors<VEC, MOST, 32>(units, f);
 }
-constexpr int kNormFwd = 32, kNormBwd = 16;  // values a thread: two rows at work in the backward
+// Values a thread: more of them share the cost of a row's reduction (forward,
+// 16384 x 4096 bfloat16: 32 values 58 us, 16 values 76, 8 values 108); the
+// backward holds column sums besides, and takes 16 only for rows too wide for 8.
+constexpr int kNormFwd = 32, kNormBwd = 8, kNormBwdWide = 16;
 
 // CTAs of the backward: what its column sums are split over.
+constexpr int64_t kMaxGrid = (1ll << 31) - 1;
 int64_t norm_ctas(int64_t N) { return std::min<int64_t>(N, kSMs * 4); }
 
 }  // namespace
@@ -235,8 +239,8 @@ int theria_norm_fwd(const void* x, const void* w, const void* b, int wdtype, voi
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
         using B = norm::Block<NW>;
         norm::fwd_kernel<T, VEC, NV, NW>
-            <<<(unsigned)std::min<int64_t>(cdiv(N, B::rows), kSMs * 32), B::threads, 0, st>>>(
-                (const T*)x, w, b, wf32, (T*)y, stats, N, (int)D, eps);
+            <<<(unsigned)std::min<int64_t>(cdiv(N, B::rows), NW == 1 ? kSMs * 32 : kMaxGrid),
+               B::threads, 0, st>>>((const T*)x, w, b, wf32, (T*)y, stats, N, (int)D, eps);
       });
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
@@ -277,17 +281,44 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC, kNormBwd>(D, [&](auto nv, auto nw) {
+      auto run = [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
         using B = norm::Block<NW>;
-        auto kern = norm::bwd_kernel<T, VEC, NV, NW>;
+        // the partial sums of a CTA's eight rows at a time
+        const int64_t sums = NW == 1 && part ? 8 * 2 * D * (int64_t)sizeof(float) : 0;
+        if constexpr (VEC > 1) {
+          const int64_t row = 2 * D * (int64_t)sizeof(T);  // of x and gy
+          if (2 * row <= 200 << 10) {
+            // rows of a batch: 4 for a warp of its own, 2 where that makes
+            // stages of at most 32 KB, else 1
+            auto batch = [&](auto rc) {
+              constexpr int R = decltype(rc)::value;
+              auto kern = norm::bwd_batch_kernel<T, VEC, NV, NW, R>;
+              const int64_t stage = B::rows * R * row;
+              const int stages = (int)std::clamp<int64_t>((96 << 10) / stage, 2, norm::MAX_STAGES);
+              const int64_t smem = std::max(sums, stage * stages);
+              if (smem > 40 << 10)  // with the kernel's static part, above the default limit
+                cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+              // one wave: each CTA has its share of the rows from the start
+              int per_sm = 1;
+              cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, B::threads, smem);
+              ctas = (int)std::min(cdiv(N, B::rows * R),
+                                   std::min<int64_t>(norm_ctas(N), kSMs * std::max(per_sm, 1)));
+              kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy,
+                                                             stats, (T*)gx, part, N, (int)D,
+                                                             stages);
+            };
+            if constexpr (NW == 1) batch(std::integral_constant<int, 4>{});
+            else if (2 * row <= 32 << 10) batch(std::integral_constant<int, 2>{});
+            else batch(std::integral_constant<int, 1>{});
+            return;
+          }
+        }
         ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
-        const size_t smem = NW == 1 && part ? 8 * 2 * D * sizeof(float) : 0;
-        if (smem > 48 * 1024)
-          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy, stats,
-                                                       (T*)gx, part, N, (int)D);
-      });
+        norm::bwd_kernel<T, VEC, NV, NW><<<(unsigned)ctas, B::threads, sums, st>>>(
+            (const T*)x, w, wf32, (const T*)gy, stats, (T*)gx, part, N, (int)D);
+      };
+      return norm_shape<VEC, kNormBwd>(D, run) || norm_shape<VEC, kNormBwdWide>(D, run);
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
                           : launch(std::integral_constant<int, 1>{});
@@ -324,7 +355,7 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC, kNormBwd>(D, [&](auto nv, auto nw) {
+      return norm_shape<VEC, kNormBwdWide>(D, [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
         using B = norm::Block<NW>;
         ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
