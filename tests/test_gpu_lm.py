@@ -84,6 +84,21 @@ def test_embedding_sums_every_token_of_one_row():
     assert gw[2].tolist() == [100_000.0] * 8 and gw[[0, 1, 3]].abs().max() == 0
 
 
+@pytest.mark.parametrize("V", [1, 2, 500, 600, 300_000])
+@pytest.mark.parametrize("n", [31, 1024, 4096, 4097, 9000, 20_000, 40_000, 131_072, 131_073,
+                               150_001])
+def test_embedding_gradient_over_token_counts(n, V):
+    # every shape of the sort, with odd row widths; whole numbers, which
+    # float32 adds exactly in any order (sums stay below 2^24)
+    g = _gen(n + V)
+    ids = (torch.rand(n, generator=g) ** 4 * V).long().clamp_(max=V - 1)
+    gy = torch.randint(-8, 9, (n, 3), generator=g).float()
+    w = torch.zeros(V, 3, device="cuda", requires_grad=True)
+    (gw,) = torch.autograd.grad(lm.embedding(ids.cuda(), w), w, gy.cuda())
+    want = torch.zeros(V, 3, dtype=torch.float64).index_add_(0, ids, gy.double())
+    assert torch.equal(gw.cpu().double(), want)
+
+
 @pytest.mark.parametrize("padding", [0, 3, -1])
 def test_embedding_padding_row_gets_no_gradient(padding):
     g = _gen(3)

@@ -67,21 +67,6 @@ struct TcArgs {
 __device__ __forceinline__ int pair_a(int i) { return (0x001102 >> (4 * i)) & 15; }
 __device__ __forceinline__ int pair_b(int i) { return (0x010120 >> (4 * i)) & 15; }
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
-               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The shared::cluster address of `p` in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tc::smem_u32(p)), "r"(rank));
-  return a;
-}
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
                : "memory");
@@ -246,7 +231,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oTmem);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::oAbort);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
+  const uint32_t rank = tc::cluster_rank();
   const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
@@ -270,7 +255,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   }
   tc::tc_fence_before();
   __syncthreads();
-  cluster_sync();
+  tc::cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const Sched<EPI> sched(args);
@@ -301,7 +286,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           uint8_t* a = smem + L::oA + slot * OPERAND;
           uint8_t* b = smem + L::oB + slot * OPERAND;
           if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
-          const uint32_t bar = map_rank(full + slot, 0);
+          const uint32_t bar = tc::map_rank(full + slot, 0);
           if constexpr (A_MN) {
             load_2d(a, pa, bar, xa + m0, k);
             load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, k);
@@ -488,7 +473,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       auto give_back = [&](uint32_t buf) {
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_cluster(map_rank(acc_empty + buf, 0));
+        if (lane == 0) arrive_cluster(tc::map_rank(acc_empty + buf, 0));
       };
 
       if constexpr (F32) {
@@ -543,7 +528,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int i = 0; i < 1000; ++i) __nanosleep(2000);
   }
   tc::tc_fence_before();
-  cluster_sync();
+  tc::cluster_sync();
   tc::tc_fence_after();
   if (warp == 1) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem),

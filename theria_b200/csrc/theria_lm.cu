@@ -66,22 +66,61 @@ struct Carver {
 
 // ------------------------------------------------------------ embedding
 struct EmbedWs {
-  uint32_t *keys[2], *vals[2], *hist, *start;
+  uint32_t *keys[2], *vals[2], *hist;
+  uint2* range;
   float* part;
   int64_t bytes;
 };
+constexpr int64_t kClusterSort = (int64_t)embed::CS_CTAS * embed::CS_THREADS * embed::CS_MOST;
 EmbedWs embed_ws(void* base, int64_t n, int64_t V, int64_t D) {
   Carver c{(char*)base};
   EmbedWs w;
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < (n <= kClusterSort ? 1 : 2); ++k) {
     w.keys[k] = c.take<uint32_t>(n);
     w.vals[k] = c.take<uint32_t>(n);
   }
-  w.hist = c.take<uint32_t>(cdiv(n, embed::TILE) * embed::BINS);
-  w.start = c.take<uint32_t>(V + 1);
+  w.hist = n <= kClusterSort ? nullptr : c.take<uint32_t>(cdiv(n, embed::TILE) * embed::BINS);
+  w.range = c.take<uint2>(V);
   w.part = c.take<float>(n / embed::CHUNK * D);
   w.bytes = c.used;
   return w;
+}
+
+// The sort of up to kClusterSort tokens: one CTA up to 4 tokens a thread, else
+// a cluster of 8.
+int embed_cluster_sort(const void* ids, int wide, const EmbedWs& ws, int64_t n, int64_t V,
+                       int64_t zero_idx, int bits, cudaStream_t st) {
+  using L = embed::ClusterSmem;
+  const int ctas = n <= 4 * embed::CS_THREADS ? 1 : embed::CS_CTAS;
+  const int64_t each = cdiv(n, (int64_t)ctas * embed::CS_THREADS);
+  const int passes = (int)cdiv(bits, embed::CS_BITS), digit = (int)cdiv(bits, passes);
+  auto launch = [&](auto rc) -> int {
+    constexpr int R = decltype(rc)::value;
+    auto kern = embed::cluster_sort_kernel<R>;
+    const int smem = L::oBuf + embed::CS_THREADS * R * 8;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess)
+      return THERIA_ERR_LAUNCH;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(embed::CS_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, ids, wide, ctas, passes, digit, ws.keys[0], ws.vals[0],
+                       ws.range, (int)n, V, zero_idx);
+    return launch_status();
+  };
+  if (each <= 1) return launch(std::integral_constant<int, 1>{});
+  if (each <= 2) return launch(std::integral_constant<int, 2>{});
+  if (each <= 4) return launch(std::integral_constant<int, 4>{});
+  if (each <= 8) return launch(std::integral_constant<int, 8>{});
+  return launch(std::integral_constant<int, embed::CS_MOST>{});
 }
 
 int embed_check(int64_t n, int64_t V, int64_t D, int dtype) {
@@ -132,27 +171,36 @@ int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* 
   if (!workspace || workspace_bytes < theria_embed_bwd_workspace_bytes(n, V, D))
     return THERIA_ERR_WORKSPACE;
   const EmbedWs ws = embed_ws(workspace, n, V, D);
-  const unsigned tiles = (unsigned)cdiv(n, embed::TILE);
   int bits = 1;  // keys are 0 .. V
   while ((V >> bits) != 0) ++bits;
   const uint32_t *keys = nullptr, *vals = nullptr;
-  int to = 0;
-  for (int shift = 0; shift < bits; shift += 8, to ^= 1) {
-    embed::hist_kernel<<<tiles, embed::SORT_THREADS, 0, st>>>(ids, wide, keys, ws.hist, n, V,
-                                                              zero_idx, shift);
+  if (n <= kClusterSort) {
+    if (int e = embed_cluster_sort(ids, wide, ws, n, V, zero_idx, bits, st)) return e;
+    keys = ws.keys[0];
+    vals = ws.vals[0];
+  } else {
+    const unsigned tiles = (unsigned)cdiv(n, embed::TILE);
+    int to = 0;
+    for (int shift = 0; shift < bits; shift += 8, to ^= 1) {
+      embed::hist_kernel<<<tiles, embed::SORT_THREADS, 0, st>>>(ids, wide, keys, ws.hist, n, V,
+                                                                zero_idx, shift);
+      if (int e = launch_status()) return e;
+      embed::scan_kernel<<<1, 1024, 0, st>>>(ws.hist, (int64_t)tiles * embed::BINS);
+      if (int e = launch_status()) return e;
+      embed::scatter_kernel<<<tiles, embed::SORT_THREADS, 0, st>>>(
+          ids, wide, keys, vals, ws.hist, ws.keys[to], ws.vals[to], n, V, zero_idx, shift);
+      if (int e = launch_status()) return e;
+      keys = ws.keys[to];
+      vals = ws.vals[to];
+    }
+    if (cudaMemsetAsync(ws.range, 0, V * sizeof(uint2), st) != cudaSuccess)
+      return THERIA_ERR_LAUNCH;
+    embed::range_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 256), kSMs * 8), 256, 0, st>>>(
+        keys, ws.range, n, V);
     if (int e = launch_status()) return e;
-    embed::scan_kernel<<<1, 1024, 0, st>>>(ws.hist, (int64_t)tiles * embed::BINS);
-    if (int e = launch_status()) return e;
-    embed::scatter_kernel<<<tiles, embed::SORT_THREADS, 0, st>>>(
-        ids, wide, keys, vals, ws.hist, ws.keys[to], ws.vals[to], n, V, zero_idx, shift);
-    if (int e = launch_status()) return e;
-    keys = ws.keys[to];
-    vals = ws.vals[to];
   }
-  embed::starts_kernel<<<(unsigned)std::min<int64_t>(cdiv(V + 1, 256), kSMs * 8), 256, 0, st>>>(
-      keys, ws.start, n, V);
-  if (int e = launch_status()) return e;
   const bool vec = vec_rows(D, dtype, {gy, gw});
+  const bool flat = tc::aligned16(gw);
   const int64_t chunks = n / embed::CHUNK;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
@@ -163,9 +211,12 @@ int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* 
           (const T*)gy, keys, vals, ws.part, chunks, V, D);
       if (int e = launch_status()) return e;
     }
-    auto kern = vec ? embed::rows_kernel<T, VEC> : embed::rows_kernel<T, 1>;
-    kern<<<(unsigned)std::min<int64_t>(V, kSMs * 32), 256, 0, st>>>(
-        (const T*)gy, vals, ws.start, ws.part, (T*)gw, V, D, scale);
+    auto kern = vec    ? embed::rows_kernel<T, VEC, true>
+                : flat ? embed::rows_kernel<T, VEC, false>
+                       : embed::rows_kernel<T, 1, true>;
+    const int64_t units = cdiv(V * D, vec || flat ? VEC : 1);
+    kern<<<(unsigned)std::min<int64_t>(cdiv(units, 1024), (1ll << 31) - 1), 256, 0, st>>>(
+        (const T*)gy, vals, ws.range, ws.part, (T*)gw, V, D, scale);
     return launch_status();
   });
 }
