@@ -37,7 +37,7 @@ int theria_embed_fwd(const void* ids, int wide, const void* w, void* out, int64_
 /* gw[v] = scale * sum over i with ids[i] == v of gy[i], summed in the order
  * of i; rows of no token, and the row `zero_idx`, are zero.  The tokens are
  * sorted by id in a workspace of theria_embed_bwd_workspace_bytes(n, V, D)
- * bytes.  n < 2^30, V < 2^31 - 1. */
+ * bytes.  n < 2^30, V < 2^31 - 1, D <= 2^21 - 32 (both directions). */
 int64_t theria_embed_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* workspace,
                      int64_t workspace_bytes, int64_t n, int64_t V, int64_t D, int dtype,

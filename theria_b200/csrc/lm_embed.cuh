@@ -4,11 +4,12 @@
 //   backward  dW_v = scale * sum_{i : id_i = v} g_i       (every row v of dW)
 //
 // The backward sorts the tokens by id with a stable radix sort, so that the
-// rows that belong to one v are neighbours and in token order, and then every
-// row of dW is one sum in a fixed order: no floating-point atomics, the same
-// bits every time, float32 throughout with one rounding at the end.  Both
-// directions are bound by HBM: the forward reads and writes n D values, the
-// backward reads n D and writes V D (mostly zeros for a large vocabulary).
+// rows that belong to one v are neighbours and in token order, and then sums
+// them in chunks of 32 sorted tokens: no floating-point atomics, the same bits
+// every time, float32 throughout with one rounding at the end.  Both directions
+// are bound by HBM: the forward reads and writes n D values, the backward
+// reads n D and writes V D (mostly zeros for a large vocabulary, written while
+// the tokens are being sorted).
 #pragma once
 
 #include "common.cuh"
@@ -85,10 +86,9 @@ fwd_kernel(const void* __restrict__ ids, int wide, const T* __restrict__ w, T* _
 // ---------------------------------------------------------------- the sort
 // Stable least-significant-digit radix sort of (key, token index): keys are the
 // ids, and V for a token without a row (outside the vocabulary, or the zero
-// row), so those come last.  What follows needs the sorted tokens and, for each
-// v, range[v] = (first position, one past the last), (0, 0) for no token.
+// row), so those come last.
 //
-// Up to 131,072 tokens one cluster does it all in one launch
+// Up to 65,536 tokens one cluster does it all in one launch
 // (cluster_sort_kernel); more tokens go through three launches a pass: a tile
 // of 2048 tokens per CTA, each warp owning 256 consecutive ones, 8 bits a pass.
 constexpr int TILE = 2048, SORT_THREADS = 256, BINS = 256;
@@ -200,50 +200,64 @@ scatter_kernel(const void* __restrict__ ids, int wide, const uint32_t* __restric
   }
 }
 
-// range[] from the sorted keys (zeroed before).
-__global__ void range_kernel(const uint32_t* __restrict__ keys, uint2* __restrict__ range,
-                             int64_t n, int64_t V) {
-  for (int64_t p = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; p < n;
-       p += (int64_t)gridDim.x * blockDim.x) {
-    const uint32_t k = keys[p];
-    if (k >= (uint32_t)V) continue;
-    if (p == 0 || keys[p - 1] != k) range[k].x = (uint32_t)p;
-    if (p == n - 1 || keys[p + 1] != k) range[k].y = (uint32_t)p + 1;
+constexpr int CS_THREADS = 1024, CS_BITS = 9, CS_BINS = 1 << CS_BITS, CS_CTAS = 8, CS_MOST = 8;
+
+// The lanes whose d (of `bits` bits) equals this lane's, among `in`: a ballot
+// per bit (match.any takes a step for each value that differs: 2.2 us a round
+// of 32 warps against 0.5).
+__device__ __forceinline__ uint32_t peers_of(uint32_t d, int bits, uint32_t in) {
+  uint32_t same = in;
+#pragma unroll
+  for (int b = 0; b < CS_BITS; ++b) {
+    if (b >= bits) break;
+    const bool one = (d >> b) & 1;
+    const uint32_t v = __ballot_sync(0xffffffffu, one);
+    same &= one ? v : ~v;
   }
+  return same;
 }
 
-// The whole sort in one cluster of 1 or 8 CTAs of 1024 threads: R tokens a
-// thread stay in registers while a pass ranks them, and go through the
+// The whole sort in the first cluster of 1 or 8 CTAs of 1024 threads: R tokens
+// a thread stay in registers while a pass ranks them, and go through the
 // distributed shared memory of the cluster to their next place (8 bytes a
 // token), 9 bits at most a pass.  A pass costs two cluster barriers instead of
-// three launches: 65,536 tokens of a 131,072-word vocabulary 84 us before, in
-// three passes of 8 bits.  R: a power of two.
-constexpr int CS_THREADS = 1024, CS_BITS = 9, CS_BINS = 1 << CS_BITS, CS_CTAS = 8, CS_MOST = 16;
+// three launches (65,536 tokens, vocabulary 131,072: 45 us, against 84 in three
+// passes of three launches).  The other clusters meanwhile write the zeros of
+// the gradient, which need no order.
 struct ClusterSmem {
   static constexpr int oCount = 0;                          // [32 warps][bins]
   static constexpr int oTotal = oCount + 32 * CS_BINS * 4;  // [bins], read by the other CTAs
   static constexpr int oBase = oTotal + CS_BINS * 4;
-  static constexpr int oWarp = oBase + CS_BINS * 4;
-  static constexpr int oBuf = oWarp + 128;                  // [1024 R] (key, index)
+  static constexpr int oOwn = oBase + CS_BINS * 4;
+  static constexpr int oWarp = oOwn + CS_BINS * 4;
+  static constexpr int oBuf = oWarp + 256;                  // 2 x [1024 R] (key, index)
 };
 template <int R>
 __global__ void __launch_bounds__(CS_THREADS)
 cluster_sort_kernel(const void* __restrict__ ids, int wide, int ctas, int passes, int bits,
-                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out,
-                    uint2* __restrict__ range, int n, int64_t V, int64_t zero_idx) {
+                    uint32_t* __restrict__ keys_out, uint32_t* __restrict__ vals_out, int n,
+                    int64_t V, int64_t zero_idx, uint4* __restrict__ zeros, int64_t zeros_bytes) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if ((int)blockIdx.x >= ctas) {
+    const int64_t n16 = zeros_bytes / 16, step = (int64_t)(gridDim.x - ctas) * CS_THREADS;
+    int64_t i = (int64_t)(blockIdx.x - ctas) * CS_THREADS + tid;
+    if (i < zeros_bytes % 16 / 2) reinterpret_cast<uint16_t*>(zeros + n16)[i] = 0;
+#pragma unroll 4
+    for (; i < n16; i += step) zeros[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   extern __shared__ __align__(16) uint8_t cs_mem[];
   using L = ClusterSmem;
   uint32_t(*count)[CS_BINS] = reinterpret_cast<uint32_t(*)[CS_BINS]>(cs_mem + L::oCount);
   uint32_t* total = reinterpret_cast<uint32_t*>(cs_mem + L::oTotal);
   uint32_t* base = reinterpret_cast<uint32_t*>(cs_mem + L::oBase);
   uint32_t* part = reinterpret_cast<uint32_t*>(cs_mem + L::oWarp);
+  uint32_t* own = reinterpret_cast<uint32_t*>(cs_mem + L::oOwn);
   uint2* buf = reinterpret_cast<uint2*>(cs_mem + L::oBuf);
+  uint2* mine = buf + CS_THREADS * R;  // this CTA's tokens by digit
   constexpr int HELD = CS_THREADS * R;  // tokens of a CTA
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = tc::cluster_rank();
   const int local = warp * 32 * R + lane, first = (int)rank * HELD + local;
-  for (int64_t v = (int64_t)rank * CS_THREADS + tid; v < V; v += (int64_t)ctas * CS_THREADS)
-    range[v] = make_uint2(0, 0);
   uint32_t key[R], val[R], at[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -260,7 +274,7 @@ cluster_sort_kernel(const void* __restrict__ ids, int wide, int ctas, int passes
     for (int r = 0; r < R; ++r) {
       const bool in = first + r * 32 < n;
       const uint32_t d = (key[r] >> shift) & mask;
-      const uint32_t peers = __match_any_sync(0xffffffffu, in ? d : CS_BINS);
+      const uint32_t peers = peers_of(d, bits, __ballot_sync(0xffffffffu, in));
       const uint32_t before = __popc(peers & ((1u << lane) - 1));
       at[r] = in ? count[warp][d] + before : 0;
       __syncwarp();
@@ -269,17 +283,20 @@ cluster_sort_kernel(const void* __restrict__ ids, int wide, int ctas, int passes
     }
     __syncthreads();
     if (tid < CS_BINS) {
-      uint32_t sum = 0;
+      uint32_t sum = 0, c[32];
+#pragma unroll
+      for (int w = 0; w < 32; ++w) c[w] = count[w][tid];
 #pragma unroll
       for (int w = 0; w < 32; ++w) {
-        const uint32_t c = count[w][tid];
         count[w][tid] = sum;
-        sum += c;
+        sum += c[w];
       }
       total[tid] = sum;
     }
     tc::cluster_sync();  // every CTA's totals are there, every token in registers
-    uint32_t all = 0, before = 0, run = 0;
+    // base[d]: where this CTA's tokens of digit d go; own[d]: their first place
+    // among its own
+    uint32_t all = 0, before = 0, run = 0, mine_d = 0, run_own = 0;
     if (tid < CS_BINS) {
       for (int c = 0; c < ctas; ++c) {
         const uint32_t t = tc::ld_cluster(tc::map_rank(total + tid, c));
@@ -287,25 +304,48 @@ cluster_sort_kernel(const void* __restrict__ ids, int wide, int ctas, int passes
         before += c < (int)rank ? t : 0;
       }
       run = all;
+      run_own = mine_d = total[tid];
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t u = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run += u;
+        const uint32_t v = __shfl_up_sync(0xffffffffu, run_own, o);
+        if (lane >= o) {
+          run += u;
+          run_own += v;
+        }
       }
-      if (lane == 31) part[warp] = run;
+      if (lane == 31) {
+        part[warp] = run;
+        part[32 + warp] = run_own;
+      }
     }
     __syncthreads();
     if (tid < CS_BINS) {
-      for (int w = 0; w < warp; ++w) before += part[w];
+      uint32_t own_before = 0;
+      for (int w = 0; w < warp; ++w) {
+        before += part[w];
+        own_before += part[32 + w];
+      }
       base[tid] = before + run - all;
+      own[tid] = own_before + run_own - mine_d;
     }
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       if (first + r * 32 >= n) continue;
       const uint32_t d = (key[r] >> shift) & mask;
-      const uint32_t to = base[d] + count[warp][d] + at[r];
-      tc::st_cluster2(tc::map_rank(buf + to % HELD, to / HELD), key[r], val[r]);
+      mine[own[d] + count[warp][d] + at[r]] = make_uint2(key[r], val[r]);
+    }
+    __syncthreads();
+    // neighbours of one digit go to neighbouring places: few segments a warp
+    const int held = n - (int)rank * HELD < HELD ? n - (int)rank * HELD : HELD;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int j = r * CS_THREADS + tid;
+      if (j >= held) break;
+      const uint2 kv = mine[j];
+      const uint32_t d = (kv.x >> shift) & mask, to = base[d] + (uint32_t)j - own[d];
+      tc::st_cluster2(tc::map_rank(buf + to % HELD, to / HELD), kv.x, kv.y);
     }
     tc::cluster_sync();
 #pragma unroll
@@ -318,159 +358,156 @@ cluster_sort_kernel(const void* __restrict__ ids, int wide, int ctas, int passes
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int p = first + r * 32, l = local + r * 32;
+    const int p = first + r * 32;
     if (p >= n) continue;
     keys_out[p] = key[r];
     vals_out[p] = val[r];
-    if (key[r] >= (uint32_t)V) continue;
-    const bool starts =
-        p == 0 || key[r] != (l > 0 ? buf[l - 1].x
-                                   : tc::ld_cluster(tc::map_rank(buf + HELD - 1, rank - 1)));
-    const bool ends = p == n - 1 || key[r] != (l < HELD - 1
-                                                   ? buf[l + 1].x
-                                                   : tc::ld_cluster(tc::map_rank(buf, rank + 1)));
-    if (starts) range[key[r]].x = (uint32_t)p;
-    if (ends) range[key[r]].y = (uint32_t)p + 1;
   }
-  tc::cluster_sync();  // no CTA ends while another reads its tokens
 }
 
 // -------------------------------------------------------------- the sums
-// Tokens are counted in aligned chunks of CHUNK sorted positions.  A chunk
-// whose tokens all have one id is summed on its own first (chunk_kernel,
-// float32), so the row of a frequent token adds a few chunk sums and at most
-// 2 * (CHUNK - 1) single rows.
+// A group of `width` threads takes one chunk of CHUNK sorted tokens and one
+// vector of columns a thread, and adds the tokens' rows in order.  A run of one
+// id that lies within the chunk is a row of gw, written at once; one that
+// reaches into a neighbouring chunk leaves its sum in part[chunk][0] (it
+// starts the chunk) or [1], for join_kernel.  Every token's row is read once,
+// and no chunk has more to do than another.
 constexpr int CHUNK = 32;
 
-// LEN consecutive values at p; `aligned`: as one 16-byte vector.
-template <typename T, int LEN, bool ALIGNED>
-__device__ __forceinline__ void load_run(const T* p, float (&v)[LEN]) {
-  if constexpr (ALIGNED) {
-    load_vec<T, LEN>(p, v);
-  } else {
-#pragma unroll
-    for (int k = 0; k < LEN; ++k) v[k] = to_f32(p[k]);
-  }
-}
-
-// acc += the rows of the tokens at sorted positions [b, e), columns c ..
-template <typename T, int LEN, bool ALIGNED>
-__device__ __forceinline__ void add_rows(const T* __restrict__ gy, const uint32_t* __restrict__ vals,
-                                         int64_t b, int64_t e, int64_t D, int64_t c,
-                                         float (&acc)[LEN]) {
-  for (; b + 4 <= e; b += 4) {
-    float v[4][LEN];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      load_run<T, LEN, ALIGNED>(gy + (int64_t)vals[b + j] * D + c, v[j]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int k = 0; k < LEN; ++k) acc[k] += v[j][k];
-  }
-  for (; b < e; ++b) {
-    float v[LEN];
-    load_run<T, LEN, ALIGNED>(gy + (int64_t)vals[b] * D + c, v);
-#pragma unroll
-    for (int k = 0; k < LEN; ++k) acc[k] += v[k];
-  }
-}
-
-// part[chunk][D] = the sum of the chunk's rows, for chunks of one id.
+// Grid (chunks / groups, column tiles).  VEC > 1: rows are whole 16-byte vectors.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 chunk_kernel(const T* __restrict__ gy, const uint32_t* __restrict__ keys,
-             const uint32_t* __restrict__ vals, float* __restrict__ part, int64_t chunks,
-             int64_t V, int64_t D) {
-  const int64_t units = (D + VEC - 1) / VEC;
-  for (int64_t j = blockIdx.x; j < chunks; j += gridDim.x) {
-    const int64_t b = j * CHUNK;
-    const uint32_t key = keys[b];
-    if (key != keys[b + CHUNK - 1] || key >= (uint32_t)V) continue;
-    for (int64_t u = threadIdx.x; u < units; u += blockDim.x) {
-      float acc[VEC];
+             const uint32_t* __restrict__ vals, float* __restrict__ part, T* __restrict__ gw,
+             int64_t n, int64_t V, int64_t D, float scale, int width) {
+  constexpr int AT_ONCE = 8;  // loads on their way
+  const int64_t chunk = (int64_t)blockIdx.x * (256 / width) + threadIdx.x / width;
+  const int64_t c = ((int64_t)blockIdx.y * width + threadIdx.x % width) * VEC;
+  const int64_t b = chunk * CHUNK, e = b + CHUNK < n ? b + CHUNK : n;
+  if (b >= n || c >= D) return;
+  float acc[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-      add_rows<T, VEC, (VEC > 1)>(gy, vals, b, b + CHUNK, D, u * VEC, acc);
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  uint32_t key = keys[b];
+  // whether the run at hand came from the chunk before, and where it began
+  bool from_before = b > 0 && keys[b - 1] == key, at_start = true;
+  const uint32_t after = e < n ? keys[e] : 0xffffffffu;
+  auto flush = [&](bool goes_on) {
+    if (key < (uint32_t)V) {
+      if (from_before || goes_on) {
+        float* p = part + (chunk * 2 + (at_start ? 0 : 1)) * D + c;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) part[j * D + u * VEC + k] = acc[k];
-    }
-  }
-}
-
-// LEN values of a row of gw (before `scale`): the tokens at [r.x, r.y).
-template <typename T, int LEN, bool ALIGNED>
-__device__ __forceinline__ void row_values(const T* __restrict__ gy,
-                                           const uint32_t* __restrict__ vals,
-                                           const float* __restrict__ part, uint2 r, int64_t D,
-                                           int64_t c, float (&acc)[LEN]) {
+        for (int k = 0; k < VEC; ++k) p[k] = acc[k];
+      } else {
 #pragma unroll
-  for (int k = 0; k < LEN; ++k) acc[k] = 0.f;
-  // whole chunks inside [r.x, r.y)
-  const int64_t cb = ((int64_t)r.x + CHUNK - 1) / CHUNK, ce = r.y / CHUNK;
-  const bool whole = cb < ce;
-  add_rows<T, LEN, ALIGNED>(gy, vals, r.x, whole ? cb * CHUNK : r.y, D, c, acc);
-  if (whole) {
-#pragma unroll 4
-    for (int64_t j = cb; j < ce; ++j)
-#pragma unroll
-      for (int k = 0; k < LEN; ++k) acc[k] += part[j * D + c + k];
-    add_rows<T, LEN, ALIGNED>(gy, vals, ce * CHUNK, r.y, D, c, acc);
-  }
-}
-
-// gw as one run of V * D values, 16 bytes a thread: zeros, or the sums of the
-// tokens' rows.  ROWS: every vector lies within a row (D a multiple of VEC) and
-// gy's rows are vectors too; else a vector may reach into the rows after its
-// first.  The large vocabulary's zeros set the pace: four vectors a thread are
-// in flight, and odd widths are written as vectors all the same.
-template <typename T, int VEC, bool ROWS>
-__global__ void __launch_bounds__(256)
-rows_kernel(const T* __restrict__ gy, const uint32_t* __restrict__ vals,
-            const uint2* __restrict__ range, const float* __restrict__ part, T* __restrict__ gw,
-            int64_t V, int64_t D, float scale) {
-  constexpr int IN_FLIGHT = 4;
-  const int64_t total = V * D, units = (total + VEC - 1) / VEC;
-  const bool small = total < (1ll << 32);
-  for (int64_t u0 = (int64_t)blockIdx.x * (256 * IN_FLIGHT) + threadIdx.x; u0 < units;
-       u0 += (int64_t)gridDim.x * (256 * IN_FLIGHT)) {
-    int64_t v[IN_FLIGHT];
-    uint2 r[IN_FLIGHT];
-#pragma unroll
-    for (int i = 0; i < IN_FLIGHT; ++i) {
-      const int64_t u = u0 + i * 256;
-      v[i] = small ? (int64_t)((uint32_t)(u * VEC) / (uint32_t)D) : u * VEC / D;
-      r[i] = u < units ? range[v[i]] : make_uint2(0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < IN_FLIGHT; ++i) {
-      const int64_t u = u0 + i * 256;
-      if (u >= units) break;
-      const int64_t c = u * VEC - v[i] * D;
-      float acc[VEC];
-      if (ROWS || c + VEC <= D) {
-        if (r[i].x == r[i].y) {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-        } else {
-          row_values<T, VEC, ROWS && (VEC > 1)>(gy, vals, part, r[i], D, c, acc);
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] *= scale;
-        }
-        store_vec<T, VEC>(gw + u * VEC, acc);
-      } else {  // the end of a row, and the start of the next ones
-#pragma unroll 1
-        for (int k = 0; k < VEC; ++k) {
-          const int64_t e = u * VEC + k;
-          if (e >= total) break;
-          const int64_t row = e / D;
-          const uint2 q = range[row];
-          float one[1];
-          row_values<T, 1, false>(gy, vals, part, q, D, e - row * D, one);
-          gw[e] = from_f32<T>(one[0] * scale);
-        }
+        for (int k = 0; k < VEC; ++k) acc[k] *= scale;
+        store_vec<T, VEC>(gw + (int64_t)key * D + c, acc);
       }
     }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    from_before = at_start = false;
+  };
+  for (int64_t p = b; p < e; p += AT_ONCE) {
+    uint32_t ks[AT_ONCE], vs[AT_ONCE];
+    float v[AT_ONCE][VEC];
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      const int64_t q = p + j < e ? p + j : e - 1;  // past the end: read again, not added
+      ks[j] = keys[q];
+      vs[j] = vals[q];
+    }
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) load_vec<T, VEC>(gy + (int64_t)vs[j] * D + c, v[j]);
+#pragma unroll
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (p + j >= e) break;
+      if (ks[j] != key) {
+        flush(false);
+        key = ks[j];
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += v[j][k];
+    }
+  }
+  flush(after == key);
+}
+
+// Rows of runs over several chunks: the CTAs of the chunk in which a run begins
+// add its parts in order, a vector of columns a thread; over more than 8 parts,
+// the 8 warps take every eighth part of 32 vectors in turn, and their sums are
+// added in order.  Grid (chunks, D / (256 VEC)): most CTAs find no such run (a
+// CTA for every 32 columns of every chunk spent 139 us, mostly on leaving).
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256)
+join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ part, T* __restrict__ gw,
+            int64_t n, int64_t V, int64_t D, float scale) {
+  __shared__ float sums[8][32][VEC + (VEC > 1)];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t j = blockIdx.x, b = j * CHUNK, e = b + CHUNK;
+  if (e >= n) return;
+  const uint32_t key = keys[e - 1], after = keys[e], at_b = keys[b];
+  const uint32_t before = b > 0 ? keys[b - 1] : 0xffffffffu;
+  if (key >= (uint32_t)V || after != key) return;
+  const bool whole = at_b == key;
+  if (whole && before == key) return;  // began earlier
+  // chunks that start within the run: [j + 1, lo), a 32-ary search
+  const int64_t chunks = (n + CHUNK - 1) / CHUNK;
+  int64_t lo = j + 2, hi = chunks;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, p = lo + lane * step;
+    const int in = __popc(__ballot_sync(0xffffffffu, p < hi && keys[p * CHUNK] == key));
+    if (in == 0) break;
+    hi = hi < lo + in * step ? hi : lo + in * step;
+    lo += (in - 1) * step + 1;
+  }
+  const float* first = part + (j * 2 + (whole ? 0 : 1)) * D;
+  if (lo - j <= 8) {
+    const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * VEC;
+    if (c >= D) return;
+    float s[VEC], v[7][VEC];
+    load_vec<float, VEC>(first + c, s);
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+      if (j + 1 + k < lo) load_vec<float, VEC>(part + (j + 1 + k) * 2 * D + c, v[k]);
+#pragma unroll
+    for (int k = 0; k < 7; ++k)
+      if (j + 1 + k < lo) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += v[k][i];
+      }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) gw[(int64_t)key * D + c + i] = from_f32<T>(s[i] * scale);
+    return;
+  }
+  for (int t = 0; t < 8; ++t) {
+    const int64_t c = (((int64_t)blockIdx.y * 8 + t) * 32 + lane) * VEC;
+    float s[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[k] = 0.f;
+    if (c < D) {
+      if (warp == 0) load_vec<float, VEC>(first + c, s);
+#pragma unroll 8
+      for (int64_t k = j + 1 + warp; k < lo; k += 8) {
+        float v[VEC];
+        load_vec<float, VEC>(part + k * 2 * D + c, v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] += v[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[warp][lane][i] = s[i];
+    __syncthreads();
+    if (warp == 0 && c < D) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s[i] += sums[w][lane][i];
+        gw[(int64_t)key * D + c + i] = from_f32<T>(s[i] * scale);
+      }
+    }
+    __syncthreads();
   }
 }
 

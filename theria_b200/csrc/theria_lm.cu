@@ -67,7 +67,6 @@ struct Carver {
 // ------------------------------------------------------------ embedding
 struct EmbedWs {
   uint32_t *keys[2], *vals[2], *hist;
-  uint2* range;
   float* part;
   int64_t bytes;
 };
@@ -80,16 +79,15 @@ EmbedWs embed_ws(void* base, int64_t n, int64_t V, int64_t D) {
     w.vals[k] = c.take<uint32_t>(n);
   }
   w.hist = n <= kClusterSort ? nullptr : c.take<uint32_t>(cdiv(n, embed::TILE) * embed::BINS);
-  w.range = c.take<uint2>(V);
-  w.part = c.take<float>(n / embed::CHUNK * D);
+  w.part = c.take<float>(cdiv(n, embed::CHUNK) * 2 * D);
   w.bytes = c.used;
   return w;
 }
 
-// The sort of up to kClusterSort tokens: one CTA up to 4 tokens a thread, else
-// a cluster of 8.
+// The sort of up to kClusterSort tokens, one CTA up to 4 tokens a thread, else a
+// cluster of 8, while further clusters zero gw (16-byte aligned).
 int embed_cluster_sort(const void* ids, int wide, const EmbedWs& ws, int64_t n, int64_t V,
-                       int64_t zero_idx, int bits, cudaStream_t st) {
+                       int64_t zero_idx, int bits, void* gw, int64_t gw_bytes, cudaStream_t st) {
   using L = embed::ClusterSmem;
   const int ctas = n <= 4 * embed::CS_THREADS ? 1 : embed::CS_CTAS;
   const int64_t each = cdiv(n, (int64_t)ctas * embed::CS_THREADS);
@@ -97,7 +95,7 @@ int embed_cluster_sort(const void* ids, int wide, const EmbedWs& ws, int64_t n, 
   auto launch = [&](auto rc) -> int {
     constexpr int R = decltype(rc)::value;
     auto kern = embed::cluster_sort_kernel<R>;
-    const int smem = L::oBuf + embed::CS_THREADS * R * 8;
+    const int smem = L::oBuf + 2 * embed::CS_THREADS * R * 8;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
         cudaSuccess)
       return THERIA_ERR_LAUNCH;
@@ -106,26 +104,29 @@ int embed_cluster_sort(const void* ids, int wide, const EmbedWs& ws, int64_t n, 
     attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas);
+    // 16 KB of zeros a CTA at least; no more clusters than run at one time
+    // beside the sort's (14 of 8: two fit a GPC)
+    const int64_t fill =
+        std::min<int64_t>(cdiv(gw_bytes, (16 << 10) * ctas), ctas > 1 ? 14 : kSMs - 1);
+    cfg.gridDim = dim3((unsigned)(ctas + ctas * std::max<int64_t>(fill, 1)));
     cfg.blockDim = dim3(embed::CS_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cudaLaunchKernelEx(&cfg, kern, ids, wide, ctas, passes, digit, ws.keys[0], ws.vals[0],
-                       ws.range, (int)n, V, zero_idx);
+                       (int)n, V, zero_idx, (uint4*)gw, gw_bytes);
     return launch_status();
   };
   if (each <= 1) return launch(std::integral_constant<int, 1>{});
   if (each <= 2) return launch(std::integral_constant<int, 2>{});
   if (each <= 4) return launch(std::integral_constant<int, 4>{});
-  if (each <= 8) return launch(std::integral_constant<int, 8>{});
   return launch(std::integral_constant<int, embed::CS_MOST>{});
 }
 
 int embed_check(int64_t n, int64_t V, int64_t D, int dtype) {
   if (n < 0 || V <= 0 || D <= 0 || !lm_dtype(dtype)) return THERIA_ERR_INVALID_ARG;
-  if (n >= (1ll << 30) || V >= (1ll << 31) - 1) return THERIA_ERR_UNSUPPORTED;
+  if (n >= (1ll << 30) || V >= (1ll << 31) - 1 || D > 32 * 65535ll) return THERIA_ERR_UNSUPPORTED;
   return THERIA_OK;
 }
 
@@ -174,8 +175,13 @@ int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* 
   int bits = 1;  // keys are 0 .. V
   while ((V >> bits) != 0) ++bits;
   const uint32_t *keys = nullptr, *vals = nullptr;
+  const int64_t gw_bytes = V * D * elem_size(dtype);
+  const bool fill = n <= kClusterSort && tc::aligned16(gw);
+  if (!fill && cudaMemsetAsync(gw, 0, gw_bytes, st) != cudaSuccess) return THERIA_ERR_LAUNCH;
   if (n <= kClusterSort) {
-    if (int e = embed_cluster_sort(ids, wide, ws, n, V, zero_idx, bits, st)) return e;
+    if (int e = embed_cluster_sort(ids, wide, ws, n, V, zero_idx, bits, gw, fill ? gw_bytes : 0,
+                                   st))
+      return e;
     keys = ws.keys[0];
     vals = ws.vals[0];
   } else {
@@ -193,30 +199,23 @@ int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* 
       keys = ws.keys[to];
       vals = ws.vals[to];
     }
-    if (cudaMemsetAsync(ws.range, 0, V * sizeof(uint2), st) != cudaSuccess)
-      return THERIA_ERR_LAUNCH;
-    embed::range_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, 256), kSMs * 8), 256, 0, st>>>(
-        keys, ws.range, n, V);
-    if (int e = launch_status()) return e;
   }
   const bool vec = vec_rows(D, dtype, {gy, gw});
-  const bool flat = tc::aligned16(gw);
-  const int64_t chunks = n / embed::CHUNK;
+  const int64_t chunks = cdiv(n, embed::CHUNK);
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
     constexpr int VEC = embed::Vec<T>::n;
-    if (chunks > 0) {
-      auto kern = vec ? embed::chunk_kernel<T, VEC> : embed::chunk_kernel<T, 1>;
-      kern<<<(unsigned)std::min<int64_t>(chunks, kSMs * 16), 256, 0, st>>>(
-          (const T*)gy, keys, vals, ws.part, chunks, V, D);
-      if (int e = launch_status()) return e;
-    }
-    auto kern = vec    ? embed::rows_kernel<T, VEC, true>
-                : flat ? embed::rows_kernel<T, VEC, false>
-                       : embed::rows_kernel<T, 1, true>;
-    const int64_t units = cdiv(V * D, vec || flat ? VEC : 1);
-    kern<<<(unsigned)std::min<int64_t>(cdiv(units, 1024), (1ll << 31) - 1), 256, 0, st>>>(
-        (const T*)gy, vals, ws.range, ws.part, (T*)gw, V, D, scale);
+    const int64_t units = cdiv(D, vec ? VEC : 1);
+    int width = 1;  // threads of a chunk: a power of two
+    while (width < 256 && width < units) width *= 2;
+    auto kern = vec ? embed::chunk_kernel<T, VEC> : embed::chunk_kernel<T, 1>;
+    kern<<<dim3((unsigned)cdiv(chunks, 256 / width), (unsigned)cdiv(units, width)), 256, 0, st>>>(
+        (const T*)gy, keys, vals, ws.part, (T*)gw, n, V, D, scale, width);
+    if (int e = launch_status()) return e;
+    if (chunks < 2) return (int)THERIA_OK;
+    auto join = D % 4 == 0 ? embed::join_kernel<T, 4> : embed::join_kernel<T, 1>;
+    join<<<dim3((unsigned)(chunks - 1), (unsigned)cdiv(D, D % 4 == 0 ? 1024 : 256)), 256, 0, st>>>(
+        keys, ws.part, (T*)gw, n, V, D, scale);
     return launch_status();
   });
 }
