@@ -442,7 +442,7 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ part, T* __restrict__ gw,
             int64_t n, int64_t V, int64_t D, float scale) {
-  __shared__ float sums[8][32][VEC + (VEC > 1)];
+  __shared__ float sums[8][256 * VEC];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j = blockIdx.x, b = j * CHUNK, e = b + CHUNK;
   if (e >= n) return;
@@ -480,34 +480,45 @@ join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ part, T
     for (int i = 0; i < VEC; ++i) gw[(int64_t)key * D + c + i] = from_f32<T>(s[i] * scale);
     return;
   }
-  for (int t = 0; t < 8; ++t) {
-    const int64_t c = (((int64_t)blockIdx.y * 8 + t) * 32 + lane) * VEC;
-    float s[VEC];
+  // a warp's parts: of 8 x 32 vectors two at a time, of narrow rows' 32 eight
+  const int64_t c0 = ((int64_t)blockIdx.y * 256 + lane) * VEC;
+  auto share = [&](auto tiles, auto parts) {
+    constexpr int TILES = decltype(tiles)::value, PARTS = decltype(parts)::value;
+    float s[TILES][VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) s[k] = 0.f;
-    if (c < D) {
-      if (warp == 0) load_vec<float, VEC>(first + c, s);
-#pragma unroll 8
-      for (int64_t k = j + 1 + warp; k < lo; k += 8) {
-        float v[VEC];
-        load_vec<float, VEC>(part + k * 2 * D + c, v);
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) s[i] += v[i];
-      }
-    }
+      for (int i = 0; i < VEC; ++i) s[t][i] = 0.f;
+    auto add = [&](const float* p) {
+      float v[TILES][VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) sums[warp][lane][i] = s[i];
-    __syncthreads();
-    if (warp == 0 && c < D) {
+      for (int t = 0; t < TILES; ++t)
+        if (c0 + t * 32 * VEC < D) load_vec<float, VEC>(p + c0 + t * 32 * VEC, v[t]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        s[i] = 0.f;
+      for (int t = 0; t < TILES; ++t)
+        if (c0 + t * 32 * VEC < D) {
 #pragma unroll
-        for (int w = 0; w < 8; ++w) s[i] += sums[w][lane][i];
-        gw[(int64_t)key * D + c + i] = from_f32<T>(s[i] * scale);
-      }
-    }
-    __syncthreads();
+          for (int i = 0; i < VEC; ++i) s[t][i] += v[t][i];
+        }
+    };
+    if (warp == 0) add(first);
+#pragma unroll PARTS
+    for (int64_t k = j + 1 + warp; k < lo; k += 8) add(part + k * 2 * D);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sums[warp][(t * 32 + lane) * VEC + i] = s[t][i];
+  };
+  if (D <= 32 * VEC) share(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+  else share(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+  __syncthreads();
+  for (int x = threadIdx.x; x < 256 * VEC; x += 256) {
+    const int64_t c = (int64_t)blockIdx.y * 256 * VEC + x;
+    if (c >= D) break;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) sum += sums[w][x];
+    gw[(int64_t)key * D + c] = from_f32<T>(sum * scale);
   }
 }
 
