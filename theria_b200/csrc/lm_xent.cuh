@@ -17,6 +17,14 @@
 namespace theria {
 namespace xent {
 
+// The split of dh's contraction over a piece of the vocabulary: parts of
+// `split_kb` k blocks, `acc_rows` rows of float32 partial sums for each.
+struct Splits {
+  int split_kb, acc_rows, splits;
+};
+constexpr int CLUSTERS = 74, TILE_ROWS = 256;
+constexpr int MAX_UNITS = 8 * CLUSTERS;  // split * tiles, where more than one split
+
 // What prep_kernel fills, and what it fills it from.
 struct Prep {
   const void* target;
@@ -31,6 +39,9 @@ struct Prep {
   const float *gloss, *lse_in, *mean_of;
   int per_row, half;
   float *lse_p, *rowscale, *post;
+  // the tensor cores' dh: how its contraction is split (see plan_splits)
+  Splits* plan;
+  int kb, d_tiles, pairs, ld_acc;
 };
 
 // float16 holds dz in units of 1 / 32768 of the largest row's factor, so that
@@ -42,6 +53,51 @@ constexpr float HALF_SCALE = 32768.f;
 // it, and after a scan over the warps numbers it; 8 loads of 32 rows are in
 // flight at a time (8192 rows: 4.5 us, against 18.8 for a thread per run).
 constexpr int PREP_BATCH = 8;
+
+// Splits dh's contraction where whole 256 x 256 tiles of the rows that count
+// would leave clusters idle.  Cost in k blocks (0.28 us): the longest cluster's
+// share with 8 for each unit's start and end, and the partials' traffic (written
+// and read, at 6.5 TB/s).  All 1024 threads; the least cost wins, then the
+// fewest splits.
+__device__ __forceinline__ void plan_splits(const Prep& a, int live) {
+  __shared__ float cost[32];
+  __shared__ int which[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rows = (live > 0 ? (live + TILE_ROWS - 1) / TILE_ROWS : 1) * TILE_ROWS;
+  const int tiles = rows / TILE_ROWS * a.d_tiles;
+  float best = INFINITY;
+  int per = a.kb;
+  const int s = threadIdx.x + 1;
+  if (s == 1 || (s <= a.kb && (int64_t)s * tiles <= MAX_UNITS)) {
+    per = (a.kb + s - 1) / s;
+    const int n = (a.kb + per - 1) / per;
+    best = (float)((n * (int64_t)tiles + CLUSTERS - 1) / CLUSTERS) * (float)(per * a.pairs + 8) +
+           (float)n * (float)rows * (float)a.ld_acc * (8.f / 6.5e12f / 0.28e-6f);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {  // the lower thread's on a tie
+    const float c = __shfl_xor_sync(0xffffffffu, best, o);
+    const int p = __shfl_xor_sync(0xffffffffu, per, o);
+    if (c < best || (c == best && p > per)) {
+      best = c;
+      per = p;
+    }
+  }
+  if (lane == 0) {
+    cost[warp] = best;
+    which[warp] = per;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w)
+      if (cost[w] < best) {
+        best = cost[w];
+        per = which[w];
+      }
+    *a.plan = Splits{per, rows, (a.kb + per - 1) / per};
+  }
+}
+
 __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
   __shared__ int part[32];
   __shared__ float peak[32];
@@ -114,6 +170,7 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
       }
     }
   }
+  if (a.plan) plan_splits(a, total);
   if (threadIdx.x == 0) {
     *a.n_live = total;
     if (a.done) *a.done = 0;

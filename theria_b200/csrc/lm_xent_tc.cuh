@@ -22,6 +22,7 @@
 
 #include "common.cuh"
 #include "lm_embed.cuh"
+#include "lm_xent.cuh"
 #include "tc_common.cuh"
 
 namespace theria {
@@ -46,7 +47,7 @@ struct TcArgs {
   int c0, Cn;           // piece of the vocabulary (kDz, kDh, kDw): start, columns
   int pairs;            // plane pairs: 1 (16-bit operands) or 6 (float32)
   int plane_a, plane_b; // elements between planes of one row
-  int splits, split_kb; // kDh: splits of the contraction, k blocks in each
+  const Splits* plan;   // kDh
   int add;              // kDh: add to what the partials hold (a later piece)
   int rows;             // all rows; if every one counts, A (B for kDw) is h itself, unpacked
   int h_plain;          // ... where h can be read as it is
@@ -57,8 +58,7 @@ struct TcArgs {
   const float* lse;     // kDz, by packed row
   const float* rowscale;
   int ld_dz;            // kDz: dz is [row][planes][ld_dz]
-  int acc_rows;         // kDh: [split][acc_rows][ld_acc] partial sums
-  int ld_acc;
+  int ld_acc;           // kDh: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
   const float* post;    // kDw: the factor of the result
 };
@@ -138,11 +138,12 @@ struct Unit {
 
 template <int EPI>
 struct Sched {
-  int mt, nt, kb, units, splits, split_kb;
+  int mt, nt, kb, units, splits, split_kb, acc_rows;
   __device__ explicit Sched(const TcArgs& a) {
     const int live = *a.n_live;
     const int rows = (live + BM - 1) / BM > 0 ? (live + BM - 1) / BM : 1;
     splits = 1;
+    acc_rows = 0;
     if (EPI == kScore || EPI == kDz) {
       mt = rows;
       nt = ((EPI == kScore ? a.V : a.Cn) + BN - 1) / BN;
@@ -151,13 +152,14 @@ struct Sched {
       mt = rows;
       nt = (a.D + BN - 1) / BN;
       kb = (a.Cn + BK - 1) / BK;
-      splits = a.splits;
+      acc_rows = a.plan->acc_rows;
     } else {
       mt = (a.Cn + BM - 1) / BM;
       nt = (a.D + BN - 1) / BN;
       kb = live > 0 ? (live + BK - 1) / BK : 1;
     }
-    split_kb = EPI == kDh ? a.split_kb : kb;
+    split_kb = EPI == kDh ? a.plan->split_kb : kb;
+    if (EPI == kDh) splits = (kb + split_kb - 1) / split_kb;
     units = mt * nt * splits;
   }
   // Tiles in groups of 8 rows of tiles, so that the clusters at work at one
@@ -446,7 +448,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           if (n >= args.ld_acc) return;
           stage_free();
           stage32<float>(out_row, lane, v, 0);
-          stage_full(n, un.split * args.acc_rows + m_warp);
+          stage_full(n, un.split * sched.acc_rows + m_warp);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= post;
@@ -586,9 +588,11 @@ pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
 template <typename O, int VEC>
 __global__ void __launch_bounds__(256)
 dh_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
-              const float* __restrict__ post, int splits, int64_t acc_rows, int ld_acc,
+              const float* __restrict__ post, const Splits* __restrict__ plan, int ld_acc,
               O* __restrict__ dh, int64_t N, int D) {
   const float f = *post;
+  const int splits = plan->splits;
+  const int64_t acc_rows = plan->acc_rows;
   const int units = D / VEC;
   for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
     const int m = pos[i];

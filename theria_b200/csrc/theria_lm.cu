@@ -451,6 +451,7 @@ struct XentRows {  // filled by prep_kernel
   int *pos, *row_of, *tgt, *n_live;
   unsigned* done;
   float *lse, *rowscale, *post;  // backward
+  xent::Splits* plan;
 };
 XentRows xent_rows(Carver& c, int64_t N) {
   XentRows r;
@@ -462,6 +463,7 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.n_live = c.take<int>(64);  // and what else is one value
   r.done = (unsigned*)r.n_live + 1;
   r.post = (float*)r.n_live + 2;
+  r.plan = (xent::Splits*)(r.n_live + 4);
   return r;
 }
 xent::Prep xent_prep(const XentRows& r, const void* target, int wide, int64_t ignore_index,
@@ -522,7 +524,8 @@ XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V) {
 }
 
 // ------------------------------------------------------- tensor-core path
-constexpr int kClusters = kSMs / 2;
+constexpr int kClusters = xent::CLUSTERS;
+static_assert(kClusters == kSMs / 2 && xent::BM == xent::TILE_ROWS, "dh's split");
 
 // Problems this small run on CUDA cores in fewer launches.
 bool xent_small(int64_t N, int64_t V, int64_t D) { return N * V * D <= (1ll << 24); }
@@ -532,7 +535,7 @@ struct TcSizes {
   int planes;
   bool pack_w;             // w needs a packed copy
   int64_t piece;           // of the vocabulary, backward
-  int64_t ld_acc, split_kb, splits;
+  int64_t ld_acc, acc_rows;  // dh's partial sums: at most these rows
 };
 TcSizes tc_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
   TcSizes z;
@@ -544,24 +547,8 @@ TcSizes tc_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
   const int64_t fit = (512ll << 20) / (z.Mp * 2 * z.planes) / xent::BN * xent::BN;
   z.piece = std::min(up(V, xent::BN), std::max<int64_t>(xent::BN, fit));
   z.ld_acc = up(D, 32);
-  // dh: the contraction over the piece is split where whole tiles would leave
-  // clusters idle.  Cost in k blocks (0.28 us): the longest cluster's share
-  // with 8 for each unit's start and end, and the partials' traffic.
-  const int64_t tiles = z.Mp / xent::BM * cdiv(D, xent::BN), kb = cdiv(z.piece, xent::BK);
-  const int pairs = z.planes > 1 ? 6 : 1;
-  double best = 1e30;
-  z.splits = 1;
-  z.split_kb = kb;
-  for (int64_t s = 1; s <= std::min<int64_t>(kClusters, kb); ++s) {
-    const int64_t per = cdiv(kb, s), n = cdiv(kb, per);
-    const double cost = (double)cdiv(tiles * n, kClusters) * (per * pairs + 8) +
-                        (double)n * z.Mp * z.ld_acc * 8 / 6.5e12 / 0.28e-6;
-    if (cost < best) {
-      best = cost;
-      z.splits = n;
-      z.split_kb = per;
-    }
-  }
+  z.acc_rows = std::max(z.Mp, std::min(xent::MAX_UNITS / cdiv(D, xent::BN) * xent::BM,
+                                       cdiv(z.piece, xent::BK) * z.Mp));
   return z;
 }
 
@@ -597,7 +584,7 @@ TcBwdWs tc_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z)
   w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
   w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
   w.dz = c.take<uint16_t>(z.Mp * z.piece * z.planes);
-  w.acc = c.take<float>(z.splits * z.Mp * z.ld_acc);
+  w.acc = c.take<float>(z.acc_rows * z.ld_acc);
   w.bytes = c.used;
   return w;
 }
@@ -713,7 +700,7 @@ struct Tc {
         !map_2d(&zk, ws.dz, op, zrow, z.Mp, xent::HALF) ||
         !map_2d(&zm, ws.dz, op, zrow, z.Mp, xent::BK) ||
         !map_2d(&zo, ws.dz, op, zrow, z.Mp, 32, z.planes > 1 ? 64 : 128) ||
-        !map_2d(&ho, ws.acc, THERIA_F32, z.ld_acc, z.splits * z.Mp, 32))
+        !map_2d(&ho, ws.acc, THERIA_F32, z.ld_acc, z.acc_rows, 32))
       return THERIA_ERR_LAUNCH;
     hk1 = hk;
     hm1 = hm;
@@ -731,17 +718,16 @@ struct Tc {
       a.lse = r.lse;
       a.rowscale = r.rowscale;
       a.ld_dz = (int)z.piece;
-      a.acc_rows = (int)z.Mp;
+      a.plan = r.plan;
       a.ld_acc = (int)z.ld_acc;
       a.out = dw_tma ? nullptr : dw;
       a.post = r.post;
-      a.split_kb = (int)z.split_kb;
-      a.splits = (int)cdiv(cdiv(C, xent::BK), z.split_kb);
       a.add = c0 > 0;
       if (int e = tc_launch<T, O, xent::kDz>(hk, wk, hk1, zo, a, mt * ct, st)) return e;
       a.plane_a = (int)z.piece;
       if (dh)
-        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, a, mt * dt * a.splits, st))
+        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, a, std::max<int64_t>(mt * dt, kClusters),
+                                                st))
           return e;
       if (dw)
         if (int e = tc_launch<T, O, xent::kDw>(zm, hm, hm1, wo, a, ct * dt, st)) return e;
@@ -750,7 +736,7 @@ struct Tc {
     constexpr int VEC = embed::Vec<O>::n;
     auto kern = vec_rows(D, dtype, {dh}) ? xent::dh_sum_kernel<O, VEC> : xent::dh_sum_kernel<O, 1>;
     kern<<<(unsigned)std::min<int64_t>(N, kSMs * 16), 256, 0, st>>>(
-        ws.acc, r.pos, r.post, (int)z.splits, z.Mp, (int)z.ld_acc, (O*)dh, N, (int)D);
+        ws.acc, r.pos, r.post, r.plan, (int)z.ld_acc, (O*)dh, N, (int)D);
     return launch_status();
   }
 };
@@ -862,6 +848,13 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   p.lse_p = r.lse;
   p.rowscale = r.rowscale;
   p.post = r.post;
+  if (tensor && dh) {
+    p.plan = r.plan;
+    p.kb = (int)cdiv(std::min(z.piece, V), xent::BK);
+    p.d_tiles = (int)cdiv(D, xent::BN);
+    p.pairs = z.planes > 1 ? 6 : 1;
+    p.ld_acc = (int)z.ld_acc;
+  }
   xent::prep_kernel<<<1, 1024, 0, st>>>(p);
   if (int e = launch_status()) return e;
   if (tensor)
