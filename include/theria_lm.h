@@ -72,8 +72,7 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
  * loss[i] = lse[i] - z[i, target[i]], 0 where target[i] == ignore_index.
  * The scores z are made in tiles and never stored.  A 16-bit w with D a
  * multiple of 8 has to start on a 16-byte boundary (else
- * THERIA_ERR_INVALID_ARG, where the problem is large enough for the
- * tensor-core kernels).
+ * THERIA_ERR_INVALID_ARG).  N, V < 2^30, D < 2^27.
  *   reduction THERIA_LOSS_NONE: loss [N]; _SUM, _MEAN: loss [1], the mean
  *   over the rows that count (NaN if there is none).
  * lse [N] and count [1] (the rows that count, float32) are what the backward

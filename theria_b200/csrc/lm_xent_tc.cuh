@@ -30,7 +30,7 @@ namespace xent {
 
 enum Epi { kScore = 0, kDz = 1, kDh = 2, kDw = 3 };
 
-constexpr int BM = 256, BN = 256, BK = 64;  // of a CTA pair
+constexpr int BM = TILE_ROWS, BN = 256, BK = K_BLOCK;  // of a CTA pair
 constexpr int HALF = 128;                   // rows of A and of B per CTA
 constexpr int SUB = 128;                    // columns per score partial
 constexpr int STAGES = 6;
@@ -47,7 +47,7 @@ struct TcArgs {
   int c0, Cn;           // piece of the vocabulary (kDz, kDh, kDw): start, columns
   int pairs;            // plane pairs: 1 (16-bit operands) or 6 (float32)
   int plane_a, plane_b; // elements between planes of one row
-  const Splits* plan;   // kDh
+  const Splits* plan;   // kDh; kDw where it is split (else NULL)
   int add;              // kDh: add to what the partials hold (a later piece)
   int rows;             // all rows; if every one counts, A (B for kDw) is h itself, unpacked
   int h_plain;          // ... where h can be read as it is
@@ -58,7 +58,7 @@ struct TcArgs {
   const float* lse;     // kDz, by packed row
   const float* rowscale;
   int ld_dz;            // kDz: dz is [row][planes][ld_dz]
-  int ld_acc;           // kDh: [split][plan->acc_rows][ld_acc] partial sums
+  int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
   const float* post;    // kDw: the factor of the result
 };
@@ -152,14 +152,17 @@ struct Sched {
       mt = rows;
       nt = (a.D + BN - 1) / BN;
       kb = (a.Cn + BK - 1) / BK;
-      acc_rows = a.plan->acc_rows;
     } else {
       mt = (a.Cn + BM - 1) / BM;
       nt = (a.D + BN - 1) / BN;
       kb = live > 0 ? (live + BK - 1) / BK : 1;
     }
-    split_kb = EPI == kDh ? a.plan->split_kb : kb;
-    if (EPI == kDh) splits = (kb + split_kb - 1) / split_kb;
+    split_kb = kb;
+    if (EPI == kDh || (EPI == kDw && a.plan)) {
+      split_kb = a.plan->split_kb;
+      acc_rows = a.plan->acc_rows;
+      splits = (kb + split_kb - 1) / split_kb;
+    }
     units = mt * nt * splits;
   }
   // Tiles in groups of 8 rows of tiles, so that the clusters at work at one
@@ -382,6 +385,11 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         rs = args.rowscale[m];
       }
 
+      // Rows past those that count: nothing of them is kept, but dz is zero up
+      // to the end of a k block of dw's contraction over the rows.
+      const bool idle = EPI == kDz ? m_warp >= (live > 0 ? (live + BK - 1) / BK * BK : BK)
+                                   : EPI != kDw && m_warp >= live;
+
       // columns n .. n + 31 of this thread's row; c: their place in the half
       auto take = [&](float (&v)[32], int c) {
         const int n = n0 + c;
@@ -444,12 +452,12 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             stage32<T>(out_row, lane, v, c % 64 / 8);
             if (c % 64 == 32) stage_full(n - 32, m_warp);
           }
-        } else if constexpr (EPI == kDh) {
+        } else if (EPI == kDh || args.plan) {
           if (n >= args.ld_acc) return;
           stage_free();
           stage32<float>(out_row, lane, v, 0);
           stage_full(n, un.split * sched.acc_rows + m_warp);
-        } else {
+        } else if constexpr (EPI == kDw) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= post;
           if (args.out) {
@@ -500,8 +508,10 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           give_back(buf);
         }
         if (!ok) break;
+        if (!idle) {
 #pragma unroll
-        for (int c = 0; c < SUB / 32; ++c) take(acc[c], c * 32);
+          for (int c = 0; c < SUB / 32; ++c) take(acc[c], c * 32);
+        }
       } else {
         const uint32_t buf = n_acc & 1;
         ok = __all_sync(0xffffffffu,
@@ -509,8 +519,9 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (!ok) break;
         ++n_acc;
         tc::tc_fence_after();
+        if (idle) give_back(buf);
 #pragma unroll 1
-        for (int c = 0; c < SUB; c += 32) {
+        for (int c = idle ? SUB : 0; c < SUB; c += 32) {
           float v[32];
           tc::tmem_ld32(src + buf * ACC_COLS + c, v);  // warp-collective
           if (c == SUB - 32) give_back(buf);
@@ -539,25 +550,30 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   }
 }
 
-// dst[m][plane][Kp] = the rows of src (by `row_of`, or all), packed: zeros
-// past D and in the rows n_live .. up to a multiple of BM.  T: the operands'
-// type; O float: three planes.
+// dst[m][plane][Kp] = the rows of src, packed: by `row_of` the n_live rows that
+// count, then zeros up to a multiple of BM; without it all `rows`.  Zeros past D.
+struct PackArgs {
+  const void* src;
+  void* dst;
+  const int *row_of, *n_live;
+  int64_t rows;
+  int vec;    // src's rows can be read 16 bytes at a time
+  int plain;  // where every row counts src is read as it is: nothing to do
+};
+// T: the operands' type; O float: three planes.
 template <typename T, typename O>
-__global__ void __launch_bounds__(256)
-pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
-            const int* __restrict__ n_live, int64_t rows, T* __restrict__ dst, int64_t D,
-            int64_t Kp, int vec, int plain) {
-  const int64_t live = n_live ? *n_live : rows;
-  if (plain && live == rows) return;  // the products read src itself
-  const int64_t end = n_live ? (live > 0 ? (live + BM - 1) / BM * BM : BM) : rows;
+__device__ __forceinline__ void pack_rows(const PackArgs& a, int64_t D, int64_t Kp, int64_t first,
+                                          int64_t step) {
+  const int64_t live = a.n_live ? *a.n_live : a.rows;
+  if (a.plain && live == a.rows) return;
+  const int64_t end = a.n_live ? (live > 0 ? (live + BM - 1) / BM * BM : BM) : a.rows;
   constexpr int planes = sizeof(O) == 4 ? 3 : 1;
   const int64_t units = Kp / 8;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < end * units;
-       e += (int64_t)gridDim.x * 256) {
+  for (int64_t e = first; e < end * units; e += step) {
     const int64_t m = e / units, k = (e - m * units) * 8;
-    const O* s = src + (m < live ? (row_of ? row_of[m] : m) : 0) * D + k;
+    const O* s = (const O*)a.src + (m < live ? (a.row_of ? a.row_of[m] : m) : 0) * D + k;
     __align__(16) O x[8];
-    if (m < live && vec && k + 8 <= D) {
+    if (m < live && a.vec && k + 8 <= D) {
 #pragma unroll
       for (int i = 0; i < (int)sizeof(O) / 2; ++i)
         reinterpret_cast<uint4*>(x)[i] = reinterpret_cast<const uint4*>(s)[i];
@@ -565,7 +581,7 @@ pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = m < live && k + i < D ? s[i] : from_f32<O>(0.f);
     }
-    T* d = dst + m * planes * Kp + k;
+    T* d = (T*)a.dst + m * planes * Kp + k;
     if constexpr (sizeof(O) == 4) {
       __nv_bfloat16 p[8][3];
 #pragma unroll
@@ -582,20 +598,31 @@ pack_kernel(const O* __restrict__ src, const int* __restrict__ row_of,
     }
   }
 }
+// h in the first `h_ctas` CTAs, w in the others (none where w is read as it is).
+template <typename T, typename O>
+__global__ void __launch_bounds__(256)
+pack_kernel(const PackArgs h, const PackArgs w, int h_ctas, int64_t D, int64_t Kp) {
+  const int b = blockIdx.x;
+  if (b < h_ctas)
+    pack_rows<T, O>(h, D, Kp, (int64_t)b * 256 + threadIdx.x, (int64_t)h_ctas * 256);
+  else
+    pack_rows<T, O>(w, D, Kp, (int64_t)(b - h_ctas) * 256 + threadIdx.x,
+                    (int64_t)(gridDim.x - h_ctas) * 256);
+}
 
-// dh[i] = post * the sum of the splits' partials of row pos[i], or zeros.
-// VEC values a thread.
+// out[i] = post * the sum of the splits' partials of row pos[i] (i itself
+// without `pos`), or zeros.  VEC values a thread.
 template <typename O, int VEC>
 __global__ void __launch_bounds__(256)
-dh_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
+split_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
               const float* __restrict__ post, const Splits* __restrict__ plan, int ld_acc,
-              O* __restrict__ dh, int64_t N, int D) {
+              O* __restrict__ out, int64_t N, int D) {
   const float f = *post;
   const int splits = plan->splits;
   const int64_t acc_rows = plan->acc_rows;
   const int units = D / VEC;
   for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
-    const int m = pos[i];
+    const int64_t m = pos ? pos[i] : i;
     for (int u = threadIdx.x; u < units; u += 256) {
       float s[VEC];
 #pragma unroll
@@ -620,7 +647,7 @@ dh_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
       }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) s[k] *= f;
-      embed::store_vec<O, VEC>(dh + i * D + u * VEC, s);
+      embed::store_vec<O, VEC>(out + i * D + u * VEC, s);
     }
   }
 }

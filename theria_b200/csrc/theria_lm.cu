@@ -442,7 +442,7 @@ namespace {
 int xent_check(int64_t N, int64_t V, int64_t D, int dtype, int reduction) {
   if (N < 0 || V <= 0 || D <= 0 || !lm_dtype(dtype)) return THERIA_ERR_INVALID_ARG;
   if (reduction < THERIA_LOSS_NONE || reduction > THERIA_LOSS_MEAN) return THERIA_ERR_INVALID_ARG;
-  if (N > 65535ll * xent::TM || V > 65535ll * xent::TN || D >= (1ll << 31))
+  if (N >= (1ll << 30) || V >= (1ll << 30) || D >= (1ll << 27))
     return THERIA_ERR_UNSUPPORTED;
   return THERIA_OK;
 }
@@ -451,7 +451,7 @@ struct XentRows {  // filled by prep_kernel
   int *pos, *row_of, *tgt, *n_live;
   unsigned* done;
   float *lse, *rowscale, *post;  // backward
-  xent::Splits* plan;
+  xent::Splits *plan_h, *plan_w;
 };
 XentRows xent_rows(Carver& c, int64_t N) {
   XentRows r;
@@ -463,7 +463,8 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.n_live = c.take<int>(64);  // and what else is one value
   r.done = (unsigned*)r.n_live + 1;
   r.post = (float*)r.n_live + 2;
-  r.plan = (xent::Splits*)(r.n_live + 4);
+  r.plan_h = (xent::Splits*)(r.n_live + 4);
+  r.plan_w = r.plan_h + 1;
   return r;
 }
 xent::Prep xent_prep(const XentRows& r, const void* target, int wide, int64_t ignore_index,
@@ -492,53 +493,22 @@ int xent_join(const XentRows& r, const float2* part, const float* zt, int tiles,
       part, zt, r.row_of, r.n_live, tiles, o.each, o.lse, r.done, o.out, o.mean, N);
   return launch_status();
 }
-// --------------------------------------------------------- CUDA-core path
-struct XentFwdWs {
-  XentRows rows;
-  float2* part;
-  float *zt, *each;
-  int64_t bytes;
-};
-XentFwdWs xent_fwd_ws(void* base, int64_t N, int64_t V) {
-  Carver c{(char*)base};
-  XentFwdWs w;
-  w.rows = xent_rows(c, N);
-  w.part = c.take<float2>(N * cdiv(V, xent::TN));
-  w.zt = c.take<float>(N);
-  w.each = c.take<float>(N);
-  w.bytes = c.used;
-  return w;
-}
-struct XentBwdWs {
-  XentRows rows;
-  float* dz;
-  int64_t bytes;
-};
-XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V) {
-  Carver c{(char*)base};
-  XentBwdWs w;
-  w.rows = xent_rows(c, N);
-  w.dz = c.take<float>(N * V);
-  w.bytes = c.used;
-  return w;
-}
-
-// ------------------------------------------------------- tensor-core path
 constexpr int kClusters = xent::CLUSTERS;
 static_assert(kClusters == kSMs / 2 && xent::BM == xent::TILE_ROWS, "dh's split");
 
-// Problems this small run on CUDA cores in fewer launches.
-bool xent_small(int64_t N, int64_t V, int64_t D) { return N * V * D <= (1ll << 24); }
-
-struct TcSizes {
+struct XentSizes {
   int64_t Mp, Kp;          // packed rows, elements of a packed row (one plane)
   int planes;
   bool pack_w;             // w needs a packed copy
   int64_t piece;           // of the vocabulary, backward
   int64_t ld_acc, acc_rows;  // dh's partial sums: at most these rows
+  // dw is split over the rows that count (and made by partial sums) where it has
+  // no more tiles than half the clusters; its partial sums' rows
+  bool split_w;
+  int64_t acc_rows_w;
 };
-TcSizes tc_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
-  TcSizes z;
+XentSizes xent_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
+  XentSizes z;
   z.Mp = up(N, xent::BM);
   z.Kp = up(D, xent::BK);
   z.planes = dtype == THERIA_F32 ? 3 : 1;
@@ -549,19 +519,22 @@ TcSizes tc_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
   z.ld_acc = up(D, 32);
   z.acc_rows = std::max(z.Mp, std::min(xent::MAX_UNITS / cdiv(D, xent::BN) * xent::BM,
                                        cdiv(z.piece, xent::BK) * z.Mp));
+  const int64_t vt = cdiv(V, xent::BM), dt = cdiv(D, xent::BN);
+  z.split_w = vt * dt * 2 <= kClusters && z.piece >= V;
+  z.acc_rows_w = std::max(vt, std::min(xent::MAX_UNITS_DW / dt, cdiv(N, xent::BK) * vt)) * xent::BM;
   return z;
 }
 
-struct TcFwdWs {
+struct XentFwdWs {
   XentRows rows;
   void *hp, *wp;
   float2* part;
   float *zt, *each;
   int64_t bytes;
 };
-TcFwdWs tc_fwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z) {
+XentFwdWs xent_fwd_ws(void* base, int64_t N, int64_t V, int64_t D, const XentSizes& z) {
   Carver c{(char*)base};
-  TcFwdWs w;
+  XentFwdWs w;
   w.rows = xent_rows(c, N);
   w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
   w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
@@ -571,20 +544,21 @@ TcFwdWs tc_fwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z)
   w.bytes = c.used;
   return w;
 }
-struct TcBwdWs {
+struct XentBwdWs {
   XentRows rows;
   void *hp, *wp, *dz;
-  float* acc;
+  float *acc, *acc_w;
   int64_t bytes;
 };
-TcBwdWs tc_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const TcSizes& z) {
+XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const XentSizes& z) {
   Carver c{(char*)base};
-  TcBwdWs w;
+  XentBwdWs w;
   w.rows = xent_rows(c, N);
   w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
   w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
   w.dz = c.take<uint16_t>(z.Mp * z.piece * z.planes);
   w.acc = c.take<float>(z.acc_rows * z.ld_acc);
+  w.acc_w = z.split_w ? c.take<float>(z.acc_rows_w * z.ld_acc) : nullptr;
   w.bytes = c.used;
   return w;
 }
@@ -622,27 +596,41 @@ int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& h,
   return launch_status();
 }
 
-template <typename T, typename O>
-int tc_pack(const void* src, const int* row_of, const int* n_live, int64_t rows, void* dst,
-            int64_t D, int64_t Kp, bool plain, cudaStream_t st) {
-  const int dtype = std::is_same<O, float>::value ? THERIA_F32 : THERIA_F16;
-  const int64_t threads = (n_live ? up(rows, xent::BM) : rows) * (Kp / 8);
-  xent::pack_kernel<T, O><<<(unsigned)std::min<int64_t>(cdiv(threads, 256), kSMs * 32), 256, 0,
-                            st>>>((const O*)src, row_of, n_live, rows, (T*)dst, D, Kp,
-                                  vec_rows(D, dtype, {src}), plain);
-  return launch_status();
-}
-
 // T: the operands' type; O: the tensors'.
 template <typename T, typename O>
 struct Tc {
   static constexpr int op = std::is_same<T, __half>::value ? THERIA_F16 : THERIA_BF16;
 
   // h can be read by TMA as it is (where every row counts)
-  static bool plain(const void* h, int64_t D, const TcSizes& z) {
+  static bool plain(const void* h, int64_t D, const XentSizes& z) {
     return z.planes == 1 && D % 8 == 0 && tc::aligned16(h);
   }
-  static xent::TcArgs common(const void* h, const XentRows& r, const TcSizes& z, int64_t N,
+  // h (the rows that count) and, where it is not read as it is, w
+  static int pack(const void* h, const void* w, const XentRows& r, void* hp, void* wp,
+                  const XentSizes& z, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
+    const int dtype = std::is_same<O, float>::value ? THERIA_F32 : op;
+    const int64_t units = z.Kp / 8;
+    auto ctas = [&](int64_t rows) {
+      return (int)std::min<int64_t>(cdiv(rows * units, 256), kSMs * 16);
+    };
+    const xent::PackArgs ph{h, hp, r.row_of, r.n_live, N, vec_rows(D, dtype, {h}), plain(h, D, z)};
+    const xent::PackArgs pw{w, wp, nullptr, nullptr, V, vec_rows(D, dtype, {w}), 0};
+    const int h_ctas = ctas(z.Mp), w_ctas = z.pack_w ? ctas(V) : 0;
+    xent::pack_kernel<T, O><<<h_ctas + w_ctas, 256, 0, st>>>(ph, pw, h_ctas, D, z.Kp);
+    return launch_status();
+  }
+  // out [rows][D] from the partial sums
+  static int sum(const float* acc, const int* pos, const float* post, const xent::Splits* plan,
+                 const XentSizes& z, void* out, int64_t rows, int64_t D, cudaStream_t st) {
+    constexpr int VEC = embed::Vec<O>::n;
+    const int dtype = std::is_same<O, float>::value ? THERIA_F32 : op;
+    auto kern = vec_rows(D, dtype, {out}) ? xent::split_sum_kernel<O, VEC>
+                                          : xent::split_sum_kernel<O, 1>;
+    kern<<<(unsigned)std::min<int64_t>(rows, kSMs * 16), 256, 0, st>>>(
+        acc, pos, post, plan, (int)z.ld_acc, (O*)out, rows, (int)D);
+    return launch_status();
+  }
+  static xent::TcArgs common(const void* h, const XentRows& r, const XentSizes& z, int64_t N,
                              int64_t V, int64_t D) {
     xent::TcArgs a{};
     a.n_live = r.n_live;
@@ -656,13 +644,10 @@ struct Tc {
     return a;
   }
 
-  static int fwd(const void* h, const void* w, const TcFwdWs& ws, const TcSizes& z,
+  static int fwd(const void* h, const void* w, const XentFwdWs& ws, const XentSizes& z,
                  const LossOut& out, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
     xent::TcArgs a = common(h, ws.rows, z, N, V, D);
-    if (int e = tc_pack<T, O>(h, ws.rows.row_of, ws.rows.n_live, N, ws.hp, D, z.Kp, a.h_plain, st))
-      return e;
-    if (z.pack_w)
-      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, false, st)) return e;
+    if (int e = pack(h, w, ws.rows, ws.hp, ws.wp, z, N, V, D, st)) return e;
     const int64_t row = z.Kp * z.planes;
     CUtensorMap ma, mb, mh;
     if (!map_2d(&ma, ws.hp, op, row, z.Mp, xent::HALF) ||
@@ -679,18 +664,15 @@ struct Tc {
     return xent_join(ws.rows, ws.part, ws.zt, a.sub_tiles, out, N, st);
   }
 
-  static int bwd(const void* h, const void* w, const TcBwdWs& ws, const TcSizes& z, void* dh,
+  static int bwd(const void* h, const void* w, const XentBwdWs& ws, const XentSizes& z, void* dh,
                  void* dw, int64_t N, int64_t V, int64_t D, int dtype, cudaStream_t st) {
     const XentRows& r = ws.rows;
     const xent::TcArgs base = common(h, r, z, N, V, D);
-    if (int e = tc_pack<T, O>(h, r.row_of, r.n_live, N, ws.hp, D, z.Kp, base.h_plain, st))
-      return e;
-    if (z.pack_w)
-      if (int e = tc_pack<T, O>(w, nullptr, nullptr, V, ws.wp, D, z.Kp, false, st)) return e;
+    if (int e = pack(h, w, r, ws.hp, ws.wp, z, N, V, D, st)) return e;
     const int64_t row = z.Kp * z.planes, zrow = z.piece * z.planes;
     const void* wsrc = z.pack_w ? ws.wp : w;
     const int64_t wrow = z.pack_w ? row : D;
-    const bool dw_tma = dw && vec_rows(D, dtype, {dw});
+    const bool dw_tma = dw && (z.split_w || vec_rows(D, dtype, {dw}));
     // contraction along the row (k) or across rows (m); outputs (o)
     CUtensorMap hk, hm, hk1, hm1, wk, wm, zk, zm, zo, ho, wo;
     if (!map_2d(&hk, ws.hp, op, row, z.Mp, xent::HALF) ||
@@ -708,7 +690,10 @@ struct Tc {
     if (base.h_plain && (!map_2d(&hk1, h, op, D, N, xent::HALF) ||
                          !map_2d(&hm1, h, op, D, N, xent::BK)))
       return THERIA_ERR_LAUNCH;
-    if (dw_tma && !map_2d(&wo, dw, dtype, D, V, 32)) return THERIA_ERR_LAUNCH;
+    if (dw_tma && !(z.split_w
+                        ? map_2d(&wo, ws.acc_w, THERIA_F32, z.ld_acc, z.acc_rows_w, 32)
+                        : map_2d(&wo, dw, dtype, D, V, 32)))
+      return THERIA_ERR_LAUNCH;
     const int64_t mt = z.Mp / xent::BM, dt = cdiv(D, xent::BN);
     for (int64_t c0 = 0; c0 < V; c0 += z.piece) {
       const int64_t C = std::min(z.piece, V - c0), ct = cdiv(C, xent::BN);
@@ -718,7 +703,7 @@ struct Tc {
       a.lse = r.lse;
       a.rowscale = r.rowscale;
       a.ld_dz = (int)z.piece;
-      a.plan = r.plan;
+      a.plan = r.plan_h;
       a.ld_acc = (int)z.ld_acc;
       a.out = dw_tma ? nullptr : dw;
       a.post = r.post;
@@ -729,15 +714,15 @@ struct Tc {
         if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, a, std::max<int64_t>(mt * dt, kClusters),
                                                 st))
           return e;
-      if (dw)
-        if (int e = tc_launch<T, O, xent::kDw>(zm, hm, hm1, wo, a, ct * dt, st)) return e;
+      if (!dw) continue;
+      a.plan = z.split_w ? r.plan_w : nullptr;
+      if (int e = tc_launch<T, O, xent::kDw>(
+              zm, hm, hm1, wo, a, z.split_w ? kClusters : ct * dt, st))
+        return e;
     }
-    if (!dh) return THERIA_OK;
-    constexpr int VEC = embed::Vec<O>::n;
-    auto kern = vec_rows(D, dtype, {dh}) ? xent::dh_sum_kernel<O, VEC> : xent::dh_sum_kernel<O, 1>;
-    kern<<<(unsigned)std::min<int64_t>(N, kSMs * 16), 256, 0, st>>>(
-        ws.acc, r.pos, r.post, r.plan, (int)z.ld_acc, (O*)dh, N, (int)D);
-    return launch_status();
+    if (dw && z.split_w)
+      if (int e = sum(ws.acc_w, nullptr, r.post, r.plan_w, z, dw, V, D, st)) return e;
+    return dh ? sum(ws.acc, r.pos, r.post, r.plan_h, z, dh, N, D, st) : (int)THERIA_OK;
   }
 };
 
@@ -754,13 +739,11 @@ extern "C" {
 
 int64_t theria_xent_fwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
-  return xent_small(N, V, D) ? xent_fwd_ws(nullptr, N, V).bytes
-                             : tc_fwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes;
+  return xent_fwd_ws(nullptr, N, V, D, xent_sizes(N, V, D, dtype)).bytes;
 }
 int64_t theria_xent_bwd_workspace_bytes(int64_t N, int64_t V, int64_t D, int dtype) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
-  return xent_small(N, V, D) ? xent_bwd_ws(nullptr, N, V).bytes
-                             : tc_bwd_ws(nullptr, N, V, D, tc_sizes(N, V, D, dtype)).bytes;
+  return xent_bwd_ws(nullptr, N, V, D, xent_sizes(N, V, D, dtype)).bytes;
 }
 
 int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
@@ -783,36 +766,22 @@ int theria_xent_fwd(const void* h, const void* w, const void* target, int wide,
                ? THERIA_OK
                : THERIA_ERR_LAUNCH;
   }
-  const bool tensor = !xent_small(N, V, D);
-  if (tensor && !w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
-  const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
-  TcFwdWs tw;
-  XentFwdWs sw;
-  if (tensor) tw = tc_fwd_ws(workspace, N, V, D, z);
-  else sw = xent_fwd_ws(workspace, N, V);
-  const XentRows& r = tensor ? tw.rows : sw.rows;
-  LossOut out{reduction == THERIA_LOSS_NONE ? loss : tensor ? tw.each : sw.each, lse,
-              reduction == THERIA_LOSS_NONE ? nullptr : loss, reduction == THERIA_LOSS_MEAN};
-  xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
+  if (!w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
+  const XentSizes z = xent_sizes(N, V, D, dtype);
+  const XentFwdWs ws = xent_fwd_ws(workspace, N, V, D, z);
+  const LossOut out{reduction == THERIA_LOSS_NONE ? loss : ws.each, lse,
+                    reduction == THERIA_LOSS_NONE ? nullptr : loss,
+                    reduction == THERIA_LOSS_MEAN};
+  xent::Prep p = xent_prep(ws.rows, target, wide, ignore_index, N, V);
   p.count = count;
   p.loss = out.each;
   p.lse = lse;
   xent::prep_kernel<<<1, 1024, 0, st>>>(p);
   if (int e = launch_status()) return e;
-  if (tensor)
-    return dtype == THERIA_F32   ? Tc<__nv_bfloat16, float>::fwd(h, w, tw, z, out, N, V, D, st)
-           : dtype == THERIA_F16 ? Tc<__half, __half>::fwd(h, w, tw, z, out, N, V, D, st)
-                                 : Tc<__nv_bfloat16, __nv_bfloat16>::fwd(h, w, tw, z, out, N, V, D,
-                                                                         st);
-  const int tiles = (int)cdiv(V, xent::TN);
-  const int e = by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    xent::score_kernel<T><<<dim3((unsigned)tiles, (unsigned)cdiv(N, xent::TM)), 256, 0, st>>>(
-        (const T*)h, (const T*)w, r.row_of, r.tgt, r.n_live, sw.part, sw.zt, V, D);
-    return launch_status();
-  });
-  if (e) return e;
-  return xent_join(r, sw.part, sw.zt, tiles, out, N, st);
+  return dtype == THERIA_F32   ? Tc<__nv_bfloat16, float>::fwd(h, w, ws, z, out, N, V, D, st)
+         : dtype == THERIA_F16 ? Tc<__half, __half>::fwd(h, w, ws, z, out, N, V, D, st)
+                               : Tc<__nv_bfloat16, __nv_bfloat16>::fwd(h, w, ws, z, out, N, V, D,
+                                                                       st);
 }
 
 int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
@@ -831,55 +800,33 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   if (!dh && !dw) return THERIA_OK;
   if (!workspace || workspace_bytes < theria_xent_bwd_workspace_bytes(N, V, D, dtype))
     return THERIA_ERR_WORKSPACE;
-  const bool tensor = !xent_small(N, V, D);
-  if (tensor && !w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
-  const TcSizes z = tensor ? tc_sizes(N, V, D, dtype) : TcSizes{};
-  TcBwdWs tw;
-  XentBwdWs ws;
-  if (tensor) tw = tc_bwd_ws(workspace, N, V, D, z);
-  else ws = xent_bwd_ws(workspace, N, V);
-  const XentRows& r = tensor ? tw.rows : ws.rows;
+  if (!w_readable(w, D, dtype)) return THERIA_ERR_INVALID_ARG;
+  const XentSizes z = xent_sizes(N, V, D, dtype);
+  const XentBwdWs ws = xent_bwd_ws(workspace, N, V, D, z);
+  const XentRows& r = ws.rows;
   xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
   p.gloss = gloss;
   p.lse_in = lse;
   p.mean_of = reduction == THERIA_LOSS_MEAN ? count : nullptr;
   p.per_row = reduction == THERIA_LOSS_NONE;
-  p.half = tensor && dtype == THERIA_F16;
+  p.half = dtype == THERIA_F16;
   p.lse_p = r.lse;
   p.rowscale = r.rowscale;
   p.post = r.post;
-  if (tensor && dh) {
-    p.plan = r.plan;
-    p.kb = (int)cdiv(std::min(z.piece, V), xent::BK);
-    p.d_tiles = (int)cdiv(D, xent::BN);
-    p.pairs = z.planes > 1 ? 6 : 1;
-    p.ld_acc = (int)z.ld_acc;
-  }
+  p.plan_h = dh ? r.plan_h : nullptr;
+  p.plan_w = dw && z.split_w ? r.plan_w : nullptr;
+  p.kb = (int)cdiv(std::min(z.piece, V), xent::BK);
+  p.d_tiles = (int)cdiv(D, xent::BN);
+  p.v_tiles = (int)cdiv(V, xent::BM);
+  p.pairs = z.planes > 1 ? 6 : 1;
+  p.ld_acc = (int)z.ld_acc;
   xent::prep_kernel<<<1, 1024, 0, st>>>(p);
   if (int e = launch_status()) return e;
-  if (tensor)
-    return dtype == THERIA_F32
-               ? Tc<__nv_bfloat16, float>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st)
-           : dtype == THERIA_F16
-               ? Tc<__half, __half>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st)
-               : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, tw, z, dh, dw, N, V, D, dtype, st);
-  const unsigned mt = (unsigned)cdiv(N, xent::TM), dt = (unsigned)cdiv(D, xent::TN),
-                 vt = (unsigned)cdiv(V, xent::TN);
-  return by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    xent::dz_kernel<T><<<dim3(vt, mt), 256, 0, st>>>((const T*)h, (const T*)w, r.row_of, r.tgt,
-                                                     r.n_live, r.lse, r.rowscale, ws.dz, V, D);
-    if (int e = launch_status()) return e;
-    if (dh) {
-      xent::dh_kernel<T><<<dim3(dt, mt), 256, 0, st>>>(ws.dz, (const T*)w, r.pos, r.post, (T*)dh,
-                                                       N, V, D);
-      if (int e = launch_status()) return e;
-    }
-    if (dw)
-      xent::dw_kernel<T><<<dim3(dt, vt), 256, 0, st>>>(ws.dz, (const T*)h, r.row_of, r.n_live,
-                                                       r.post, (T*)dw, V, D);
-    return dw ? launch_status() : THERIA_OK;
-  });
+  return dtype == THERIA_F32
+             ? Tc<__nv_bfloat16, float>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
+         : dtype == THERIA_F16
+             ? Tc<__half, __half>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
+             : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st);
 }
 
 }  // extern "C"
