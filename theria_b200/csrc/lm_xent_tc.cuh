@@ -611,43 +611,54 @@ pack_kernel(const PackArgs h, const PackArgs w, int h_ctas, int64_t D, int64_t K
 }
 
 // out[i] = post * the sum of the splits' partials of row pos[i] (i itself
-// without `pos`), or zeros.  VEC values a thread.
+// without `pos`), or zeros, for dh and dw: the first `a_ctas` CTAs take a, the
+// others b.  VEC values a thread.
+struct SumArgs {
+  const float* acc;
+  const int* pos;
+  const Splits* plan;
+  void* out;
+  int64_t rows;
+};
 template <typename O, int VEC>
 __global__ void __launch_bounds__(256)
-split_sum_kernel(const float* __restrict__ acc, const int* __restrict__ pos,
-              const float* __restrict__ post, const Splits* __restrict__ plan, int ld_acc,
-              O* __restrict__ out, int64_t N, int D) {
+split_sum_kernel(const SumArgs a, const SumArgs b, int a_ctas, const float* __restrict__ post,
+                 int ld_acc, int D) {
+  const bool is_a = (int)blockIdx.x < a_ctas;
+  const SumArgs& s = is_a ? a : b;
+  const int64_t first = is_a ? blockIdx.x : blockIdx.x - a_ctas;
+  const int64_t step = is_a ? a_ctas : (int)gridDim.x - a_ctas;
   const float f = *post;
-  const int splits = plan->splits;
-  const int64_t acc_rows = plan->acc_rows;
+  const int splits = s.plan->splits;
+  const int64_t acc_rows = s.plan->acc_rows;
   const int units = D / VEC;
-  for (int64_t i = blockIdx.x; i < N; i += gridDim.x) {
-    const int64_t m = pos ? pos[i] : i;
+  for (int64_t i = first; i < s.rows; i += step) {
+    const int64_t m = s.pos ? s.pos[i] : i;
     for (int u = threadIdx.x; u < units; u += 256) {
-      float s[VEC];
+      float x[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s[k] = 0.f;
+      for (int k = 0; k < VEC; ++k) x[k] = 0.f;
       if (m >= 0) {
 #pragma unroll 4
         for (int k = 0; k < splits; ++k) {
-          const float* p = acc + (k * acc_rows + m) * ld_acc + u * VEC;
+          const float* p = s.acc + (k * acc_rows + m) * ld_acc + u * VEC;
           if constexpr (VEC == 1) {
-            s[0] += p[0];
+            x[0] += p[0];
           } else {
 #pragma unroll
             for (int q = 0; q < VEC / 4; ++q) {
-              const float4 x = reinterpret_cast<const float4*>(p)[q];
-              s[4 * q] += x.x;
-              s[4 * q + 1] += x.y;
-              s[4 * q + 2] += x.z;
-              s[4 * q + 3] += x.w;
+              const float4 y = reinterpret_cast<const float4*>(p)[q];
+              x[4 * q] += y.x;
+              x[4 * q + 1] += y.y;
+              x[4 * q + 2] += y.z;
+              x[4 * q + 3] += y.w;
             }
           }
         }
       }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s[k] *= f;
-      embed::store_vec<O, VEC>(out + i * D + u * VEC, s);
+      for (int k = 0; k < VEC; ++k) x[k] *= f;
+      embed::store_vec<O, VEC>((O*)s.out + i * D + u * VEC, x);
     }
   }
 }

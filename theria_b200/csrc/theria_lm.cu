@@ -619,15 +619,17 @@ struct Tc {
     xent::pack_kernel<T, O><<<h_ctas + w_ctas, 256, 0, st>>>(ph, pw, h_ctas, D, z.Kp);
     return launch_status();
   }
-  // out [rows][D] from the partial sums
-  static int sum(const float* acc, const int* pos, const float* post, const xent::Splits* plan,
-                 const XentSizes& z, void* out, int64_t rows, int64_t D, cudaStream_t st) {
+  // dh and dw from their partial sums (either may have no rows)
+  static int sum(const xent::SumArgs& a, const xent::SumArgs& b, const float* post,
+                 const XentSizes& z, int64_t D, cudaStream_t st) {
     constexpr int VEC = embed::Vec<O>::n;
     const int dtype = std::is_same<O, float>::value ? THERIA_F32 : op;
-    auto kern = vec_rows(D, dtype, {out}) ? xent::split_sum_kernel<O, VEC>
-                                          : xent::split_sum_kernel<O, 1>;
-    kern<<<(unsigned)std::min<int64_t>(rows, kSMs * 16), 256, 0, st>>>(
-        acc, pos, post, plan, (int)z.ld_acc, (O*)out, rows, (int)D);
+    auto kern = vec_rows(D, dtype, {a.out, b.out}) ? xent::split_sum_kernel<O, VEC>
+                                                   : xent::split_sum_kernel<O, 1>;
+    const int a_ctas = (int)std::min<int64_t>(a.rows, kSMs * 16);
+    const int b_ctas = (int)std::min<int64_t>(b.rows, kSMs * 16);
+    if (a_ctas + b_ctas == 0) return THERIA_OK;
+    kern<<<a_ctas + b_ctas, 256, 0, st>>>(a, b, a_ctas, post, (int)z.ld_acc, (int)D);
     return launch_status();
   }
   static xent::TcArgs common(const void* h, const XentRows& r, const XentSizes& z, int64_t N,
@@ -720,9 +722,8 @@ struct Tc {
               zm, hm, hm1, wo, a, z.split_w ? kClusters : ct * dt, st))
         return e;
     }
-    if (dw && z.split_w)
-      if (int e = sum(ws.acc_w, nullptr, r.post, r.plan_w, z, dw, V, D, st)) return e;
-    return dh ? sum(ws.acc, r.pos, r.post, r.plan_h, z, dh, N, D, st) : (int)THERIA_OK;
+    return sum({ws.acc, r.pos, r.plan_h, dh, dh ? N : 0},
+               {ws.acc_w, nullptr, r.plan_w, dw, dw && z.split_w ? V : 0}, r.post, z, D, st);
   }
 };
 
