@@ -85,6 +85,33 @@ inline int launch_status() {
   return THERIA_ERR_LAUNCH;
 }
 
+// Chained launches of one call: the kernel starts (its prologue, on the SMs that
+// become free) while the one before it in the stream still runs, and waits with
+// grid_wait() before it reads or writes anything; grid_launch() lets the next
+// one start the same way.  What the chain's kernels write for one another is
+// not read through `const __restrict__`, whose loads may be moved up before
+// the wait.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+int launch_chained(void (*kern)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                   A&&... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+  return launch_status();
+}
+
 inline int64_t elem_size(int dtype) { return dtype == THERIA_F32 ? 4 : 2; }
 
 // Device-side error word (one per device that loads the library); a kernel

@@ -101,6 +101,7 @@ __device__ __forceinline__ void plan_splits(Splits* out, int kb, int rows, int t
 }
 
 __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
+  grid_launch();
   __shared__ int part[32];
   __shared__ float peak[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -194,13 +195,12 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
 // per row.  `out` not NULL: the CTA that ends last adds all N rows' losses in
 // a fixed order (mean: over *count).
 __global__ void __launch_bounds__(256)
-join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
-            const int* __restrict__ row_of, const int* __restrict__ n_live, int tiles,
-            float* __restrict__ loss, float* __restrict__ lse, unsigned* __restrict__ done,
-            float* __restrict__ out, int mean, int64_t N) {
+join_kernel(const float2* part, const float* zt, const int* row_of, const int* n_live, int tiles,
+            float* loss, float* lse, unsigned* done, float* out, int mean, int64_t N) {
   __shared__ float warps[8];
   __shared__ bool last;
   const int lane = threadIdx.x & 31;
+  grid_wait();
   const int n = *n_live;
   for (int m = blockIdx.x * 8 + (threadIdx.x >> 5); m < n; m += gridDim.x * 8) {
     const float2* p = part + (int64_t)m * tiles;

@@ -263,6 +263,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   tc::cluster_sync();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_launch();
+  grid_wait();
   const Sched<EPI> sched(args);
   // k blocks per accumulation
   const auto chunk = [](const Unit& un) { return F32 ? F32_CHUNK : un.kbs; };
@@ -603,6 +605,8 @@ template <typename T, typename O>
 __global__ void __launch_bounds__(256)
 pack_kernel(const PackArgs h, const PackArgs w, int h_ctas, int64_t D, int64_t Kp) {
   const int b = blockIdx.x;
+  grid_launch();
+  grid_wait();
   if (b < h_ctas)
     pack_rows<T, O>(h, D, Kp, (int64_t)b * 256 + threadIdx.x, (int64_t)h_ctas * 256);
   else
@@ -622,12 +626,13 @@ struct SumArgs {
 };
 template <typename O, int VEC>
 __global__ void __launch_bounds__(256)
-split_sum_kernel(const SumArgs a, const SumArgs b, int a_ctas, const float* __restrict__ post,
+split_sum_kernel(const SumArgs a, const SumArgs b, int a_ctas, const float* post,
                  int ld_acc, int D) {
   const bool is_a = (int)blockIdx.x < a_ctas;
   const SumArgs& s = is_a ? a : b;
   const int64_t first = is_a ? blockIdx.x : blockIdx.x - a_ctas;
   const int64_t step = is_a ? a_ctas : (int)gridDim.x - a_ctas;
+  grid_wait();
   const float f = *post;
   const int splits = s.plan->splits;
   const int64_t acc_rows = s.plan->acc_rows;

@@ -489,9 +489,9 @@ struct LossOut {
 };
 int xent_join(const XentRows& r, const float2* part, const float* zt, int tiles,
               const LossOut& o, int64_t N, cudaStream_t st) {
-  xent::join_kernel<<<(unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8), 256, 0, st>>>(
-      part, zt, r.row_of, r.n_live, tiles, o.each, o.lse, r.done, o.out, o.mean, N);
-  return launch_status();
+  return launch_chained(xent::join_kernel, dim3((unsigned)std::min<int64_t>(cdiv(N, 8), kSMs * 8)),
+                        dim3(256), 0, st, part, zt, r.row_of, r.n_live, tiles, o.each, o.lse,
+                        r.done, o.out, o.mean, N);
 }
 constexpr int kClusters = xent::CLUSTERS;
 static_assert(kClusters == kSMs / 2 && xent::BM == xent::TILE_ROWS, "dh's split");
@@ -592,8 +592,8 @@ int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& h,
                            xent::TcSmem::kAlloc) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(units, kClusters);
-  kern<<<grid, xent::TC_THREADS, xent::TcSmem::kAlloc, st>>>(a, b, h, o, args);
-  return launch_status();
+  return launch_chained(kern, dim3(grid), dim3(xent::TC_THREADS), xent::TcSmem::kAlloc, st, a, b, h,
+                        o, args);
 }
 
 // T: the operands' type; O: the tensors'.
@@ -616,8 +616,8 @@ struct Tc {
     const xent::PackArgs ph{h, hp, r.row_of, r.n_live, N, vec_rows(D, dtype, {h}), plain(h, D, z)};
     const xent::PackArgs pw{w, wp, nullptr, nullptr, V, vec_rows(D, dtype, {w}), 0};
     const int h_ctas = ctas(z.Mp), w_ctas = z.pack_w ? ctas(V) : 0;
-    xent::pack_kernel<T, O><<<h_ctas + w_ctas, 256, 0, st>>>(ph, pw, h_ctas, D, z.Kp);
-    return launch_status();
+    return launch_chained(xent::pack_kernel<T, O>, dim3(h_ctas + w_ctas), dim3(256), 0, st, ph, pw,
+                          h_ctas, D, z.Kp);
   }
   // dh and dw from their partial sums (either may have no rows)
   static int sum(const xent::SumArgs& a, const xent::SumArgs& b, const float* post,
@@ -629,8 +629,8 @@ struct Tc {
     const int a_ctas = (int)std::min<int64_t>(a.rows, kSMs * 16);
     const int b_ctas = (int)std::min<int64_t>(b.rows, kSMs * 16);
     if (a_ctas + b_ctas == 0) return THERIA_OK;
-    kern<<<a_ctas + b_ctas, 256, 0, st>>>(a, b, a_ctas, post, (int)z.ld_acc, (int)D);
-    return launch_status();
+    return launch_chained(kern, dim3(a_ctas + b_ctas), dim3(256), 0, st, a, b, a_ctas, post,
+                          (int)z.ld_acc, (int)D);
   }
   static xent::TcArgs common(const void* h, const XentRows& r, const XentSizes& z, int64_t N,
                              int64_t V, int64_t D) {
