@@ -462,6 +462,10 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   const int g = threadIdx.x % G, q = threadIdx.x / G;
   const float inv = 1.f / (float)D;
   Ring ring(full, &abort, ring_mem, x, gy, ROWS, stages, N, (int64_t)D * sizeof(T));
+  float wr[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    if ((j * G + g) * VEC < D) affine_vec<T, VEC>(w, wf32, (j * G + g) * VEC, 1.f, wr[j]);
   float aw[NV][VEC], ab[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -481,8 +485,8 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   int before = -1;  // the stage of the batch before, read by every thread at the next barrier
   for (int64_t blk = blockIdx.x; blk < ring.blocks; blk += gridDim.x) {
     ring.wait();
-    const T* sx = reinterpret_cast<const T*>(ring.at(ring.stage)) + (int64_t)q * R * D;
-    const T* sg = sx + (int64_t)ROWS * D;
+    const T* sx = reinterpret_cast<const T*>(ring.at(ring.stage)) + q * R * D;
+    const T* sg = sx + ROWS * D;
     const int64_t r0 = blk * ROWS + q * R;
     float m[R], rs[R], s[2 * R];
 #pragma unroll
@@ -496,19 +500,17 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
       if (c >= D) continue;
-      float wv[VEC];
-      affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         if (r0 + i >= N) continue;
         float h[VEC], u[VEC];
-        load_vec<T, VEC>(sx + (int64_t)i * D + c, h);
-        load_vec<T, VEC>(sg + (int64_t)i * D + c, u);
+        load_vec<T, VEC>(sx + i * D + c, h);
+        load_vec<T, VEC>(sg + i * D + c, u);
         vshift(h, -m[i]);  // in this order: a mean far above the deviations loses nothing
         vscale(h, h, rs[i], 0.f);
         vfma(aw[j], u, h, aw[j]);
         vadd(ab[j], u);
-        vmul(u, wv);
+        vmul(u, wr[j]);
         vsum(su[i], u);
         vdot(sh[i], u, h);
       }
@@ -528,21 +530,18 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
       for (int j = 0; j < NV; ++j) {
         const int c = (j * G + g) * VEC;
         if (c >= D) continue;
-        float wv[VEC];
-        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
           if (r0 + i >= N) continue;
           float h[VEC], u[VEC];
-          load_vec<T, VEC>(sx + (int64_t)i * D + c, h);
-          load_vec<T, VEC>(sg + (int64_t)i * D + c, u);
+          load_vec<T, VEC>(sx + i * D + c, h);
+          load_vec<T, VEC>(sg + i * D + c, u);
           vshift(h, -m[i]);
-          vscale(h, h, rs[i], 0.f);
           // the means first: where they cancel u, they do so before rstd
           // enlarges it
-          vmul(u, wv);
+          vmul(u, wr[j]);
           vshift(u, -s[2 * i] * inv);
-          vaxpy(u, h, -s[2 * i + 1] * inv);
+          vaxpy(u, h, -s[2 * i + 1] * inv * rs[i]);
           vscale(u, u, rs[i], 0.f);
           store_vec<T, VEC>(gx + (r0 + i) * D + c, u);
         }
