@@ -174,75 +174,120 @@ template <int NW> struct Block {
   static constexpr int rows = threads / G; // rows at a time
 };
 
-// One row of the forward in registers: x in v becomes y; the statistics to
-// `stats` (may be NULL).
-template <typename T, int VEC, int NV, int NW>
-__device__ __forceinline__ void fwd_row(float (&v)[NV][VEC], const void* w, const void* b,
-                                        int wf32, float* stats, int64_t N, int64_t r, int D,
-                                        float inv, float eps, float (*red)[32][SUMS], int& turn) {
-  constexpr int G = Block<NW>::G;
-  const int g = threadIdx.x % G;
-  Pair sum, dev, sq;
+// Sums of M values (a power of two) over NW warps.  Each step of the butterfly
+// halves the values a lane keeps, so M sums cost little more than one.
+template <int NW, int M>
+__device__ __forceinline__ void batch_sum(float (&s)[M], float (*red)[32][8], int& turn) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int LANES = 32 / M;  // lanes that end with the same value
+  float t[M];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if ((j * G + g) * VEC < D) vsum(sum, v[j]);
-  float s[1] = {sum.total()};
-  row_sum<NW>(s, red, turn);
-  const float mean = s[0] * inv;
+  for (int i = 0; i < M; ++i) t[i] = s[i];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    if ((j * G + g) * VEC < D) {
-      vshift(v[j], -mean);
-      vdot(sq, v[j], v[j]);
-      vsum(dev, v[j]);
-    }
-  float q[2] = {sq.total(), dev.total()};
-  row_sum<NW>(q, red, turn);
-  // what the rounding of a large mean left in the deviations
-  const float left = q[1] * inv;
-  const float rstd = rsqrtf(fmaxf(q[0] * inv - left * left, 0.f) + eps);
-  const float off = -left * rstd;
+  for (int m = M, o = 16; o > 0; m >>= 1, o >>= 1) {
+    if (m > 1) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * G + g) * VEC;
-    if (c < D) {
-      float wv[VEC], bv[VEC];
-      affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
-      affine_vec<T, VEC>(b, wf32, c, 0.f, bv);
-      vscale(v[j], v[j], rstd, off);
-      vfma(v[j], v[j], wv, bv);
+      for (int i = 0; i < m / 2; ++i) {
+        const bool upper = lane & o;
+        const float give = upper ? t[i] : t[i + m / 2], keep = upper ? t[i + m / 2] : t[i];
+        t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+      }
+    } else {
+      t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
     }
   }
-  if (stats && g == 0) {
-    stats[r] = mean + left;
-    stats[N + r] = rstd;
+  if constexpr (NW > 1) {
+    float (*r)[8] = red[turn];
+    turn ^= 1;
+    if (lane % LANES == 0) r[warp][lane / LANES] = t[0];
+    __syncthreads();
+    t[0] = 0.f;
+#pragma unroll
+    for (int w = 0; w < (NW + LANES - 1) / LANES; ++w)
+      if (w * LANES + lane % LANES < NW) t[0] += r[w * LANES + lane % LANES][lane / LANES];
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
   }
+#pragma unroll
+  for (int i = 0; i < M; ++i) s[i] = __shfl_sync(0xffffffffu, t[0], i * LANES);
 }
 
-// NW warps per row, NV vectors of VEC values per thread; 1024 threads an SM
-// (64 registers), so that as many rows as possible are on their way.
-template <typename T, int VEC, int NV, int NW>
+// NW warps per row, R rows at a time, NV vectors of VEC values of each per
+// thread; the rows go through the reductions together and share the affine
+// values.  1024 threads an SM (64 registers), so that as many rows as possible
+// are on their way.
+template <typename T, int VEC, int NV, int NW, int R>
 __global__ void __launch_bounds__(Block<NW>::threads, 1024 / Block<NW>::threads)
 fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __restrict__ b,
            int wf32, T* __restrict__ y, float* __restrict__ stats, int64_t N, int D, float eps) {
-  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows;
-  __shared__ float red[2][32][SUMS];
+  constexpr int G = Block<NW>::G, ROWS = Block<NW>::rows * R;
+  __shared__ float red[2][32][8];
   int turn = 0;
   const int g = threadIdx.x % G;
   const float inv = 1.f / (float)D;
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
-       r += (int64_t)gridDim.x * ROWS) {
-    float v[NV][VEC];
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS + threadIdx.x / G * R; r0 < N;
+       r0 += (int64_t)gridDim.x * ROWS) {
+    float v[R][NV][VEC];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = (j * G + g) * VEC;
-      if (c < D) load_vec<T, VEC>(x + r * D + c, v[j]);
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * G + g) * VEC;
+        // past the last row: the last one again, not stored
+        if (c < D) load_vec<T, VEC>(x + (r0 + i < N ? r0 + i : N - 1) * D + c, v[i][j]);
+      }
+    float s[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      Pair sum;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if ((j * G + g) * VEC < D) vsum(sum, v[i][j]);
+      s[i] = sum.total();
     }
-    fwd_row<T, VEC, NV, NW>(v, w, b, wf32, stats, N, r, D, inv, eps, red, turn);
+    batch_sum<NW>(s, red, turn);
+    float q[2 * R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      Pair dev, sq;
+      s[i] *= inv;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if ((j * G + g) * VEC < D) {
+          vshift(v[i][j], -s[i]);
+          vdot(sq, v[i][j], v[i][j]);
+          vsum(dev, v[i][j]);
+        }
+      q[2 * i] = sq.total();
+      q[2 * i + 1] = dev.total();
+    }
+    batch_sum<NW>(q, red, turn);
+    float rstd[R], off[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      // what the rounding of a large mean left in the deviations
+      const float left = q[2 * i + 1] * inv;
+      rstd[i] = rsqrtf(fmaxf(q[2 * i] * inv - left * left, 0.f) + eps);
+      off[i] = -left * rstd[i];
+      if (stats && g == 0 && r0 + i < N) {
+        stats[r0 + i] = s[i] + left;
+        stats[N + r0 + i] = rstd[i];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + g) * VEC;
-      if (c < D) store_vec<T, VEC>(y + r * D + c, v[j]);
+      if (c < D) {
+        float wv[VEC], bv[VEC];
+        affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
+        affine_vec<T, VEC>(b, wf32, c, 0.f, bv);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          vscale(v[i][j], v[i][j], rstd[i], off[i]);
+          vfma(v[i][j], v[i][j], wv, bv);
+          if (r0 + i < N) store_vec<T, VEC>(y + (r0 + i) * D + c, v[i][j]);
+        }
+      }
     }
   }
 }
@@ -355,44 +400,6 @@ bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
     }
   }
   if (part) store_part<NW, NV, VEC>(aw, ab, part, D);
-}
-
-// Sums of M values (a power of two) over NW warps.  Each step of the butterfly
-// halves the values a lane keeps, so M sums cost little more than one.
-template <int NW, int M>
-__device__ __forceinline__ void batch_sum(float (&s)[M], float (*red)[32][8], int& turn) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int LANES = 32 / M;  // lanes that end with the same value
-  float t[M];
-#pragma unroll
-  for (int i = 0; i < M; ++i) t[i] = s[i];
-#pragma unroll
-  for (int m = M, o = 16; o > 0; m >>= 1, o >>= 1) {
-    if (m > 1) {
-#pragma unroll
-      for (int i = 0; i < m / 2; ++i) {
-        const bool upper = lane & o;
-        const float give = upper ? t[i] : t[i + m / 2], keep = upper ? t[i + m / 2] : t[i];
-        t[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-      }
-    } else {
-      t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
-    }
-  }
-  if constexpr (NW > 1) {
-    float (*r)[8] = red[turn];
-    turn ^= 1;
-    if (lane % LANES == 0) r[warp][lane / LANES] = t[0];
-    __syncthreads();
-    t[0] = 0.f;
-#pragma unroll
-    for (int w = 0; w < (NW + LANES - 1) / LANES; ++w)
-      if (w * LANES + lane % LANES < NW) t[0] += r[w * LANES + lane % LANES][lane / LANES];
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) t[0] += __shfl_xor_sync(0xffffffffu, t[0], o);
-  }
-#pragma unroll
-  for (int i = 0; i < M; ++i) s[i] = __shfl_sync(0xffffffffu, t[0], i * LANES);
 }
 
 // Blocks of consecutive rows, of x and of gy, in a ring of shared-memory

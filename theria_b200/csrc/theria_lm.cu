@@ -285,13 +285,20 @@ int theria_norm_fwd(const void* x, const void* w, const void* b, int wdtype, voi
     using T = decltype(t);
     auto launch = [&](auto vecn) {
       constexpr int VEC = decltype(vecn)::value;
-      return norm_shape<VEC, kNormFwd>(D, [&](auto nv, auto nw) {
-        constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
+      auto run = [&](auto nv, auto nw, auto rc) {
+        constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value, R = decltype(rc)::value;
         using B = norm::Block<NW>;
-        norm::fwd_kernel<T, VEC, NV, NW>
-            <<<(unsigned)std::min<int64_t>(cdiv(N, B::rows), NW == 1 ? kSMs * 32 : kMaxGrid),
+        norm::fwd_kernel<T, VEC, NV, NW, R>
+            <<<(unsigned)std::min<int64_t>(cdiv(N, B::rows * R), NW == 1 ? kSMs * 32 : kMaxGrid),
                B::threads, 0, st>>>((const T*)x, w, b, wf32, (T*)y, stats, N, (int)D, eps);
-      });
+      };
+      auto four = [&](auto nv, auto nw) { run(nv, nw, std::integral_constant<int, 4>{}); };
+      auto two = [&](auto nv, auto nw) { run(nv, nw, std::integral_constant<int, 2>{}); };
+      auto one = [&](auto nv, auto nw) { run(nv, nw, std::integral_constant<int, 1>{}); };
+      // a warp takes as many rows at a time as make kNormFwd values a lane
+      const int64_t units = cdiv(D, VEC);
+      return norm_vectors<VEC, kNormFwd / 4, 1>(units, four) ||
+             norm_vectors<VEC, kNormFwd / 2, 1>(units, two) || norm_shape<VEC, kNormFwd>(D, one);
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
                           : launch(std::integral_constant<int, 1>{});
