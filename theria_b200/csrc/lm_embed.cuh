@@ -203,8 +203,7 @@ scatter_kernel(const void* __restrict__ ids, int wide, const uint32_t* __restric
 constexpr int CS_THREADS = 1024, CS_BITS = 9, CS_BINS = 1 << CS_BITS, CS_CTAS = 8, CS_MOST = 8;
 
 // The lanes whose d (of `bits` bits) equals this lane's, among `in`: a ballot
-// per bit (match.any takes a step for each value that differs: 2.2 us a round
-// of 32 warps against 0.5).
+// per bit.
 __device__ __forceinline__ uint32_t peers_of(uint32_t d, int bits, uint32_t in) {
   uint32_t same = in;
 #pragma unroll
