@@ -445,15 +445,18 @@ join_kernel(const uint32_t* __restrict__ keys, const float* __restrict__ part, T
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j = blockIdx.x, b = j * CHUNK, e = b + CHUNK;
   if (e >= n) return;
+  const int64_t chunks = (n + CHUNK - 1) / CHUNK;
   const uint32_t key = keys[e - 1], after = keys[e], at_b = keys[b];
   const uint32_t before = b > 0 ? keys[b - 1] : 0xffffffffu;
+  const int64_t ahead = j + 2 + lane;  // the next 32 chunks but one, at the same time
+  const uint32_t probe = ahead < chunks ? keys[ahead * CHUNK] : 0xffffffffu;
   if (key >= (uint32_t)V || after != key) return;
   const bool whole = at_b == key;
   if (whole && before == key) return;  // began earlier
-  // chunks that start within the run: [j + 1, lo), a 32-ary search
-  const int64_t chunks = (n + CHUNK - 1) / CHUNK;
-  int64_t lo = j + 2, hi = chunks;
-  while (lo < hi) {
+  // chunks that start within the run: [j + 1, lo)
+  int64_t lo = j + 2 + __popc(__ballot_sync(0xffffffffu, probe == key)), hi = chunks;
+  if (lo < j + 34) hi = lo;
+  while (lo < hi) {  // a 32-ary search
     const int64_t step = (hi - lo + 31) / 32, p = lo + lane * step;
     const int in = __popc(__ballot_sync(0xffffffffu, p < hi && keys[p * CHUNK] == key));
     if (in == 0) break;

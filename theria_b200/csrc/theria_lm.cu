@@ -346,13 +346,18 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
         if constexpr (VEC > 1) {
           const int64_t row = 2 * D * (int64_t)sizeof(T);  // of x and gy
           if (2 * row <= 200 << 10) {
-            // rows of a batch: 4 for a warp of its own, 2 where that makes
-            // stages of at most 32 KB, else 1
+            // Rows of a batch: 4 for a warp of its own and where they make a
+            // stage of at most 16 KB (65536 x 1024 bfloat16: 80 us, with 2 rows
+            // 86, with one 103), 2 up to 32 KB (16384 x 4096 bfloat16: 93 us,
+            // with one 103, with 4 115), else 1.
             auto batch = [&](auto rc) {
               constexpr int R = decltype(rc)::value;
               auto kern = norm::bwd_batch_kernel<T, VEC, NV, NW, R>;
               const int64_t stage = B::rows * R * row;
-              const int stages = (int)std::clamp<int64_t>((96 << 10) / stage, 2, norm::MAX_STAGES);
+              // float32 rows need more bytes on their way (16384 x 4096: 128 KB
+              // 130 us, 96 KB 143), 16-bit rows a second CTA (93 us, 100)
+              const int64_t ring = (sizeof(T) == 4 ? 128 : 96) << 10;
+              const int stages = (int)std::clamp<int64_t>(ring / stage, 2, norm::MAX_STAGES);
               const int64_t smem = std::max(sums, stage * stages);
               if (smem > 40 << 10)  // with the kernel's static part, above the default limit
                 cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -366,6 +371,7 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
                                                              stages);
             };
             if constexpr (NW == 1) batch(std::integral_constant<int, 4>{});
+            else if (4 * row <= 16 << 10) batch(std::integral_constant<int, 4>{});
             else if (2 * row <= 32 << 10) batch(std::integral_constant<int, 2>{});
             else batch(std::integral_constant<int, 1>{});
             return;
