@@ -15,6 +15,11 @@
 // TMEM in each CTA) is double-buffered: eight warps read one while the next
 // tile is being multiplied.
 //
+// 16-bit dz of few rows (FEW_ROWS) is held as two planes, value and rounding
+// error: with one row, or a few, the rounding of one dominant score's gradient
+// is the whole gradient's error (1.8 times that of its own final rounding);
+// over many rows it averages (1.0 to 1.4 times).
+//
 // float32 operands come as three bfloat16 planes (x = hi + mid + lo exactly,
 // 8 bits each) and the contraction runs over six of the nine plane pairs,
 // smallest products first; what is left out is below 2^-24 of a product.
@@ -31,6 +36,7 @@ namespace xent {
 enum Epi { kScore = 0, kDz = 1, kDh = 2, kDw = 3 };
 
 constexpr int BM = TILE_ROWS, BN = 256, BK = K_BLOCK;  // of a CTA pair
+constexpr int FEW_ROWS = 64;
 constexpr int HALF = 128;                   // rows of A and of B per CTA
 constexpr int SUB = 128;                    // columns per score partial
 constexpr int STAGES = 6;
@@ -45,7 +51,7 @@ struct TcArgs {
   const int* n_live;
   int V, D;
   int c0, Cn;           // piece of the vocabulary (kDz, kDh, kDw): start, columns
-  int pairs;            // plane pairs: 1 (16-bit operands) or 6 (float32)
+  int pairs;            // plane pairs: 6 (float32); 16-bit operands 1, or 2 of a dz of two planes
   int plane_a, plane_b; // elements between planes of one row
   const Splits* plan;   // kDh; kDw where it is split (else NULL)
   int add;              // kDh: add to what the partials hold (a later piece)
@@ -57,7 +63,7 @@ struct TcArgs {
   float* zt;
   const float* lse;     // kDz, by packed row
   const float* rowscale;
-  int ld_dz;            // kDz: dz is [row][planes][ld_dz]
+  int ld_dz, dz_planes; // kDz: dz is [row][planes][ld_dz]
   int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
   const float* post;    // kDw: the factor of the result
@@ -210,15 +216,17 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
   p[2] = __float2bfloat16_rz(r1 - __bfloat162float(p[1]));
 }
 
-// k blocks that one accumulation in TMEM runs over for float32.  The tensor
-// core cuts each sum to the accumulator's precision instead of rounding it,
-// which over a long contraction leaves a bias of about one unit in the last
-// place per step; the sums of short chunks are added in registers instead.
-constexpr int F32_CHUNK = 4;
+// k blocks that one accumulation in TMEM runs over where sums of chunks are
+// added in registers.  The tensor core cuts each sum to the accumulator's
+// precision instead of rounding it, which over a long contraction leaves a bias
+// of about one unit in the last place per step: float32 results (4 blocks: dw
+// over 2048 rows 2.6e-6 -> 4e-7), and the float32 loss of 16-bit operands wider
+// than DEEP (16 blocks: 1.3e-6 at 4096 -> below 5e-7).
+constexpr int F32_CHUNK = 4, DEEP_CHUNK = 16, DEEP = 2048;
 
 // T: the operands' type.  O: the type of the user's tensors (float32 with T =
-// bfloat16 planes, else T).
-template <typename T, typename O, int EPI>
+// bfloat16 planes, else T).  CHUNKS: sums of chunks in registers.
+template <typename T, typename O, int EPI, bool CHUNKS>
 __global__ void __launch_bounds__(TC_THREADS, 1) __cluster_dims__(2, 1, 1)
 tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_o,
@@ -267,7 +275,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   grid_wait();
   const Sched<EPI> sched(args);
   // k blocks per accumulation
-  const auto chunk = [](const Unit& un) { return F32 ? F32_CHUNK : un.kbs; };
+  constexpr int CHUNK_KB = F32 ? F32_CHUNK : DEEP_CHUNK;
+  const auto chunk = [](const Unit& un) { return CHUNKS ? CHUNK_KB : un.kbs; };
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------ loads, in both CTAs
@@ -288,7 +297,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             break;
           }
           const int pr = i / len, k = (un.kb0 + kc + i - pr * len) * BK;
-          const int xa = F32 ? pair_a(pr) * args.plane_a : 0;
+          // 16-bit: dz's second plane first, where it has one
+          const int xa = (F32 ? pair_a(pr) : args.pairs - 1 - pr) * args.plane_a;
           const int xb = F32 ? pair_b(pr) * args.plane_b : 0;
           uint8_t* a = smem + L::oA + slot * OPERAND;
           uint8_t* b = smem + L::oB + slot * OPERAND;
@@ -427,20 +437,24 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (n + i == t) p -= 1.f;
             v[i] = (m < live && i < valid) ? rs * p : 0.f;
           }
-          if constexpr (F32) {
-            // 32 columns of the three planes: planes 0, 1 side by side in one
-            // stage would split a box, so each is staged on its own
+          if (F32 || args.dz_planes > 1) {
+            // 32 columns of each plane in turn, in rows of 64 bytes
 #pragma unroll
-            for (int pl = 0; pl < 3; ++pl) {
+            for (int pl = 0; pl < (F32 ? 3 : 2); ++pl) {
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
-                const __nv_bfloat16 x = __float2bfloat16_rz(v[2 * i]);
-                const __nv_bfloat16 y = __float2bfloat16_rz(v[2 * i + 1]);
-                const __nv_bfloat162 q = __halves2bfloat162(x, y);
-                w[i] = *reinterpret_cast<const uint32_t*>(&q);
-                v[2 * i] -= __bfloat162float(x);
-                v[2 * i + 1] -= __bfloat162float(y);
+                float x, y;
+                if constexpr (F32) {
+                  const __nv_bfloat162 q = __halves2bfloat162(__float2bfloat16_rz(v[2 * i]),
+                                                              __float2bfloat16_rz(v[2 * i + 1]));
+                  w[i] = *reinterpret_cast<const uint32_t*>(&q);
+                } else {
+                  w[i] = tc::pack2<T>(v[2 * i], v[2 * i + 1]);
+                }
+                tc::unpack2<T>(w[i], x, y);
+                v[2 * i] -= x;
+                v[2 * i + 1] -= y;
               }
               stage_free();
 #pragma unroll
@@ -488,13 +502,13 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (lane == 0) arrive_cluster(tc::map_rank(acc_empty + buf, 0));
       };
 
-      if constexpr (F32) {
+      if constexpr (CHUNKS) {
         float acc[SUB / 32][32];
 #pragma unroll
         for (int c = 0; c < SUB / 32; ++c)
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
-        for (int kc = 0; kc < un.kbs; kc += F32_CHUNK, ++n_acc) {
+        for (int kc = 0; kc < un.kbs; kc += CHUNK_KB, ++n_acc) {
           const uint32_t buf = n_acc & 1;
           ok = __all_sync(0xffffffffu,
                           tc::mbar_wait(acc_full + buf, (n_acc >> 1) & 1, abort, POLLS));
