@@ -221,8 +221,12 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
 // precision instead of rounding it, which over a long contraction leaves a bias
 // of about one unit in the last place per step: float32 results (4 blocks: dw
 // over 2048 rows 2.6e-6 -> 4e-7), and the float32 loss of 16-bit operands wider
-// than DEEP (16 blocks: 1.3e-6 at 4096 -> below 5e-7).
-constexpr int F32_CHUNK = 4, DEEP_CHUNK = 16, DEEP = 2048;
+// than DEEP over few words (16 blocks; 100 words, width 4000: 1.3e-6 -> 3e-7).
+// Over many words the scores' sums are larger and the same bias is less of them
+// (131,072 words, width 4096: 4.8e-7), and the second read of the accumulators
+// costs up to 8 % under the power cap: not where there are more tiles than
+// DEEP_UNITS.
+constexpr int F32_CHUNK = 4, DEEP_CHUNK = 16, DEEP = 1024, DEEP_UNITS = 4 * CLUSTERS;
 
 // T: the operands' type.  O: the type of the user's tensors (float32 with T =
 // bfloat16 planes, else T).  CHUNKS: sums of chunks in registers.

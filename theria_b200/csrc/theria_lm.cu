@@ -675,7 +675,7 @@ struct Tc {
     a.sub_tiles = (int)cdiv(V, xent::SUB);
     a.zt = ws.zt;
     const int64_t units = z.Mp / xent::BM * cdiv(V, xent::BN);
-    if (int e = D > xent::DEEP
+    if (int e = D > xent::DEEP && units <= xent::DEEP_UNITS
                     ? tc_launch<T, O, xent::kScore, true>(ma, mb, mh, ma, a, units, st)
                     : tc_launch<T, O, xent::kScore>(ma, mb, mh, ma, a, units, st))
       return e;
