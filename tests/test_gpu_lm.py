@@ -170,6 +170,20 @@ def test_ids_outside_the_vocabulary_are_reported():
         theria_b200.check_device_error()
 
 
+def test_embedding_offsets_past_32_bits():
+    # 4.5e9 elements: the last rows lie beyond 2^32
+    V, D = 2_200_000, 2048
+    w = torch.zeros(V, D, device="cuda", dtype=torch.bfloat16)
+    w[V - 2:] = torch.randn(2, D, device="cuda").bfloat16()
+    w.requires_grad_(True)
+    ids = torch.tensor([V - 1, 0, V - 2, V - 1], device="cuda")
+    y = lm.embedding(ids, w)
+    assert torch.equal(y[0], w[V - 1]) and torch.equal(y[2], w[V - 2]) and y[1].abs().max() == 0
+    (gw,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert (gw[V - 1] == 2).all() and (gw[V - 2] == 1).all() and (gw[0] == 1).all()
+    assert gw[1:V - 2].any().item() is False
+
+
 # ----------------------------------------------------------------- layer norm
 NORM_SHAPES = [(1, 1), (1, 64), (5, 31), (300, 33), (17, 64), (3, 256), (9, 257), (4, 1000),
                (33, 1111), (7, 2048), (300, 4096), (3, 8192), (5, 8200), (2, 20001)]
@@ -287,6 +301,19 @@ def test_layer_norm_strides_empty_and_streams():
     _near(y, F.layer_norm(x.double(), (32,)), torch.float32)
 
 
+def test_layer_norm_offsets_past_32_bits():
+    N, D = 1_050_000, 4096
+    x = torch.empty(N, D, device="cuda", dtype=torch.bfloat16).normal_().requires_grad_(True)
+    y = lm.layer_norm(x)
+    _near(y[-3:], F.layer_norm(x.detach()[-3:].double(), (D,)), torch.bfloat16)
+    (gx,) = torch.autograd.grad(y, x, x.detach())
+    xr = x.detach()[-3:].double().requires_grad_(True)
+    (want,) = torch.autograd.grad(F.layer_norm(xr, (D,)), xr, xr.detach())
+    # the upstream gradient x is nearly all mean and xhat: gx is what is left,
+    # the rounding of x's own 8 bits cancels in it to float32's
+    assert (gx[-3:].double() - want).abs().max() <= 2 ** -8 * want.abs().max() + 2 ** -20
+
+
 def test_layer_norm_gradient_against_differences():
     # float32 central differences of <y, r> along a direction: with step 1e-2
     # the truncation error is ~ 1e-4 of the slope and the float32 sum's
@@ -351,6 +378,25 @@ def test_linear_cross_entropy_and_its_gradients(N, V, D, dtype):
         assert torch.equal(lm.linear_cross_entropy(hd, wd, t.cuda()), got)
     again = torch.autograd.grad(lm.linear_cross_entropy(hd, wd, t.cuda()), (hd, wd), up.cuda())
     assert torch.equal(again[0], gh) and torch.equal(again[1], gw)
+
+
+@pytest.mark.parametrize("dtype,N,V,D", [(torch.bfloat16, 16384, 20000, 64),
+                                         (torch.float32, 8192, 12000, 40)])
+def test_linear_cross_entropy_in_pieces_of_the_vocabulary(dtype, N, V, D):
+    # dz of all words would take over 512 MB: two pieces, dh added up over them
+    g = _gen(18)
+    h = torch.randn(N, D, generator=g).to(dtype).cuda().requires_grad_(True)
+    w = (torch.randn(V, D, generator=g) / math.sqrt(D)).to(dtype).cuda().requires_grad_(True)
+    t = torch.randint(V, (N,), generator=g).cuda()
+    t[::7] = -100
+    got = lm.linear_cross_entropy(h, w, t, reduction="sum")
+    gh, gw = torch.autograd.grad(got, (h, w))
+    hr, wr = (x.detach().double().requires_grad_(True) for x in (h, w))
+    want = F.cross_entropy(hr @ wr.t(), t, reduction="sum")
+    dh, dw = torch.autograd.grad(want, (hr, wr))
+    assert abs(got.item() / want.item() - 1) <= 4e-6
+    _near(gh, dh, dtype)
+    _near(gw, dw, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
