@@ -45,6 +45,7 @@ constexpr int EPI_WARPS = 8;
 constexpr int STAGE_OUT = 4096;             // a warp's stage of results: 32 rows of 128 bytes
 constexpr int TC_THREADS = 128 + EPI_WARPS * 32;
 constexpr uint32_t ACC_COLS = 256;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr uint32_t POLLS = 1u << 20;  // bound of one wait; a poll suspends the thread for a while
 
 struct TcArgs {
@@ -422,24 +423,54 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int i = 0; i < 32; ++i)
               if (n + i == t) args.zt[m] = v[i];
           }
-          float most = v[0];
+          // four chains of three-input maxima, four sums in two pairs
+          float top4[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-          for (int i = 1; i < 32; ++i) most = fmaxf(most, v[i]);
-          const float now = fmaxf(top, most);
-          const float base = now == -INFINITY ? 0.f : now * 1.4426950408889634f;
-          sum *= tc::ex2(fmaf(top, 1.4426950408889634f, -base));
+          for (int i = 4; i < 28; i += 8)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sum += tc::ex2(fmaf(v[i], 1.4426950408889634f, -base));
+            for (int k = 0; k < 4; ++k) top4[k] = tc::max3(top4[k], v[i + k], v[i + k + 4]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], v[28 + k]);
+          const float now = fmaxf(tc::max3(top4[0], top4[1], top4[2]), fmaxf(top4[3], top));
+          const float base = now == -INFINITY ? 0.f : now * LOG2E;
+          float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            float e0, e1, e2, e3;
+            tc::fma2(e0, e1, v[i], v[i + 1], LOG2E, LOG2E, -base, -base);
+            tc::fma2(e2, e3, v[i + 2], v[i + 3], LOG2E, LOG2E, -base, -base);
+            tc::add2(s0, s1, s0, s1, tc::ex2(e0), tc::ex2(e1));
+            tc::add2(s2, s3, s2, s3, tc::ex2(e2), tc::ex2(e3));
+          }
+          sum = fmaf(sum, tc::ex2(fmaf(top, LOG2E, -base)), (s0 + s1) + (s2 + s3));
           top = now;
         } else if constexpr (EPI == kDz) {
-          const int valid = args.Cn - n;
+          // Rows that do not count are zeros of h: their scores are 0 and their
+          // factor rs is 0.
+          if constexpr (F32) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float p;
-            if constexpr (F32) p = expf(v[i] - l);
-            else p = tc::ex2((v[i] - l) * 1.4426950408889634f);
-            if (n + i == t) p -= 1.f;
-            v[i] = (m < live && i < valid) ? rs * p : 0.f;
+            for (int i = 0; i < 32; ++i) v[i] = expf(v[i] - l);
+          } else {
+            const float off = -l * LOG2E;
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float e0, e1;
+              tc::fma2(e0, e1, v[i], v[i + 1], LOG2E, LOG2E, off, off);
+              v[i] = tc::ex2(e0);
+              v[i + 1] = tc::ex2(e1);
+            }
+          }
+          if (t >= n && t < n + 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (n + i == t) v[i] -= 1.f;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) tc::mul2(v[i], v[i + 1], v[i], v[i + 1], rs, rs);
+          if (args.Cn - n < 32) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= args.Cn - n) v[i] = 0.f;
           }
           if (F32 || args.dz_planes > 1) {
             // 32 columns of each plane in turn, in rows of 64 bytes
@@ -539,13 +570,22 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         if (!ok) break;
         ++n_acc;
         tc::tc_fence_after();
-        if (idle) give_back(buf);
-#pragma unroll 1
-        for (int c = idle ? SUB : 0; c < SUB; c += 32) {
-          float v[32];
-          tc::tmem_ld32(src + buf * ACC_COLS + c, v);  // warp-collective
-          if (c == SUB - 32) give_back(buf);
-          take(v, c);
+        if (idle) {
+          give_back(buf);
+        } else {
+          // the next 32 columns are on their way while these are worked on
+          uint32_t raw[2][32];
+          tc::tmem_start32(src + buf * ACC_COLS, raw[0]);
+#pragma unroll
+          for (int c = 0; c < SUB / 32; ++c) {
+            tc::tmem_wait32(raw[c & 1]);
+            if (c + 1 < SUB / 32) tc::tmem_start32(src + buf * ACC_COLS + (c + 1) * 32, raw[(c + 1) & 1]);
+            else give_back(buf);
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[c & 1][i]);
+            take(v, c * 32);
+          }
         }
       }
       if (EPI == kScore && m < live && n0 < args.V)
