@@ -74,9 +74,11 @@ struct TcArgs {
 __device__ __forceinline__ int pair_a(int i) { return (0x001102 >> (4 * i)) & 15; }
 __device__ __forceinline__ int pair_b(int i) { return (0x010120 >> (4 * i)) & 15; }
 
+// Arrives on a barrier of the pair.  What it orders is the reads of TMEM before
+// it (tcgen05 fences); at cluster scope it would wait for this thread's global
+// stores as well.
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr)
-               : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // A warp's staged 32 x 128-byte tile to (x, y) of `map`, or added to it
 // (float32); one bulk group of this thread.
@@ -387,20 +389,40 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         else store_2d(&map_o, out, x, y);
       }
     };
+    // What a unit's row needs, fetched while the unit before is worked on: with
+    // short contractions the latency would otherwise be a third of a unit.
+    struct Row {
+      Unit un;
+      int t;
+      float l, rs;
+    };
+    auto fetch = [&](int u) {
+      Row r;
+      r.t = -1;
+      r.l = r.rs = 0.f;
+      if (u >= sched.units) return r;
+      r.un = sched.at(u);
+      const int m = r.un.m0 + rank * HALF + quarter * 32 + lane;
+      if (EPI <= kDz && m < live) {
+        r.t = args.tgt[m] - (EPI == kDz ? args.c0 : 0);
+        if (EPI == kDz) {
+          r.l = args.lse[m];
+          r.rs = args.rowscale[m];
+        }
+      }
+      return r;
+    };
     uint32_t n_acc = 0;
     bool ok = true;
+    Row next = fetch(cluster);
     for (int u = cluster; ok && u < sched.units; u += clusters) {
-      const Unit un = sched.at(u);
+      const Unit un = next.un;
+      const int t = next.t;
+      const float l = next.l, rs = next.rs;
+      next = fetch(u + clusters);
       const int m_warp = un.m0 + rank * HALF + quarter * 32, m = m_warp + lane;
       const int n0 = un.n0 + side * SUB;
-      // what the row needs, fetched while the product is still running
-      int t = -1;
-      float l = 0.f, rs = 0.f, top = -INFINITY, sum = 0.f;
-      if (EPI <= kDz && m < live) t = args.tgt[m] - (EPI == kDz ? args.c0 : 0);
-      if (EPI == kDz && m < live) {
-        l = args.lse[m];
-        rs = args.rowscale[m];
-      }
+      float top = -INFINITY, sum = 0.f;
 
       // Rows past those that count: nothing of them is kept, but dz is zero up
       // to the end of a k block of dw's contraction over the rows.
