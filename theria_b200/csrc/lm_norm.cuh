@@ -16,6 +16,12 @@
 // nothing to cancellation.  Statistics, sums and the weight gradients are
 // float32; each result is rounded once.  The sums over rows go through per-CTA
 // partials added by a second kernel in a fixed order: the same bits every time.
+//
+// Measured: 16384 x 4096 bfloat16 forward 56 us (4.8 TB/s; bound by the latency
+// of a row's two reductions), backward 87 us (4.6 TB/s; by instruction issue) and
+// 6 us for the column sums; float32 85 us (6.3 TB/s) and 130 (6.2 TB/s).  Rows
+// that are no 16-byte vectors go value by value: 32768 x 1111 float16 104 us (1.4
+// TB/s) and 225.
 #pragma once
 
 #include "common.cuh"

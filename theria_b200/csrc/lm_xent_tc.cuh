@@ -23,6 +23,13 @@
 // float32 operands come as three bfloat16 planes (x = hi + mid + lo exactly,
 // 8 bits each) and the contraction runs over six of the nine plane pairs,
 // smallest products first; what is left out is below 2^-24 of a product.
+//
+// Measured (bfloat16, one launch alone): 4096 x 16384 x 2048 scores 183 us (1505
+// TFLOP/s, tensor pipe 80 % busy), dz 194, dh 194, dw 179 us.  Bound by the
+// tensor cores (by the power cap in a long run) from a width of about 512 on;
+// below it by the exponentials of the scores' epilogue and by dz in HBM (8192 x
+// 32768 x 64: scores 125 us, of which 60 the exponentials; dz 137, dh 98, dw 104,
+// of which 82 each its 537 MB).
 #pragma once
 
 #include "common.cuh"
