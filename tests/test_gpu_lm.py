@@ -508,6 +508,59 @@ def test_linear_cross_entropy_refuses_a_second_derivative():
         gh.sum().backward()
 
 
+# --------------------------------------------------------- streams and graphs
+def _step(ids, target, table, w, b):
+    x = lm.embedding(ids, table, scale=4.0)
+    loss = lm.linear_cross_entropy(lm.layer_norm(x, w, b), table, target)
+    return (loss, *torch.autograd.grad(loss, (table, w, b)))
+
+
+def _step_inputs(seed):
+    g = _gen(seed)
+    ids, target = (torch.randint(700, (6, 90), generator=g).cuda() for _ in range(2))
+    target[2, 10:] = -100
+    table = (torch.randn(700, 64, generator=g) * 0.2).cuda().bfloat16().requires_grad_(True)
+    w, b = (torch.randn(64, generator=g).cuda().requires_grad_(True) for _ in range(2))
+    return ids, target, table, w, b
+
+
+def test_training_step_in_a_cuda_graph():
+    # captured once, replayed on other tokens: the number of rows that count and
+    # the splits chosen from it are found on the device
+    ids, target, table, w, b = _step_inputs(20)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _step(ids, target, table, w, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(ids, target, table, w, b)
+    ids2, target2, *_ = _step_inputs(21)
+    target2[4:] = -100
+    for i, t in ((ids2, target2), (ids.clone(), target.clone())):
+        ids.copy_(i)
+        target.copy_(t)
+        graph.replay()
+        for x, y in zip(out, _step(i, t, table, w, b)):
+            assert torch.equal(x, y)
+
+
+def test_training_steps_on_two_streams():
+    first, second = _step_inputs(22), _step_inputs(23)
+    want = [[t.clone() for t in _step(*x)] for x in (first, second)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(5):
+        for k, x in enumerate((first, second)):
+            with torch.cuda.stream(streams[k]):
+                got[k] = _step(*x)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals():
     w = torch.randn(8, 16, device="cuda")
