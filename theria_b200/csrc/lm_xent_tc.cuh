@@ -297,39 +297,45 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const bool plain = args.h_plain && *args.n_live == args.rows;
     const CUtensorMap* pa = EPI <= kDz && plain ? &map_h : &map_a;
     const CUtensorMap* pb = EPI == kDw && plain ? &map_h : &map_b;
-    uint32_t it = 0;
+    const uint32_t bars = tc::map_rank(full, 0);
+    uint32_t slot = 0, phase = 1, it = 0;
     bool ok = true;
     for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = sched.at(u);
       const int m0 = un.m0 + rank * HALF, n0 = un.n0 + rank * HALF;
       for (int kc = 0; ok && kc < un.kbs; kc += chunk(un)) {
-        const int len = min(chunk(un), un.kbs - kc);
-        for (int i = 0, n = args.pairs * len; i < n; ++i, ++it) {
-          const int slot = it % STAGES;
-          if (!tc::mbar_wait(empty + slot, ((it / STAGES) & 1) ^ 1, abort, POLLS)) {
-            ok = false;
-            break;
-          }
-          const int pr = i / len, k = (un.kb0 + kc + i - pr * len) * BK;
+        const int k0 = un.kb0 + kc, k1 = k0 + min(chunk(un), un.kbs - kc);
+        for (int pr = 0; ok && pr < args.pairs; ++pr) {
           // 16-bit: dz's second plane first, where it has one
           const int xa = (F32 ? pair_a(pr) : args.pairs - 1 - pr) * args.plane_a;
           const int xb = F32 ? pair_b(pr) * args.plane_b : 0;
-          uint8_t* a = smem + L::oA + slot * OPERAND;
-          uint8_t* b = smem + L::oB + slot * OPERAND;
-          if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
-          const uint32_t bar = tc::map_rank(full + slot, 0);
-          if constexpr (A_MN) {
-            load_2d(a, pa, bar, xa + m0, k);
-            load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, k);
-          } else {
-            load_2d(a, pa, bar, xa + k, m0);
-          }
-          if constexpr (B_MN) {
-            const int y = (EPI == kDh ? args.c0 : 0) + k;
-            load_2d(b, pb, bar, xb + n0, y);
-            load_2d(b + OPERAND / 2, pb, bar, xb + n0 + 64, y);
-          } else {
-            load_2d(b, pb, bar, xb + k, (EPI == kDz ? args.c0 : 0) + n0);
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            if (!tc::mbar_wait(empty + slot, phase, abort, POLLS)) {
+              ok = false;
+              break;
+            }
+            const int k = kb * BK;
+            uint8_t* a = smem + L::oA + slot * OPERAND;
+            uint8_t* b = smem + L::oB + slot * OPERAND;
+            if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
+            const uint32_t bar = bars + slot * 8;
+            if constexpr (A_MN) {
+              load_2d(a, pa, bar, xa + m0, k);
+              load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, k);
+            } else {
+              load_2d(a, pa, bar, xa + k, m0);
+            }
+            if constexpr (B_MN) {
+              const int y = (EPI == kDh ? args.c0 : 0) + k;
+              load_2d(b, pb, bar, xb + n0, y);
+              load_2d(b + OPERAND / 2, pb, bar, xb + n0 + 64, y);
+            } else {
+              load_2d(b, pb, bar, xb + k, (EPI == kDz ? args.c0 : 0) + n0);
+            }
+            if (++slot == STAGES) {
+              slot = 0;
+              phase ^= 1;
+            }
           }
         }
       }
@@ -345,7 +351,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     constexpr uint32_t step_a = A_MN ? 2048 : 32, step_b = B_MN ? 2048 : 32;
     const uint64_t da = tc::sw128_desc(tc::smem_u32(smem + L::oA), A_MN ? OPERAND / 2 : 16, 1024);
     const uint64_t db = tc::sw128_desc(tc::smem_u32(smem + L::oB), B_MN ? OPERAND / 2 : 16, 1024);
-    uint32_t it = 0, n_acc = 0;
+    uint32_t slot = 0, phase = 0, n_acc = 0;
     bool ok = true;
     for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = sched.at(u);
@@ -358,9 +364,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         tc::tc_fence_after();
         const uint32_t d = tmem + buf * ACC_COLS;
         const int len = min(chunk(un), un.kbs - kc);
-        for (int i = 0, n = args.pairs * len; i < n; ++i, ++it) {
-          const int slot = it % STAGES;
-          if (!tc::mbar_wait(full + slot, (it / STAGES) & 1, abort, POLLS)) {
+        for (int i = 0, n = args.pairs * len; i < n; ++i) {
+          if (!tc::mbar_wait(full + slot, phase, abort, POLLS)) {
             ok = false;
             break;
           }
@@ -371,6 +376,10 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             mma_pair(d, tc::desc_at(a, k * step_a), tc::desc_at(b, k * step_b), id,
                      (i > 0 || k > 0) ? 1u : 0u);
           commit_pair(empty + slot);
+          if (++slot == STAGES) {
+            slot = 0;
+            phase ^= 1;
+          }
         }
         if (ok) commit_pair(acc_full + buf);
       }
