@@ -24,8 +24,8 @@
 // 8 bits each) and the contraction runs over six of the nine plane pairs,
 // smallest products first; what is left out is below 2^-24 of a product.
 //
-// Measured (bfloat16, one launch alone): 4096 x 16384 x 2048 scores 183 us (1505
-// TFLOP/s, tensor pipe 80 % busy), dz 194, dh 194, dw 179 us.  Bound by the
+// Measured (bfloat16, one launch alone): 8192 x 32768 x 2048 scores 716 us (1535
+// TFLOP/s), dz 737, dh 721, dw 720 us; tensor pipe about 80 % busy.  Bound by the
 // tensor cores (by the power cap in a long run) from a width of about 512 on;
 // below it by the exponentials of the scores' epilogue and by dz in HBM (8192 x
 // 32768 x 64: scores 125 us, of which 60 the exponentials; dz 137, dh 98, dw 104,
@@ -297,6 +297,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const bool plain = args.h_plain && *args.n_live == args.rows;
     const CUtensorMap* pa = EPI <= kDz && plain ? &map_h : &map_a;
     const CUtensorMap* pb = EPI == kDw && plain ? &map_h : &map_b;
+    // no division and no mapping in the loop: with four loads a k block it sets
+    // the pace (dw of 8192 x 32768 x 2048: 777 -> 720 us)
     const uint32_t bars = tc::map_rank(full, 0);
     uint32_t slot = 0, phase = 1, it = 0;
     bool ok = true;
