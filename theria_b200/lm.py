@@ -16,6 +16,9 @@ A token id or target outside the vocabulary is found on the device, where it
 cannot raise: it counts as a row of zeros (an ignored row in the loss), and
 ``theria_b200.check_device_error()`` then raises.
 
+There is no forward mode: a tensor that carries a tangent is refused with
+NotImplementedError, as an input or as a gradient that arrives.
+
 The reference library has no such operators; its decoder example composes them
 from torch modules (``examples/minimal_decoder_transformer.py:82-263``).
 """
@@ -23,6 +26,7 @@ from torch modules (``examples/minimal_decoder_transformer.py:82-263``).
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from theria_b200 import _lib
@@ -81,6 +85,13 @@ def _check_ids(what, name, ids, device):
         raise AssertionError(f"{what}: {name} is on {ids.device}, not {device}")
 
 
+def _no_tangents(what, *tensors):
+    """Forward mode is refused: a tangent left out would read as a derivative of 0."""
+    for t in tensors:
+        if t is not None and unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward mode derivative")
+
+
 def _wide(ids):
     return int(ids.dtype == torch.int64)
 
@@ -121,6 +132,7 @@ class _EmbeddingBackward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, u):
+        _no_tangents("theria embedding", u)
         (ids,) = ctx.saved_tensors
         return _embed(ids, u.contiguous(), ctx.scale, ctx.padding), None, None, None, None
 
@@ -134,6 +146,7 @@ class _Embedding(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
+        _no_tangents("theria embedding", gy)
         (ids,) = ctx.saved_tensors
         grad = _EmbeddingBackward.apply if torch.is_grad_enabled() else _embed_grad
         return grad(gy, ids, ctx.V, ctx.scale, ctx.padding), None, None, None
@@ -151,6 +164,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     _check_ids("theria embedding", "ids", ids, weight.device)
     if weight.ndim != 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise AssertionError("weight must have shape (V,D)")
+    _no_tangents("theria embedding", weight)
     V = weight.shape[0]
     padding = -1
     if padding_idx is not None:
@@ -208,6 +222,7 @@ class _LayerNormBackward(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, u, a, c):
+        _no_tangents("theria layer_norm", u, a, c)
         x, w, b, gy, stats = ctx.saved_tensors
         D = x.shape[-1]
         N = x.numel() // D
@@ -230,6 +245,7 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
+        _no_tangents("theria layer_norm", gy)
         x, w, b, stats = ctx.saved_tensors
         need = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():
@@ -257,6 +273,7 @@ def layer_norm(x, weight=None, bias=None, eps=EPS):
             raise AssertionError(f"{name} dtype must be {x.dtype} or float32")
     if weight is not None and bias is not None and weight.dtype is not bias.dtype:
         raise AssertionError("weight and bias must share one dtype")
+    _no_tangents(what, x, weight, bias)
     x = x.contiguous()
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
@@ -318,6 +335,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g):
+        _no_tangents("theria linear_cross_entropy", g)
         h, w, target, stats = ctx.saved_tensors
         grad = _LinearCrossEntropyBackward.apply if torch.is_grad_enabled() else _loss_grad
         dh, dw = grad(h, w, g, target, stats, *ctx.rest, ctx.needs_input_grad[:2])
@@ -355,6 +373,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, redu
         raise AssertionError(f"target shape must be {tuple(hidden.shape[:-1])}")
     if reduction not in _REDUCTIONS:
         raise AssertionError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    _no_tangents(what, hidden, weight)
     h, w, t = hidden.contiguous(), _aligned(weight), target.contiguous()
     if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
         return _LinearCrossEntropy.apply(h, w, t, int(ignore_index), _REDUCTIONS[reduction])
