@@ -67,3 +67,23 @@ def test_a_second_cotangent_with_a_tangent_is_refused():
             u = [fwAD.make_dual(torch.ones_like(t), torch.ones_like(t)) for t in first]
             with pytest.raises(NotImplementedError, match="forward mode"):
                 torch.autograd.grad(first, g, u)
+
+
+def test_layer_norm_refuses_a_third_derivative():
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    r = torch.randn(4, 16, device="cuda")
+    (gx,) = torch.autograd.grad((lm.layer_norm(x) * r).sum(), x, create_graph=True)
+    (g2,) = torch.autograd.grad((gx * r).sum(), x, create_graph=True)
+    assert g2.requires_grad  # not silently cut off
+    with pytest.raises(RuntimeError, match="differentiable twice"):
+        g2.sum().backward()
+
+
+def test_embedding_has_every_derivative_of_a_linear_map():
+    # the second derivative's own: linear in its cotangent, constant in the table
+    ids = torch.tensor([1, 0, 5, 1], device="cuda")
+    w = torch.randn(8, 16, device="cuda", requires_grad=True)
+    g = torch.randn(4, 16, device="cuda", requires_grad=True)
+    (gw,) = torch.autograd.grad(lm.embedding(ids, w, scale=2.0), w, g, create_graph=True)
+    (gg,) = torch.autograd.grad(gw, g, torch.ones_like(gw), create_graph=True)
+    assert not gg.requires_grad and (gg == 2).all()

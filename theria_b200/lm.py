@@ -209,6 +209,33 @@ def _norm_grad(x, w, b, stats, gy, need):
     return gx, gw if need[1] else None, gb if need[2] else None
 
 
+def _norm_grad2(x, w, b, gy, stats, u, a, c):
+    D = x.shape[-1]
+    N = x.numel() // D
+    u, a, c = (None if t is None else t.contiguous() for t in (u, a, c))
+    dx, dgy = torch.empty_like(x), torch.empty_like(x)
+    dw = None if w is None else torch.empty_like(w)
+    ws, size = _workspace("theria_norm_bwd_workspace_bytes", x.device, N, D)
+    _call("theria_norm_bwd2", x.device, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
+          gy.data_ptr(), stats.data_ptr(), _ptr(u), _ptr(a), _ptr(c), dx.data_ptr(),
+          _ptr(dw), dgy.data_ptr(), ws.data_ptr(), size, N, D, _DTYPES[x.dtype])
+    return dx, dw, dgy
+
+
+class _LayerNormBackward2(torch.autograd.Function):
+    """Cotangents of the backward -> (dx, dw, dgy); a third derivative is refused
+    (once_differentiable would cut it off where no cotangent needs a gradient)."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _norm_grad2(*args)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("theria layer_norm is differentiable twice: its second derivatives "
+                           "have no derivative here")
+
+
 class _LayerNormBackward(torch.autograd.Function):
     """(x, w, gy) -> (gx, gw, gb); its backward is the second derivative.
     The statistics are functions of x, differentiated through there."""
@@ -220,19 +247,10 @@ class _LayerNormBackward(torch.autograd.Function):
         return _norm_grad(x, w, b, stats, gy, need)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, u, a, c):
         _no_tangents("theria layer_norm", u, a, c)
-        x, w, b, gy, stats = ctx.saved_tensors
-        D = x.shape[-1]
-        N = x.numel() // D
-        u, a, c = (None if t is None else t.contiguous() for t in (u, a, c))
-        dx, dgy = torch.empty_like(x), torch.empty_like(x)
-        dw = None if w is None else torch.empty_like(w)
-        ws, size = _workspace("theria_norm_bwd_workspace_bytes", x.device, N, D)
-        _call("theria_norm_bwd2", x.device, x.data_ptr(), _ptr(w), _affine_dtype(x, w, b),
-              gy.data_ptr(), stats.data_ptr(), _ptr(u), _ptr(a), _ptr(c), dx.data_ptr(),
-              _ptr(dw), dgy.data_ptr(), ws.data_ptr(), size, N, D, _DTYPES[x.dtype])
+        grad = _LayerNormBackward2.apply if torch.is_grad_enabled() else _norm_grad2
+        dx, dw, dgy = grad(*ctx.saved_tensors, u, a, c)
         return dx, dw, None, dgy, None, None
 
 
