@@ -185,9 +185,11 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
     if (a.done) *a.done = 0;
     if (a.count) *a.count = (float)total;
     if (a.post)
-      *a.post = (a.per_row ? most
-                 : a.mean_of ? (total > 0 ? a.gloss[0] / *a.mean_of : 0.f)
-                             : a.gloss[0]) / unit;
+      // no row: zeros, whatever the upstream gradient is
+      *a.post = (a.per_row    ? most
+                 : total == 0 ? 0.f
+                 : a.mean_of  ? a.gloss[0] / *a.mean_of
+                              : a.gloss[0]) / unit;
   }
 }
 

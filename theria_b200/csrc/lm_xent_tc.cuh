@@ -759,8 +759,10 @@ split_sum_kernel(const SumArgs a, const SumArgs b, int a_ctas, const float* post
           }
         }
       }
+      if (m >= 0) {  // a row that does not count stays 0, also where f is not finite
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] *= f;
+        for (int k = 0; k < VEC; ++k) x[k] *= f;
+      }
       embed::store_vec<O, VEC>((O*)s.out + i * D + u * VEC, x);
     }
   }
