@@ -485,8 +485,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           sum = fmaf(sum, tc::ex2(fmaf(top, LOG2E, -base)), (s0 + s1) + (s2 + s3));
           top = now;
         } else if constexpr (EPI == kDz) {
-          // Rows that do not count are zeros of h: their scores are 0 and their
-          // factor rs is 0.
+          // Rows that do not count are zeros of h: their scores are 0, or NaN
+          // beside a weight that is not finite; their dz is 0.
           if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = expf(v[i] - l);
@@ -507,10 +507,11 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) tc::mul2(v[i], v[i + 1], v[i], v[i + 1], rs, rs);
-          if (args.Cn - n < 32) {
+          const int valid = m < live ? args.Cn - n : 0;
+          if (valid < 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i >= args.Cn - n) v[i] = 0.f;
+              if (i >= valid) v[i] = 0.f;
           }
           if (F32 || args.dz_planes > 1) {
             // 32 columns of each plane in turn, in rows of 64 bytes
