@@ -29,6 +29,90 @@ def _rel(got, want):
 
 
 # ------------------------------------------------------- linear cross entropy
+# Scores are sums of D products to which the tensor cores add 16 at a time; each
+# addition cuts the sum by less than a unit in its last place, 2^-23 of the next
+# power of two above the largest score: `_score_error` for the difference of two
+# scores.  Against that, and relative to the result, stands what float32 softmax
+# arithmetic around the maximum costs in absolute terms: sums of V exponentials
+# beside a 1 go through at most 20 roundings of 2^-24 (8 in a chain of a row's 32
+# columns, 5 for joining chains and blocks, 7 for the tiles and the logarithm),
+# which over many rows average to the size of 3.
+def _score_error(top, D):
+    return 2 * math.ceil(D / 16) * 2.0 ** -23 * 2.0 ** math.ceil(math.log2(top))
+
+
+def _certain(N, V, D, score, gap, dtype, seed):
+    """Targets whose score is about `score`, `gap` above all others'."""
+    g = _gen(seed)
+    w = torch.randn(V, D, generator=g) / math.sqrt(D)
+    t = torch.randint(V, (N,), generator=g)
+    h = gap * w[t]
+    h[:, 0], w[:, 0] = 8.0, (score - gap) / 8  # the others' common score
+    return h.to(dtype), w.to(dtype), t
+
+
+def _exact_loss(h, w, t):
+    """loss, dz and z_t - lse of each row, in float64 without cancellation."""
+    z = h.double() @ w.double().t()
+    z = z - z.gather(1, t[:, None])
+    others = z.exp().scatter(1, t[:, None], 0.0).sum(1)
+    dz = z.exp() / (1 + others)[:, None]
+    dz.scatter_(1, t[:, None], (-others / (1 + others))[:, None])
+    return torch.log1p(others), dz
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("score,gap", [(20, 8), (20, 20), (60, 14), (100, 8), (100, 20)])
+@pytest.mark.parametrize("N,V,D", [(200, 256, 64), (300, 1000, 72)])
+def test_loss_and_gradients_of_nearly_certain_tokens(N, V, D, score, gap, dtype):
+    h, w, t = _certain(N, V, D, float(score), float(gap), dtype, score + gap + N)
+    want, dz = _exact_loss(h, w, t)
+    rel = _score_error(2 * score, D) + 2 ** -21  # of a small loss, and of its gradient
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = lm.linear_cross_entropy(hd, wd, t.cuda(), reduction="none")
+    err = (loss.detach().cpu().double() - want).abs()
+    assert (loss >= 0).all()
+    assert (err <= rel * want + 20 * 2 ** -24).all()
+    assert err.mean() <= rel * want.mean() + 3 * 2 ** -24
+    # an upstream gradient that keeps float16 results above their smallest numbers
+    (gh,) = torch.autograd.grad(loss, hd, torch.full_like(loss, 1024.0))
+    dh = dz @ w.double()
+    size = dz.abs() @ w.double().abs()  # of dh's terms
+    # dz in 16 bits: 2^-8 and 2^-11 of each, and the result's own rounding
+    unit = {torch.float32: 2 ** -22, torch.float16: 2 ** -10, torch.bfloat16: 2 ** -7}[dtype]
+    err = (gh.cpu().double() / 1024 - dh).abs()
+    p = 2 ** -24 * w.double().abs()[t]  # the absolute error is that of the target's term
+    tiny = 2 ** -34 if dtype == torch.float16 else 0.0  # the spacing of its smallest numbers
+    assert (err <= (rel + unit) * size + 20 * p + tiny).all()
+    assert err.mean() <= (rel + unit) * size.mean() + 3 * p.mean() + tiny
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64])
+def test_loss_of_one_word_is_exactly_zero(D, dtype):
+    g = _gen(D)
+    h, w = torch.randn(90, D, generator=g).to(dtype), torch.randn(1, D, generator=g).to(dtype)
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = lm.linear_cross_entropy(hd, wd, torch.zeros(90, dtype=torch.long, device="cuda"),
+                                   reduction="none")
+    assert (loss == 0).all()
+    for grad in torch.autograd.grad(loss, (hd, wd), torch.ones_like(loss)):
+        assert (grad == 0).all()
+
+
+def test_loss_of_extreme_scores_to_its_own_size():
+    h = torch.tensor([[1.0, 0.0], [0.0, 1.0], [1.0, 1.0], [0.0, 1.0]])
+    w = torch.tensor([[30000.0, -30000.0], [-30000.0, 30000.0], [0.0, 0.0]])
+    t = torch.tensor([0, 0, 2, 1])
+    want = torch.tensor([0.0, 60000.0, math.log(3.0), 0.0], dtype=torch.float64)
+    for dtype in (torch.float32, torch.bfloat16):
+        wd = w.to(dtype)
+        scale = wd[0, 0].item() / 30000  # bfloat16 has no 30000
+        got = lm.linear_cross_entropy(h.to("cuda", dtype), wd.cuda(), t.cuda(), reduction="none")
+        want_d = want * torch.tensor([1, scale, 1, 1])
+        assert ((got.cpu().double() - want_d).abs() <= 2 ** -22 * want_d).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
 @pytest.mark.parametrize("up", [math.nan, math.inf])

@@ -36,8 +36,8 @@ struct Prep {
   unsigned* done;                    // zeroed for join_kernel
   // forward: the rows that do not count get 0 here
   float *count, *loss, *lse;
-  // backward, by packed row: lse and the row's factor of dz, and the factor of
-  // the results
+  // backward, by packed row: lse [2][N] and the row's factor of dz, and the
+  // factor of the results
   const float *gloss, *lse_in, *mean_of;
   int per_row, half;
   float *lse_p, *rowscale, *post;
@@ -165,11 +165,12 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
         a.tgt[to] = (int)t[k];
         if (a.lse_p) {
           a.lse_p[to] = a.lse_in[i];
+          a.lse_p[a.N + to] = a.lse_in[a.N + i];
           a.rowscale[to] = unit * (a.per_row ? a.gloss[i] / most : 1.f);
         }
       } else {
         if (a.loss) a.loss[i] = 0.f;
-        if (a.lse) a.lse[i] = 0.f;
+        if (a.lse) a.lse[i] = a.lse[a.N + i] = 0.f;
       }
     }
   }
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
   }
 }
 
-// lse and loss of each row that counts, from its tiles' (max, sum); a warp
+// lse [2][N] and loss of each row that counts, from its tiles' (max, sum); a warp
 // per row.  `out` not NULL: the CTA that ends last adds all N rows' losses in
 // a fixed order (mean: over *count).
 __global__ void __launch_bounds__(256)
@@ -213,9 +214,13 @@ join_kernel(const float2* part, const float* zt, const int* row_of, const int* n
     sum = warp_sum(sum);
     if (lane == 0) {
       const int64_t i = row_of[m];
-      const float l = top + logf(sum);
+      // log(sum) is small beside top for a nearly certain token, and all of its
+      // loss: it is never rounded to top's last place.  lse keeps what its own
+      // rounding leaves (the error of a sum of two, Knuth's TwoSum).
+      const float log_sum = logf(sum), l = top + log_sum, back = l - top;
       lse[i] = l;
-      loss[i] = l - zt[m];
+      lse[N + i] = (top - (l - back)) + (log_sum - back);
+      loss[i] = log_sum + (top - zt[m]);
     }
   }
   if (out == nullptr) return;

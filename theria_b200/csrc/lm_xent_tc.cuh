@@ -69,7 +69,7 @@ struct TcArgs {
   float2* part;         // kScore: [row][sub_tiles]
   int sub_tiles;
   float* zt;
-  const float* lse;     // kDz, by packed row
+  const float* lse;     // kDz, by packed row: [2][rows], lse and what its rounding left
   const float* rowscale;
   int ld_dz, dz_planes; // kDz: dz is [row][planes][ld_dz]
   int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
@@ -412,12 +412,12 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     struct Row {
       Unit un;
       int t;
-      float l, rs;
+      float l, lo, rs;
     };
     auto fetch = [&](int u) {
       Row r;
       r.t = -1;
-      r.l = r.rs = 0.f;
+      r.l = r.lo = r.rs = 0.f;
       if (u >= sched.units) return r;
       r.un = sched.at(u);
       const int m = r.un.m0 + rank * HALF + quarter * 32 + lane;
@@ -425,6 +425,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         r.t = args.tgt[m] - (EPI == kDz ? args.c0 : 0);
         if (EPI == kDz) {
           r.l = args.lse[m];
+          r.lo = args.lse[args.rows + m];
           r.rs = args.rowscale[m];
         }
       }
@@ -436,7 +437,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = next.un;
       const int t = next.t;
-      const float l = next.l, rs = next.rs;
+      const float l = next.l, lo = next.lo, rs = next.rs;
       next = fetch(u + clusters);
       const int m_warp = un.m0 + rank * HALF + quarter * 32, m = m_warp + lane;
       const int n0 = un.n0 + side * SUB;
@@ -472,38 +473,53 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
           for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], v[28 + k]);
           const float now = fmaxf(tc::max3(top4[0], top4[1], top4[2]), fmaxf(top4[3], top));
-          const float base = now == -INFINITY ? 0.f : now * LOG2E;
+          // The difference first: the maximum's own term is exactly 1 then, and the
+          // others' errors are relative to their distance, not to their size.
+          const float ref = now == -INFINITY ? 0.f : now;
           float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             float e0, e1, e2, e3;
-            tc::fma2(e0, e1, v[i], v[i + 1], LOG2E, LOG2E, -base, -base);
-            tc::fma2(e2, e3, v[i + 2], v[i + 3], LOG2E, LOG2E, -base, -base);
+            tc::add2(e0, e1, v[i], v[i + 1], -ref, -ref);
+            tc::add2(e2, e3, v[i + 2], v[i + 3], -ref, -ref);
+            tc::mul2(e0, e1, e0, e1, LOG2E, LOG2E);
+            tc::mul2(e2, e3, e2, e3, LOG2E, LOG2E);
             tc::add2(s0, s1, s0, s1, tc::ex2(e0), tc::ex2(e1));
             tc::add2(s2, s3, s2, s3, tc::ex2(e2), tc::ex2(e3));
           }
-          sum = fmaf(sum, tc::ex2(fmaf(top, LOG2E, -base)), (s0 + s1) + (s2 + s3));
+          sum = fmaf(sum, tc::ex2((top - ref) * LOG2E), (s0 + s1) + (s2 + s3));
           top = now;
         } else if constexpr (EPI == kDz) {
           // Rows that do not count are zeros of h: their scores are 0, or NaN
           // beside a weight that is not finite; their dz is 0.
+          // z - lse as (z - l) - lo, the first exact near the maximum; the
+          // target's p - 1 without the subtraction, which would leave 2^-24.
+          const bool target = t >= n && t < n + 32;
+          float less = 0.f;
+          if (target) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (n + i == t) less = v[i];
+            less = expm1f((less - l) - lo);
+          }
           if constexpr (F32) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = expf(v[i] - l);
+            for (int i = 0; i < 32; ++i) v[i] = expf((v[i] - l) - lo);
           } else {
-            const float off = -l * LOG2E;
+            const float off = -lo * LOG2E;
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float e0, e1;
-              tc::fma2(e0, e1, v[i], v[i + 1], LOG2E, LOG2E, off, off);
+              tc::add2(e0, e1, v[i], v[i + 1], -l, -l);
+              tc::fma2(e0, e1, e0, e1, LOG2E, LOG2E, off, off);
               v[i] = tc::ex2(e0);
               v[i + 1] = tc::ex2(e1);
             }
           }
-          if (t >= n && t < n + 32) {
+          if (target) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (n + i == t) v[i] -= 1.f;
+              if (n + i == t) v[i] = less;
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) tc::mul2(v[i], v[i + 1], v[i], v[i + 1], rs, rs);

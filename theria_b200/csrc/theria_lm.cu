@@ -471,7 +471,7 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.pos = c.take<int>(N);
   r.row_of = c.take<int>(N);
   r.tgt = c.take<int>(N);
-  r.lse = c.take<float>(N);
+  r.lse = c.take<float>(2 * N);
   r.rowscale = c.take<float>(N);
   r.n_live = c.take<int>(64);  // and what else is one value
   r.done = (unsigned*)r.n_live + 1;
