@@ -75,10 +75,10 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
  * THERIA_ERR_INVALID_ARG).  N, V < 2^30, D < 2^27.
  *   reduction THERIA_LOSS_NONE: loss [N]; _SUM, _MEAN: loss [1], the mean
  *   over the rows that count (NaN if there is none).
- * lse [2, N] and count [1] (the rows that count, float32) are what the backward
- * needs: the lse of each row, then what its rounding to float32 left (without
- * it the gradient of a nearly certain token, p - 1, would be lost); rows that
- * do not count leave both 0. */
+ * lse [3, N] and count [1] (the rows that count, float32) are what the backward
+ * needs: the lse of each row, what its rounding to float32 left, and the row's
+ * loss (of which the gradient of a nearly certain token, p - 1, is made); rows
+ * that do not count leave 0. */
 #define THERIA_LOSS_NONE 0
 #define THERIA_LOSS_SUM 1
 #define THERIA_LOSS_MEAN 2

@@ -36,11 +36,11 @@ struct Prep {
   unsigned* done;                    // zeroed for join_kernel
   // forward: the rows that do not count get 0 here
   float *count, *loss, *lse;
-  // backward, by packed row: lse [2][N] and the row's factor of dz, and the
-  // factor of the results
+  // backward, by packed row: lse [2][N], the row's factor of dz, dz of its
+  // target, and the factor of the results
   const float *gloss, *lse_in, *mean_of;
   int per_row, half;
-  float *lse_p, *rowscale, *post;
+  float *lse_p, *rowscale, *less, *post;
   // how dh's and dw's contractions are split (see plan_splits); NULL: not
   Splits *plan_h, *plan_w;
   int kb, d_tiles, v_tiles, pairs, ld_acc;
@@ -166,11 +166,14 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
         if (a.lse_p) {
           a.lse_p[to] = a.lse_in[i];
           a.lse_p[a.N + to] = a.lse_in[a.N + i];
-          a.rowscale[to] = unit * (a.per_row ? a.gloss[i] / most : 1.f);
+          const float rs = unit * (a.per_row ? a.gloss[i] / most : 1.f);
+          a.rowscale[to] = rs;
+          // p - 1 of a nearly certain token from its loss: p itself is rounded at 1
+          a.less[to] = rs * expm1f(-a.lse_in[2 * a.N + i]);
         }
       } else {
         if (a.loss) a.loss[i] = 0.f;
-        if (a.lse) a.lse[i] = a.lse[a.N + i] = 0.f;
+        if (a.lse) a.lse[i] = a.lse[a.N + i] = a.lse[2 * a.N + i] = 0.f;
       }
     }
   }
@@ -194,7 +197,7 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
   }
 }
 
-// lse [2][N] and loss of each row that counts, from its tiles' (max, sum); a warp
+// lse [3][N] and loss of each row that counts, from its tiles' (max, sum); a warp
 // per row.  `out` not NULL: the CTA that ends last adds all N rows' losses in
 // a fixed order (mean: over *count).
 __global__ void __launch_bounds__(256)
@@ -220,7 +223,7 @@ join_kernel(const float2* part, const float* zt, const int* row_of, const int* n
       const float log_sum = logf(sum), l = top + log_sum, back = l - top;
       lse[i] = l;
       lse[N + i] = (top - (l - back)) + (log_sum - back);
-      loss[i] = log_sum + (top - zt[m]);
+      loss[i] = lse[2 * N + i] = log_sum + (top - zt[m]);
     }
   }
   if (out == nullptr) return;

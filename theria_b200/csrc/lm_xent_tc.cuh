@@ -70,7 +70,7 @@ struct TcArgs {
   int sub_tiles;
   float* zt;
   const float* lse;     // kDz, by packed row: [2][rows], lse and what its rounding left
-  const float* rowscale;
+  const float *rowscale, *less;
   int ld_dz, dz_planes; // kDz: dz is [row][planes][ld_dz]
   int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
@@ -412,12 +412,12 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     struct Row {
       Unit un;
       int t;
-      float l, lo, rs;
+      float l, lo, rs, less;
     };
     auto fetch = [&](int u) {
       Row r;
       r.t = -1;
-      r.l = r.lo = r.rs = 0.f;
+      r.l = r.lo = r.rs = r.less = 0.f;
       if (u >= sched.units) return r;
       r.un = sched.at(u);
       const int m = r.un.m0 + rank * HALF + quarter * 32 + lane;
@@ -427,6 +427,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           r.l = args.lse[m];
           r.lo = args.lse[args.rows + m];
           r.rs = args.rowscale[m];
+          r.less = args.less[m];
         }
       }
       return r;
@@ -437,7 +438,9 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     for (int u = cluster; ok && u < sched.units; u += clusters) {
       const Unit un = next.un;
       const int t = next.t;
-      const float l = next.l, lo = next.lo, rs = next.rs;
+      const float l = next.l, lo = next.lo, rs = next.rs, less = next.less;
+      const float base = l * LOG2E;
+      const float rs_p = rs * tc::ex2(-fmaf(lo, LOG2E, fmaf(l, LOG2E, -base)));
       next = fetch(u + clusters);
       const int m_warp = un.m0 + rank * HALF + quarter * 32, m = m_warp + lane;
       const int n0 = un.n0 + side * SUB;
@@ -492,37 +495,25 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         } else if constexpr (EPI == kDz) {
           // Rows that do not count are zeros of h: their scores are 0, or NaN
           // beside a weight that is not finite; their dz is 0.
-          // z - lse as (z - l) - lo, the first exact near the maximum; the
-          // target's p - 1 without the subtraction, which would leave 2^-24.
-          const bool target = t >= n && t < n + 32;
-          float less = 0.f;
-          if (target) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (n + i == t) less = v[i];
-            less = expm1f((less - l) - lo);
-          }
           if constexpr (F32) {
+            // lse is l + lo; z - l is exact near the maximum
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = expf((v[i] - l) - lo);
+            for (int i = 0; i < 32; ++i) v[i] = expf((v[i] - l) - lo) * rs;
           } else {
-            const float off = -lo * LOG2E;
+            // z log2(e) - base in one step, rounded once; what base leaves of lse
+            // log2(e) is a factor of the row, in rs_p
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
               float e0, e1;
-              tc::add2(e0, e1, v[i], v[i + 1], -l, -l);
-              tc::fma2(e0, e1, e0, e1, LOG2E, LOG2E, off, off);
-              v[i] = tc::ex2(e0);
-              v[i + 1] = tc::ex2(e1);
+              tc::fma2(e0, e1, v[i], v[i + 1], LOG2E, LOG2E, -base, -base);
+              tc::mul2(v[i], v[i + 1], tc::ex2(e0), tc::ex2(e1), rs_p, rs_p);
             }
           }
-          if (target) {
+          if (t >= n && t < n + 32) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (n + i == t) v[i] = less;
           }
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) tc::mul2(v[i], v[i + 1], v[i], v[i + 1], rs, rs);
           const int valid = m < live ? args.Cn - n : 0;
           if (valid < 32) {
 #pragma unroll

@@ -463,7 +463,7 @@ int xent_check(int64_t N, int64_t V, int64_t D, int dtype, int reduction) {
 struct XentRows {  // filled by prep_kernel
   int *pos, *row_of, *tgt, *n_live;
   unsigned* done;
-  float *lse, *rowscale, *post;  // backward
+  float *lse, *rowscale, *less, *post;  // backward
   xent::Splits *plan_h, *plan_w;
 };
 XentRows xent_rows(Carver& c, int64_t N) {
@@ -473,6 +473,7 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.tgt = c.take<int>(N);
   r.lse = c.take<float>(2 * N);
   r.rowscale = c.take<float>(N);
+  r.less = c.take<float>(N);
   r.n_live = c.take<int>(64);  // and what else is one value
   r.done = (unsigned*)r.n_live + 1;
   r.post = (float*)r.n_live + 2;
@@ -720,6 +721,7 @@ struct Tc {
       a.Cn = (int)C;
       a.lse = r.lse;
       a.rowscale = r.rowscale;
+      a.less = r.less;
       a.ld_dz = (int)z.piece;
       a.dz_planes = z.dz_planes;
       a.plan = r.plan_h;
@@ -831,6 +833,7 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   p.half = dtype == THERIA_F16;
   p.lse_p = r.lse;
   p.rowscale = r.rowscale;
+  p.less = r.less;
   p.post = r.post;
   p.plan_h = dh ? r.plan_h : nullptr;
   p.plan_w = dw && z.split_w ? r.plan_w : nullptr;

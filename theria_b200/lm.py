@@ -307,11 +307,11 @@ def _loss(h, w, target, ignore_index, reduction):
     V, D = w.shape
     N, dt, dev = target.numel(), _DTYPES[h.dtype], h.device
     loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
-    stats = torch.empty(2 * N + 1, dtype=torch.float32, device=dev)  # lse [2, N], count
+    stats = torch.empty(3 * N + 1, dtype=torch.float32, device=dev)  # lse [3, N], count
     ws, size = _workspace("theria_xent_fwd_workspace_bytes", dev, N, V, D, dt)
     lse = stats.data_ptr()
     _call("theria_xent_fwd", dev, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
-          ignore_index, reduction, loss.data_ptr(), lse, lse + 8 * N, ws.data_ptr(), size, N, V,
+          ignore_index, reduction, loss.data_ptr(), lse, lse + 12 * N, ws.data_ptr(), size, N, V,
           D, dt)
     return loss, stats
 
@@ -325,7 +325,7 @@ def _loss_grad(h, w, g, target, stats, ignore_index, reduction, need):
     ws, size = _workspace("theria_xent_bwd_workspace_bytes", dev, N, V, D, dt)
     lse = stats.data_ptr()
     _call("theria_xent_bwd", dev, h.data_ptr(), w.data_ptr(), target.data_ptr(), _wide(target),
-          ignore_index, reduction, g.data_ptr(), lse, lse + 8 * N, _ptr(dh), _ptr(dw),
+          ignore_index, reduction, g.data_ptr(), lse, lse + 12 * N, _ptr(dh), _ptr(dw),
           ws.data_ptr(), size, N, V, D, dt)
     return dh, dw
 
