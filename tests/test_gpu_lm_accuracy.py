@@ -88,7 +88,7 @@ def test_loss_and_gradients_of_nearly_certain_tokens(N, V, D, score, gap, dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("D", [64])
+@pytest.mark.parametrize("D", [64, 2048])
 def test_loss_of_one_word_is_exactly_zero(D, dtype):
     g = _gen(D)
     h, w = torch.randn(90, D, generator=g).to(dtype), torch.randn(1, D, generator=g).to(dtype)
@@ -111,6 +111,64 @@ def test_loss_of_extreme_scores_to_its_own_size():
         got = lm.linear_cross_entropy(h.to("cuda", dtype), wd.cuda(), t.cuda(), reduction="none")
         want_d = want * torch.tensor([1, scale, 1, 1])
         assert ((got.cpu().double() - want_d).abs() <= 2 ** -22 * want_d).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(70, 512), (3, 300)])
+def test_gradients_of_certain_tokens_in_wide_rows(N, V, dtype):
+    # few tiles of wide 16-bit rows: the backward's scores have to be the
+    # forward's to the bit, or their difference is what is left of p - 1
+    D = 2048
+    h, w, t = _certain(N, V, D, 60.0, 14.0, dtype, V)
+    want, dz = _exact_loss(h, w, t)
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = lm.linear_cross_entropy(hd, wd, t.cuda(), reduction="none")
+    (gh,) = torch.autograd.grad(loss, hd, torch.full_like(loss, 1024.0))
+    dh, size = dz @ w.double(), dz.abs() @ w.double().abs()
+    unit = {torch.float16: 2 ** -10, torch.bfloat16: 2 ** -7}[dtype]
+    err = (gh.cpu().double() / 1024 - dh).abs()
+    p = 2 ** -24 * w.double().abs()[t]
+    assert (err <= (_score_error(120, D) + unit) * size + 20 * p + 2 ** -34).all()
+    assert err.mean() <= (_score_error(120, D) + unit) * size.mean() + 3 * p.mean() + 2 ** -34
+
+
+def test_float32_products_keep_their_low_bits():
+    # 1 + 2^-7 - 2^-23 as bfloat16 parts cut toward zero leaves products 7.8 * 2^-24
+    # short.  Here: at most one unit for what three parts rounded to nearest leave
+    # out, one for the accumulator's cut, half a one for the last rounding.
+    x = 1 + 2.0 ** -7 - 2.0 ** -23
+    bound = 2.5 * 2.0 ** -23
+    h = torch.full((8, 16), x, device="cuda")
+    w = torch.zeros(2, 16, device="cuda")
+    w[0] = x
+    one = torch.ones(8, dtype=torch.long, device="cuda")
+    loss = lm.linear_cross_entropy(h, w, one, reduction="none").cpu().double()
+    z = 16 * x * x
+    assert (loss / (z + math.log1p(math.exp(-z))) - 1).abs().max() <= bound
+    # scores of 0: dz = +-x for the upstream gradient 2 x, and dh = x * x
+    hz = torch.zeros(8, 16, device="cuda", requires_grad=True)
+    w = torch.zeros(2, 16, device="cuda")
+    w[1] = -x
+    loss = lm.linear_cross_entropy(hz, w, one, reduction="none")
+    (gh,) = torch.autograd.grad(loss, hz, torch.full_like(loss, 2 * x))
+    assert (gh.cpu().double() / (x * x) - 1).abs().max() <= bound
+
+
+def test_float32_loss_of_the_largest_numbers():
+    # rounded to nearest, the leading part of the largest float32 would be infinite
+    big = torch.finfo(torch.float32).max
+    h = torch.tensor([[big], [-big]], device="cuda")
+    w = torch.tensor([[2.0 ** -120], [0.0]], device="cuda", requires_grad=True)
+    loss = lm.linear_cross_entropy(h, w, torch.tensor([1, 0], device="cuda"), reduction="none")
+    assert ((loss.detach().cpu().double() / (big * 2.0 ** -120)) - 1).abs().max() <= 2 ** -20
+    (gw,) = torch.autograd.grad(loss, w, torch.tensor([1.0, 0.0], device="cuda"))
+    assert (gw[:, 0].cpu().double() / torch.tensor([big, -big]).double() - 1).abs().max() <= 2 ** -20
+    hs = torch.zeros(1, 1, device="cuda", requires_grad=True)
+    ws = torch.tensor([[0.5], [-0.5]], device="cuda")
+    loss = lm.linear_cross_entropy(hs, ws, torch.zeros(1, dtype=torch.long, device="cuda"),
+                                   reduction="none")
+    (gh,) = torch.autograd.grad(loss, hs, torch.full_like(loss, big))
+    assert abs(gh.item() / (-0.5 * big) - 1) <= 2 ** -20
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -21,8 +21,11 @@
 // over many rows it averages (1.0 to 1.4 times).
 //
 // float32 operands come as three bfloat16 planes (x = hi + mid + lo exactly,
-// 8 bits each) and the contraction runs over six of the nine plane pairs,
-// smallest products first; what is left out is below 2^-24 of a product.
+// each rounded to nearest, so mid is at most 2^-8 and lo 2^-17 of x's power of
+// two) and the contraction runs over six of the nine plane pairs, smallest
+// products first; what is left out, 2 mid lo + lo lo, is at most 2^-24 of a
+// product and has either sign.  (Cut toward zero instead, the planes left out
+// up to 2^-21, always of the product's sign: a bias.)
 //
 // Measured (bfloat16, one launch alone): 8192 x 32768 x 2048 scores 716 us (1535
 // TFLOP/s), dz 737, dh 721, dw 720 us; tensor pipe about 80 % busy.  Bound by the
@@ -218,12 +221,14 @@ __device__ __forceinline__ void stage32(uint32_t row, int lane, const float (&v)
   }
 }
 
-// x = hi + mid + lo, each the leading 8 bits of what the ones before leave.
+// x = hi + mid + lo, each the nearest 8 bits of what the ones before leave; hi
+// is cut where the nearest would be infinite.
 __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
-  p[0] = __float2bfloat16_rz(x);
+  p[0] = __float2bfloat16_rn(x);
+  if (isinf(__bfloat162float(p[0]))) p[0] = __float2bfloat16_rz(x);
   const float r1 = isfinite(x) ? x - __bfloat162float(p[0]) : 0.f;
-  p[1] = __float2bfloat16_rz(r1);
-  p[2] = __float2bfloat16_rz(r1 - __bfloat162float(p[1]));
+  p[1] = __float2bfloat16_rn(r1);
+  p[2] = __float2bfloat16_rn(r1 - __bfloat162float(p[1]));
 }
 
 // k blocks that one accumulation in TMEM runs over where sums of chunks are
@@ -521,19 +526,20 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               if (i >= valid) v[i] = 0.f;
           }
           if (F32 || args.dz_planes > 1) {
-            // 32 columns of each plane in turn, in rows of 64 bytes
+            // 32 columns of each plane in turn, in rows of 64 bytes; |dz| <= |rs|, and
+            // the nearest of the largest float32 numbers would be infinite
+            const bool huge = F32 && fabsf(rs) > 1e38f;
 #pragma unroll
             for (int pl = 0; pl < (F32 ? 3 : 2); ++pl) {
               uint32_t w[16];
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float x, y;
-                if constexpr (F32) {
+                w[i] = tc::pack2<T>(v[2 * i], v[2 * i + 1]);
+                if (F32 && huge && pl == 0) {
                   const __nv_bfloat162 q = __halves2bfloat162(__float2bfloat16_rz(v[2 * i]),
                                                               __float2bfloat16_rz(v[2 * i + 1]));
                   w[i] = *reinterpret_cast<const uint32_t*>(&q);
-                } else {
-                  w[i] = tc::pack2<T>(v[2 * i], v[2 * i + 1]);
                 }
                 tc::unpack2<T>(w[i], x, y);
                 v[2 * i] -= x;
