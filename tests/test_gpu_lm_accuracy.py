@@ -171,6 +171,28 @@ def test_float32_loss_of_the_largest_numbers():
     assert abs(gh.item() / (-0.5 * big) - 1) <= 2 ** -20
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("N,live", [(64, 64), (65, 1), (500, 3), (1000, 64)])
+def test_few_scored_rows_among_many_keep_their_gradients(N, live, dtype):
+    # The rows that count decide how finely dz is held: the error is that of the
+    # results' own rounding (a fifth more for results that round the other way).
+    g = _gen(N + live)
+    D, V = 256, 700
+    h = torch.randn(N, D, generator=g).to(dtype)
+    w = (torch.randn(V, D, generator=g) * 0.2).to(dtype)
+    t = torch.full((N,), -100)
+    t[torch.randperm(N, generator=g)[:live]] = torch.randint(V, (live,), generator=g)
+    up = 64.0
+    hr, wr = h.double().requires_grad_(True), w.double().requires_grad_(True)
+    want = torch.autograd.grad(F.cross_entropy(hr @ wr.t(), t, reduction="sum"), (hr, wr),
+                               torch.tensor(up).double())
+    hd, wd = h.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    loss = lm.linear_cross_entropy(hd, wd, t.cuda(), reduction="sum")
+    got = torch.autograd.grad(loss, (hd, wd), torch.tensor(up, device="cuda"))
+    for a, b in zip(got, want):
+        assert _rel(a, b) <= 1.2 * _rel(b.to(dtype), b)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reduction", ["sum", "mean"])
 @pytest.mark.parametrize("up", [math.nan, math.inf])

@@ -23,6 +23,7 @@ struct Splits {
   int split_kb, acc_rows, splits;
 };
 constexpr int CLUSTERS = 74, TILE_ROWS = 256, K_BLOCK = 64;
+constexpr int FEW_ROWS = 64;  // that count: 16-bit dz in two planes
 // splits * tiles, where there is more than one split: of dh (over a piece of the
 // vocabulary) and of dw (over the rows that count, where it has few tiles)
 constexpr int MAX_UNITS = 8 * CLUSTERS, MAX_UNITS_DW = 2 * CLUSTERS;
@@ -43,7 +44,7 @@ struct Prep {
   float *lse_p, *rowscale, *less, *post;
   // how dh's and dw's contractions are split (see plan_splits); NULL: not
   Splits *plan_h, *plan_w;
-  int kb, d_tiles, v_tiles, pairs, ld_acc;
+  int kb, d_tiles, v_tiles, f32, ld_acc;
 };
 
 // float16 holds dz in units of 1 / 32768 of the largest row's factor, so that
@@ -178,12 +179,13 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
     }
   }
   const int live_tiles = total > 0 ? (total + TILE_ROWS - 1) / TILE_ROWS : 1;
+  const int pairs = a.f32 ? 6 : total <= FEW_ROWS ? 2 : 1;  // of planes
   if (a.plan_h)
-    plan_splits(a.plan_h, a.kb, live_tiles * TILE_ROWS, live_tiles * a.d_tiles, MAX_UNITS, a.pairs,
+    plan_splits(a.plan_h, a.kb, live_tiles * TILE_ROWS, live_tiles * a.d_tiles, MAX_UNITS, pairs,
                 a.ld_acc);
   if (a.plan_w)
     plan_splits(a.plan_w, total > 0 ? (total + K_BLOCK - 1) / K_BLOCK : 1, a.v_tiles * TILE_ROWS,
-                a.v_tiles * a.d_tiles, MAX_UNITS_DW, a.pairs, a.ld_acc);
+                a.v_tiles * a.d_tiles, MAX_UNITS_DW, pairs, a.ld_acc);
   if (threadIdx.x == 0) {
     *a.n_live = total;
     if (a.done) *a.done = 0;

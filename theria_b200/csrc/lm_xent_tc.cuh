@@ -15,10 +15,12 @@
 // TMEM in each CTA) is double-buffered: eight warps read one while the next
 // tile is being multiplied.
 //
-// 16-bit dz of few rows (FEW_ROWS) is held as two planes, value and rounding
-// error: with one row, or a few, the rounding of one dominant score's gradient
-// is the whole gradient's error (1.8 times that of its own final rounding);
-// over many rows it averages (1.0 to 1.4 times).
+// 16-bit dz of few rows that count (FEW_ROWS) is held as two planes, value and
+// rounding error: with one row, or a few, the rounding of one dominant score's
+// gradient is the whole gradient's error (1.8 times that of its own final
+// rounding); over many rows it averages (1.0 to 1.4 times).  The second plane
+// lies HALF rows below the first, in a part of dz's first tile of rows that so
+// few leave unused; how many count is known on the device only.
 //
 // float32 operands come as three bfloat16 planes (x = hi + mid + lo exactly,
 // each rounded to nearest, so mid is at most 2^-8 and lo 2^-17 of x's power of
@@ -46,9 +48,9 @@ namespace xent {
 enum Epi { kScore = 0, kDz = 1, kDh = 2, kDw = 3 };
 
 constexpr int BM = TILE_ROWS, BN = 256, BK = K_BLOCK;  // of a CTA pair
-constexpr int FEW_ROWS = 64;
 constexpr int HALF = 128;                   // rows of A and of B per CTA
 constexpr int SUB = 128;                    // columns per score partial
+static_assert(FEW_ROWS <= BK && BK <= HALF, "both planes of few rows in one tile");
 constexpr int STAGES = 6;
 constexpr int OPERAND = HALF * BK * 2;      // bytes of one operand's stage
 constexpr int EPI_WARPS = 8;
@@ -62,7 +64,6 @@ struct TcArgs {
   const int* n_live;
   int V, D;
   int c0, Cn;           // piece of the vocabulary (kDz, kDh, kDw): start, columns
-  int pairs;            // plane pairs: 6 (float32); 16-bit operands 1, or 2 of a dz of two planes
   int plane_a, plane_b; // elements between planes of one row
   const Splits* plan;   // kDh; kDw where it is split (else NULL)
   int add;              // kDh: add to what the partials hold (a later piece)
@@ -74,7 +75,7 @@ struct TcArgs {
   float* zt;
   const float* lse;     // kDz, by packed row: [2][rows], lse and what its rounding left
   const float *rowscale, *less;
-  int ld_dz, dz_planes; // kDz: dz is [row][planes][ld_dz]
+  int ld_dz;            // kDz: dz is [row][planes][ld_dz]
   int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
   const float* post;    // kDw: the factor of the result
@@ -249,7 +250,7 @@ template <typename T, typename O, int EPI, bool CHUNKS>
 __global__ void __launch_bounds__(TC_THREADS, 1) __cluster_dims__(2, 1, 1)
 tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
           const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_o,
-          const __grid_constant__ TcArgs args) {
+          const __grid_constant__ CUtensorMap map_p, const __grid_constant__ TcArgs args) {
   constexpr bool A_MN = EPI == kDw, B_MN = EPI == kDh || EPI == kDw;
   constexpr bool F32 = sizeof(O) == 4;
   using L = TcSmem;
@@ -293,6 +294,8 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
   grid_launch();
   grid_wait();
   const Sched<EPI> sched(args);
+  const bool few = !F32 && *args.n_live <= FEW_ROWS;  // two planes of dz
+  const int pairs = F32 ? 6 : EPI >= kDh && few ? 2 : 1;
   // k blocks per accumulation
   constexpr int CHUNK_KB = F32 ? F32_CHUNK : DEEP_CHUNK;
   const auto chunk = [](const Unit& un) { return CHUNKS ? CHUNK_KB : un.kbs; };
@@ -312,9 +315,10 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       const int m0 = un.m0 + rank * HALF, n0 = un.n0 + rank * HALF;
       for (int kc = 0; ok && kc < un.kbs; kc += chunk(un)) {
         const int k0 = un.kb0 + kc, k1 = k0 + min(chunk(un), un.kbs - kc);
-        for (int pr = 0; ok && pr < args.pairs; ++pr) {
+        for (int pr = 0; ok && pr < pairs; ++pr) {
           // 16-bit: dz's second plane first, where it has one
-          const int xa = (F32 ? pair_a(pr) : args.pairs - 1 - pr) * args.plane_a;
+          const int xa = F32 ? pair_a(pr) * args.plane_a : 0;
+          const int ya = F32 ? 0 : (pairs - 1 - pr) * HALF;
           const int xb = F32 ? pair_b(pr) * args.plane_b : 0;
           for (int kb = k0; kb < k1; ++kb, ++it) {
             if (!tc::mbar_wait(empty + slot, phase, abort, POLLS)) {
@@ -327,10 +331,10 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             if (rank == 0) tc::mbar_expect_tx(full + slot, 4 * OPERAND);
             const uint32_t bar = bars + slot * 8;
             if constexpr (A_MN) {
-              load_2d(a, pa, bar, xa + m0, k);
-              load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, k);
+              load_2d(a, pa, bar, xa + m0, ya + k);
+              load_2d(a + OPERAND / 2, pa, bar, xa + m0 + 64, ya + k);
             } else {
-              load_2d(a, pa, bar, xa + k, m0);
+              load_2d(a, pa, bar, xa + k, ya + m0);
             }
             if constexpr (B_MN) {
               const int y = (EPI == kDh ? args.c0 : 0) + k;
@@ -371,7 +375,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         tc::tc_fence_after();
         const uint32_t d = tmem + buf * ACC_COLS;
         const int len = min(chunk(un), un.kbs - kc);
-        for (int i = 0, n = args.pairs * len; i < n; ++i) {
+        for (int i = 0, n = pairs * len; i < n; ++i) {
           if (!tc::mbar_wait(full + slot, phase, abort, POLLS)) {
             ok = false;
             break;
@@ -404,12 +408,12 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       if (lane == 0) tc::bulk_wait_read_all();
       __syncwarp();
     };
-    auto stage_full = [&](int x, int y) {
+    auto stage_full = [&](int x, int y, const CUtensorMap* map) {
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (EPI == kDh && args.add) add_2d(&map_o, out, x, y);
-        else store_2d(&map_o, out, x, y);
+        if (EPI == kDh && args.add) add_2d(map, out, x, y);
+        else store_2d(map, out, x, y);
       }
     };
     // What a unit's row needs, fetched while the unit before is worked on: with
@@ -525,7 +529,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             for (int i = 0; i < 32; ++i)
               if (i >= valid) v[i] = 0.f;
           }
-          if (F32 || args.dz_planes > 1) {
+          if (F32 || few) {
             // 32 columns of each plane in turn, in rows of 64 bytes; |dz| <= |rs|, and
             // the nearest of the largest float32 numbers would be infinite
             const bool huge = F32 && fabsf(rs) > 1e38f;
@@ -550,18 +554,19 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               for (int i = 0; i < 4; ++i)
                 tc::st_shared_v4(tc::smem_u32(out) + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4),
                                  w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-              stage_full(pl * args.ld_dz + n, m_warp);
+              if (F32) stage_full(pl * args.ld_dz + n, m_warp, &map_p);
+              else stage_full(n, pl * HALF + m_warp, &map_p);
             }
           } else {
             if (c % 64 == 0) stage_free();
             stage32<T>(out_row, lane, v, c % 64 / 8);
-            if (c % 64 == 32) stage_full(n - 32, m_warp);
+            if (c % 64 == 32) stage_full(n - 32, m_warp, &map_o);
           }
         } else if (EPI == kDh || args.plan) {
           if (n >= args.ld_acc) return;
           stage_free();
           stage32<float>(out_row, lane, v, 0);
-          stage_full(n, un.split * sched.acc_rows + m_warp);
+          stage_full(n, un.split * sched.acc_rows + m_warp, &map_o);
         } else if constexpr (EPI == kDw) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] *= post;
@@ -575,12 +580,12 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
           } else if constexpr (F32) {
             stage_free();
             stage32<float>(out_row, lane, v, 0);
-            if (n < args.D && m_warp < args.Cn) stage_full(n, args.c0 + m_warp);
+            if (n < args.D && m_warp < args.Cn) stage_full(n, args.c0 + m_warp, &map_o);
           } else {
             if (c % 64 == 0) stage_free();
             stage32<O>(out_row, lane, v, c % 64 / 8);
             if (c % 64 == 32 && n - 32 < args.D && m_warp < args.Cn)
-              stage_full(n - 32, args.c0 + m_warp);
+              stage_full(n - 32, args.c0 + m_warp, &map_o);
           }
         }
       };

@@ -512,7 +512,7 @@ static_assert(kClusters == kSMs / 2 && xent::BM == xent::TILE_ROWS, "dh's split"
 
 struct XentSizes {
   int64_t Mp, Kp;          // packed rows, elements of a packed row (one plane)
-  int planes, dz_planes;
+  int planes;              // of a value, dz's as well
   bool pack_w;             // w needs a packed copy
   int64_t piece;           // of the vocabulary, backward
   int64_t ld_acc, acc_rows;  // dh's partial sums: at most these rows
@@ -526,10 +526,9 @@ XentSizes xent_sizes(int64_t N, int64_t V, int64_t D, int dtype) {
   z.Mp = up(N, xent::BM);
   z.Kp = up(D, xent::BK);
   z.planes = dtype == THERIA_F32 ? 3 : 1;
-  z.dz_planes = dtype == THERIA_F32 ? 3 : N <= xent::FEW_ROWS ? 2 : 1;
   z.pack_w = z.planes > 1 || D % 8 != 0;
   // dz of a piece within 512 MB
-  const int64_t fit = (512ll << 20) / (z.Mp * 2 * z.dz_planes) / xent::BN * xent::BN;
+  const int64_t fit = (512ll << 20) / (z.Mp * 2 * z.planes) / xent::BN * xent::BN;
   z.piece = std::min(up(V, xent::BN), std::max<int64_t>(xent::BN, fit));
   z.ld_acc = up(D, 32);
   z.acc_rows = std::max(z.Mp, std::min(xent::MAX_UNITS / cdiv(D, xent::BN) * xent::BM,
@@ -571,7 +570,7 @@ XentBwdWs xent_bwd_ws(void* base, int64_t N, int64_t V, int64_t D, const XentSiz
   w.rows = xent_rows(c, N);
   w.hp = c.take<uint16_t>(z.Mp * z.Kp * z.planes);
   w.wp = z.pack_w ? c.take<uint16_t>(V * z.Kp * z.planes) : nullptr;
-  w.dz = c.take<uint16_t>(z.Mp * z.piece * z.dz_planes);
+  w.dz = c.take<uint16_t>(z.Mp * z.piece * z.planes);
   w.acc = c.take<float>(z.acc_rows * z.ld_acc);
   w.acc_w = z.split_w ? c.take<float>(z.acc_rows_w * z.ld_acc) : nullptr;
   w.bytes = c.used;
@@ -601,14 +600,15 @@ bool map_2d(CUtensorMap* map, const void* base, int dtype, int64_t inner, int64_
 
 template <typename T, typename O, int EPI, bool CHUNKS = sizeof(O) == 4>
 int tc_launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& h,
-              const CUtensorMap& o, const xent::TcArgs& args, int64_t units, cudaStream_t st) {
+              const CUtensorMap& o, const CUtensorMap& p, const xent::TcArgs& args, int64_t units,
+              cudaStream_t st) {
   auto kern = xent::tc_kernel<T, O, EPI, CHUNKS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            xent::TcSmem::kAlloc) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
   const unsigned grid = 2 * (unsigned)std::min<int64_t>(units, kClusters);
   return launch_chained(kern, dim3(grid), dim3(xent::TC_THREADS), xent::TcSmem::kAlloc, st, a, b, h,
-                        o, args);
+                        o, p, args);
 }
 
 // T: the operands' type; O: the tensors'.
@@ -653,7 +653,6 @@ struct Tc {
     a.n_live = r.n_live;
     a.V = (int)V;
     a.D = (int)D;
-    a.pairs = z.planes > 1 ? 6 : 1;
     a.plane_a = a.plane_b = (int)z.Kp;
     a.tgt = r.tgt;
     a.rows = (int)N;
@@ -677,8 +676,8 @@ struct Tc {
     a.zt = ws.zt;
     const int64_t units = z.Mp / xent::BM * cdiv(V, xent::BN);
     if (int e = D > xent::DEEP && units <= xent::DEEP_UNITS
-                    ? tc_launch<T, O, xent::kScore, true>(ma, mb, mh, ma, a, units, st)
-                    : tc_launch<T, O, xent::kScore>(ma, mb, mh, ma, a, units, st))
+                    ? tc_launch<T, O, xent::kScore, true>(ma, mb, mh, ma, ma, a, units, st)
+                    : tc_launch<T, O, xent::kScore>(ma, mb, mh, ma, ma, a, units, st))
       return e;
     return xent_join(ws.rows, ws.part, ws.zt, a.sub_tiles, out, N, st);
   }
@@ -688,19 +687,19 @@ struct Tc {
     const XentRows& r = ws.rows;
     const xent::TcArgs base = common(h, r, z, N, V, D);
     if (int e = pack(h, w, r, ws.hp, ws.wp, z, N, V, D, st)) return e;
-    const int64_t row = z.Kp * z.planes, zrow = z.piece * z.dz_planes;
+    const int64_t row = z.Kp * z.planes, zrow = z.piece * z.planes;
     const void* wsrc = z.pack_w ? ws.wp : w;
     const int64_t wrow = z.pack_w ? row : D;
     const bool dw_tma = dw && (z.split_w || vec_rows(D, dtype, {dw}));
     // contraction along the row (k) or across rows (m); outputs (o)
-    CUtensorMap hk, hm, hk1, hm1, wk, wm, zk, zm, zo, ho, wo;
+    CUtensorMap hk, hm, hk1, hm1, wk, wm, zk, zm, zo, zp, ho, wo;
     if (!map_2d(&hk, ws.hp, op, row, z.Mp, xent::HALF) ||
         !map_2d(&hm, ws.hp, op, row, z.Mp, xent::BK) ||
         !map_2d(&wk, wsrc, op, wrow, V, xent::HALF) ||
         !map_2d(&wm, wsrc, op, wrow, V, xent::BK) ||
         !map_2d(&zk, ws.dz, op, zrow, z.Mp, xent::HALF) ||
         !map_2d(&zm, ws.dz, op, zrow, z.Mp, xent::BK) ||
-        !map_2d(&zo, ws.dz, op, zrow, z.Mp, 32, z.dz_planes > 1 ? 64 : 128) ||
+        !map_2d(&zo, ws.dz, op, zrow, z.Mp, 32) || !map_2d(&zp, ws.dz, op, zrow, z.Mp, 32, 64) ||
         !map_2d(&ho, ws.acc, THERIA_F32, z.ld_acc, z.acc_rows, 32))
       return THERIA_ERR_LAUNCH;
     hk1 = hk;
@@ -723,23 +722,21 @@ struct Tc {
       a.rowscale = r.rowscale;
       a.less = r.less;
       a.ld_dz = (int)z.piece;
-      a.dz_planes = z.dz_planes;
       a.plan = r.plan_h;
       a.ld_acc = (int)z.ld_acc;
       a.out = dw_tma ? nullptr : dw;
       a.post = r.post;
       a.add = c0 > 0;
-      if (int e = tc_launch<T, O, xent::kDz>(hk, wk, hk1, zo, a, mt * ct, st)) return e;
+      if (int e = tc_launch<T, O, xent::kDz>(hk, wk, hk1, zo, zp, a, mt * ct, st)) return e;
       a.plane_a = (int)z.piece;
-      a.pairs = z.planes > 1 ? 6 : z.dz_planes;
       if (dh)
-        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, a, std::max<int64_t>(mt * dt, kClusters),
+        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, ho, a, std::max<int64_t>(mt * dt, kClusters),
                                                 st))
           return e;
       if (!dw) continue;
       a.plan = z.split_w ? r.plan_w : nullptr;
       if (int e = tc_launch<T, O, xent::kDw>(
-              zm, hm, hm1, wo, a, z.split_w ? kClusters : ct * dt, st))
+              zm, hm, hm1, wo, wo, a, z.split_w ? kClusters : ct * dt, st))
         return e;
     }
     return sum({ws.acc, r.pos, r.plan_h, dh, dh ? N : 0},
@@ -840,7 +837,7 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   p.kb = (int)cdiv(std::min(z.piece, V), xent::BK);
   p.d_tiles = (int)cdiv(D, xent::BN);
   p.v_tiles = (int)cdiv(V, xent::BM);
-  p.pairs = z.planes > 1 ? 6 : z.dz_planes;
+  p.f32 = dtype == THERIA_F32;
   p.ld_acc = (int)z.ld_acc;
   xent::prep_kernel<<<1, 1024, 0, st>>>(p);
   if (int e = launch_status()) return e;
