@@ -46,8 +46,9 @@ int theria_embed_bwd(const void* ids, int wide, const void* gy, void* gw, void* 
 /* ------------------------------------------------------------ layer norm
  * y = (x - mean) * rstd * w + b over rows of D values, rstd = (var +
  * eps)^-1/2; x, y [N, D] of `dtype`; w, b [D] of `wdtype` (`dtype` or
- * THERIA_F32), either may be NULL.  stats (may be NULL) receives [2, N]
- * float32: the means, then the reciprocal standard deviations. */
+ * THERIA_F32), either may be NULL.  stats (may be NULL; 16-byte
+ * aligned) receives [N, 4] float32: the row's mean, its reciprocal standard
+ * deviation, what the mean's rounding to float32 left, and 0. */
 int theria_norm_fwd(const void* x, const void* w, const void* b, int wdtype, void* y,
                     float* stats, int64_t N, int64_t D, int dtype, float eps, void* stream);
 

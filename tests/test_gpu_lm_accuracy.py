@@ -162,7 +162,8 @@ def test_float32_loss_of_the_largest_numbers():
     loss = lm.linear_cross_entropy(h, w, torch.tensor([1, 0], device="cuda"), reduction="none")
     assert ((loss.detach().cpu().double() / (big * 2.0 ** -120)) - 1).abs().max() <= 2 ** -20
     (gw,) = torch.autograd.grad(loss, w, torch.tensor([1.0, 0.0], device="cuda"))
-    assert (gw[:, 0].cpu().double() / torch.tensor([big, -big]).double() - 1).abs().max() <= 2 ** -20
+    want = torch.tensor([big, -big]).double()
+    assert (gw[:, 0].cpu().double() / want - 1).abs().max() <= 2 ** -20
     hs = torch.zeros(1, 1, device="cuda", requires_grad=True)
     ws = torch.tensor([[0.5], [-0.5]], device="cuda")
     loss = lm.linear_cross_entropy(hs, ws, torch.zeros(1, dtype=torch.long, device="cuda"),
@@ -240,3 +241,30 @@ def test_a_word_whose_scores_are_minus_infinity(dtype):
     assert abs(got.item() / loss.item() - 1) <= 4e-6
     assert (gw[0] == 0).all()
     assert _rel(gw[1:], want) <= {torch.float16: 8e-4, torch.bfloat16: 6e-3}[dtype]
+
+
+# ----------------------------------------------------------------- layer norm
+def _norm_grads(fn, x, w, b, gy, dev, dt):
+    xs = [t.to(dev, dt).requires_grad_(True) for t in (x, w, b)]
+    g = gy.to(dev, dt).requires_grad_(True)
+    y = fn(*xs)
+    first = torch.autograd.grad(y, xs, g, create_graph=True)
+    second = torch.autograd.grad(first[0], (xs[0], xs[1], g), g.detach().roll(1, 0))
+    return [t.detach() for t in (y, *first, *second)]
+
+
+@pytest.mark.parametrize("N,D", [(64, 512), (70, 64), (64, 511), (33, 4096), (5, 16392),
+                                 (3, 33001)])
+@pytest.mark.parametrize("mean", [100.0, 1000.0, 10000.0])
+def test_layer_norm_gradients_of_rows_with_a_large_mean(N, D, mean):
+    # x - mean is exact near the mean: nothing is lost that float32 rows around
+    # zero would keep, so the bound is theirs (64 units of 2^-24)
+    g = _gen(N + D)
+    x = mean + torch.randn(N, D, generator=g)
+    w, b = 1 + 0.3 * torch.randn(D, generator=g), torch.randn(D, generator=g)
+    gy = torch.randn(N, D, generator=g)
+    got = _norm_grads(lm.layer_norm, x, w, b, gy, "cuda", torch.float32)
+    want = _norm_grads(lambda x, w, b: F.layer_norm(x, (D,), w, b), x, w, b, gy, "cpu",
+                       torch.float64)
+    for p, q in zip(got, want):
+        assert _rel(p, q) <= 4e-6

@@ -10,6 +10,10 @@
 //                                          + P(<u, xhat> g + <g, xhat> u)).
 // P is linear, so all of a row's sums in these are taken in one reduction.
 //
+// The mean is kept as two floats, itself and what its rounding left (`left`):
+// with a mean far above the deviations half a unit of the one float would shift
+// every xhat of the row.
+//
 // Both directions are bound by HBM: x read and y written once, then x and gy
 // read and gx written once.  A row stays in registers between its load and
 // its store; the variance is taken around the mean already known, so it loses
@@ -168,6 +172,36 @@ __device__ __forceinline__ void vmul(float (&d)[VEC], const float (&a)[VEC]) {
   }
 }
 
+// A row's statistics, 16 bytes: the mean rounded, the reciprocal standard
+// deviation, what the mean's rounding left, and 0.  xhat = (x - mean) rstd + off,
+// where the difference is exact for a mean far above the deviations.
+struct Stats {
+  float mean, rstd, off;
+  __device__ __forceinline__ explicit Stats(const float* p) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    mean = v.x;
+    rstd = v.y;
+    off = -v.z * v.y;
+  }
+  __device__ __forceinline__ float xhat(float x) const { return fmaf(x - mean, rstd, off); }
+};
+// Stores row r's, where `own`; the mean comes as `mean` + `left`.  One predicated
+// store whose address is made here: as an expression it becomes a pointer carried
+// through the rows' loop, two registers that the row needs (65536 x 1024 bfloat16
+// 58 us, this way 54).
+__device__ __forceinline__ void store_stats(float* stats, int64_t r, bool own, float mean,
+                                            float left, float rstd) {
+  const float m = mean + left, rest = (mean - m) + left;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t.reg .b64 a;\n\t"
+      "setp.ne.s32 q, %0, 0;\n\t"
+      "shl.b64 a, %1, 4;\n\t"
+      "add.s64 a, a, %2;\n\t"
+      "@q st.global.v4.f32 [a], {%3, %4, %5, %6};\n\t}" ::"r"((int)own),
+      "l"(r), "l"(stats), "f"(m), "f"(rstd), "f"(rest), "f"(0.f)
+      : "memory");
+}
+
 // One affine value, for the kernels of wide rows.
 __device__ __forceinline__ float affine(const void* p, int dtype, int64_t i, float none) {
   return p ? load_any(p, i, dtype) : none;
@@ -178,6 +212,8 @@ template <int NW> struct Block {
   static constexpr int threads = NW == 1 ? 256 : NW * 32;
   static constexpr int G = NW * 32;        // threads of a row
   static constexpr int rows = threads / G; // rows at a time
+  // CTAs an SM, for 128 registers a thread at most
+  static constexpr int least = threads < 512 ? 512 / threads : 1;
 };
 
 // Sums of M values (a power of two) over NW warps.  Each step of the butterfly
@@ -275,10 +311,7 @@ fwd_kernel(const T* __restrict__ x, const void* __restrict__ w, const void* __re
       const float left = q[2 * i + 1] * inv;
       rstd[i] = rsqrtf(fmaxf(q[2 * i] * inv - left * left, 0.f) + eps);
       off[i] = -left * rstd[i];
-      if (stats && g == 0 && r0 + i < N) {
-        stats[r0 + i] = s[i] + left;
-        stats[N + r0 + i] = rstd[i];
-      }
+      store_stats(stats, r0 + i, stats && g == 0 && r0 + i < N, s[i], left, rstd[i]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -334,7 +367,7 @@ __device__ __forceinline__ void store_part(const float (&a)[NV][VEC], const floa
 template <typename T, int VEC, int NV, int NW>
 __device__ __forceinline__ void bwd_row(float (&h)[NV][VEC], float (&u)[NV][VEC],
                                         float (&aw)[NV][VEC], float (&ab)[NV][VEC],
-                                        const void* w, int wf32, float mean, float rstd, int D,
+                                        const void* w, int wf32, const Stats& st, int D,
                                         float inv, float (*red)[32][SUMS], int& turn) {
   constexpr int G = Block<NW>::G;
   const int g = threadIdx.x % G;
@@ -345,8 +378,8 @@ __device__ __forceinline__ void bwd_row(float (&h)[NV][VEC], float (&u)[NV][VEC]
     if (c < D) {
       float wv[VEC];
       affine_vec<T, VEC>(w, wf32, c, 1.f, wv);
-      vshift(h[j], -mean);  // in this order: a mean far above the deviations loses nothing
-      vscale(h[j], h[j], rstd, 0.f);
+      vshift(h[j], -st.mean);
+      vscale(h[j], h[j], st.rstd, st.off);
       vfma(aw[j], u[j], h[j], aw[j]);
       vadd(ab[j], u[j]);
       vmul(u[j], wv);
@@ -363,7 +396,7 @@ __device__ __forceinline__ void bwd_row(float (&h)[NV][VEC], float (&u)[NV][VEC]
     if ((j * G + g) * VEC < D) {
       vshift(u[j], c0);
       vaxpy(u[j], h[j], c1);
-      vscale(u[j], u[j], rstd, 0.f);
+      vscale(u[j], u[j], st.rstd, 0.f);
     }
   }
 }
@@ -396,7 +429,7 @@ bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
         load_vec<T, VEC>(gy + r * D + c, u[j]);
       }
     }
-    bwd_row<T, VEC, NV, NW>(h, u, aw, ab, w, wf32, stats[r], stats[N + r], D, inv, red, turn);
+    bwd_row<T, VEC, NV, NW>(h, u, aw, ab, w, wf32, Stats(stats + 4 * r), D, inv, red, turn);
     if (gx) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -408,22 +441,23 @@ bwd_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   if (part) store_part<NW, NV, VEC>(aw, ab, part, D);
 }
 
-// Blocks of consecutive rows, of x and of gy, in a ring of shared-memory
-// stages filled by bulk copies.  A wait that gives up sets the device error
+// Blocks of consecutive rows, of x, of gy and of the statistics, in a ring of
+// shared-memory stages filled by bulk copies.  A wait that gives up sets the device error
 // word, and the kernel goes on with what the stage holds.
 constexpr int MAX_STAGES = 4;
 struct Ring {
   uint64_t* full;
   volatile int* abort;
   uint8_t* mem;
-  const uint8_t *x, *gy;
+  const uint8_t *x, *gy, *stats;
   int rows, stages, stage = 0;
   uint32_t phase = 0;
   int64_t N, row_bytes, blocks;
   __device__ Ring(uint64_t* f, volatile int* a, uint8_t* m, const void* x_, const void* gy_,
-                  int rows_, int stages_, int64_t n, int64_t rb)
-      : full(f), abort(a), mem(m), x((const uint8_t*)x_), gy((const uint8_t*)gy_), rows(rows_),
-        stages(stages_), N(n), row_bytes(rb), blocks((n + rows_ - 1) / rows_) {
+                  const float* stats_, int rows_, int stages_, int64_t n, int64_t rb)
+      : full(f), abort(a), mem(m), x((const uint8_t*)x_), gy((const uint8_t*)gy_),
+        stats((const uint8_t*)stats_), rows(rows_), stages(stages_), N(n), row_bytes(rb),
+        blocks((n + rows_ - 1) / rows_) {
     if (threadIdx.x == 0) {
       for (int i = 0; i < MAX_STAGES; ++i) tc::mbar_init(full + i, 1);
       *abort = 0;
@@ -432,15 +466,17 @@ struct Ring {
     }
     __syncthreads();
   }
-  __device__ uint8_t* at(int s) const { return mem + (int64_t)s * 2 * rows * row_bytes; }
+  __device__ uint8_t* at(int s) const { return mem + (int64_t)s * rows * (2 * row_bytes + 16); }
   // block b into stage s, by one thread
   __device__ void fetch(int64_t b, int s) {
     if (b >= blocks) return;
     const int64_t r0 = b * rows;
-    const uint32_t bytes = (uint32_t)((N - r0 < rows ? N - r0 : rows) * row_bytes);
-    tc::mbar_expect_tx(full + s, 2 * bytes);
+    const int n = (int)(N - r0 < rows ? N - r0 : rows);
+    const uint32_t bytes = (uint32_t)(n * row_bytes);
+    tc::mbar_expect_tx(full + s, 2 * bytes + 16 * n);
     tc::bulk_load(at(s), x + r0 * row_bytes, bytes, full + s);
     tc::bulk_load(at(s) + rows * row_bytes, gy + r0 * row_bytes, bytes, full + s);
+    tc::bulk_load(at(s) + 2 * rows * row_bytes, stats + r0 * 16, 16 * n, full + s);
   }
   __device__ void wait() { tc::mbar_wait(full + stage, phase, abort); }
   __device__ void next() {
@@ -474,7 +510,7 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   int turn = 0;
   const int g = threadIdx.x % G, q = threadIdx.x / G;
   const float inv = 1.f / (float)D;
-  Ring ring(full, &abort, ring_mem, x, gy, ROWS, stages, N, (int64_t)D * sizeof(T));
+  Ring ring(full, &abort, ring_mem, x, gy, stats, ROWS, stages, N, (int64_t)D * sizeof(T));
   float wr[NV][VEC];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -484,30 +520,15 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int k = 0; k < VEC; ++k) aw[j][k] = ab[j][k] = 0.f;
-  // of the batch to come
-  float mean[R], rstd[R];
-  auto statistics = [&](int64_t blk) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int64_t r = blk * ROWS + q * R + i;
-      mean[i] = r < N ? stats[r] : 0.f;
-      rstd[i] = r < N ? stats[N + r] : 0.f;
-    }
-  };
-  statistics(blockIdx.x);
   int before = -1;  // the stage of the batch before, read by every thread at the next barrier
   for (int64_t blk = blockIdx.x; blk < ring.blocks; blk += gridDim.x) {
     ring.wait();
     const T* sx = reinterpret_cast<const T*>(ring.at(ring.stage)) + q * R * D;
     const T* sg = sx + ROWS * D;
     const int64_t r0 = blk * ROWS + q * R;
-    float m[R], rs[R], s[2 * R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      m[i] = mean[i];
-      rs[i] = rstd[i];
-    }
-    statistics(blk + gridDim.x);
+    const float* row_stats =
+        reinterpret_cast<const float*>(sx + (2 * ROWS - q * R) * D) + 4 * q * R;
+    float s[2 * R];
     Pair su[R], sh[R];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -519,8 +540,9 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
         float h[VEC], u[VEC];
         load_vec<T, VEC>(sx + i * D + c, h);
         load_vec<T, VEC>(sg + i * D + c, u);
-        vshift(h, -m[i]);  // in this order: a mean far above the deviations loses nothing
-        vscale(h, h, rs[i], 0.f);
+        const Stats st(row_stats + 4 * i);
+        vshift(h, -st.mean);
+        vscale(h, h, st.rstd, st.off);
         vfma(aw[j], u, h, aw[j]);
         vadd(ab[j], u);
         vmul(u, wr[j]);
@@ -549,13 +571,14 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
           float h[VEC], u[VEC];
           load_vec<T, VEC>(sx + i * D + c, h);
           load_vec<T, VEC>(sg + i * D + c, u);
-          vshift(h, -m[i]);
+          const Stats st(row_stats + 4 * i);
+          vshift(h, -st.mean);
           // the means first: where they cancel u, they do so before rstd
           // enlarges it
           vmul(u, wr[j]);
-          vshift(u, -s[2 * i] * inv);
-          vaxpy(u, h, -s[2 * i + 1] * inv * rs[i]);
-          vscale(u, u, rs[i], 0.f);
+          vshift(u, -fmaf(st.off, s[2 * i + 1], s[2 * i]) * inv);
+          vaxpy(u, h, -s[2 * i + 1] * inv * st.rstd);
+          vscale(u, u, st.rstd, 0.f);
           store_vec<T, VEC>(gx + (r0 + i) * D + c, u);
         }
       }
@@ -592,10 +615,7 @@ fwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, const void*
     for (int64_t c = threadIdx.x; c < D; c += 256)
       y[r * D + c] = from_f32<T>(fmaf((to_f32(row[c]) - mean - left) * rstd,
                                       affine(w, wdtype, c, 1.f), affine(b, wdtype, c, 0.f)));
-    if (stats && threadIdx.x == 0) {
-      stats[r] = mean + left;
-      stats[N + r] = rstd;
-    }
+    store_stats(stats, r, stats && threadIdx.x == 0, mean, left, rstd);
   }
 }
 
@@ -612,10 +632,10 @@ bwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
   if (mine)
     for (int64_t c = threadIdx.x; c < D; c += 256) mine[c] = mine[D + c] = 0.f;
   for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-    const float mean = stats[r], rstd = stats[N + r];
+    const Stats st(stats + 4 * r);
     float s[2] = {0.f, 0.f};
     for (int64_t c = threadIdx.x; c < D; c += 256) {
-      const float h = (to_f32(x[r * D + c]) - mean) * rstd, u = to_f32(gy[r * D + c]);
+      const float h = st.xhat(to_f32(x[r * D + c])), u = to_f32(gy[r * D + c]);
       if (mine) {
         mine[c] = fmaf(u, h, mine[c]);
         mine[D + c] += u;
@@ -629,9 +649,9 @@ bwd_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype,
     s[0] /= (float)D;
     s[1] /= (float)D;
     for (int64_t c = threadIdx.x; c < D; c += 256) {
-      const float h = (to_f32(x[r * D + c]) - mean) * rstd;
+      const float h = st.xhat(to_f32(x[r * D + c]));
       const float uw = to_f32(gy[r * D + c]) * affine(w, wdtype, c, 1.f);
-      gx[r * D + c] = from_f32<T>(rstd * (uw - s[0] - h * s[1]));
+      gx[r * D + c] = from_f32<T>(st.rstd * (uw - s[0] - h * s[1]));
     }
   }
 }
@@ -672,7 +692,7 @@ __device__ __forceinline__ void second_terms(float (&s)[SUMS], float h, float u,
 // The backward's backward; u, a, c may be NULL (zero).  part[cta][2][D]: the
 // CTA's sums for dw (the second half is unused, zero).
 template <typename T, int VEC, int NV, int NW>
-__global__ void __launch_bounds__(Block<NW>::threads)
+__global__ void __launch_bounds__(Block<NW>::threads, Block<NW>::least)
 bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
             const T* __restrict__ gy, const float* __restrict__ stats, const T* __restrict__ u,
             const void* __restrict__ a, const void* __restrict__ c, T* __restrict__ dx,
@@ -688,7 +708,8 @@ bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
     for (int k = 0; k < VEC; ++k) aw[j][k] = none[j][k] = 0.f;
   for (int64_t r = (int64_t)blockIdx.x * ROWS + threadIdx.x / G; r < N;
        r += (int64_t)gridDim.x * ROWS) {
-    const float mean = stats[r], rstd = stats[N + r];
+    const Stats st(stats + 4 * r);
+    const float rstd = st.rstd;
     float h[NV][VEC], g[NV][VEC], v[NV][VEC], s[SUMS];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) s[i] = 0.f;
@@ -709,7 +730,7 @@ bwd2_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
         affine_vec<T, VEC>(a, wf32, col, 0.f, av);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
-          h[j][k] = (h[j][k] - mean) * rstd;
+          h[j][k] = st.xhat(h[j][k]);
           second_terms(s, h[j][k], v[j][k], g[j][k] * wv[k], g[j][k] * av[k]);
         }
       }
@@ -751,19 +772,20 @@ bwd2_wide_kernel(const T* __restrict__ x, const void* __restrict__ w, int wdtype
   float* mine = part + (int64_t)blockIdx.x * 2 * D;
   for (int64_t e = threadIdx.x; e < D; e += 256) mine[e] = mine[D + e] = 0.f;
   for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
-    const float mean = stats[r], rstd = stats[N + r];
+    const Stats st(stats + 4 * r);
+    const float rstd = st.rstd;
     float s[SUMS];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) s[i] = 0.f;
     for (int64_t e = threadIdx.x; e < D; e += 256) {
-      const float h = (to_f32(x[r * D + e]) - mean) * rstd, g = to_f32(gy[r * D + e]);
+      const float h = st.xhat(to_f32(x[r * D + e])), g = to_f32(gy[r * D + e]);
       second_terms(s, h, u ? to_f32(u[r * D + e]) : 0.f, g * affine(w, wdtype, e, 1.f),
                    g * affine(a, wdtype, e, 0.f));
     }
     row_sum<8>(s, red, turn);
     const Second f(s, D, rstd);
     for (int64_t e = threadIdx.x; e < D; e += 256) {
-      const float h = (to_f32(x[r * D + e]) - mean) * rstd, g = to_f32(gy[r * D + e]);
+      const float h = st.xhat(to_f32(x[r * D + e])), g = to_f32(gy[r * D + e]);
       const float uu = u ? to_f32(u[r * D + e]) : 0.f, pu = f.pu(uu, h);
       const float wk = affine(w, wdtype, e, 1.f), ak = affine(a, wdtype, e, 0.f);
       mine[e] = fmaf(rstd * g, pu, mine[e]);

@@ -267,6 +267,15 @@ constexpr int kNormFwd = 32, kNormBwd = 8, kNormBwdWide = 16;
 // CTAs of the backward: what its column sums are split over.
 constexpr int64_t kMaxGrid = (1ll << 31) - 1;
 int64_t norm_ctas(int64_t N) { return std::min<int64_t>(N, kSMs * 4); }
+// What of them runs at one time: with more, some SMs would take another whole
+// share of the rows (32768 x 1111 float16, three CTAs an SM instead of the four
+// asked for: second derivative 868 us, with their number 484).
+template <typename K>
+int64_t norm_wave(K kern, int threads, size_t smem, int64_t N) {
+  int per_sm = 1;
+  cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem);
+  return std::min<int64_t>(norm_ctas(N), kSMs * std::max(per_sm, 1));
+}
 
 }  // namespace
 }  // namespace theria
@@ -277,7 +286,7 @@ int theria_norm_fwd(const void* x, const void* w, const void* b, int wdtype, voi
                     float* stats, int64_t N, int64_t D, int dtype, float eps, void* stream) {
   if (int e = norm_check(N, D, dtype, wdtype)) return e;
   if (N == 0) return THERIA_OK;
-  if (!x || !y) return THERIA_ERR_INVALID_ARG;
+  if (!x || !y || !tc::aligned16(stats)) return THERIA_ERR_INVALID_ARG;
   cudaStream_t st = (cudaStream_t)stream;
   const bool vec = vec_rows(D, dtype, {x, y, w, b});
   const int wf32 = wdtype == THERIA_F32;
@@ -326,7 +335,7 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
     }
     return THERIA_OK;
   }
-  if (!x || !gy || !stats) return THERIA_ERR_INVALID_ARG;
+  if (!x || !gy || !stats || !tc::aligned16(stats)) return THERIA_ERR_INVALID_ARG;
   if (!gx && !gw) return THERIA_OK;
   if (gw && (!workspace || workspace_bytes < theria_norm_bwd_workspace_bytes(N, D)))
     return THERIA_ERR_WORKSPACE;
@@ -345,7 +354,7 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
         const int64_t sums = NW == 1 && part ? 8 * 2 * D * (int64_t)sizeof(float) : 0;
         if constexpr (VEC > 1) {
           const int64_t row = 2 * D * (int64_t)sizeof(T);  // of x and gy
-          if (2 * row <= 200 << 10) {
+          if (2 * (row + 16) <= 201 << 10) {  // and the row's statistics
             // Rows of a batch: 4 for a warp of its own and where they make a
             // stage of at most 16 KB (65536 x 1024 bfloat16: 80 us, with 2 rows
             // 86, with one 103), 2 up to 32 KB (16384 x 4096 bfloat16: 93 us,
@@ -353,19 +362,15 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
             auto batch = [&](auto rc) {
               constexpr int R = decltype(rc)::value;
               auto kern = norm::bwd_batch_kernel<T, VEC, NV, NW, R>;
-              const int64_t stage = B::rows * R * row;
+              const int64_t rows = B::rows * R, stage = rows * row;
               // float32 rows need more bytes on their way (16384 x 4096: 128 KB
               // 130 us, 96 KB 143), 16-bit rows a second CTA (93 us, 100)
               const int64_t ring = (sizeof(T) == 4 ? 128 : 96) << 10;
               const int stages = (int)std::clamp<int64_t>(ring / stage, 2, norm::MAX_STAGES);
-              const int64_t smem = std::max(sums, stage * stages);
+              const int64_t smem = std::max(sums, (stage + 16 * rows) * stages);
               if (smem > 40 << 10)  // with the kernel's static part, above the default limit
                 cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-              // one wave: each CTA has its share of the rows from the start
-              int per_sm = 1;
-              cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, B::threads, smem);
-              ctas = (int)std::min(cdiv(N, B::rows * R),
-                                   std::min<int64_t>(norm_ctas(N), kSMs * std::max(per_sm, 1)));
+              ctas = (int)std::min(cdiv(N, rows), norm_wave(kern, B::threads, smem, N));
               kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy,
                                                              stats, (T*)gx, part, N, (int)D,
                                                              stages);
@@ -377,8 +382,9 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
             return;
           }
         }
-        ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
-        norm::bwd_kernel<T, VEC, NV, NW><<<(unsigned)ctas, B::threads, sums, st>>>(
+        auto kern = norm::bwd_kernel<T, VEC, NV, NW>;
+        ctas = (int)std::min(cdiv(N, B::rows), norm_wave(kern, B::threads, sums, N));
+        kern<<<(unsigned)ctas, B::threads, sums, st>>>(
             (const T*)x, w, wf32, (const T*)gy, stats, (T*)gx, part, N, (int)D);
       };
       return norm_shape<VEC, kNormBwd>(D, run) || norm_shape<VEC, kNormBwdWide>(D, run);
@@ -407,7 +413,8 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
     if (dw) cudaMemsetAsync(dw, 0, D * elem_size(wdtype), st);
     return THERIA_OK;
   }
-  if (!x || !gy || !stats || !dx || !dgy || (dw && !w)) return THERIA_ERR_INVALID_ARG;
+  if (!x || !gy || !stats || !dx || !dgy || (dw && !w) || !tc::aligned16(stats))
+    return THERIA_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < theria_norm_bwd_workspace_bytes(N, D))
     return THERIA_ERR_WORKSPACE;
   const bool vec = vec_rows(D, dtype, {x, gy, u, dx, dgy, w, a, c});
@@ -421,11 +428,11 @@ int theria_norm_bwd2(const void* x, const void* w, int wdtype, const void* gy,
       return norm_shape<VEC, kNormBwdWide>(D, [&](auto nv, auto nw) {
         constexpr int NV = decltype(nv)::value, NW = decltype(nw)::value;
         using B = norm::Block<NW>;
-        ctas = (int)std::min<int64_t>(cdiv(N, B::rows), norm_ctas(N));
         auto kern = norm::bwd2_kernel<T, VEC, NV, NW>;
         const size_t smem = NW == 1 ? 8 * 2 * D * sizeof(float) : 0;
         if (smem > 48 * 1024)
           cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        ctas = (int)std::min(cdiv(N, B::rows), norm_wave(kern, B::threads, smem, N));
         kern<<<(unsigned)ctas, B::threads, smem, st>>>((const T*)x, w, wf32, (const T*)gy, stats,
                                                 (const T*)u, a, c, (T*)dx, (T*)dgy, part, N,
                                                 (int)D);

@@ -182,7 +182,7 @@ def _norm(x, w, b, eps, need_stats):
     D = x.shape[-1]
     N = x.numel() // D
     y = torch.empty_like(x)
-    stats = torch.empty(2, N, dtype=torch.float32, device=x.device) if need_stats else None
+    stats = torch.empty(N, 4, dtype=torch.float32, device=x.device) if need_stats else None
     _call("theria_norm_fwd", x.device, x.data_ptr(), _ptr(w), _ptr(b), _affine_dtype(x, w, b),
           y.data_ptr(), _ptr(stats), N, D, _DTYPES[x.dtype], eps)
     return y, stats
