@@ -268,3 +268,19 @@ def test_layer_norm_gradients_of_rows_with_a_large_mean(N, D, mean):
                        torch.float64)
     for p, q in zip(got, want):
         assert _rel(p, q) <= 4e-6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,D", [(5, 12808), (3, 16384), (4, 16385), (2, 32768), (3, 32776),
+                                 (2, 40001)])
+def test_layer_norm_of_the_widest_rows(N, D, dtype):
+    # past each width that a kernel keeps in registers or in its ring: forward up
+    # to 32768, backward and second derivative up to 16384
+    tol = {torch.float32: 4e-6, torch.float16: 8e-4, torch.bfloat16: 6e-3}[dtype]
+    g = _gen(N + D)
+    x, w, b, gy = (torch.randn(*s, generator=g).to(dtype) for s in ((N, D), (D,), (D,), (N, D)))
+    got = _norm_grads(lm.layer_norm, x, w, b, gy, "cuda", dtype)
+    want = _norm_grads(lambda x, w, b: F.layer_norm(x, (D,), w, b), x, w, b, gy, "cpu",
+                       torch.float64)
+    for p, q in zip(got, want):
+        assert _rel(p, q) <= tol

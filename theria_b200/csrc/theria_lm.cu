@@ -387,7 +387,12 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
         kern<<<(unsigned)ctas, B::threads, sums, st>>>(
             (const T*)x, w, wf32, (const T*)gy, stats, (T*)gx, part, N, (int)D);
       };
-      return norm_shape<VEC, kNormBwd>(D, run) || norm_shape<VEC, kNormBwdWide>(D, run);
+      if (norm_shape<VEC, kNormBwd>(D, run)) return true;
+      // wider rows need all 32 warps
+      constexpr int NV = kNormBwdWide / VEC;
+      if (cdiv(D, VEC) > 32 * 32 * NV) return false;
+      run(std::integral_constant<int, NV>{}, std::integral_constant<int, 32>{});
+      return true;
     };
     const bool done = vec ? launch(std::integral_constant<int, embed::Vec<T>::n>{})
                           : launch(std::integral_constant<int, 1>{});
