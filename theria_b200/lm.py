@@ -26,7 +26,7 @@ from torch modules (``examples/minimal_decoder_transformer.py:82-263``).
 from __future__ import annotations
 
 import torch
-from torch.autograd.forward_ad import unpack_dual
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from theria_b200 import _lib
@@ -87,8 +87,10 @@ def _check_ids(what, name, ids, device):
 
 def _no_tangents(what, *tensors):
     """Forward mode is refused: a tangent left out would read as a derivative of 0."""
+    if forward_ad._current_level < 0:  # no tensor carries one (looking at each costs 0.3 us)
+        return
     for t in tensors:
-        if t is not None and unpack_dual(t).tangent is not None:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what} has no forward mode derivative")
 
 
