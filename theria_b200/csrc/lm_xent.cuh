@@ -37,11 +37,11 @@ struct Prep {
   unsigned* done;                    // zeroed for join_kernel
   // forward: the rows that do not count get 0 here
   float *count, *loss, *lse;
-  // backward, by packed row: lse [2][N], the row's factor of dz, dz of its
-  // target, and the factor of the results
-  const float *gloss, *lse_in, *mean_of;
+  // backward: the upstream gradient; the largest row's factor (1 but for
+  // float16) and the factor of the results
+  const float *gloss, *mean_of;
   int per_row, half;
-  float *lse_p, *rowscale, *less, *post;
+  float *most, *post;
   // how dh's and dw's contractions are split (see plan_splits); NULL: not
   Splits *plan_h, *plan_w;
   int kb, d_tiles, v_tiles, f32, ld_acc;
@@ -148,7 +148,6 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
     most = fmaxf(most, peak[w]);
   }
   if (most == 0.f) most = 1.f;
-  const float unit = a.half ? HALF_SCALE : 1.f;
   for (int64_t i0 = b; i0 < e; i0 += PREP_BATCH * 32) {
     int64_t t[PREP_BATCH];
     load(i0, t);
@@ -164,14 +163,6 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
       if (is) {
         a.row_of[to] = (int)i;
         a.tgt[to] = (int)t[k];
-        if (a.lse_p) {
-          a.lse_p[to] = a.lse_in[i];
-          a.lse_p[a.N + to] = a.lse_in[a.N + i];
-          const float rs = unit * (a.per_row ? a.gloss[i] / most : 1.f);
-          a.rowscale[to] = rs;
-          // p - 1 of a nearly certain token from its loss: p itself is rounded at 1
-          a.less[to] = rs * expm1f(-a.lse_in[2 * a.N + i]);
-        }
       } else {
         if (a.loss) a.loss[i] = 0.f;
         if (a.lse) a.lse[i] = a.lse[a.N + i] = a.lse[2 * a.N + i] = 0.f;
@@ -188,6 +179,7 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
                 a.v_tiles * a.d_tiles, MAX_UNITS_DW, pairs, a.ld_acc);
   if (threadIdx.x == 0) {
     *a.n_live = total;
+    if (a.most) *a.most = most;
     if (a.done) *a.done = 0;
     if (a.count) *a.count = (float)total;
     if (a.post)
@@ -195,7 +187,7 @@ __global__ void __launch_bounds__(1024) prep_kernel(const Prep a) {
       *a.post = (a.per_row    ? most
                  : total == 0 ? 0.f
                  : a.mean_of  ? a.gloss[0] / *a.mean_of
-                              : a.gloss[0]) / unit;
+                              : a.gloss[0]) / (a.half ? HALF_SCALE : 1.f);
   }
 }
 

@@ -2,7 +2,7 @@
 // with four epilogues.
 //
 //   kScore  z  = h w^T    -> per row and 128 columns (max, sum exp), target score
-//   kDz     z  = h w^T    -> dz = rowscale * (exp(z - lse) - onehot), stored
+//   kDz     z  = h w^T    -> dz = c (exp(z - lse) - onehot), stored
 //   kDh     dh = dz w     -> float32 partial sums, per split of the vocabulary
 //   kDw     dw = dz^T h   -> the result, scaled and rounded once
 //
@@ -73,8 +73,7 @@ struct TcArgs {
   float2* part;         // kScore: [row][sub_tiles]
   int sub_tiles;
   float* zt;
-  const float* lse;     // kDz, by packed row: [2][rows], lse and what its rounding left
-  const float *rowscale, *less;
+  const float4* row;    // kDz: see RowArgs
   int ld_dz;            // kDz: dz is [row][planes][ld_dz]
   int ld_acc;           // with a plan: [split][plan->acc_rows][ld_acc] partial sums
   void* out;            // kDw: [V][D], where it cannot be stored by TMA
@@ -433,10 +432,11 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
       if (EPI <= kDz && m < live) {
         r.t = args.tgt[m] - (EPI == kDz ? args.c0 : 0);
         if (EPI == kDz) {
-          r.l = args.lse[m];
-          r.lo = args.lse[args.rows + m];
-          r.rs = args.rowscale[m];
-          r.less = args.less[m];
+          const float4 s = args.row[m];
+          r.l = s.x;
+          r.lo = s.y;
+          r.rs = s.z;
+          r.less = s.w;
         }
       }
       return r;
@@ -717,13 +717,35 @@ __device__ __forceinline__ void pack_rows(const PackArgs& a, int64_t D, int64_t 
     }
   }
 }
+// out[m] of each row that counts, for dz's epilogue: its lse, what that one's
+// rounding left, its factor of dz, and dz of its target.
+struct RowArgs {
+  const float* lse;    // [3][N]: lse, what its rounding left, the row's loss
+  const float* gloss;  // the rows' upstream gradients (NULL: 1) ...
+  const float* most;   // ... in units of the largest
+  float unit;
+  float4* out;         // NULL: nothing to do (forward)
+};
+__device__ __forceinline__ void make_rows(const RowArgs& a, const int* row_of, int live, int64_t N,
+                                          int first, int step) {
+  const float most = a.gloss ? *a.most : 1.f;
+  for (int m = first; m < live; m += step) {
+    const int64_t i = row_of[m];
+    const float rs = (a.gloss ? a.gloss[i] / most : 1.f) * a.unit;
+    // p - 1 of a nearly certain token from its loss: p itself is rounded at 1
+    a.out[m] = make_float4(a.lse[i], a.lse[N + i], rs, rs * expm1f(-a.lse[2 * N + i]));
+  }
+}
 // h in the first `h_ctas` CTAs, w in the others (none where w is read as it is).
 template <typename T, typename O>
 __global__ void __launch_bounds__(256)
-pack_kernel(const PackArgs h, const PackArgs w, int h_ctas, int64_t D, int64_t Kp) {
+pack_kernel(const PackArgs h, const PackArgs w, const RowArgs rows, int h_ctas, int64_t D,
+            int64_t Kp) {
   const int b = blockIdx.x;
   grid_launch();
   grid_wait();
+  if (b < h_ctas && rows.out)
+    make_rows(rows, h.row_of, *h.n_live, h.rows, b * 256 + threadIdx.x, h_ctas * 256);
   if (b < h_ctas)
     pack_rows<T, O>(h, D, Kp, (int64_t)b * 256 + threadIdx.x, (int64_t)h_ctas * 256);
   else

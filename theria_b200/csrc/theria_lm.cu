@@ -475,7 +475,8 @@ int xent_check(int64_t N, int64_t V, int64_t D, int dtype, int reduction) {
 struct XentRows {  // filled by prep_kernel
   int *pos, *row_of, *tgt, *n_live;
   unsigned* done;
-  float *lse, *rowscale, *less, *post;  // backward
+  float4* row;  // backward, by packed row (see RowArgs)
+  float *post, *most;
   xent::Splits *plan_h, *plan_w;
 };
 XentRows xent_rows(Carver& c, int64_t N) {
@@ -483,12 +484,11 @@ XentRows xent_rows(Carver& c, int64_t N) {
   r.pos = c.take<int>(N);
   r.row_of = c.take<int>(N);
   r.tgt = c.take<int>(N);
-  r.lse = c.take<float>(2 * N);
-  r.rowscale = c.take<float>(N);
-  r.less = c.take<float>(N);
+  r.row = c.take<float4>(N);
   r.n_live = c.take<int>(64);  // and what else is one value
   r.done = (unsigned*)r.n_live + 1;
   r.post = (float*)r.n_live + 2;
+  r.most = r.post + 1;
   r.plan_h = (xent::Splits*)(r.n_live + 4);
   r.plan_w = r.plan_h + 1;
   return r;
@@ -632,9 +632,10 @@ struct Tc {
   static bool plain(const void* h, int64_t D, const XentSizes& z) {
     return z.planes == 1 && D % 8 == 0 && tc::aligned16(h);
   }
-  // h (the rows that count) and, where it is not read as it is, w
-  static int pack(const void* h, const void* w, const XentRows& r, void* hp, void* wp,
-                  const XentSizes& z, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
+  // h (the rows that count) and, where it is not read as it is, w; and `rows`
+  static int pack(const void* h, const void* w, const XentRows& r, const xent::RowArgs& rows,
+                  void* hp, void* wp, const XentSizes& z, int64_t N, int64_t V, int64_t D,
+                  cudaStream_t st) {
     const int dtype = std::is_same<O, float>::value ? THERIA_F32 : op;
     const int64_t units = z.Kp / 8;
     auto ctas = [&](int64_t rows) {
@@ -644,7 +645,7 @@ struct Tc {
     const xent::PackArgs pw{w, wp, nullptr, nullptr, V, vec_rows(D, dtype, {w}), 0};
     const int h_ctas = ctas(z.Mp), w_ctas = z.pack_w ? ctas(V) : 0;
     return launch_chained(xent::pack_kernel<T, O>, dim3(h_ctas + w_ctas), dim3(256), 0, st, ph, pw,
-                          h_ctas, D, z.Kp);
+                          rows, h_ctas, D, z.Kp);
   }
   // dh and dw from their partial sums (either may have no rows)
   static int sum(const xent::SumArgs& a, const xent::SumArgs& b, const float* post,
@@ -675,7 +676,7 @@ struct Tc {
   static int fwd(const void* h, const void* w, const XentFwdWs& ws, const XentSizes& z,
                  const LossOut& out, int64_t N, int64_t V, int64_t D, cudaStream_t st) {
     xent::TcArgs a = common(h, ws.rows, z, N, V, D);
-    if (int e = pack(h, w, ws.rows, ws.hp, ws.wp, z, N, V, D, st)) return e;
+    if (int e = pack(h, w, ws.rows, {}, ws.hp, ws.wp, z, N, V, D, st)) return e;
     const int64_t row = z.Kp * z.planes;
     CUtensorMap ma, mb, mh;
     if (!map_2d(&ma, ws.hp, op, row, z.Mp, xent::HALF) ||
@@ -694,11 +695,14 @@ struct Tc {
     return xent_join(ws.rows, ws.part, ws.zt, a.sub_tiles, out, N, st);
   }
 
-  static int bwd(const void* h, const void* w, const XentBwdWs& ws, const XentSizes& z, void* dh,
-                 void* dw, int64_t N, int64_t V, int64_t D, int dtype, cudaStream_t st) {
+  // gloss: the rows' upstream gradients; NULL where there is one for all
+  static int bwd(const void* h, const void* w, const float* lse, const float* gloss,
+                 const XentBwdWs& ws, const XentSizes& z, void* dh, void* dw, int64_t N,
+                 int64_t V, int64_t D, int dtype, cudaStream_t st) {
     const XentRows& r = ws.rows;
     const xent::TcArgs base = common(h, r, z, N, V, D);
-    if (int e = pack(h, w, r, ws.hp, ws.wp, z, N, V, D, st)) return e;
+    const xent::RowArgs rows{lse, gloss, r.most, op == THERIA_F16 ? xent::HALF_SCALE : 1.f, r.row};
+    if (int e = pack(h, w, r, rows, ws.hp, ws.wp, z, N, V, D, st)) return e;
     const int64_t row = z.Kp * z.planes, zrow = z.piece * z.planes;
     const void* wsrc = z.pack_w ? ws.wp : w;
     const int64_t wrow = z.pack_w ? row : D;
@@ -730,9 +734,7 @@ struct Tc {
       xent::TcArgs a = base;
       a.c0 = (int)c0;
       a.Cn = (int)C;
-      a.lse = r.lse;
-      a.rowscale = r.rowscale;
-      a.less = r.less;
+      a.row = r.row;
       a.ld_dz = (int)z.piece;
       a.plan = r.plan_h;
       a.ld_acc = (int)z.ld_acc;
@@ -742,8 +744,8 @@ struct Tc {
       if (int e = tc_launch<T, O, xent::kDz>(hk, wk, hk1, zo, zp, a, mt * ct, st)) return e;
       a.plane_a = (int)z.piece;
       if (dh)
-        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, ho, a, std::max<int64_t>(mt * dt, kClusters),
-                                                st))
+        if (int e = tc_launch<T, O, xent::kDh>(zk, wm, zk, ho, ho, a,
+                                                std::max<int64_t>(mt * dt, kClusters), st))
           return e;
       if (!dw) continue;
       a.plan = z.split_w ? r.plan_w : nullptr;
@@ -836,13 +838,10 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   const XentRows& r = ws.rows;
   xent::Prep p = xent_prep(r, target, wide, ignore_index, N, V);
   p.gloss = gloss;
-  p.lse_in = lse;
   p.mean_of = reduction == THERIA_LOSS_MEAN ? count : nullptr;
   p.per_row = reduction == THERIA_LOSS_NONE;
   p.half = dtype == THERIA_F16;
-  p.lse_p = r.lse;
-  p.rowscale = r.rowscale;
-  p.less = r.less;
+  p.most = r.most;
   p.post = r.post;
   p.plan_h = dh ? r.plan_h : nullptr;
   p.plan_w = dw && z.split_w ? r.plan_w : nullptr;
@@ -853,11 +852,13 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   p.ld_acc = (int)z.ld_acc;
   xent::prep_kernel<<<1, 1024, 0, st>>>(p);
   if (int e = launch_status()) return e;
-  return dtype == THERIA_F32
-             ? Tc<__nv_bfloat16, float>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
-         : dtype == THERIA_F16
-             ? Tc<__half, __half>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st)
-             : Tc<__nv_bfloat16, __nv_bfloat16>::bwd(h, w, ws, z, dh, dw, N, V, D, dtype, st);
+  auto run = [&](auto tc) {
+    return decltype(tc)::bwd(h, w, lse, p.per_row ? gloss : nullptr, ws, z, dh, dw, N, V, D, dtype,
+                             st);
+  };
+  return dtype == THERIA_F32   ? run(Tc<__nv_bfloat16, float>{})
+         : dtype == THERIA_F16 ? run(Tc<__half, __half>{})
+                               : run(Tc<__nv_bfloat16, __nv_bfloat16>{});
 }
 
 }  // extern "C"
