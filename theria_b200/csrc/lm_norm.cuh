@@ -527,7 +527,7 @@ bwd_batch_kernel(const T* __restrict__ x, const void* __restrict__ w, int wf32,
     const T* sg = sx + ROWS * D;
     const int64_t r0 = blk * ROWS + q * R;
     const float* row_stats =
-        reinterpret_cast<const float*>(sx + (2 * ROWS - q * R) * D) + 4 * q * R;
+        reinterpret_cast<const float*>(sx - q * R * D + 2 * ROWS * D) + 4 * q * R;
     float s[2 * R];
     Pair su[R], sh[R];
 #pragma unroll
