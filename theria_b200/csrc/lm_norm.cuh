@@ -21,11 +21,16 @@
 // float32; each result is rounded once.  The sums over rows go through per-CTA
 // partials added by a second kernel in a fixed order: the same bits every time.
 //
-// Measured: 16384 x 4096 bfloat16 forward 56 us (4.8 TB/s; bound by the latency
-// of a row's two reductions), backward 87 us (4.6 TB/s; by instruction issue) and
-// 6 us for the column sums; float32 85 us (6.3 TB/s) and 130 (6.2 TB/s).  Rows
-// that are no 16-byte vectors go value by value: 32768 x 1111 float16 104 us (1.4
-// TB/s) and 225.
+// Measured: 16384 x 4096 bfloat16 forward 54 us (5.0 TB/s), backward 78 us (5.1
+// TB/s) and 3 us for the column sums, second derivative 243 us (2.8 TB/s);
+// float32 83 us (6.5 TB/s), 128 (6.3) and 305 (4.4).  By its counters no unit is
+// full in either 16-bit direction: the forward issues in 67 % of its cycles (19
+// instructions a value), and its warps, 46 % of the most an SM holds, mostly wait
+// for loads; the backward issues in 62 % (25 instructions a value), uses 45 % of
+// the shared-memory pipe and 57 % of DRAM.  For each of its instructions 2.6 warps
+// stand ready but not chosen and 1.7 wait for the arithmetic pipe: work in bursts,
+// between the barriers of a batch's rows.  Rows that are no 16-byte vectors go
+// value by value: 32768 x 1111 float16 104, 132 and 460 us.
 #pragma once
 
 #include "common.cuh"

@@ -29,12 +29,13 @@
 // product and has either sign.  (Cut toward zero instead, the planes left out
 // up to 2^-21, always of the product's sign: a bias.)
 //
-// Measured (bfloat16, one launch alone): 8192 x 32768 x 2048 scores 716 us (1535
-// TFLOP/s), dz 737, dh 721, dw 720 us; tensor pipe about 80 % busy.  Bound by the
+// Measured (bfloat16, one launch alone): 8192 x 32768 x 2048 scores 723 us (1520
+// TFLOP/s), dz 749, dh 736, dw 732 us; tensor pipe about 80 % busy.  Bound by the
 // tensor cores (by the power cap in a long run) from a width of about 512 on;
 // below it by the exponentials of the scores' epilogue and by dz in HBM (8192 x
-// 32768 x 64: scores 125 us, of which 60 the exponentials; dz 137, dh 98, dw 104,
-// of which 82 each its 537 MB).
+// 32768 x 64: scores 130 us, of which 60 the exponentials; dz 147, dh 96, dw 97,
+// of which 82 each its 537 MB).  Taking the maximum off each score before the
+// factor log2(e), instead of one fused step, costs 4 % of those 130 us.
 #pragma once
 
 #include "common.cuh"
@@ -240,7 +241,8 @@ __device__ __forceinline__ void split3(float x, __nv_bfloat16 (&p)[3]) {
 // Over many words the scores' sums are larger and the same bias is less of them
 // (131,072 words, width 4096: 4.8e-7), and the second read of the accumulators
 // costs up to 8 % under the power cap: not where there are more tiles than
-// DEEP_UNITS.
+// DEEP_UNITS.  dz's scores of 16-bit operands go without: an error of a score is
+// one of its p relative to p, and the target's p - 1 is not made from them.
 constexpr int F32_CHUNK = 4, DEEP_CHUNK = 16, DEEP = 1024, DEEP_UNITS = 4 * CLUSTERS;
 
 // T: the operands' type.  O: the type of the user's tensors (float32 with T =
@@ -638,8 +640,10 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
 #pragma unroll
           for (int c = 0; c < SUB / 32; ++c) {
             tc::tmem_wait32(raw[c & 1]);
-            if (c + 1 < SUB / 32) tc::tmem_start32(src + buf * ACC_COLS + (c + 1) * 32, raw[(c + 1) & 1]);
-            else give_back(buf);
+            if (c + 1 < SUB / 32)
+              tc::tmem_start32(src + buf * ACC_COLS + (c + 1) * 32, raw[(c + 1) & 1]);
+            else
+              give_back(buf);
             float v[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(raw[c & 1][i]);

@@ -356,15 +356,15 @@ int theria_norm_bwd(const void* x, const void* w, int wdtype, const void* gy,
           const int64_t row = 2 * D * (int64_t)sizeof(T);  // of x and gy
           if (2 * (row + 16) <= 201 << 10) {  // and the row's statistics
             // Rows of a batch: 4 for a warp of its own and where they make a
-            // stage of at most 16 KB (65536 x 1024 bfloat16: 80 us, with 2 rows
-            // 86, with one 103), 2 up to 32 KB (16384 x 4096 bfloat16: 93 us,
-            // with one 103, with 4 115), else 1.
+            // stage of at most 16 KB (65536 x 1024 bfloat16: 73 us, with 2 rows
+            // 80, with one 97), 2 up to 32 KB (16384 x 4096 bfloat16: 78 us,
+            // with one 94, with 4 106), else 1.
             auto batch = [&](auto rc) {
               constexpr int R = decltype(rc)::value;
               auto kern = norm::bwd_batch_kernel<T, VEC, NV, NW, R>;
               const int64_t rows = B::rows * R, stage = rows * row;
               // float32 rows need more bytes on their way (16384 x 4096: 128 KB
-              // 130 us, 96 KB 143), 16-bit rows a second CTA (93 us, 100)
+              // 128 us, 96 KB 140), 16-bit rows a second CTA (78 us, 82)
               const int64_t ring = (sizeof(T) == 4 ? 128 : 96) << 10;
               const int stages = (int)std::clamp<int64_t>(ring / stage, 2, norm::MAX_STAGES);
               const int64_t smem = std::max(sums, (stage + 16 * rows) * stages);
