@@ -2,7 +2,8 @@
  * theria_lm.h -- C ABI of the language-model operators around the attention
  * (libtheria_sm100.so): the scaled token embedding, the layer norm of any
  * width, and the linear layer to the vocabulary fused with its softmax cross
- * entropy, each with its gradient.
+ * entropy, rotary positions, and the gradients' global norm and clipping, each
+ * with its gradient.
  *
  * Raw device pointers to contiguous row-major tensors, int64 sizes, dtype
  * codes THERIA_F32 / THERIA_F16 / THERIA_BF16 (theria_sdpa.h), cudaStream_t
@@ -101,6 +102,52 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
                     const float* count, void* dh, void* dw, void* workspace,
                     int64_t workspace_bytes, int64_t N, int64_t V, int64_t D, int dtype,
                     void* stream);
+
+/* ------------------------------------------------------- rotary positions
+ * Pair m of a head's first 2 * pairs values turns by the angle t *
+ * frequencies[m] (float64, device memory) at position t: (a, b) -> amplitude *
+ * (a cos - b sin, b cos + a sin), the values behind pass through; `back` != 0
+ * turns the other way (the gradient).  Pairs are (2m, 2m + 1) if `interleaved`,
+ * else (m, m + pairs).
+ *
+ * q, yq [B, T, Hq, D] and k, yk [B, T, Hk, D] (either with no heads) lie at
+ * strides[12] elements (host memory): batch, token and head of q, of yq, of k,
+ * of yk; a head's D values side by side.  yq may not overlap q, nor yk k.
+ *
+ * Positions (int64 if `wide`, else int32): positions[n_positions], token i of
+ * B * T taking positions[i % n_positions]; or offsets[S + 1] of S packed
+ * sequences in each T, counting from its sequence's first token (0 for a token
+ * of none); or neither, counting from the first of T.  D <= 4096. */
+int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_t* strides,
+                  int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int dtype,
+                  const void* positions, int64_t n_positions, const void* offsets, int64_t S,
+                  int wide, const double* frequencies, int64_t pairs, float amplitude,
+                  int interleaved, int back, void* stream);
+
+/* ---------------------------------------------- gradient norm and clipping
+ * n tensors: arrays (host memory) of their device pointers, their numbers of
+ * values, and dtype codes; tensor i of every pointer array has dtypes[i].
+ *
+ * parts receives theria_grads_parts(sizes, n) float64 sums that add up to the
+ * sum of x * u over all values of all tensors (u NULL: of x * x). */
+int64_t theria_grads_parts(const int64_t* sizes, int64_t n);
+int theria_grads_dot(const void* const* x, const void* const* u, const int64_t* sizes,
+                     const int* dtypes, int64_t n, double* parts, void* stream);
+
+/* From the sums of x * x: norm [1] = their root (may be NULL), y = c x with c =
+ * min(1, max_norm / norm), stats [2] = {norm, c} (NULL: not wanted; norm or
+ * stats is).  y NULL: the norm alone.  y may be x.  With a norm that is NaN every
+ * y is NaN; with an infinite one c is 0. */
+int theria_grads_clip(const void* const* x, void* const* y, const int64_t* sizes,
+                      const int* dtypes, int64_t n, const double* parts, double max_norm,
+                      float* norm, double* stats, void* stream);
+
+/* dx of <y, u> + gnorm * norm: parts from theria_grads_dot(x, u), stats from the
+ * clip.  u (with parts) or gnorm may be NULL (zero). */
+int theria_grads_clip_bwd(const void* const* x, const void* const* u, void* const* dx,
+                          const int64_t* sizes, const int* dtypes, int64_t n,
+                          const double* parts, const double* stats, const float* gnorm,
+                          void* stream);
 
 #ifdef __cplusplus
 }

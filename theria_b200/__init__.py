@@ -8,6 +8,7 @@ a C ABI (include/theria_sdpa.h, libtheria_sm100.so).
 """
 
 from theria_b200._lib import check_device_error  # noqa: F401
+from theria_b200.attention.ragged import sdpa_ragged  # noqa: F401
 from theria_b200.autograd.sdpa_function import sdpa  # noqa: F401
 
 __version__ = "0.1.0"

@@ -31,9 +31,10 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> (restype, argtypes); must mirror include/theria_sdpa.h,
-# include/theria_ln.h and include/theria_lm.h exactly.
+# include/theria_ln.h, include/theria_lm.h and include/theria_ragged.h exactly.
 SIGNATURES = {
     "theria_status_string": (ctypes.c_char_p, [_i]),
     "theria_version": (ctypes.c_char_p, []),
@@ -78,6 +79,16 @@ SIGNATURES = {
     "theria_xent_bwd_workspace_bytes": (_i64, [_i64] * 3 + [_i]),
     "theria_xent_bwd": (_i, [_vp, _vp, _vp, _i, _i64, _i] + [_vp] * 6 + [_i64, _i64, _i64, _i64,
                                                                         _i, _vp]),
+    "theria_rotary": (_i, [_vp] * 5 + [_i64] * 5 + [_i, _vp, _i64, _vp, _i64, _i, _vp, _i64, _f,
+                                                    _i, _i, _vp]),
+    "theria_grads_parts": (_i64, [_vp, _i64]),
+    "theria_grads_dot": (_i, [_vp] * 4 + [_i64, _vp, _vp]),
+    "theria_grads_clip": (_i, [_vp] * 4 + [_i64, _vp, _d, _vp, _vp, _vp]),
+    "theria_grads_clip_bwd": (_i, [_vp] * 5 + [_i64] + [_vp] * 4),
+    "theria_ragged_fwd_workspace_bytes": (_i64, [_i64] * 4),
+    "theria_ragged_fwd": (_i, [_vp] * 5 + [_i] + [_vp] * 3 + [_i64] * 6 + [_i, _f, _i, _vp]),
+    "theria_ragged_bwd_workspace_bytes": (_i64, [_i64] * 5),
+    "theria_ragged_bwd": (_i, [_vp] * 5 + [_i] + [_vp] * 7 + [_i64] * 6 + [_i, _f, _i, _vp]),
     "theria_get_device_error": (_i, [ctypes.POINTER(ctypes.c_int), _vp]),
     "theria_clear_device_error": (_i, [_vp]),
     "theria_diag_bounded_wait": (_i, [_i, _vp, _vp]),

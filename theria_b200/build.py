@@ -2,8 +2,8 @@
 
     python -m theria_b200.build [--verbose]
 
-The library is two translation units (csrc/theria_sm100.cu, csrc/theria_lm.cu)
-compiled side by side for ``arch=compute_100a,code=sm_100a``; nvcc
+The library is three translation units (csrc/theria_sm100.cu, csrc/theria_lm.cu,
+csrc/theria_ragged.cu) compiled side by side for ``arch=compute_100a,code=sm_100a``; nvcc
 cross-compiles them on a machine without a GPU.  The output lands next to this
 file so it travels with the source tree.
 """
@@ -21,7 +21,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtheria_sm100.so")
 ROOT = os.path.dirname(HERE)
 OBJ = os.path.join(HERE, "_build")
-UNITS = ("theria_sm100", "theria_lm")
+UNITS = ("theria_sm100", "theria_lm", "theria_ragged")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -56,11 +56,13 @@ def _newer(out, deps):
 
 
 def _deps(unit):
-    # the language-model headers (csrc/lm_*) belong to theria_lm alone
-    own = [p for p in sources() if os.path.basename(p).startswith("lm_")]
+    # the headers csrc/lm_* belong to theria_lm alone, csrc/ragged_* to theria_ragged
+    def belongs(p):
+        first = os.path.basename(p).split("_")[0]
+        return first not in ("lm", "ragged") or unit == "theria_" + first
     cu = os.path.join(CSRC, unit + ".cu")
-    deps = [p for p in sources() if p.endswith(".cuh") and p not in own]
-    return [cu] + deps + (own if unit == "theria_lm" else []) + headers() + [__file__]
+    deps = [p for p in sources() if p.endswith(".cuh") and belongs(p)]
+    return [cu] + deps + headers() + [__file__]
 
 
 def up_to_date():

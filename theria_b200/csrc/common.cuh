@@ -116,8 +116,8 @@ inline int64_t elem_size(int dtype) { return dtype == THERIA_F32 ? 4 : 2; }
 
 // Device-side error word (one per device that loads the library); a kernel
 // whose bounded wait runs out sets it instead of spinning forever, as does one
-// that meets a token id outside the vocabulary.  Each of the library's two
-// translation units has its own; theria_get_device_error reads both.
+// that meets a token id outside the vocabulary.  Each of the library's three
+// translation units has its own; theria_get_device_error reads them all.
 static __device__ int g_device_error = 0;
 
 }  // namespace theria

@@ -1,0 +1,370 @@
+// Attention over packed sequences on the CUDA cores: float32 (always in
+// float32), and 16-bit tensors that the tensor-core kernels cannot take
+// (more than 64 query heads a key head, or rows off 16-byte boundaries).
+//
+// Tiles of 64 rows by 64 columns, 16 x 16 threads: a thread holds 4 x 4 of the
+// tile's scores (rows 4 ty + i, columns tx + 16 j) and, of the sums over its
+// columns, the same 4 rows of DT / 16 values.  Operands lie in shared memory as
+// float32 rows of DT + 4 values: a step of 4 along a row is one 16-byte load,
+// free of bank conflicts down the columns' 16 rows.  A score step of 4 costs 8
+// such loads for 64 products, a sums step of 4 columns 4 + 4 * DT / 64 for 16 *
+// DT / 16 * 4; the loads and the FMA pipe are about evenly used.
+//
+// The backward is one kernel for both sides.  Its tile stays on 64 rows x1, x2
+// and walks over tiles of 64 y1, y2:
+//     queries: x = (q, do), y = (k, v):  dq += ds k
+//     keys:    x = (k, v), y = (q, do):  dk += ds^T q, dv += p^T do
+// so no sum is shared between blocks and nothing is added atomically.
+#pragma once
+
+#include "ragged_plan.cuh"
+#include "tc_common.cuh"
+
+namespace theria {
+namespace ragged {
+
+constexpr int SR = 64;             // rows and columns of a tile
+constexpr int SIMT_THREADS = 256;
+
+template <int DT>
+struct SimtSmem {
+  static constexpr int kRow = DT + 4;            // floats of an operand's row
+  static constexpr int kTile = SR * kRow;
+  static constexpr int kS = SR * (SR + 4);       // a tile of scores
+  static constexpr int kFwd = (3 * kTile + kS) * 4;
+  static constexpr int kBwd = (4 * kTile + 2 * kS + 2 * SR) * 4;
+};
+
+// 64 rows of a tensor into shared memory as float32, zero beyond row `n` and
+// column D.  row_at(r): the element where row r starts.
+template <typename T, int DT, typename F>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int n, int D, F row_at) {
+  for (int i = threadIdx.x; i < SR * DT; i += SIMT_THREADS) {
+    const int r = i / DT, d = i % DT;
+    dst[r * SimtSmem<DT>::kRow + d] = r < n && d < D ? to_f32<T>(src[row_at(r) + d]) : 0.f;
+  }
+}
+
+// s[i][j] = x[4 ty + i] . y[tx + 16 j]
+template <int DT>
+__device__ __forceinline__ void tile_scores(float (&s)[4][4], const float* x, const float* y) {
+  constexpr int K = SimtSmem<DT>::kRow;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DT; d += 4) {
+    float4 a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(x + (4 * ty + i) * K + d);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(y + (tx + 16 * j) * K + d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+        s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+        s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+        s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+      }
+  }
+}
+
+// The columns of DT that a thread sums: DT / 16 of them, in runs of up to 4.
+template <int DT>
+struct Cols {
+  static constexpr int n = DT / 16;
+  static constexpr int run = n < 4 ? n : 4;
+  __device__ static int at(int c) {  // column of the thread's value c
+    return (c / run) * (16 * run) + (threadIdx.x & 15) * run + c % run;
+  }
+};
+
+// acc[i][c] += sum over the tile's columns e of p[4 ty + i][e] * y[e][column c]
+template <int DT>
+__device__ __forceinline__ void tile_sums(float (&acc)[4][DT / 16], const float* p,
+                                          const float* y) {
+  constexpr int K = SimtSmem<DT>::kRow, KS = SR + 4, RUN = Cols<DT>::run;
+  const int ty = threadIdx.x >> 4;
+#pragma unroll 2
+  for (int e = 0; e < SR; e += 4) {
+    float4 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * KS + e);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float* row = y + (e + u) * K;
+#pragma unroll
+      for (int c = 0; c < DT / 16; c += RUN) {
+        float b[RUN];
+        if constexpr (RUN == 4) {
+          const float4 t = *reinterpret_cast<const float4*>(row + Cols<DT>::at(c));
+          b[0] = t.x; b[1] = t.y; b[2] = t.z; b[3] = t.w;
+        } else if constexpr (RUN == 2) {
+          const float2 t = *reinterpret_cast<const float2*>(row + Cols<DT>::at(c));
+          b[0] = t.x; b[1] = t.y;
+        } else {
+          b[0] = row[Cols<DT>::at(c)];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float pi = u == 0 ? a[i].x : u == 1 ? a[i].y : u == 2 ? a[i].z : a[i].w;
+#pragma unroll
+          for (int x = 0; x < RUN; ++x) acc[i][c + x] = fmaf(pi, b[x], acc[i][c + x]);
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ void put_scores(float* p, const float (&s)[4][4]) {
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[(4 * ty + i) * (SR + 4) + tx + 16 * j] = s[i][j];
+}
+
+template <typename T, int DT>
+__global__ void __launch_bounds__(SIMT_THREADS)
+simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                T* __restrict__ o, float* __restrict__ lse, const int4* items, const int* count,
+                Problem pr) {
+  using L = SimtSmem<DT>;
+  extern __shared__ float4 smem4[];
+  float* xs = reinterpret_cast<float*>(smem4);
+  float *ks = xs + L::kTile, *vs = ks + L::kTile, *ps = vs + L::kTile;
+  grid_wait();
+  const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
+  if (tile >= *count) return;
+  const int4 it = items[tile];
+  const int G = pr.G, len = it.y, first = it.z;
+  const int rows = min(SR, (int)min((int64_t)len * G - first, (int64_t)SR));
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  load_tile<T, DT>(xs, q, rows, pr.D, [&](int r) {
+    const int p = first + r;
+    return (int64_t)(it.x + p / G) * pr.q_t + (int64_t)(hk * G + p % G) * pr.q_h;
+  });
+  const int last = (first + rows - 1) / G;  // the last row's token
+  const int keys = pr.causal ? last + 1 : len;
+  const float c = pr.scale * kLog2e;
+  float m[4], l[4], acc[4][DT / 16];
+  int lim[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    lim[i] = pr.causal ? min((first + 4 * ty + i) / G + 1, len) : len;
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) acc[i][x] = 0.f;
+  }
+  for (int j0 = 0; j0 < keys; j0 += SR) {
+    const int n = min(SR, len - j0);
+    __syncthreads();
+    load_tile<T, DT>(ks, k, n, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
+    });
+    load_tile<T, DT>(vs, v, n, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
+    });
+    __syncthreads();
+    float s[4][4];
+    tile_scores<DT>(s, xs, ks);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mt = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = j0 + tx + 16 * j < lim[i] ? s[i][j] * c : -INFINITY;
+        mt = fmaxf(mt, s[i][j]);
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
+      const float mn = fmaxf(m[i], mt), sub = mn == -INFINITY ? 0.f : mn;
+      const float alpha = exp2f(m[i] - sub);
+      m[i] = mn;
+      float rs = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = exp2f(s[i][j] - sub);
+        rs += s[i][j];
+      }
+      l[i] = l[i] * alpha + rs;
+#pragma unroll
+      for (int x = 0; x < DT / 16; ++x) acc[i][x] *= alpha;
+    }
+    put_scores(ps, s);
+    __syncthreads();
+    tile_sums<DT>(acc, ps, vs);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float sum = l[i];
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int r = 4 * ty + i;
+    if (r >= rows) continue;
+    const int p = first + r;
+    const int64_t row = (int64_t)(it.x + p / G) * pr.H + hk * G + p % G;
+    const float inv = 1.f / sum;
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) {
+      const int d = Cols<DT>::at(x);
+      if (d < pr.D) o[row * pr.D + d] = from_f32<T>(acc[i][x] * inv);
+    }
+    if (lse != nullptr && tx == 0) lse[row] = (m[i] + log2f(sum)) * kLn2;
+  }
+}
+
+// terms[row] = {-lse * log2(e), -rowsum(do * o)} for every row [T, H], a warp a
+// row.  Rows of no sequence get whatever their memory holds: no tile reads them.
+template <typename T>
+__global__ void __launch_bounds__(256)
+terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse,
+             float2* __restrict__ terms, int64_t rows, int D) {
+  grid_launch();
+  grid_wait();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
+       r += (int64_t)gridDim.x * 8) {
+    float z = 0.f;
+    for (int d = lane; d < D; d += 32)
+      z = fmaf(to_f32<T>(o[r * D + d]), to_f32<T>(dout[r * D + d]), z);
+    z = warp_sum(z);
+    if (lane == 0) terms[r] = make_float2(-lse[r] * kLog2e, -z);
+  }
+}
+
+// One split of a backward tile (see above).  part: NULL where there is one
+// split (results rounded to T at once), else float32 [splits][2][T * Hkv][D].
+template <typename T, int DT, bool KEYS>
+__global__ void __launch_bounds__(SIMT_THREADS)
+simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
+                const T* __restrict__ dout, const float2* terms, T* __restrict__ out1,
+                T* __restrict__ out2, float* part, const int4* items, const int* count,
+                Problem pr) {
+  using L = SimtSmem<DT>;
+  extern __shared__ float4 smem4[];
+  float* x1 = reinterpret_cast<float*>(smem4);
+  float *x2 = x1 + L::kTile, *y1 = x2 + L::kTile, *y2 = y1 + L::kTile;
+  float *ps = y2 + L::kTile, *ds = ps + L::kS;
+  float2* ts = reinterpret_cast<float2*>(ds + L::kS);
+  grid_wait();
+  const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
+  if (tile >= *count) return;
+  const int4 it = items[tile];
+  const int G = pr.G, len = it.y, first = it.z;
+  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int64_t q_rows = (int64_t)len * G;
+  const int rows = (int)min((int64_t)SR, (KEYS ? len : q_rows) - first);
+  auto q_at = [&](int64_t p, int64_t st, int64_t sh) {
+    return (it.x + p / G) * st + (hk * G + p % G) * sh;
+  };
+  auto load_q = [&](float* a, float* b, int64_t p0, int n) {
+    load_tile<T, DT>(a, q, n, pr.D, [&](int r) { return q_at(p0 + r, pr.q_t, pr.q_h); });
+    load_tile<T, DT>(b, dout, n, pr.D,
+                     [&](int r) { return q_at(p0 + r, (int64_t)pr.H * pr.D, pr.D); });
+    if (threadIdx.x < SR)
+      ts[threadIdx.x] = (int)threadIdx.x < n ? terms[q_at(p0 + threadIdx.x, pr.H, 1)]
+                                             : make_float2(-INFINITY, 0.f);
+  };
+  auto load_k = [&](float* a, float* b, int j0, int n) {
+    load_tile<T, DT>(a, k, n, pr.D,
+                     [&](int r) { return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h; });
+    load_tile<T, DT>(b, v, n, pr.D,
+                     [&](int r) { return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h; });
+  };
+  if (KEYS) load_k(x1, x2, first, rows); else load_q(x1, x2, first, rows);
+  // the tiles of y, and this split's share of them
+  int64_t y_from = 0, y_to = KEYS ? q_rows : len;
+  if (pr.causal && KEYS) y_from = (int64_t)first * G;
+  if (pr.causal && !KEYS) y_to = (first + rows - 1) / G + 1;
+  const int n_y = (int)((y_to - y_from + SR - 1) / SR), splits = gridDim.y;
+  const int t0 = (int)((int64_t)n_y * blockIdx.y / splits);
+  const int t1 = (int)((int64_t)n_y * (blockIdx.y + 1) / splits);
+  const float c = pr.scale * kLog2e;
+  float a1[4][DT / 16], a2[KEYS ? 4 : 1][DT / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) {
+      a1[i][x] = 0.f;
+      if (KEYS) a2[KEYS ? i : 0][x] = 0.f;
+    }
+  for (int t = t0; t < t1; ++t) {
+    const int64_t e0 = y_from + (int64_t)t * SR;
+    const int n = (int)min((int64_t)SR, (KEYS ? q_rows : len) - e0);
+    __syncthreads();
+    if (KEYS) load_q(y1, y2, e0, n); else load_k(y1, y2, (int)e0, n);
+    __syncthreads();
+    float s[4][4], dp[4][4];
+    tile_scores<DT>(s, x1, y1);
+    tile_scores<DT>(dp, x2, y2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * ty + i, e = tx + 16 * j;
+        const float2 tm = ts[KEYS ? e : r];
+        const int64_t qr = KEYS ? e0 + e : (int64_t)first + r;      // query row
+        const int64_t key = KEYS ? (int64_t)first + r : e0 + e;
+        const bool on = key < len && qr < q_rows && (!pr.causal || key <= qr / G);
+        const float p = on ? exp2f(fmaf(s[i][j], c, tm.x)) : 0.f;
+        s[i][j] = p;
+        dp[i][j] = on ? p * (dp[i][j] + tm.y) : 0.f;
+      }
+    if (KEYS) put_scores(ps, s);
+    put_scores(ds, dp);
+    __syncthreads();
+    tile_sums<DT>(a1, ds, y1);
+    if constexpr (KEYS) tile_sums<DT>(a2, ps, y2);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * ty + i;
+    if (r >= rows) continue;
+    const int64_t row = KEYS ? (int64_t)(it.x + first + r) * pr.Hkv + hk : q_at(first + r, pr.H, 1);
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) {
+      const int d = Cols<DT>::at(x);
+      if (d >= pr.D) continue;
+      if (part == nullptr) {
+        out1[row * pr.D + d] = from_f32<T>(a1[i][x] * pr.scale);
+        if constexpr (KEYS) out2[row * pr.D + d] = from_f32<T>(a2[i][x]);
+      } else {
+        const int64_t plane = (int64_t)pr.T * pr.Hkv * pr.D;
+        float* to = part + 2 * plane * blockIdx.y + row * pr.D + d;
+        to[0] = a1[i][x] * pr.scale;
+        if constexpr (KEYS) to[plane] = a2[i][x];
+      }
+    }
+  }
+}
+
+// dk, dv from the splits' float32 sums, added in the splits' order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+join_kernel(const float* part, int splits, const int* count, const void* offsets, int wide,
+            T* __restrict__ dk, T* __restrict__ dv, Problem pr) {
+  grid_wait();
+  if (*count == 0) return;
+  const int64_t row = (int64_t)pr.Hkv * pr.D, plane = row * pr.T;
+  const int64_t lo = offset_at(offsets, wide, 0) * row, hi = offset_at(offsets, wide, pr.S) * row;
+  const int64_t all = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += all) {
+    if (i < lo || i >= hi) continue;  // zeroed with the other rows of no sequence
+    float a = 0.f, b = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      a += part[2 * plane * s + i];
+      b += part[2 * plane * s + plane + i];
+    }
+    dk[i] = from_f32<T>(a);
+    dv[i] = from_f32<T>(b);
+  }
+}
+
+}  // namespace ragged
+}  // namespace theria

@@ -4,7 +4,9 @@
 
 #include "common.cuh"
 #include "lm_embed.cuh"
+#include "lm_grads.cuh"
 #include "lm_norm.cuh"
+#include "lm_rotary.cuh"
 #include "lm_xent.cuh"
 #include "lm_xent_tc.cuh"
 #include "tc_host.cuh"
@@ -859,6 +861,192 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
   return dtype == THERIA_F32   ? run(Tc<__nv_bfloat16, float>{})
          : dtype == THERIA_F16 ? run(Tc<__half, __half>{})
                                : run(Tc<__nv_bfloat16, __nv_bfloat16>{});
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- rotary
+extern "C" {
+
+int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_t* strides,
+                  int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int dtype,
+                  const void* positions, int64_t n_positions, const void* offsets, int64_t S,
+                  int wide, const double* frequencies, int64_t pairs, float amplitude,
+                  int interleaved, int back, void* stream) {
+  if (B < 0 || T < 0 || Hq < 0 || Hk < 0 || D <= 0 || pairs < 0 || 2 * pairs > D || S < 0 ||
+      !lm_dtype(dtype) || (positions && (offsets || n_positions <= 0)))
+    return THERIA_ERR_INVALID_ARG;
+  if (D > 4096 || Hq + Hk > 65535 || T >= (1ll << 31) || S >= (1ll << 31) ||
+      (B > 0 && T > (1ll << 40) / B))
+    return THERIA_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0 || Hq + Hk == 0) return THERIA_OK;
+  if (!strides || (Hq > 0 && (!q || !yq)) || (Hk > 0 && (!k || !yk)) ||
+      (pairs > 0 && !frequencies))
+    return THERIA_ERR_INVALID_ARG;
+  rotary::Args a{};
+  const void* xs[2] = {q, k};
+  void* ys[2] = {yq, yk};
+  a.heads[0] = (int)Hq;
+  a.heads[1] = (int)Hk;
+  const int64_t es = elem_size(dtype), vec = 16 / es;
+  bool aligned = D % vec == 0;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = strides + 6 * i;
+    a.s[i] = rotary::Side{xs[i], ys[i], s[0], s[1], s[2], s[3], s[4], s[5]};
+    if (a.heads[i] == 0) continue;
+    aligned = aligned && tc::aligned16(xs[i]) && tc::aligned16(ys[i]);
+    for (int j = 0; j < 6; ++j) aligned = aligned && s[j] % vec == 0;
+  }
+  a.T = (int)T;
+  a.D = (int)D;
+  a.pairs = (int)pairs;
+  a.n = B * T;
+  a.positions = positions;
+  a.n_positions = n_positions;
+  a.offsets = offsets;
+  a.S = (int)S;
+  a.wide = wide;
+  a.freq = frequencies;
+  a.amplitude = amplitude;
+  a.back = back;
+  // about two angles a thread, but the tokens spread over the GPU first
+  const int64_t share = std::max<int64_t>(1, a.n / (2 * kSMs));
+  a.tokens = (int)std::max<int64_t>(
+      1, std::min<int64_t>({share, rotary::MOST_TOKENS, 512 / std::max<int64_t>(pairs, 1)}));
+  const int64_t blocks = cdiv(a.n, a.tokens);
+  if (blocks >= (1ll << 31)) return THERIA_ERR_UNSUPPORTED;
+  const size_t smem = (size_t)a.tokens * pairs * sizeof(float2);  // 16 KB at most
+  return by_type(dtype, [&](auto t) {
+    using E = decltype(t);
+    constexpr int VEC = embed::Vec<E>::n;
+    using namespace rotary;
+    auto kern = interleaved ? (aligned ? rotary_kernel<E, VEC, kInterleaved>
+                                       : rotary_kernel<E, 1, kInterleaved>)
+                : !aligned  ? rotary_kernel<E, 1, kHalvesAnywhere>
+                : pairs % VEC == 0 ? rotary_kernel<E, VEC, kHalves>
+                                   : rotary_kernel<E, VEC, kHalvesAnywhere>;
+    kern<<<(unsigned)blocks, THREADS, smem, (cudaStream_t)stream>>>(a);
+    return launch_status();
+  });
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------- gradient norm
+namespace theria {
+namespace {
+
+int grads_check(const int64_t* sizes, const int* dtypes, int64_t n) {
+  if (n < 0 || (n > 0 && (!sizes || !dtypes))) return THERIA_ERR_INVALID_ARG;
+  int64_t chunks = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    if (sizes[i] < 0 || !lm_dtype(dtypes[i])) return THERIA_ERR_INVALID_ARG;
+    chunks += cdiv(sizes[i], grads::CHUNK);
+    if (chunks >= (1ll << 30)) return THERIA_ERR_UNSUPPORTED;
+  }
+  return THERIA_OK;
+}
+
+// Calls f(table, chunks) for every group of up to MOST tensors that are not empty.
+template <typename F>
+int grads_groups(const void* const* x, const void* const* u, void* const* out,
+                 const int64_t* sizes, const int* dtypes, int64_t n, F f) {
+  grads::Table t;
+  t.n = 0;
+  int64_t chunks = 0;
+  auto flush = [&]() -> int {
+    if (t.n == 0) return THERIA_OK;
+    t.first[t.n] = (int)chunks;
+    const int e = f(t, (int)chunks);
+    t.n = 0;
+    chunks = 0;
+    return e;
+  };
+  for (int64_t i = 0; i < n; ++i) {
+    if (sizes[i] == 0) continue;
+    if (!x[i] || (u && !u[i]) || (out && !out[i])) return THERIA_ERR_INVALID_ARG;
+    const int k = t.n++;
+    t.x[k] = x[i];
+    t.u[k] = u ? u[i] : nullptr;
+    t.out[k] = out ? out[i] : nullptr;
+    t.size[k] = sizes[i];
+    t.dtype[k] = (unsigned char)dtypes[i];
+    t.vec[k] = tc::aligned16(x[i]) && tc::aligned16(t.u[k]) && tc::aligned16(t.out[k]);
+    t.first[k] = (int)chunks;
+    chunks += cdiv(sizes[i], grads::CHUNK);
+    if (t.n == grads::MOST)
+      if (int e = flush()) return e;
+  }
+  return flush();
+}
+
+}  // namespace
+}  // namespace theria
+
+extern "C" {
+
+int64_t theria_grads_parts(const int64_t* sizes, int64_t n) {
+  int64_t parts = 0, chunks = 0, k = 0;
+  for (int64_t i = 0; sizes && i < n; ++i) {
+    if (sizes[i] <= 0) continue;
+    chunks += cdiv(sizes[i], grads::CHUNK);
+    if (++k == grads::MOST) {
+      parts += std::min<int64_t>(chunks, grads::MOST_BLOCKS);
+      k = chunks = 0;
+    }
+  }
+  return parts + std::min<int64_t>(chunks, grads::MOST_BLOCKS);
+}
+
+int theria_grads_dot(const void* const* x, const void* const* u, const int64_t* sizes,
+                     const int* dtypes, int64_t n, double* parts, void* stream) {
+  if (int e = grads_check(sizes, dtypes, n)) return e;
+  if (theria_grads_parts(sizes, n) == 0) return THERIA_OK;
+  if (!x || !parts) return THERIA_ERR_INVALID_ARG;
+  return grads_groups(x, u, nullptr, sizes, dtypes, n, [&](const grads::Table& t, int chunks) {
+    const int blocks = std::min(chunks, grads::MOST_BLOCKS);
+    grads::dot_kernel<<<blocks, grads::THREADS, 0, (cudaStream_t)stream>>>(t, parts);
+    parts += blocks;
+    return launch_status();
+  });
+}
+
+int theria_grads_clip(const void* const* x, void* const* y, const int64_t* sizes,
+                      const int* dtypes, int64_t n, const double* parts, double max_norm,
+                      float* norm, double* stats, void* stream) {
+  if (int e = grads_check(sizes, dtypes, n)) return e;
+  if (!(max_norm >= 0.0)) return THERIA_ERR_INVALID_ARG;
+  const int np = (int)theria_grads_parts(sizes, n);
+  if ((np > 0 && (!x || !parts)) || (!norm && !stats)) return THERIA_ERR_INVALID_ARG;
+  cudaStream_t st = (cudaStream_t)stream;
+  auto launch = [&](const grads::Table& t, int chunks) {
+    // (two more of the launches may run beside: 8 blocks an SM)
+    return launch_chained(grads::clip_kernel, dim3(std::max(1, std::min(chunks, kSMs * 8))),
+                          dim3(grads::THREADS), 0, st, t, parts, np, max_norm, norm, stats);
+  };
+  if (y == nullptr || np == 0) {
+    grads::Table t;
+    t.n = 0;
+    return launch(t, 0);
+  }
+  return grads_groups(x, nullptr, y, sizes, dtypes, n, launch);
+}
+
+int theria_grads_clip_bwd(const void* const* x, const void* const* u, void* const* dx,
+                          const int64_t* sizes, const int* dtypes, int64_t n,
+                          const double* parts, const double* stats, const float* gnorm,
+                          void* stream) {
+  if (int e = grads_check(sizes, dtypes, n)) return e;
+  const int np = (int)theria_grads_parts(sizes, n);
+  if (np == 0) return THERIA_OK;
+  if (!x || !dx || !stats || (u && !parts) || (!u && !gnorm)) return THERIA_ERR_INVALID_ARG;
+  // the kernel's first operand is what the factor c takes
+  return grads_groups(u ? u : x, u ? x : nullptr, dx, sizes, dtypes, n,
+                      [&](const grads::Table& t, int chunks) {
+    return launch_chained(grads::clip_bwd_kernel, dim3(std::min(chunks, kSMs * 8)),
+                          dim3(grads::THREADS), 0, (cudaStream_t)stream, t, parts, u ? np : 0,
+                          stats, gnorm);
+  });
 }
 
 }  // extern "C"

@@ -1,0 +1,289 @@
+// The attention over packed sequences of include/theria_ragged.h: argument
+// checks, workspace carving and kernel selection.
+#include <algorithm>
+
+#include "common.cuh"
+#include "ragged_plan.cuh"
+#include "ragged_simt.cuh"
+#include "tc_host.cuh"
+#include "../../include/theria_ragged.h"
+
+namespace theria {
+
+// This translation unit's copy of the device error word, for
+// theria_get_device_error / theria_clear_device_error.
+int ragged_read_device_error(int* out, cudaStream_t st) {
+  return cudaMemcpyFromSymbolAsync(out, g_device_error, sizeof(int), 0, cudaMemcpyDeviceToHost,
+                                   st) == cudaSuccess
+             ? THERIA_OK
+             : THERIA_ERR_LAUNCH;
+}
+int ragged_clear_device_error(cudaStream_t st) {
+  static const int zero = 0;
+  return cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice,
+                                 st) == cudaSuccess
+             ? THERIA_OK
+             : THERIA_ERR_LAUNCH;
+}
+
+namespace ragged {
+namespace {
+
+constexpr int kSMs = 148;
+constexpr int kBlankBlocks = 32;  // CTAs that zero the rows of no sequence
+
+int64_t up(int64_t x) { return (x + 255) / 256 * 256; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Carver {
+  char* base;
+  int64_t used = 0;
+  template <typename T>
+  T* take(int64_t count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += up(count * (int64_t)sizeof(T));
+    return p;
+  }
+};
+
+// The most tiles of `step` rows that T tokens of `per` rows in S sequences make.
+int64_t most_items(int64_t T, int64_t S, int64_t per, int64_t step) {
+  return T * per / step + std::min(S, T);
+}
+// The smallest step of any kernel's list is 64 rows of packed heads.
+List take_list(Carver& c, const Problem& p, int per, int step, int by_key) {
+  List l{};
+  l.per = per;
+  l.step = step;
+  l.by_key = by_key;
+  l.items = c.take<int4>(most_items(p.T, p.S, per, step));
+  l.count = c.take<int>(1);
+  l.base = c.take<int>(p.S);
+  return l;
+}
+
+int check(const Problem& p, int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype) {
+  if (T < 0 || S < 0 || H <= 0 || Hkv <= 0 || D <= 0 || H % Hkv) return THERIA_ERR_INVALID_ARG;
+  if (dtype != THERIA_F32 && dtype != THERIA_F16 && dtype != THERIA_BF16)
+    return THERIA_ERR_INVALID_ARG;
+  if (D > THERIA_MAX_HEAD_DIM || T >= (1ll << 30) || S >= (1ll << 30) || H >= 65536 ||
+      T * H >= (1ll << 31))
+    return THERIA_ERR_UNSUPPORTED;
+  return THERIA_OK;
+}
+
+Problem problem(const int64_t* st, int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D,
+                float scale, int causal) {
+  Problem p{};
+  p.T = (int)T;
+  p.S = (int)S;
+  p.H = (int)H;
+  p.Hkv = (int)Hkv;
+  p.G = Hkv > 0 ? (int)(H / Hkv) : 0;
+  p.D = (int)D;
+  if (st != nullptr) {
+    p.q_t = st[0];
+    p.q_h = st[1];
+    p.k_t = st[2];
+    p.k_h = st[3];
+    p.v_t = st[4];
+    p.v_h = st[5];
+  }
+  p.scale = scale;
+  p.causal = causal != 0;
+  return p;
+}
+
+template <typename F>
+int by_type(int dtype, F f) {
+  if (dtype == THERIA_F32) return f(float{});
+  if (dtype == THERIA_F16) return f(__half{});
+  return f(__nv_bfloat16{});
+}
+template <typename F>
+int by_width(int D, F f) {
+  if (D <= 16) return f(std::integral_constant<int, 16>{});
+  if (D <= 32) return f(std::integral_constant<int, 32>{});
+  if (D <= 64) return f(std::integral_constant<int, 64>{});
+  return f(std::integral_constant<int, 128>{});
+}
+
+int run_plan(const void* offsets, int wide, const Problem& p, const List& a, const List& b,
+             const Blank& blank, cudaStream_t st) {
+  plan_kernel<<<2 + kBlankBlocks, kPlanThreads, 0, st>>>(offsets, wide, p.S, p.T, p.causal, a, b,
+                                                         blank);
+  return launch_status();
+}
+
+// Parts that a key tile's queries are split into: until the tiles of an even
+// batch would fill the GPU twice, and no more than 32.
+int key_splits(const Problem& p, int step) {
+  const int64_t tiles = std::max<int64_t>(1, cdiv(p.T, step) * p.Hkv);
+  return (int)std::min<int64_t>(32, std::max<int64_t>(1, 2 * kSMs / tiles));
+}
+
+struct FwdWs {
+  List list;
+  int64_t bytes;
+};
+FwdWs fwd_ws(void* base, const Problem& p) {
+  Carver c{(char*)base};
+  FwdWs w{};
+  w.list = take_list(c, p, p.G, SR, 0);
+  w.bytes = c.used;
+  return w;
+}
+
+struct BwdWs {
+  List lq, lk;
+  float2* terms;
+  float* part;
+  int splits;
+  int64_t bytes;
+};
+BwdWs bwd_ws(void* base, const Problem& p) {
+  Carver c{(char*)base};
+  BwdWs w{};
+  w.lq = take_list(c, p, p.G, SR, 0);
+  w.lk = take_list(c, p, 1, SR, 1);
+  w.terms = c.take<float2>((int64_t)p.T * p.H);
+  w.splits = key_splits(p, SR);
+  w.part = w.splits > 1 ? c.take<float>(2ll * w.splits * p.T * p.Hkv * p.D) : nullptr;
+  w.bytes = c.used;
+  return w;
+}
+
+// Blocks: the key heads of a tile side by side.
+bool grid_fits(const Problem& p) {
+  return (most_items(p.T, p.S, p.G, SR) + 1) * p.Hkv < (1ll << 31);
+}
+unsigned blocks(const Problem& p, int per, int step) {
+  return (unsigned)(std::max<int64_t>(1, most_items(p.T, p.S, per, step)) * p.Hkv);
+}
+
+template <typename T>
+int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const FwdWs& ws,
+             const Problem& p, cudaStream_t st) {
+  return by_width(p.D, [&](auto w) {
+    constexpr int DT = decltype(w)::value;
+    auto kern = simt_fwd_kernel<T, DT>;
+    constexpr int smem = SimtSmem<DT>::kFwd;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess)
+      return (int)THERIA_ERR_LAUNCH;
+    return launch_chained(kern, dim3(blocks(p, p.G, SR)), dim3(SIMT_THREADS), smem, st, (const T*)q,
+                          (const T*)k, (const T*)v, (T*)o, lse,
+                          (const int4*)ws.list.items, (const int*)ws.list.count, p);
+  });
+}
+
+template <typename T>
+int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
+             void* dv, const BwdWs& ws, const void* offsets, int wide, const Problem& p,
+             cudaStream_t st) {
+  return by_width(p.D, [&](auto w) {
+    constexpr int DT = decltype(w)::value;
+    constexpr int smem = SimtSmem<DT>::kBwd;
+    auto run = [&](auto kern, const List& l, int splits, void* o1, void* o2, float* part) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+          cudaSuccess)
+        return (int)THERIA_ERR_LAUNCH;
+      return launch_chained(kern, dim3(blocks(p, l.per, SR), (unsigned)splits), dim3(SIMT_THREADS),
+                            smem, st, (const T*)q, (const T*)k, (const T*)v,
+                            (const T*)dout, (const float2*)ws.terms, (T*)o1, (T*)o2, part,
+                            (const int4*)l.items, (const int*)l.count, p);
+    };
+    if (dq != nullptr)
+      if (int e = run(simt_bwd_kernel<T, DT, false>, ws.lq, 1, dq, nullptr, nullptr)) return e;
+    if (dk != nullptr) {
+      if (int e = run(simt_bwd_kernel<T, DT, true>, ws.lk, ws.splits, dk, dv, ws.part)) return e;
+      if (ws.part != nullptr)
+        return launch_chained(join_kernel<T>, dim3(kSMs * 4), dim3(256), 0, st,
+                              (const float*)ws.part, ws.splits, (const int*)ws.lk.count, offsets,
+                              wide, (T*)dk, (T*)dv, p);
+    }
+    return (int)THERIA_OK;
+  });
+}
+
+}  // namespace
+}  // namespace ragged
+}  // namespace theria
+
+using namespace theria;
+using namespace theria::ragged;
+
+extern "C" {
+
+int64_t theria_ragged_fwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv) {
+  const Problem p = problem(nullptr, T, S, H, Hkv, 1, 0.f, 0);
+  if (check(p, T, S, H, Hkv, 1, THERIA_F32) != THERIA_OK) return 0;
+  return fwd_ws(nullptr, p).bytes;
+}
+
+int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                      const void* offsets, int wide, void* o, float* lse, void* workspace,
+                      int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
+                      int64_t D, int dtype, float scale, int causal, void* stream) {
+  const Problem p = problem(strides, T, S, H, Hkv, D, scale, causal);
+  if (int e = check(p, T, S, H, Hkv, D, dtype)) return e;
+  if (T == 0) return THERIA_OK;
+  if (!q || !k || !v || !strides || !offsets || !o) return THERIA_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < theria_ragged_fwd_workspace_bytes(T, S, H, Hkv))
+    return THERIA_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  const FwdWs ws = fwd_ws(workspace, p);
+  if (!grid_fits(p)) return THERIA_ERR_UNSUPPORTED;
+  Blank blank{};
+  blank.p[0] = o;
+  blank.row_bytes[0] = H * D * elem_size(dtype);
+  if (int e = run_plan(offsets, wide, p, ws.list, List{}, blank, st)) return e;
+  return by_type(dtype, [&](auto t) {
+    return simt_fwd<decltype(t)>(q, k, v, o, lse, ws, p, st);
+  });
+}
+
+int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv,
+                                          int64_t D) {
+  const Problem p = problem(nullptr, T, S, H, Hkv, D, 0.f, 0);
+  if (check(p, T, S, H, Hkv, D, THERIA_F32) != THERIA_OK) return 0;
+  return bwd_ws(nullptr, p).bytes;
+}
+
+int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                      const void* offsets, int wide, const void* o, const void* dout,
+                      const float* lse, void* dq, void* dk, void* dv, void* workspace,
+                      int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
+                      int64_t D, int dtype, float scale, int causal, void* stream) {
+  const Problem p = problem(strides, T, S, H, Hkv, D, scale, causal);
+  if (int e = check(p, T, S, H, Hkv, D, dtype)) return e;
+  if ((dk == nullptr) != (dv == nullptr)) return THERIA_ERR_INVALID_ARG;
+  if (T == 0 || (dq == nullptr && dk == nullptr)) return THERIA_OK;
+  if (!q || !k || !v || !strides || !offsets || !o || !dout || !lse)
+    return THERIA_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < theria_ragged_bwd_workspace_bytes(T, S, H, Hkv, D))
+    return THERIA_ERR_WORKSPACE;
+  cudaStream_t st = (cudaStream_t)stream;
+  const BwdWs ws = bwd_ws(workspace, p);
+  if (!grid_fits(p)) return THERIA_ERR_UNSUPPORTED;
+  Blank blank{};
+  blank.p[0] = dq;
+  blank.p[1] = dk;
+  blank.p[2] = dv;
+  blank.row_bytes[0] = H * D * elem_size(dtype);
+  blank.row_bytes[1] = blank.row_bytes[2] = Hkv * D * elem_size(dtype);
+  if (int e = run_plan(offsets, wide, p, dq ? ws.lq : List{}, dk ? ws.lk : List{}, blank, st))
+    return e;
+  return by_type(dtype, [&](auto t) {
+    using E = decltype(t);
+    const int64_t rows = T * H;
+    if (int e = launch_chained(terms_kernel<E>,
+                               dim3((unsigned)std::min<int64_t>(cdiv(rows, 8), kSMs * 32)),
+                               dim3(256), 0, st, (const E*)o, (const E*)dout, lse, ws.terms, rows,
+                               (int)D))
+      return e;
+    return simt_bwd<E>(q, k, v, dout, dq, dk, dv, ws, offsets, wide, p, st);
+  });
+}
+
+}  // extern "C"

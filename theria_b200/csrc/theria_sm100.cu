@@ -1,8 +1,8 @@
 // libtheria_sm100.so: the C ABI declared in include/theria_sdpa.h.
 //
-// The library is two translation units without relocatable device code: the
-// language-model operators of include/theria_lm.h are in theria_lm.cu, and
-// this file includes the kernel headers and implements argument checking,
+// The library is three translation units without relocatable device code: the
+// language-model operators of include/theria_lm.h are in theria_lm.cu, the
+// attention of include/theria_ragged.h in theria_ragged.cu, and this file includes the kernel headers and implements argument checking,
 // workspace carving and kernel selection for each entry point.
 #include <algorithm>
 #include <cstdio>
@@ -28,6 +28,9 @@ namespace theria {
 // The device error word of theria_lm.cu's kernels.
 int lm_read_device_error(int* out, cudaStream_t st);
 int lm_clear_device_error(cudaStream_t st);
+// ... and of theria_ragged.cu's.
+int ragged_read_device_error(int* out, cudaStream_t st);
+int ragged_clear_device_error(cudaStream_t st);
 
 namespace {
 
@@ -837,13 +840,15 @@ int theria_diag_bounded_wait(int max_polls, int* out, void* stream) {
 int theria_get_device_error(int* out_flag, void* stream) {
   if (!out_flag) return THERIA_ERR_INVALID_ARG;
   cudaStream_t st = (cudaStream_t)stream;
-  int lm_flag = 0;  // the word of the other translation unit's kernels
+  int lm_flag = 0, ragged_flag = 0;  // the words of the other translation units' kernels
   if (cudaMemcpyFromSymbolAsync(out_flag, g_device_error, sizeof(int), 0,
                                 cudaMemcpyDeviceToHost, st) != cudaSuccess ||
       theria::lm_read_device_error(&lm_flag, st) != THERIA_OK ||
+      theria::ragged_read_device_error(&ragged_flag, st) != THERIA_OK ||
       cudaStreamSynchronize(st) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
   if (*out_flag == THERIA_OK) *out_flag = lm_flag;
+  if (*out_flag == THERIA_OK) *out_flag = ragged_flag;
   return THERIA_OK;
 }
 
@@ -852,7 +857,8 @@ int theria_clear_device_error(void* stream) {
   if (cudaMemcpyToSymbolAsync(g_device_error, &zero, sizeof(int), 0, cudaMemcpyHostToDevice,
                               (cudaStream_t)stream) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
-  return theria::lm_clear_device_error((cudaStream_t)stream);
+  if (int e = theria::lm_clear_device_error((cudaStream_t)stream)) return e;
+  return theria::ragged_clear_device_error((cudaStream_t)stream);
 }
 
 // ---------------------------------------------------------------------------

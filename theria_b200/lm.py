@@ -1,9 +1,11 @@
 """Language-model operators around the attention: what stands before, between
-and after the blocks of a pre-LN decoder.
+and after the blocks of a pre-LN decoder, and at the end of its training step.
 
     embedding(ids, weight, scale)                 scale * weight[ids]
     layer_norm(x, weight, bias)                   over the last axis, any width
     linear_cross_entropy(hidden, weight, target)  cross entropy of hidden @ weight.T
+    rotary(q, k, frequencies)                     rotary positions of queries and keys
+    clip_gradients(tensors, max_norm)             by their global norm
 
 Each runs hand-written kernels of libtheria_sm100.so (``include/theria_lm.h``)
 on float32, float16 and bfloat16 CUDA tensors, on torch's current stream, and
@@ -24,6 +26,9 @@ from torch modules (``examples/minimal_decoder_transformer.py:82-263``).
 """
 
 from __future__ import annotations
+
+import ctypes
+import math
 
 import torch
 from torch.autograd import forward_ad
@@ -400,4 +405,311 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, redu
     return _loss(h, w, t, int(ignore_index), _REDUCTIONS[reduction])[0]
 
 
-__all__ = ["embedding", "layer_norm", "linear_cross_entropy"]
+# --------------------------------------------------------------------- rotary
+SCALINGS = (None, "linear", "ntk", "by_parts")
+
+
+def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None,
+                       low=1.0, high=32.0, device="cuda"):
+    """The angular frequencies ``base ** (-2 m / dim)`` of the dim / 2 pairs, float64,
+    for ``rotary``; made once and kept, like a weight.
+
+    ``scaling`` stretches them for contexts ``factor`` times as long as the
+    model was trained on:
+
+    - "linear": all frequencies divided by factor (positions interpolated);
+    - "ntk": base times factor ** (dim / (dim - 2)), which divides the lowest
+      frequency by factor and keeps the highest;
+    - "by_parts": a pair that turns fewer than ``low`` times within
+      ``original_length`` is divided by factor, one that turns more than ``high``
+      times is kept, with a linear passage between them (its scores are usually
+      also sharpened by ``rotary(..., amplitude=0.1 * log(factor) + 1)``).
+    """
+    if dim <= 0 or dim % 2:
+        raise AssertionError(f"dim must be positive and even, got {dim}")
+    if scaling not in SCALINGS:
+        raise AssertionError(f"scaling must be one of {SCALINGS}")
+    if not factor > 0 or not base > 0:
+        raise AssertionError("base and factor must be positive")
+    if scaling == "ntk" and dim > 2:
+        base = base * factor ** (dim / (dim - 2))
+    m = torch.arange(0, dim, 2, dtype=torch.float64)
+    f = base ** (-m / dim)
+    if scaling == "linear":
+        f = f / factor
+    if scaling == "by_parts":
+        if original_length is None or original_length <= 0 or not high > low:
+            raise AssertionError("by_parts needs original_length, and low < high")
+        keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+        f = f / factor * (1 - keep) + f * keep
+    return f.to(device)
+
+
+def _rotary_layout(t):
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _rotate(q, k, frequencies, positions, offsets, interleaved, amplitude, back):
+    """Rotated q and k (each may be None)."""
+    out, strides = [], []
+    for x in (q, k):
+        if x is None:
+            out.append(None)
+            strides += [0] * 6
+            continue
+        x = _rotary_layout(x)
+        y = torch.empty_like(x)
+        if y.stride(-1) != 1:
+            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out.append((x, y))
+        for t in (x, y):
+            strides += t.stride()[:3] if t.ndim == 4 else (0, *t.stride()[:2])
+    x = (out[0] or out[1])[0]
+    B, T, D = x.shape[0] if x.ndim == 4 else 1, x.shape[-3], x.shape[-1]
+    at = positions if positions is not None else offsets
+    (xq, yq), (xk, yk) = (o or (None, None) for o in out)
+    _call("theria_rotary", x.device, _ptr(xq), _ptr(xk), _ptr(yq), _ptr(yk),
+          (ctypes.c_int64 * 12)(*strides), B, T, 0 if xq is None else xq.shape[-2],
+          0 if xk is None else xk.shape[-2], D, _DTYPES[x.dtype], _ptr(positions),
+          0 if positions is None else positions.numel(), _ptr(offsets),
+          0 if offsets is None else offsets.numel() - 1, 0 if at is None else _wide(at),
+          frequencies.data_ptr(), frequencies.numel(), amplitude, interleaved, back)
+    return yq, yk
+
+
+class _Rotary(torch.autograd.Function):
+    """Linear in (q, k): its backward is itself with the angles negated."""
+
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, offsets, *rest):
+        ctx.save_for_backward(frequencies, positions, offsets)
+        ctx.rest = rest
+        ctx.set_materialize_grads(False)
+        out = _rotate(q, k, frequencies, positions, offsets, *rest)
+        ctx.mark_non_differentiable(*(y for y, need in zip(out, ctx.needs_input_grad)
+                                      if y is not None and not need))
+        return out
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        what = "theria rotary"
+        _no_tangents(what, gq, gk)
+        if gq is None and gk is None:
+            return (None,) * 8
+        *rest, back = ctx.rest
+        turn = _Rotary.apply if torch.is_grad_enabled() else _rotate
+        gq, gk = turn(gq, gk, *ctx.saved_tensors, *rest, 1 - back)
+        return gq, gk, None, None, None, None, None, None
+
+
+@_opaque
+def rotary(q, k, frequencies, positions=None, offsets=None, interleaved=False, amplitude=1.0):
+    """Rotary positions: q [T, Hq, D] and k [T, Hk, D], or [B, T, H, D] each, any
+    strides (heads-first tensors are passed as ``q.transpose(1, 2)``, and come back
+    in the same order of memory); k may be None.  Returns the pair, or q alone.
+
+    The pair m of each head's first ``2 * len(frequencies)`` values turns by
+    ``position * frequencies[m]`` and is multiplied by ``amplitude``; the values
+    behind pass through.  Pairs are (m, m + len(frequencies)), or with
+    ``interleaved`` (2 m, 2 m + 1).  ``frequencies`` is float64 (see
+    ``rotary_frequencies``); angles are reduced in float64, so positions may be far.
+
+    Positions: ``positions`` (int64 or int32) [T] or [B, T]; or ``offsets`` [S + 1]
+    of packed sequences, each counted from its first token (tokens of no sequence
+    stand at 0); else 0 .. T - 1.  Differentiable in q and k, any number of times.
+    """
+    what = "theria rotary"
+    _check(what, "q", q)
+    if q.ndim not in (3, 4) or q.shape[-1] == 0:
+        raise AssertionError("q must have shape (T,H,D) or (B,T,H,D)")
+    if k is not None:
+        _check(what, "k", k, q.device)
+        if k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+            raise AssertionError("k must have q's shape up to the number of heads")
+        if k.dtype != q.dtype:
+            raise AssertionError("q and k must share one dtype")
+    if frequencies.dtype is not torch.float64 or frequencies.device != q.device:
+        raise AssertionError("frequencies must be float64 on q's device")
+    if frequencies.ndim != 1 or 2 * frequencies.numel() > q.shape[-1]:
+        raise AssertionError("frequencies must have shape (pairs,) with 2 * pairs <= D")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise AssertionError("theria rotary has no gradient for its frequencies")
+    if positions is not None and offsets is not None:
+        raise AssertionError("theria rotary takes positions or offsets, not both")
+    for name, t in (("positions", positions), ("offsets", offsets)):
+        if t is not None:
+            _check_ids(what, name, t, q.device)
+    tokens = q.shape[:-2]
+    if positions is not None and positions.shape not in (tokens, tokens[-1:]):
+        raise AssertionError(f"positions must have shape {tuple(tokens)} or {tuple(tokens[-1:])}")
+    if offsets is not None and (offsets.ndim != 1 or offsets.shape[0] == 0):
+        raise AssertionError("offsets must have shape (S+1,)")
+    _no_tangents(what, q, k)
+    if q.numel() == 0 and (k is None or k.numel() == 0):
+        out = torch.empty_like(q), None if k is None else torch.empty_like(k)
+        return out if k is not None else out[0]
+    positions = None if positions is None else positions.contiguous()
+    offsets = None if offsets is None else offsets.contiguous()
+    args = (q, k, frequencies.contiguous(), positions, offsets, int(bool(interleaved)),
+            float(amplitude), 0)
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        out = _Rotary.apply(*args)
+    else:
+        out = _rotate(*args)
+    return out if k is not None else out[0]
+
+
+# ------------------------------------------------------ gradient norm, clipping
+def _grads_table(tensors):
+    n = len(tensors)
+    return ((ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
+            (ctypes.c_int * n)(*[_DTYPES[t.dtype] for t in tensors]))
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _grads_dot(x, u, sizes, dtypes, dev):
+    parts = torch.empty(max(1, _fn("theria_grads_parts")(sizes, len(x))), dtype=torch.float64,
+                        device=dev)
+    _call("theria_grads_dot", dev, _pointers(x), None if u is None else _pointers(u), sizes,
+          dtypes, len(x), parts.data_ptr())
+    return parts
+
+
+def _clip(x, out, max_norm):
+    """norm [] of x, and its stats; out (None: not wanted) receives x clipped."""
+    dev, (sizes, dtypes) = x[0].device, _grads_table(x)
+    parts = _grads_dot(x, None, sizes, dtypes, dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty(2, dtype=torch.float64, device=dev)
+    _call("theria_grads_clip", dev, _pointers(x), None if out is None else _pointers(out), sizes,
+          dtypes, len(x), parts.data_ptr(), max_norm, norm.data_ptr(), stats.data_ptr())
+    return norm, stats
+
+
+def _clip_grad(x, u, gnorm, stats):
+    dev, (sizes, dtypes) = x[0].device, _grads_table(x)
+    parts = None
+    if u is not None:
+        u = [t.contiguous() for t in u]
+        parts = _grads_dot(x, u, sizes, dtypes, dev)
+    dx = [torch.empty_like(t) for t in x]
+    gnorm = None if gnorm is None else gnorm.to(torch.float32).contiguous()
+    _call("theria_grads_clip_bwd", dev, _pointers(x), None if u is None else _pointers(u),
+          _pointers(dx), sizes, dtypes, len(x), _ptr(parts), stats.data_ptr(), _ptr(gnorm))
+    return dx
+
+
+class _ClipBackward(torch.autograd.Function):
+    """(x, u, gnorm) -> dx; a second derivative is refused."""
+
+    @staticmethod
+    def forward(ctx, n, stats, gnorm, *xu):
+        return tuple(_clip_grad(xu[:n], xu[n:] or None, gnorm, stats))
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("theria clip_gradients is differentiable once: its gradients have no "
+                           "second derivative here")
+
+
+class _Clip(torch.autograd.Function):
+    """tensors -> (norm, *clipped); clip false: the norm alone."""
+
+    @staticmethod
+    def forward(ctx, max_norm, clip, *x):
+        y = [torch.empty_like(t) for t in x] if clip else None
+        norm, stats = _clip(x, y, max_norm)
+        ctx.save_for_backward(stats, *x)
+        ctx.set_materialize_grads(False)
+        return (norm, *y) if clip else norm
+
+    @staticmethod
+    def backward(ctx, gnorm, *gy):
+        _no_tangents("theria clip_gradients", gnorm, *gy)
+        stats, *x = ctx.saved_tensors
+        some = any(g is not None for g in gy)
+        if not some and gnorm is None:
+            return (None, None, *(None for _ in x))
+        u = [torch.zeros_like(t) if g is None else g for t, g in zip(x, gy)] if some else []
+        if torch.is_grad_enabled():
+            dx = _ClipBackward.apply(len(x), stats, gnorm, *x, *u)
+        else:
+            dx = _clip_grad(x, u or None, gnorm, stats)
+        return (None, None, *dx)
+
+
+def _check_grads(what, tensors):
+    tensors = list(tensors)
+    if not tensors:
+        raise AssertionError(f"{what} needs at least one tensor")
+    for i, t in enumerate(tensors):
+        _check(what, f"tensor {i}", t, tensors[0].device)
+    _no_tangents(what, *tensors)
+    return tensors
+
+
+def _check_max(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise AssertionError(f"max_norm must not be negative, got {max_norm}")
+    return max_norm
+
+
+@_opaque
+def gradient_norm(tensors):
+    """The 2-norm of all values of the tensors together (float32, on the device);
+    differentiable once.  Any shapes and mixed types; sums are taken to float64, so
+    very large and very small gradients neither overflow nor vanish."""
+    x = [t.contiguous() for t in _check_grads("theria gradient_norm", tensors)]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in x):
+        return _Clip.apply(0.0, False, *x)
+    return _clip(x, None, 0.0)[0]
+
+
+@_opaque
+def clip_gradients(tensors, max_norm):
+    """``([t * c for t in tensors], norm)`` with ``norm = gradient_norm(tensors)`` and
+    ``c = min(1, max_norm / norm)``; differentiable once, so that clipped steps can be
+    part of an adapted model.  A norm that is NaN makes every value NaN, an
+    infinite one makes c 0."""
+    what = "theria clip_gradients"
+    x = [t.contiguous() for t in _check_grads(what, tensors)]
+    max_norm = _check_max(max_norm)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in x):
+        norm, *y = _Clip.apply(max_norm, True, *x)
+        return y, norm
+    y = [torch.empty_like(t) for t in x]
+    return y, _clip(x, y, max_norm)[0]
+
+
+@_opaque
+def clip_gradients_(tensors, max_norm):
+    """clip_gradients in place; returns the norm.  No two tensors may overlap, and
+    none may need a gradient (under ``torch.no_grad()`` they may)."""
+    what = "theria clip_gradients_"
+    tensors = _check_grads(what, tensors)
+    max_norm = _check_max(max_norm)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise AssertionError(f"{what} changes its tensors: none may require a gradient")
+    x = [t.contiguous() for t in tensors]
+    for t, c in zip(tensors, x):
+        if t is not c and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise AssertionError(f"{what} changes its tensors: none may be an expanded view")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                   for t in x if t.numel())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise AssertionError(f"{what} changes its tensors: no two may overlap")
+    norm, _ = _clip(x, x, max_norm)
+    for t, c in zip(tensors, x):
+        if t is not c:
+            t.copy_(c)
+        elif not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+    return norm
+
+
+__all__ = ["embedding", "layer_norm", "linear_cross_entropy", "rotary", "rotary_frequencies",
+           "gradient_norm", "clip_gradients", "clip_gradients_"]

@@ -19,6 +19,7 @@ from __future__ import annotations
 import torch
 import torch.distributed as dist
 
+from theria_b200.lm import clip_gradients_
 from theria_b200.maml.loops import meta_loss_batched
 from theria_b200.maml.tasks import TaskBatch
 
@@ -38,16 +39,23 @@ def shard_range(meta_batch: int, rank: int, world: int) -> tuple[int, int]:
 
 
 class MetaStep:
-    """One outer step: local batched adaptation, one gradient all-reduce, Adam."""
+    """One outer step: local batched adaptation, one gradient all-reduce, Adam.
+
+    ``max_norm`` clips the whole meta-gradient by its norm before Adam, after the
+    exchange (``lm.clip_gradients_``: CUDA parameters); ``grad_norm`` then holds
+    the norm of the last step's gradient.
+    """
 
     def __init__(self, model, *, meta_batch=32, inner_lr=0.4, inner_steps=5, fo=False,
-                 outer_lr=1e-3, world=1, capturable=False):
+                 outer_lr=1e-3, world=1, capturable=False, max_norm=None):
         self.model = model
         self.meta_batch = meta_batch
         self.inner_lr = inner_lr
         self.inner_steps = inner_steps
         self.fo = fo
         self.world = world
+        self.max_norm = max_norm
+        self.grad_norm = None
         self.params = [p for p in model.parameters()]
         # one fused kernel per step on the GPU (foreach kernels elsewhere)
         fused = self.params[0].is_cuda
@@ -76,6 +84,8 @@ class MetaStep:
                 n = p.numel()
                 p.grad = self.bucket[off:off + n].view_as(p)  # views of the bucket
                 off += n
+        if self.max_norm is not None:
+            self.grad_norm = clip_gradients_([self.bucket], self.max_norm)
         self.opt.step()
 
     def step(self, tasks: TaskBatch) -> torch.Tensor:

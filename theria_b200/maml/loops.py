@@ -25,6 +25,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch.func import functional_call
 
+from theria_b200.lm import clip_gradients
 from theria_b200.maml.tasks import TaskBatch
 
 Params = "OrderedDict[str, torch.Tensor]"
@@ -44,13 +45,20 @@ def loss_fn(logits: torch.Tensor, y: torch.Tensor) -> torch.Tensor:
 
 def inner_adapt(model: nn.Module, params: Mapping[str, torch.Tensor],
                 buffers: Mapping[str, torch.Tensor], task: TaskBatch, *,
-                inner_lr: float = 0.1, inner_steps: int = 1, fo: bool = False):
-    """phi <- phi - lr * grad L_support(phi), ``inner_steps`` times."""
+                inner_lr: float = 0.1, inner_steps: int = 1, fo: bool = False,
+                max_norm: float | None = None):
+    """phi <- phi - lr * grad L_support(phi), ``inner_steps`` times.
+
+    ``max_norm`` clips each step's gradients by their global norm
+    (``lm.clip_gradients``: CUDA tensors), and the meta-gradient goes through it.
+    """
     phi = OrderedDict(params.items())
     for _ in range(inner_steps):
         loss_s = loss_fn(functional_call(model, (phi, buffers), (task.x_s,)), task.y_s)
         grads = torch.autograd.grad(loss_s, tuple(phi.values()), create_graph=not fo,
                                     retain_graph=True, allow_unused=False)
+        if max_norm is not None:
+            grads, _ = clip_gradients(grads, max_norm)
         phi = OrderedDict((n, p - inner_lr * g) for (n, p), g in zip(phi.items(), grads))
     return phi
 
@@ -61,14 +69,15 @@ def outer_loss(model, phi, buffers, task: TaskBatch) -> torch.Tensor:
 
 def meta_loss_on_tasks(model: nn.Module, tasks: list[TaskBatch], *, inner_lr: float = 0.1,
                        inner_steps: int = 1, fo: bool = False, fo_strict: bool = False,
-                       return_metrics: bool = False):
-    """J(theta) = mean over tasks of L_query(phi_K(theta; support); query)."""
+                       return_metrics: bool = False, max_norm: float | None = None):
+    """J(theta) = mean over tasks of L_query(phi_K(theta; support); query);
+    ``max_norm`` as in ``inner_adapt``."""
     params = named_params(model)
     buffers = named_buffers(model)
     losses, accs = [], []
     for task in tasks:
         phi = inner_adapt(model, params, buffers, task, inner_lr=inner_lr,
-                          inner_steps=inner_steps, fo=fo)
+                          inner_steps=inner_steps, fo=fo, max_norm=max_norm)
         if fo_strict:
             phi = OrderedDict((k, v.detach().clone()) for k, v in phi.items())
         logits_q = functional_call(model, (phi, buffers), (task.x_q,))
