@@ -6,7 +6,11 @@ ds k and ds^T q, and every result: each is off by u times the same sum of
 absolute values.  z = o . do is taken from the rounded o, which is off by
 u (p |v| + |o|), so ds is off by p * dz besides.  What float32 adds is at most
 (terms of the sum + 8 max|s| + 32) 2^-24 of the sums of absolute values: one
-rounding a term, the scores' own error in the exponent, and the exponential's."""
+rounding a term, the scores' own error in the exponent, and the exponential's.
+
+float16 has no relative precision below 2^-14: p and ds are off by 2^-25 besides
+there (half its smallest step), each time the sum of the sizes that it multiplies;
+in the forward p is at least 1 in each row's maximum, and the row's sum l >= 1."""
 
 import math
 
@@ -38,7 +42,7 @@ def _inputs(lengths, H, Hkv, D, dtype, seed=0, lead=0, tail=0):
 def _plain(q, k, v, do, lengths, lead, causal, scale):
     """Results, and how far each may be off, in float64."""
     u = torch.finfo(q.dtype).eps / 2
-    half = q.dtype != torch.float32
+    half, q_type = q.dtype != torch.float32, q.dtype
     q, k, v, do = (t.double() for t in (q, k, v, do))
     G = q.shape[1] // k.shape[1]
     D = q.shape[2]
@@ -63,15 +67,17 @@ def _plain(q, k, v, do, lengths, lead, causal, scale):
             smax = s[s > -math.inf].abs().max().item()
             f = (max(n, n * G) + D + 8 * smax + 32) * 2.0 ** -24
             w = (u if half else 0.0) + f
+            # float16's smallest half step, for each pair that is not masked
+            sub = (s > -math.inf).double() * (2.0 ** -25 if q_type is torch.float16 else 0.0)
             a_o = p @ vs.abs()
-            e_o = w * a_o + u * o.abs()
+            e_o = w * a_o + u * o.abs() + sub @ vs.abs()
             # dp - z: float32 sums of D terms, and z from the o that was stored
             e_dp = f * (ds_o.abs() @ vs.abs().transpose(1, 2))
             e_z = (ds_o.abs() * (e_o + f * o.abs())).sum(-1, keepdim=True)
-            e_ds = w * ds.abs() + scale * p * (e_dp + e_z + f * (dp - z).abs())
+            e_ds = w * ds.abs() + scale * sub + scale * p * (e_dp + e_z + f * (dp - z).abs())
             e_dq = (e_ds + f * ds.abs()) @ ks.abs() + u * dq.abs()
             e_dk = (e_ds + f * ds.abs()).transpose(1, 2) @ qs.abs()
-            e_dv = w * (p.transpose(1, 2) @ ds_o.abs())
+            e_dv = (w * p + sub).transpose(1, 2) @ ds_o.abs()
             per = lambda t: t.unflatten(0, (-1, G)).sum(1)  # noqa: E731
             dk, dv = per(dk), per(dv)
             e_dk, e_dv = per(e_dk) + u * dk.abs(), per(e_dv) + u * dv.abs()

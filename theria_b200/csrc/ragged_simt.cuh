@@ -35,6 +35,19 @@ struct SimtSmem {
   static constexpr int kBwd = (4 * kTile + 2 * kS + 2 * SR) * 4;
 };
 
+// 16 bytes (VEC > 1) or one value, as floats.
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = to_f32<T>(*p);
+  } else {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32<T>(e[i]);
+  }
+}
+
 // 64 rows of a tensor into shared memory as float32, zero beyond row `n` and
 // column D.  row_at(r): the element where row r starts.
 template <typename T, int DT, typename F>
@@ -219,22 +232,32 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   }
 }
 
-// terms[row] = {-lse * log2(e), -rowsum(do * o)} for every row [T, H], a warp a
-// row.  Rows of no sequence get whatever their memory holds: no tile reads them.
-template <typename T>
+// terms[row] = {-lse * log2(e), -rowsum(do * o)} for every row [T, H]: LANES
+// neighbouring lanes a row, each on VEC of its values at a time.  Rows of no
+// sequence get whatever their memory holds: no tile reads them.
+template <typename T, int VEC, int LANES>
 __global__ void __launch_bounds__(256)
 terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse,
              float2* __restrict__ terms, int64_t rows, int D) {
   grid_launch();
   grid_wait();
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows;
-       r += (int64_t)gridDim.x * 8) {
+  const int lane = threadIdx.x % LANES;
+  const int64_t all = (int64_t)gridDim.x * (256 / LANES);
+  const int64_t r0 = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  for (int64_t base = 0; base < rows; base += all) {  // the same trips for every lane
+    const int64_t r = base + r0;
     float z = 0.f;
-    for (int d = lane; d < D; d += 32)
-      z = fmaf(to_f32<T>(o[r * D + d]), to_f32<T>(dout[r * D + d]), z);
-    z = warp_sum(z);
-    if (lane == 0) terms[r] = make_float2(-lse[r] * kLog2e, -z);
+    if (r < rows)
+      for (int d = lane * VEC; d < D; d += LANES * VEC) {
+        float a[VEC], b[VEC];
+        load_vec<T, VEC>(o + r * D + d, a);
+        load_vec<T, VEC>(dout + r * D + d, b);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z = fmaf(a[i], b[i], z);
+      }
+#pragma unroll
+    for (int x = LANES / 2; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+    if (r < rows && lane == 0) terms[r] = make_float2(-lse[r] * kLog2e, -z);
   }
 }
 

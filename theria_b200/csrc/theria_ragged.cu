@@ -5,6 +5,8 @@
 #include "common.cuh"
 #include "ragged_plan.cuh"
 #include "ragged_simt.cuh"
+#include "ragged_tc_bwd.cuh"
+#include "ragged_tc_fwd.cuh"
 #include "tc_host.cuh"
 #include "../../include/theria_ragged.h"
 
@@ -50,7 +52,6 @@ struct Carver {
 int64_t most_items(int64_t T, int64_t S, int64_t per, int64_t step) {
   return T * per / step + std::min(S, T);
 }
-// The smallest step of any kernel's list is 64 rows of packed heads.
 List take_list(Carver& c, const Problem& p, int per, int step, int by_key) {
   List l{};
   l.per = per;
@@ -122,6 +123,14 @@ int key_splits(const Problem& p, int step) {
   return (int)std::min<int64_t>(32, std::max<int64_t>(1, 2 * kSMs / tiles));
 }
 
+// Lists have room for the CUDA-core kernels' tiles of 64 packed rows; the
+// tensor-core kernels' are larger, hence fewer (128 / G, rounded down, is at
+// least 64 / G).
+void retile(List& l, int per, int step) {
+  l.per = per;
+  l.step = step;
+}
+
 struct FwdWs {
   List list;
   int64_t bytes;
@@ -137,8 +146,7 @@ FwdWs fwd_ws(void* base, const Problem& p) {
 struct BwdWs {
   List lq, lk;
   float2* terms;
-  float* part;
-  int splits;
+  float* part;  // room for the larger tiles' splits
   int64_t bytes;
 };
 BwdWs bwd_ws(void* base, const Problem& p) {
@@ -147,8 +155,8 @@ BwdWs bwd_ws(void* base, const Problem& p) {
   w.lq = take_list(c, p, p.G, SR, 0);
   w.lk = take_list(c, p, 1, SR, 1);
   w.terms = c.take<float2>((int64_t)p.T * p.H);
-  w.splits = key_splits(p, SR);
-  w.part = w.splits > 1 ? c.take<float>(2ll * w.splits * p.T * p.Hkv * p.D) : nullptr;
+  const int splits = key_splits(p, BX);
+  w.part = splits > 1 ? c.take<float>(2ll * splits * p.T * p.Hkv * p.D) : nullptr;
   w.bytes = c.used;
   return w;
 }
@@ -178,6 +186,13 @@ int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, c
 }
 
 template <typename T>
+int run_join(const BwdWs& ws, int splits, const void* offsets, int wide, void* dk, void* dv,
+             const Problem& p, cudaStream_t st) {
+  return launch_chained(join_kernel<T>, dim3(kSMs * 4), dim3(256), 0, st, (const float*)ws.part,
+                        splits, (const int*)ws.lk.count, offsets, wide, (T*)dk, (T*)dv, p);
+}
+
+template <typename T>
 int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
              void* dv, const BwdWs& ws, const void* offsets, int wide, const Problem& p,
              cudaStream_t st) {
@@ -189,21 +204,142 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
           cudaSuccess)
         return (int)THERIA_ERR_LAUNCH;
       return launch_chained(kern, dim3(blocks(p, l.per, SR), (unsigned)splits), dim3(SIMT_THREADS),
-                            smem, st, (const T*)q, (const T*)k, (const T*)v,
-                            (const T*)dout, (const float2*)ws.terms, (T*)o1, (T*)o2, part,
-                            (const int4*)l.items, (const int*)l.count, p);
+                            smem, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout,
+                            (const float2*)ws.terms, (T*)o1, (T*)o2, part, (const int4*)l.items,
+                            (const int*)l.count, p);
     };
     if (dq != nullptr)
       if (int e = run(simt_bwd_kernel<T, DT, false>, ws.lq, 1, dq, nullptr, nullptr)) return e;
-    if (dk != nullptr) {
-      if (int e = run(simt_bwd_kernel<T, DT, true>, ws.lk, ws.splits, dk, dv, ws.part)) return e;
-      if (ws.part != nullptr)
-        return launch_chained(join_kernel<T>, dim3(kSMs * 4), dim3(256), 0, st,
-                              (const float*)ws.part, ws.splits, (const int*)ws.lk.count, offsets,
-                              wide, (T*)dk, (T*)dv, p);
-    }
-    return (int)THERIA_OK;
+    if (dk == nullptr) return (int)THERIA_OK;
+    const int splits = key_splits(p, SR);
+    if (int e = run(simt_bwd_kernel<T, DT, true>, ws.lk, splits, dk, dv,
+                    splits > 1 ? ws.part : nullptr))
+      return e;
+    return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : (int)THERIA_OK;
   });
+}
+
+// ------------------------------------------------------ tensor-core launches
+// Rows of 16 bytes on 16-byte boundaries, and a group that a tile of 64 rows
+// holds.  (Measured against the CUDA-core kernels: see ragged_tc_bwd.cuh.)
+bool use_tc(int dtype, const Problem& p, std::initializer_list<const void*> ptrs) {
+  if (dtype == THERIA_F32 || p.D % 8 || p.G > BY || tc::encode_fn() == nullptr) return false;
+  for (const void* x : ptrs)
+    if (!tc::aligned16(x)) return false;
+  for (int64_t s : {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h})
+    if (s % 8 || s <= 0 || s >= (1ll << 38)) return false;
+  return true;
+}
+
+bool encode(CUtensorMap* m, const void* base, int dtype, int rank, const cuuint64_t* dims,
+            const cuuint64_t* strides, const cuuint32_t* box) {
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  return tc::encode_fn()(m,
+                         dtype == THERIA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                         rank, const_cast<void*>(base), dims, strides, box, one,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Keys or values [T, Hkv, D]: box {64 values, `rows` tokens, 1 head}.
+bool key_map(CUtensorMap* m, const void* base, int dtype, const Problem& p, int64_t st, int64_t sh,
+             int rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)p.D, (cuuint64_t)p.T, (cuuint64_t)p.Hkv};
+  const cuuint64_t strides[2] = {(cuuint64_t)(2 * st), (cuuint64_t)(2 * sh)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)rows, 1};
+  return encode(m, base, dtype, 3, dims, strides, box);
+}
+// Queries (or their gradients) [T, Hkv, G, D]: box {64 values, G heads, `tokens`, 1}.
+bool row_map(CUtensorMap* m, const void* base, int dtype, const Problem& p, int64_t st, int64_t sh,
+             int tokens) {
+  const cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.G, (cuuint64_t)p.T,
+                              (cuuint64_t)p.Hkv};
+  const cuuint64_t strides[3] = {(cuuint64_t)(2 * sh), (cuuint64_t)(2 * st),
+                                 (cuuint64_t)(2 * sh * p.G)};
+  const cuuint32_t box[4] = {64, (cuuint32_t)p.G, (cuuint32_t)tokens, 1};
+  return encode(m, base, dtype, 4, dims, strides, box);
+}
+
+template <typename T, int HD, bool CAUSAL>
+int tc_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const FwdWs& ws,
+           int dtype, const Problem& p, cudaStream_t st) {
+  CUtensorMap mq, mk, mv;
+  if (!row_map(&mq, q, dtype, p, p.q_t, p.q_h, FM / p.G) ||
+      !key_map(&mk, k, dtype, p, p.k_t, p.k_h, FN) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, FN))
+    return THERIA_ERR_UNSUPPORTED;
+  auto kern = tc_fwd_kernel<T, HD, CAUSAL>;
+  constexpr int smem = FwdCfg<HD>::kAlloc;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return THERIA_ERR_LAUNCH;
+  return launch_chained(kern, dim3(blocks(p, ws.list.per, ws.list.step)),
+                        dim3(FwdCfg<HD>::kThreads), smem, st, mq, mk, mv, (T*)o, lse,
+                        (const int4*)ws.list.items, (const int*)ws.list.count, p);
+}
+
+template <typename T, int HD, bool CAUSAL>
+int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
+           void* dv, const BwdWs& ws, const void* offsets, int wide, int dtype, const Problem& p,
+           cudaStream_t st) {
+  constexpr int smem = BwdCfg<HD>::kAlloc;
+  const int64_t o_t = (int64_t)p.H * p.D, o_h = p.D;
+  auto run = [&](auto kern, const CUtensorMap (&m)[4], const List& l, int splits, void* o1,
+                 void* o2, float* part) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess)
+      return (int)THERIA_ERR_LAUNCH;
+    return launch_chained(kern, dim3(blocks(p, l.per, l.step), (unsigned)splits), dim3(B_THREADS),
+                          smem, st, m[0], m[1], m[2], m[3], (const float2*)ws.terms, (T*)o1,
+                          (T*)o2, part, (const int4*)l.items, (const int*)l.count, p);
+  };
+  CUtensorMap m[4];
+  if (dq != nullptr) {
+    if (!row_map(m, q, dtype, p, p.q_t, p.q_h, BX / p.G) ||
+        !row_map(m + 1, dout, dtype, p, o_t, o_h, BX / p.G) ||
+        !key_map(m + 2, k, dtype, p, p.k_t, p.k_h, BY) ||
+        !key_map(m + 3, v, dtype, p, p.v_t, p.v_h, BY))
+      return THERIA_ERR_UNSUPPORTED;
+    if (int e = run(tc_bwd_kernel<T, HD, false, CAUSAL>, m, ws.lq, 1, dq, nullptr, nullptr))
+      return e;
+  }
+  if (dk == nullptr) return THERIA_OK;
+  if (!key_map(m, k, dtype, p, p.k_t, p.k_h, BX) || !key_map(m + 1, v, dtype, p, p.v_t, p.v_h, BX) ||
+      !row_map(m + 2, q, dtype, p, p.q_t, p.q_h, BY / p.G) ||
+      !row_map(m + 3, dout, dtype, p, o_t, o_h, BY / p.G))
+    return THERIA_ERR_UNSUPPORTED;
+  const int splits = key_splits(p, BX);
+  if (int e = run(tc_bwd_kernel<T, HD, true, CAUSAL>, m, ws.lk, splits, dk, dv,
+                  splits > 1 ? ws.part : nullptr))
+    return e;
+  return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : THERIA_OK;
+}
+
+// Calls f(HD, CAUSAL) as integral constants.
+template <typename F>
+int by_tile(const Problem& p, F f) {
+  using W64 = std::integral_constant<int, 64>;
+  using W128 = std::integral_constant<int, 128>;
+  if (p.D <= 64)
+    return p.causal ? f(W64{}, std::true_type{}) : f(W64{}, std::false_type{});
+  return p.causal ? f(W128{}, std::true_type{}) : f(W128{}, std::false_type{});
+}
+
+template <typename T>
+int run_terms(const void* o, const void* dout, const float* lse, const BwdWs& ws, const Problem& p,
+              cudaStream_t st) {
+  const int64_t rows = (int64_t)p.T * p.H;
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = p.D % VEC == 0 && tc::aligned16(o) && tc::aligned16(dout);
+  const int64_t units = vec ? p.D / VEC : p.D;  // a row's
+  auto run = [&](auto kern, int lanes) {
+    const int64_t need = cdiv(rows, 256 / lanes);
+    return launch_chained(kern, dim3((unsigned)std::min<int64_t>(need, kSMs * 32)), dim3(256), 0,
+                          st, (const T*)o, (const T*)dout, lse, ws.terms, rows, p.D);
+  };
+  if (!vec) return run(terms_kernel<T, 1, 32>, 32);
+  if (units <= 4) return run(terms_kernel<T, VEC, 4>, 4);
+  if (units <= 8) return run(terms_kernel<T, VEC, 8>, 8);
+  return run(terms_kernel<T, VEC, 16>, 16);
 }
 
 }  // namespace
@@ -232,14 +368,23 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
   if (!workspace || workspace_bytes < theria_ragged_fwd_workspace_bytes(T, S, H, Hkv))
     return THERIA_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  const FwdWs ws = fwd_ws(workspace, p);
+  FwdWs ws = fwd_ws(workspace, p);
   if (!grid_fits(p)) return THERIA_ERR_UNSUPPORTED;
+  const bool on_tc = use_tc(dtype, p, {q, k, v, o});
+  if (on_tc) retile(ws.list, 1, 2 * (FM / p.G));
   Blank blank{};
   blank.p[0] = o;
   blank.row_bytes[0] = H * D * elem_size(dtype);
   if (int e = run_plan(offsets, wide, p, ws.list, List{}, blank, st)) return e;
-  return by_type(dtype, [&](auto t) {
-    return simt_fwd<decltype(t)>(q, k, v, o, lse, ws, p, st);
+  return by_type(dtype, [&](auto t) -> int {
+    using E = decltype(t);
+    if constexpr (!std::is_same<E, float>::value)
+      if (on_tc)
+        return by_tile(p, [&](auto hd, auto causal_) {
+          return tc_fwd<E, decltype(hd)::value, decltype(causal_)::value>(q, k, v, o, lse, ws,
+                                                                          dtype, p, st);
+        });
+    return simt_fwd<E>(q, k, v, o, lse, ws, p, st);
   });
 }
 
@@ -264,8 +409,13 @@ int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t
   if (!workspace || workspace_bytes < theria_ragged_bwd_workspace_bytes(T, S, H, Hkv, D))
     return THERIA_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  const BwdWs ws = bwd_ws(workspace, p);
+  BwdWs ws = bwd_ws(workspace, p);
   if (!grid_fits(p)) return THERIA_ERR_UNSUPPORTED;
+  const bool on_tc = use_tc(dtype, p, {q, k, v, dout, dq, dk, dv});
+  if (on_tc) {
+    retile(ws.lq, 1, BX / p.G);
+    retile(ws.lk, 1, BX);
+  }
   Blank blank{};
   blank.p[0] = dq;
   blank.p[1] = dk;
@@ -274,14 +424,15 @@ int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t
   blank.row_bytes[1] = blank.row_bytes[2] = Hkv * D * elem_size(dtype);
   if (int e = run_plan(offsets, wide, p, dq ? ws.lq : List{}, dk ? ws.lk : List{}, blank, st))
     return e;
-  return by_type(dtype, [&](auto t) {
+  return by_type(dtype, [&](auto t) -> int {
     using E = decltype(t);
-    const int64_t rows = T * H;
-    if (int e = launch_chained(terms_kernel<E>,
-                               dim3((unsigned)std::min<int64_t>(cdiv(rows, 8), kSMs * 32)),
-                               dim3(256), 0, st, (const E*)o, (const E*)dout, lse, ws.terms, rows,
-                               (int)D))
-      return e;
+    if (int e = run_terms<E>(o, dout, lse, ws, p, st)) return e;
+    if constexpr (!std::is_same<E, float>::value)
+      if (on_tc)
+        return by_tile(p, [&](auto hd, auto causal_) {
+          return tc_bwd<E, decltype(hd)::value, decltype(causal_)::value>(
+              q, k, v, dout, dq, dk, dv, ws, offsets, wide, dtype, p, st);
+        });
     return simt_bwd<E>(q, k, v, dout, dq, dk, dv, ws, offsets, wide, p, st);
   });
 }
