@@ -14,9 +14,15 @@
 // tile of rows (as in the forward), so dk and dv sum over the group in TMEM.
 //
 //     warp 0       TMA producer; keys: also each tile's row terms
-//     warp 1       issues s and dp into one of two buffers
-//     warp 2       issues the sums
-//     warps 3..10  p and ds, two groups on 32 of a tile's 64 columns each
+//     warps 1..4   one thread each issues s, dp, the sum of ds y1, that of p y2
+//     warps 5..20  p and ds: eight warps take the even tiles, eight the odd ones, each
+//                  32 rows (a TMEM lane quarter) by 32 of the 64 columns
+// A hop from one of these to the next (a commit or an arrival, a wait that returns)
+// takes a few hundred cycles, and so does a wait that finds its barrier passed: with
+// two buffers the hops of the ring s -> p -> sum -> s set the pace unless each product
+// is its own step with its own barrier and its own waiting thread.  Measured at 8192
+// tokens of two sequences, 16 heads of 128: one issuing thread for all products
+// 2640 / 1170 us (both sides / queries), two (s and dp, the sums) 2260 / 1010.
 // TMEM: buffer b at [128 b, +64) s and [128 b + 64, +64) dp; the sums at 256 and
 // 256 + HD; where there is room (queries, or HD = 64) x1 and x2 as 16-bit pairs
 // at [384, ...): A operands from TMEM leave shared memory, which otherwise sets
@@ -34,8 +40,16 @@
 namespace theria {
 namespace ragged {
 
+__device__ __forceinline__ float2 ld_shared_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 constexpr int BX = 128, BY = 64;
-constexpr int B_COMPUTE = 256, B_THREADS = 96 + B_COMPUTE;
+constexpr int B_SET = 256;  // threads that make one tile's p and ds
+constexpr int B_CTL = 5;    // control warps
+constexpr int B_THREADS = 32 * B_CTL + 2 * B_SET;
 
 template <int HD>
 struct BwdCfg {
@@ -44,10 +58,11 @@ struct BwdCfg {
   static constexpr int oX1 = 0, oX2 = kX;
   static constexpr int oY1 = 2 * kX;              // [YST]
   static constexpr int oY2 = oY1 + YST * kY;      // [YST]
-  static constexpr int oTerm = oY2 + YST * kY;    // [YST][64] float2
+  static constexpr int oTerm = oY2 + YST * kY;    // [YST][2][64] floats
   static constexpr int oBar = oTerm + YST * BY * 8;
-  // x_full, x_tmem, edge, drain[2], s_full[2], p_full[2], done[2], y_full[], y_empty[]
-  static constexpr int nBar = 11 + 2 * YST;
+  // x_full, x_tmem, edge, drain[4], and per buffer s_full, s_free, dp_full, dp_free,
+  // p_full, ds_full; y_full[], y_empty[]
+  static constexpr int nBar = 7 + 12 + 2 * YST;
   static constexpr int oTmem = oBar + nBar * 8;
   static constexpr int oAbort = oTmem + 4;
   static constexpr int kAlloc = oAbort + 4 + 1024;
@@ -66,9 +81,12 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBar);
-  uint64_t *x_full = bars, *x_tmem = bars + 1, *edge = bars + 2, *drain = bars + 3;
-  uint64_t *s_full = bars + 5, *p_full = bars + 7, *done = bars + 9;
-  uint64_t *y_full = bars + 11, *y_empty = y_full + YST;
+  uint64_t *x_full = bars, *x_tmem = bars + 1, *edge = bars + 2, *drain = bars + 3;  // drain [4]
+  uint64_t *s_full = bars + 7, *dp_full = bars + 9;    // products done
+  uint64_t *p_full = bars + 11, *ds_full = bars + 13;  // pairs written (keys; both)
+  // s's columns free: keys, when p y2 is done; queries, when the warps have read s
+  uint64_t *s_free = bars + 15, *dp_free = bars + 17;  // dp's: when ds y1 is done
+  uint64_t *y_full = bars + 19, *y_empty = y_full + YST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oTmem);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::oAbort);
 
@@ -91,17 +109,20 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
 
   if (threadIdx.x == 0) {
     tc::mbar_init(x_full, 1);
-    tc::mbar_init(x_tmem, B_COMPUTE);
+    tc::mbar_init(x_tmem, B_SET / 32);
     tc::mbar_init(edge, 1);
+    for (int b = 0; b < 4; ++b) tc::mbar_init(drain + b, 1);
     for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(drain + b, 1);
       tc::mbar_init(s_full + b, 1);
-      tc::mbar_init(p_full + b, B_COMPUTE);
-      tc::mbar_init(done + b, 1);
+      tc::mbar_init(dp_full + b, 1);
+      tc::mbar_init(p_full + b, B_SET / 32);  // a warp arrives once
+      tc::mbar_init(ds_full + b, B_SET / 32);
+      tc::mbar_init(s_free + b, KEYS ? 1 : B_SET / 32);
+      tc::mbar_init(dp_free + b, 1);
     }
     for (int s = 0; s < YST; ++s) {
       tc::mbar_init(y_full + s, KEYS ? 2 : 1);  // the tile (and its row terms)
-      tc::mbar_init(y_empty + s, 1);
+      tc::mbar_init(y_empty + s, KEYS ? 2 : 1);  // the sums (s and dp read it before)
     }
     *abort = 0;
     tc::fence_barrier_init();
@@ -171,9 +192,11 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
           }
         }
         if (KEYS) {
-          float2* rt = reinterpret_cast<float2*>(smem + L::oTerm + st * BY * 8);
-          rt[lane] = rv[0];
-          rt[32 + lane] = rv[1];
+          float* rt = reinterpret_cast<float*>(smem + L::oTerm + st * BY * 8);
+          rt[lane] = rv[0].x;
+          rt[32 + lane] = rv[1].x;
+          rt[BY + lane] = rv[0].y;
+          rt[BY + 32 + lane] = rv[1].y;
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(y_full + st);
           if (t + 1 < n_iter) load_terms(t + 1);
@@ -197,58 +220,57 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
           tc::mbar_wait_drain(y_full + t % YST, (t / YST) & 1);
       }
     }
-  } else if (warp == 1 || warp == 2) {
+  } else if (warp < B_CTL) {
     // ------------------------------------------------------------ issuers
-    if (lane == 0 && n_iter > 0) {
+    if (lane == 0 && n_iter > 0 && (KEYS || warp != 4)) {
       constexpr int ab = tc::AbFmt<T>::v;
-      const uint32_t a_y1 = tc::smem_u32(smem + L::oY1), a_y2 = tc::smem_u32(smem + L::oY2);
-      if (warp == 1) {
+      if (warp <= 2) {
+        // s = x1 y1^T (warp 1) or dp = x2 y2^T (warp 2)
         constexpr uint32_t id_s = tc::idesc_f16(BX, BY, ab, 0, 0);
-        const uint64_t x1 = tc::sw128_desc(tc::smem_u32(smem + L::oX1), 16, 1024);
-        const uint64_t x2 = tc::sw128_desc(tc::smem_u32(smem + L::oX2), 16, 1024);
-        const uint64_t y1 = tc::sw128_desc(a_y1, 16, 1024), y2 = tc::sw128_desc(a_y2, 16, 1024);
-        bool ok = kXT ? tc::mbar_wait(x_tmem, 0, abort) : tc::mbar_wait(x_full, 0, abort);
+        const bool is_s = warp == 1;
+        const uint64_t x = tc::sw128_desc(tc::smem_u32(smem + (is_s ? L::oX1 : L::oX2)), 16, 1024);
+        const uint64_t y = tc::sw128_desc(tc::smem_u32(smem + (is_s ? L::oY1 : L::oY2)), 16, 1024);
+        const uint32_t t_x = is_s ? t_x1 : t_x2, t_d = tmem + (is_s ? 0 : 64);
+        uint64_t *full = is_s ? s_full : dp_full, *free_ = is_s ? s_free : dp_free;
+        const bool ok = tc::mbar_wait(kXT ? x_tmem : x_full, 0, abort);
         for (int t = 0; ok && t < n_iter; ++t) {
           const int st = t % YST, b = t & 1;
           if (!tc::mbar_wait(y_full + st, (t / YST) & 1, abort)) break;
-          if (t >= 2 && !tc::mbar_wait(done + b, ((t >> 1) - 1) & 1, abort)) break;
+          if (t >= 2 && !tc::mbar_wait(free_ + b, ((t >> 1) - 1) & 1, abort)) break;
           tc::tc_fence_after();
-          const uint32_t t_s = tmem + b * 128;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t xo = (kk / 4) * (BX * 128) + (kk % 4) * 32;
-            const uint32_t yo = st * L::kY + (kk / 4) * (BY * 128) + (kk % 4) * 32;
-            if constexpr (kXT) {
-              tc::mma_ts(t_s, t_x1 + kk * 8, tc::desc_at(y1, yo), id_s, kk > 0 ? 1u : 0u);
-              tc::mma_ts(t_s + 64, t_x2 + kk * 8, tc::desc_at(y2, yo), id_s, kk > 0 ? 1u : 0u);
-            } else {
-              tc::mma_ss(t_s, tc::desc_at(x1, xo), tc::desc_at(y1, yo), id_s, kk > 0 ? 1u : 0u);
-              tc::mma_ss(t_s + 64, tc::desc_at(x2, xo), tc::desc_at(y2, yo), id_s,
-                         kk > 0 ? 1u : 0u);
-            }
+            const uint64_t yd =
+                tc::desc_at(y, st * L::kY + (kk / 4) * (BY * 128) + (kk % 4) * 32);
+            if constexpr (kXT)
+              tc::mma_ts(t_d + b * 128, t_x + kk * 8, yd, id_s, kk > 0 ? 1u : 0u);
+            else
+              tc::mma_ss(t_d + b * 128, tc::desc_at(x, (kk / 4) * (BX * 128) + (kk % 4) * 32), yd,
+                         id_s, kk > 0 ? 1u : 0u);
           }
-          tc::mma_commit(s_full + b);
+          tc::mma_commit(full + b);
         }
       } else {
+        // the sums of ds y1 (warp 3) or p y2 (warp 4), the tile's rows as contraction
         constexpr uint32_t id_a = tc::idesc_f16(BX, HD, ab, 0, 1);
-        const uint64_t y1 = tc::sw128_desc(a_y1, BY * 128, 1024);
-        const uint64_t y2 = tc::sw128_desc(a_y2, BY * 128, 1024);
+        const bool is_ds = warp == 3;
+        const uint64_t y =
+            tc::sw128_desc(tc::smem_u32(smem + (is_ds ? L::oY1 : L::oY2)), BY * 128, 1024);
+        const uint32_t t_d = is_ds ? t_a1 : t_a2, t_p = tmem + (is_ds ? 64 : 0);
+        uint64_t* full = is_ds ? ds_full : p_full;
         for (int t = 0; t < n_iter; ++t) {
           const int st = t % YST, b = t & 1;
-          if (!tc::mbar_wait(p_full + b, (t >> 1) & 1, abort)) break;
+          if (!tc::mbar_wait(full + b, (t >> 1) & 1, abort)) break;
           tc::tc_fence_after();
-          const uint32_t t_p = tmem + b * 128;
 #pragma unroll
-          for (int kk = 0; kk < BY / 16; ++kk) {
+          for (int kk = 0; kk < BY / 16; ++kk)
             // 16 columns of the tile: 8 TMEM columns of pairs, in the half of the
-            // group that wrote them
-            const uint32_t po = (kk / 2) * 32 + (kk % 2) * 8, yo = st * L::kY + kk * 2048;
-            const uint32_t acc = t > 0 || kk > 0 ? 1u : 0u;
-            tc::mma_ts(t_a1, t_p + 64 + po, tc::desc_at(y1, yo), id_a, acc);
-            if constexpr (KEYS) tc::mma_ts(t_a2, t_p + po, tc::desc_at(y2, yo), id_a, acc);
-          }
-          tc::mma_commit(done + b);
-          tc::mma_commit(y_empty + st);  // s and dp of the tile read it before
+            // warps that wrote them
+            tc::mma_ts(t_d, t_p + b * 128 + (kk / 2) * 32 + (kk % 2) * 8,
+                       tc::desc_at(y, st * L::kY + kk * 2048), id_a, t > 0 || kk > 0 ? 1u : 0u);
+          if (is_ds) tc::mma_commit(dp_free + b);
+          else tc::mma_commit(s_free + b);
+          tc::mma_commit(y_empty + st);
         }
       }
       tc::mma_commit(drain + warp - 1);
@@ -256,7 +278,7 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
     }
   } else {
     // ------------------------------------------------------------ p and ds
-    const int grp = (warp - 3) >> 2, quarter = warp & 3;
+    const int grp = ((warp - B_CTL) >> 2) & 1, quarter = warp & 3, set = (warp - B_CTL) >> 3;
     const int r = quarter * 32 + lane;  // TMEM lane: the row of x
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const int tok = first + (KEYS ? r : r / G);      // its token
@@ -266,7 +288,7 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort));
     };
-    if (kXT && n_iter > 0) {
+    if (kXT && set == 0 && n_iter > 0) {
       // this row of x1 (group 0) or x2 (group 1) into TMEM: the 128-byte
       // swizzled row of 64 values is 32 pairs, one a column
       ok = wait(x_full, 0);
@@ -288,21 +310,19 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
         }
         tc::tmem_wait_st();
         tc::tc_fence_before();
-        tc::mbar_arrive(x_tmem);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(x_tmem);
       }
     }
     float2 mine = make_float2(-INFINITY, 0.f);  // queries: this row's terms
     if (!KEYS && live) mine = terms[(int64_t)(start + tok) * pr.H + hk * G + r % G];
     const int warp_tok = first + quarter * 32 / G;  // queries: the first token of the warp
-    for (int t = 0; ok && t < n_iter; ++t) {
-      const int b = t & 1, st = t % YST, y0 = tok_of(t);
+    for (int t = set; ok && t < n_iter; t += 2) {
+      const int b = set, st = t % YST, y0 = tok_of(t);
       const uint32_t t_s = tmem + b * 128 + grp * 32 + lane_off;
       if (KEYS && !wait(y_full + st, (t / YST) & 1)) { ok = false; break; }  // the terms
       if (!wait(s_full + b, (t >> 1) & 1)) { ok = false; break; }
       tc::tc_fence_after();
-      float s[32], dp[32];
-      tc::tmem_ld32(t_s, s);
-      tc::tmem_ld32(t_s + 64, dp);
       // Tiles on the diagonal and (queries) at the sequence's end need a mask; the
       // test is the same for a whole warp.  Valid: columns from `lo` on (keys), or
       // below `hi` (queries).
@@ -315,54 +335,80 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
         masked = y0 + BY > len || (CAUSAL && y0 + BY - 1 > warp_tok);
         hi = (CAUSAL ? min(len, tok + 1) : len) - y0 - grp * 32;
       }
-      const uint32_t rows_at = tc::smem_u32(smem + L::oTerm + st * BY * 8) + grp * 32 * 8;
-      auto make = [&](auto mk) {
+      // the row terms of this warp's columns: all -lse log2 e of a tile, then all -z
+      const uint32_t lse_at = tc::smem_u32(smem + L::oTerm + st * BY * 8) + grp * 32 * 4;
+      const uint32_t z_at = lse_at + BY * 4;
+      float s[32];
+      tc::tmem_ld32(t_s, s);
+      if constexpr (!KEYS) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(s_free + b);
+      }
+      auto on = [&](int e) { return KEYS ? e >= lo : e < hi; };
+      // p = exp2(scale s - lse); rows past the end of y: exp2(-inf) = 0
+      auto make_p = [&](auto mk) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-          float nl0, nl1, nz0, nz1;
+          float nl0 = mine.x, nl1 = mine.x;
           if constexpr (KEYS) {
-            const float4 rr = tc::ld_shared_f4(rows_at + e * 8);
-            nl0 = rr.x; nz0 = rr.y; nl1 = rr.z; nz1 = rr.w;
-          } else {
-            nl0 = nl1 = mine.x;
-            nz0 = nz1 = mine.y;
+            const float2 rr = ld_shared_f2(lse_at + e * 4);
+            nl0 = rr.x;
+            nl1 = rr.y;
           }
-          float x0, x1, g0, g1;
-          tc::fma2(x0, x1, s[e], s[e + 1], scale_log2, scale_log2, nl0, nl1);
-          float p0 = tc::ex2(x0), p1 = tc::ex2(x1);
-          tc::add2(g0, g1, dp[e], dp[e + 1], nz0, nz1);
-          tc::mul2(g0, g1, p0, p1, g0, g1);
+          tc::fma2(s[e], s[e + 1], s[e], s[e + 1], scale_log2, scale_log2, nl0, nl1);
+          s[e] = tc::ex2(s[e]);
+          s[e + 1] = tc::ex2(s[e + 1]);
           if constexpr (decltype(mk)::value) {
-            const bool on0 = KEYS ? e >= lo : e < hi, on1 = KEYS ? e + 1 >= lo : e + 1 < hi;
-            p0 = on0 ? p0 : 0.f;
-            p1 = on1 ? p1 : 0.f;
-            g0 = on0 ? g0 : 0.f;
-            g1 = on1 ? g1 : 0.f;
+            s[e] = on(e) ? s[e] : 0.f;
+            s[e + 1] = on(e + 1) ? s[e + 1] : 0.f;
           }
-          s[e] = p0;
-          s[e + 1] = p1;
-          dp[e] = g0;
-          dp[e + 1] = g1;
         }
       };
-      if (masked) make(std::true_type{}); else make(std::false_type{});
-      uint32_t pk[16];
+      if (masked) make_p(std::true_type{}); else make_p(std::false_type{});
+      uint32_t pk[16];  // 16-bit pairs
       if constexpr (KEYS) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) pk[i] = tc::pack2<T>(s[2 * i], s[2 * i + 1]);
         tc::tmem_st16(t_s, pk);
+        tc::tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full + b);
       }
+      if (!wait(dp_full + b, (t >> 1) & 1)) { ok = false; break; }
+      tc::tc_fence_after();
+      float dp[32];
+      tc::tmem_ld32(t_s + 64, dp);
+      // ds = p (dp - z)
+      auto make_ds = [&](auto mk) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) pk[i] = tc::pack2<T>(dp[2 * i], dp[2 * i + 1]);
+        for (int e = 0; e < 32; e += 2) {
+          float nz0 = mine.y, nz1 = mine.y, g0, g1;
+          if constexpr (KEYS) {
+            const float2 rr = ld_shared_f2(z_at + e * 4);
+            nz0 = rr.x;
+            nz1 = rr.y;
+          }
+          tc::add2(g0, g1, dp[e], dp[e + 1], nz0, nz1);
+          tc::mul2(g0, g1, s[e], s[e + 1], g0, g1);
+          if constexpr (decltype(mk)::value) {
+            g0 = on(e) ? g0 : 0.f;
+            g1 = on(e + 1) ? g1 : 0.f;
+          }
+          pk[e / 2] = tc::pack2<T>(g0, g1);
+        }
+      };
+      if (masked) make_ds(std::true_type{}); else make_ds(std::false_type{});
       tc::tmem_st16(t_s + 64, pk);
       tc::tmem_wait_st();
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full + b);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(ds_full + b);
     }
     // ------------------------------------------------------------ results
     if (ok && n_iter > 0) {
-      const int tl = n_iter - 1;
-      ok = wait(done + (tl & 1), (tl >> 1) & 1);
+      ok = wait(drain + 2, 0) && (!KEYS || wait(drain + 3, 0));  // the sums are complete
       if (ok) tc::tc_fence_after();
     }
     if (ok) {
@@ -375,7 +421,7 @@ tc_bwd_kernel(const __grid_constant__ CUtensorMap tm_x1, const __grid_constant__
         T* out = which == 0 ? out1 : out2;
         float* sums = part == nullptr ? nullptr : part + (2 * blockIdx.y + which) * plane;
 #pragma unroll 1
-        for (int c = grp * (HD / 64); c < (grp + 1) * (HD / 64); ++c) {
+        for (int c = grp + 2 * set; c < HD / 32; c += 4) {
           float v[32];
           if (n_iter > 0) {
             tc::tmem_ld32((which == 0 ? t_a1 : t_a2) + lane_off + c * 32, v);

@@ -126,7 +126,7 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     }
     for (int t = 0; t < 2; ++t) {
       tc::mbar_init(s_full + t, 1);
-      tc::mbar_init(p_full + t, 128 * L::kHalves);
+      tc::mbar_init(p_full + t, 4 * L::kHalves);  // a warp arrives once
       tc::mbar_init(o_done + t, 1);
       tc::mbar_init(s_read + t, 4 * L::kHalves);
       tc::mbar_init(pv_done + t, 1);
@@ -440,7 +440,8 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
       tc::tmem_wait_st();
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full + t);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(p_full + t);
     }
     // ------------------------------------------------------------ epilogue
     if (nt > 0) {
