@@ -15,9 +15,9 @@
 //
 // A thread multiplies and adds 8 values at a time in float32 and takes those
 // sums to float64, which costs an eighth of the conversions (16 a cycle and SM:
-// at one a value they would bound 16-bit tensors).  Where eight products
-// overflow or come near the smallest float32, they are done again in float64, so
-// that norms of very large and very small gradients are right.
+// at one a value they would bound 16-bit tensors).  A thread that meets very large
+// or very small values does its part of the chunk again in float64, so that norms
+// of such gradients are right.
 #pragma once
 
 #include "common.cuh"
@@ -59,43 +59,38 @@ __device__ __forceinline__ int tensor_of(const Table& t, int chunk) {
   return lo;
 }
 
-// sum of a[i] * b[i]
-template <int N>
-__device__ __forceinline__ double dot(const float (&a)[N], const float (&b)[N]) {
-  float s = 0.f, big = 0.f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    s = fmaf(a[i], b[i], s);
-    big = fmaxf(big, fabsf(a[i] * b[i]));
-  }
-  if (big > 1e-28f && big < 1e37f) return (double)s;
-  double d = 0.0;
-#pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (a[i] != 0.f && b[i] != 0.f) d = fma((double)a[i], (double)b[i], d);
-  return d;
+// Values whose products, or sums of a few, may leave float32's range.
+__device__ __forceinline__ bool extreme(float big) {
+  return big > 1e17f || (big < 1e-13f && big != 0.f);
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+// 8 values as they lie in memory, so that a thread can have several in flight.
+template <typename T>
+struct Eight {
+  static constexpr int n = 8 * sizeof(T) / 16;
+  uint4 r[n];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-  for (int i = 0; i < 8; i += VEC) {
-    float w[VEC];
-    embed::load_vec<T, VEC>(p + i, w);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[i + k] = w[k];
+    for (int i = 0; i < n; ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const T* e = reinterpret_cast<const T*>(r);
 #pragma unroll
-  for (int i = 0; i < 8; i += VEC) {
-    float w[VEC];
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) w[k] = v[i + k];
-    embed::store_vec<T, VEC>(p + i, w);
+    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(e[i]);
   }
-}
+  __device__ __forceinline__ void set(const float (&v)[8]) {
+    T* e = reinterpret_cast<T*>(r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < n; ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+  }
+};
+// A thread's eights of a whole chunk, and how many of them it has in flight (64 bytes).
+constexpr int EIGHTS = CHUNK / (THREADS * 8);
+template <typename T> constexpr int kFlight = 64 / (8 * (int)sizeof(T));
 
 // The block's sum, in every thread.
 __device__ __forceinline__ double block_sum(double x) {
@@ -121,8 +116,9 @@ __device__ __forceinline__ void chunk_at(const Table& t, int chunk, F f) {
   by_type(t.dtype[i], [&](auto e) { f(e, i, from, n); });
 }
 
-// part[block] = the block's share of sum x u (u NULL: of sum x^2).
-__global__ void __launch_bounds__(THREADS)
+// part[block] = the block's share of sum x u (SAME: of sum x^2).
+template <bool SAME>
+__global__ void __launch_bounds__(THREADS, SAME ? 4 : 3)
 dot_kernel(const __grid_constant__ Table t, double* part) {
   grid_launch();
   grid_wait();
@@ -131,28 +127,49 @@ dot_kernel(const __grid_constant__ Table t, double* part) {
     chunk_at(t, c, [&](auto e, int i, int64_t from, int n) {
       using T = decltype(e);
       const T* x = static_cast<const T*>(t.x[i]) + from;
-      const T* u = static_cast<const T*>(t.u[i] ? t.u[i] : t.x[i]) + from;
-      const bool same = x == u;
+      const T* u = static_cast<const T*>(SAME ? t.x[i] : t.u[i]) + from;
+      bool odd = false;  // an eight of this thread is extreme
+      double sum = 0.0;
       int at = 0;
       if (t.vec[i]) {
-        constexpr int VEC = embed::Vec<T>::n;
-#pragma unroll 4
-        for (int k = threadIdx.x * 8; k + 8 <= n; k += THREADS * 8) {
-          float a[8], b[8];
-          load8<T, VEC>(x + k, a);
-          if (same) {
-            acc += dot<8>(a, a);
-          } else {
-            load8<T, VEC>(u + k, b);
-            acc += dot<8>(a, b);
+        constexpr int F = kFlight<T>;
+#pragma unroll 1
+        for (int j0 = 0; j0 < EIGHTS; j0 += F) {
+          Eight<T> ra[F], rb[F];
+#pragma unroll
+          for (int j = 0; j < F; ++j) {
+            const int k = ((j0 + j) * THREADS + threadIdx.x) * 8;
+            if (k + 8 > n) continue;
+            ra[j].load(x + k);
+            if constexpr (!SAME) rb[j].load(u + k);
+          }
+#pragma unroll
+          for (int j = 0; j < F; ++j) {
+            if (((j0 + j) * THREADS + (int)threadIdx.x) * 8 + 8 > n) continue;
+            float a[8], b[8], s = 0.f, ma = 0.f, mb = 0.f;
+            ra[j].get(a);
+            if constexpr (!SAME) rb[j].get(b);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              s = fmaf(a[e], SAME ? a[e] : b[e], s);
+              ma = fmaxf(ma, fabsf(a[e]));
+              if constexpr (!SAME) mb = fmaxf(mb, fabsf(b[e]));
+            }
+            odd |= extreme(ma) || (!SAME && extreme(mb));
+            sum += (double)s;
           }
         }
         at = n / 8 * 8;
       }
-      for (int k = at + threadIdx.x; k < n; k += THREADS) {
-        const float a[1] = {to_f32<T>(x[k])}, b[1] = {to_f32<T>(u[k])};
-        acc += dot<1>(a, b);
+      if (odd) {  // the thread's eights again, in float64
+        sum = 0.0;
+        for (int k0 = threadIdx.x * 8; k0 + 8 <= n; k0 += THREADS * 8)
+          for (int k = k0; k < k0 + 8; ++k)
+            sum = fma((double)to_f32<T>(x[k]), (double)to_f32<T>(u[k]), sum);
       }
+      for (int k = at + threadIdx.x; k < n; k += THREADS)
+        sum = fma((double)to_f32<T>(x[k]), (double)to_f32<T>(u[k]), sum);
+      acc += sum;
     });
   acc = block_sum(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
@@ -164,38 +181,53 @@ __device__ __forceinline__ double all_parts(const double* part, int parts) {
   return block_sum(s);
 }
 
-// out = a x + b u, from the values a, b (u NULL: a x)
+// out = a x + b u (TWO false: a x)
+template <bool TWO>
 __device__ __forceinline__ void combine(const Table& t, float a, float b) {
   const int last = t.first[t.n] - 1;
   for (int c = blockIdx.x; c <= last; c += gridDim.x)
     chunk_at(t, last - c, [&](auto e, int i, int64_t from, int n) {
       using T = decltype(e);
       const T* x = static_cast<const T*>(t.x[i]) + from;
-      const T* u = t.u[i] ? static_cast<const T*>(t.u[i]) + from : nullptr;
+      const T* u = static_cast<const T*>(TWO ? t.u[i] : t.x[i]) + from;
       T* out = static_cast<T*>(t.out[i]) + from;
       int at = 0;
       if (t.vec[i]) {
-        constexpr int VEC = embed::Vec<T>::n;
-#pragma unroll 4
-        for (int k = threadIdx.x * 8; k + 8 <= n; k += THREADS * 8) {
-          float v[8], w[8];
-          load8<T, VEC>(x + k, v);
-          if (u != nullptr) load8<T, VEC>(u + k, w);
+        constexpr int F = kFlight<T>;
+#pragma unroll 1
+        for (int j0 = 0; j0 < EIGHTS; j0 += F) {
+          Eight<T> rx[F], ru[F];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = u != nullptr ? fmaf(a, v[j], b * w[j]) : a * v[j];
-          store8<T, VEC>(out + k, v);
+          for (int j = 0; j < F; ++j) {
+            const int k = ((j0 + j) * THREADS + threadIdx.x) * 8;
+            if (k + 8 > n) continue;
+            rx[j].load(x + k);
+            if constexpr (TWO) ru[j].load(u + k);
+          }
+#pragma unroll
+          for (int j = 0; j < F; ++j) {
+            const int k = ((j0 + j) * THREADS + threadIdx.x) * 8;
+            if (k + 8 > n) continue;
+            float v[8], w[8];
+            rx[j].get(v);
+            if constexpr (TWO) ru[j].get(w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = TWO ? fmaf(a, v[e], b * w[e]) : a * v[e];
+            rx[j].set(v);
+            rx[j].store(out + k);
+          }
         }
         at = n / 8 * 8;
       }
       for (int k = at + threadIdx.x; k < n; k += THREADS) {
         const float v = to_f32<T>(x[k]);
-        out[k] = from_f32<T>(u != nullptr ? fmaf(a, v, b * to_f32<T>(u[k])) : a * v);
+        out[k] = from_f32<T>(TWO ? fmaf(a, v, b * to_f32<T>(u[k])) : a * v);
       }
     });
 }
 
 // out = c x (out may be x; t.n == 0: the norm alone).  stats receives {norm, c}.
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 4)
 clip_kernel(const __grid_constant__ Table t, const double* part, int parts, double most,
             float* norm, double* stats) {
   grid_wait();
@@ -210,11 +242,12 @@ clip_kernel(const __grid_constant__ Table t, const double* part, int parts, doub
   }
   if (t.n == 0) return;
   if (c == 1.0 && t.out[0] == t.x[0]) return;  // in place, nothing to clip
-  combine(t, (float)c, 0.f);
+  combine<false>(t, (float)c, 0.f);
 }
 
 // out = a u + b x (see above); u NULL: out = b x.  part: the sums of x u.
-__global__ void __launch_bounds__(THREADS)
+template <bool TWO>
+__global__ void __launch_bounds__(THREADS, TWO ? 3 : 4)
 clip_bwd_kernel(const __grid_constant__ Table t, const double* part, int parts,
                 const double* stats, const float* gnorm) {
   grid_wait();
@@ -226,7 +259,7 @@ clip_bwd_kernel(const __grid_constant__ Table t, const double* part, int parts,
     if (c != 1.0) b -= c * xu / n / n;
   }
   // with u, the table has it first: combine's x is u, its u is x
-  combine(t, parts > 0 ? (float)c : (float)b, (float)b);
+  combine<TWO>(t, TWO ? (float)c : (float)b, (float)b);
 }
 
 }  // namespace grads

@@ -10,9 +10,10 @@
 // turns less their nearest integer it is exact to 2^-52 t w / 2 pi turns, and the
 // remaining half turn at most is float32's to compute (sincospi, 1 to 2 units).
 //
-// With the halves apart a thread moves 16 bytes of each half where a half is a
-// whole number of such vectors, else 16 bytes of the output whose partners it
-// reads one by one (from the cache: a neighbour has just loaded them).
+// A thread stays on one column of 16 bytes of the heads and has the loads of four
+// rows (token, head) in flight.  With the halves apart it moves 16 bytes of each half where a half is a whole number
+// of such vectors, else 16 bytes of the output whose partners it reads one by one
+// (from the cache: a neighbour has just loaded them).
 #pragma once
 
 #include "common.cuh"
@@ -44,6 +45,7 @@ struct Args {
   const double* freq;    // [pairs]
   float amplitude;
   int back, tokens;      // the angle negated; tokens of a block
+  unsigned magic;        // ceil(2^32 / heads): row / heads as a product's high half
 };
 
 __device__ __forceinline__ int64_t int_at(const void* p, int wide, int64_t i) {
@@ -64,84 +66,126 @@ __device__ __forceinline__ int64_t position_of(const Args& a, int64_t i) {
   return i - int_at(a.offsets, a.wide, lo);
 }
 
+// VEC values as they lie in memory.
+template <typename T, int VEC>
+struct Raw {
+  uint4 r;
+  __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = r; }
+  __device__ __forceinline__ float get(int e) const {
+    return to_f32<T>(reinterpret_cast<const T*>(&r)[e]);
+  }
+  __device__ __forceinline__ void set(int e, float v) { reinterpret_cast<T*>(&r)[e] = from_f32<T>(v); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  T r;
+  __device__ __forceinline__ void load(const T* p) { r = *p; }
+  __device__ __forceinline__ void store(T* p) const { *p = r; }
+  __device__ __forceinline__ float get(int) const { return to_f32<T>(r); }
+  __device__ __forceinline__ void set(int, float v) { r = from_f32<T>(v); }
+};
+
 template <typename T, int VEC, int LAYOUT>
-__global__ void __launch_bounds__(THREADS) rotary_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
   extern __shared__ float2 turn[];  // [tokens][pairs] {cos, sin} * amplitude
+  __shared__ double at_pos[MOST_TOKENS];
+  __shared__ int64_t base[MOST_TOKENS][4];  // where the token's q, yq, k, yk start
+  constexpr int LOADS = LAYOUT == kHalves ? 2 : 4;  // heads in flight
+  using R = Raw<T, VEC>;
   const int64_t first = (int64_t)blockIdx.x * a.tokens;
   const int tokens = (int)min((int64_t)a.tokens, a.n - first);
+  if ((int)threadIdx.x < tokens) {
+    const int64_t tok = first + threadIdx.x, b = tok / a.T, at = tok - b * a.T;
+    at_pos[threadIdx.x] = (double)position_of(a, tok);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      base[threadIdx.x][2 * i] = b * a.s[i].xb + at * a.s[i].xt;
+      base[threadIdx.x][2 * i + 1] = b * a.s[i].yb + at * a.s[i].yt;
+    }
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < tokens * a.pairs; i += THREADS) {
-    const int t = i / a.pairs, m = i % a.pairs;
-    const double turns = (double)position_of(a, first + t) * a.freq[m] * 0.15915494309189533577;
+    const int t = i / a.pairs, m = i - t * a.pairs;
+    const double turns = at_pos[t] * a.freq[m] * 0.15915494309189533577;
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
     turn[i] = make_float2(c * a.amplitude, (a.back ? -s : s) * a.amplitude);
   }
   __syncthreads();
-  const int halves = LAYOUT == kHalves ? a.pairs / VEC : 0;  // units of both halves at once
-  const unsigned units = a.D / VEC - halves;                // a head's
-  const unsigned heads = a.heads[0] + a.heads[1];
-  const unsigned all = (unsigned)tokens * heads * units;
-  for (unsigned i = threadIdx.x; i < all; i += THREADS) {
-    const unsigned th = i / units, u = i - th * units;
-    const unsigned t = th / heads;
-    int h = th - t * heads;
-    const int side = h >= a.heads[0];
-    if (side) h -= a.heads[0];
-    const Side& sd = a.s[side];
-    const int64_t tok = first + t, b = tok / a.T, at = tok - b * a.T;
-    const T* x = static_cast<const T*>(sd.x) + b * sd.xb + at * sd.xt + h * sd.xh;
-    T* y = static_cast<T*>(sd.y) + b * sd.yb + at * sd.yt + h * sd.yh;
-    const float2* cs = turn + t * a.pairs;
-    if constexpr (LAYOUT == kHalves) {
-      if ((int)u < halves) {
-        const int m = u * VEC;
-        float p[VEC], q[VEC];
-        embed::load_vec<T, VEC>(x + m, p);
-        embed::load_vec<T, VEC>(x + a.pairs + m, q);
+  const int halves = LAYOUT == kHalves ? a.pairs / VEC : 0;  // columns of both halves at once
+  const int columns = a.D / VEC - halves;                   // of a head
+  const unsigned heads = a.heads[0] + a.heads[1], all = tokens * heads;
+  // threads over the columns of a head, then over the rows (token, head)
+  const int wide = min(columns, THREADS), step = THREADS / wide;
+  const int row0 = threadIdx.x / wide;
+  if (row0 >= step) return;
+  for (int u = threadIdx.x % wide; u < columns; u += wide) {
+    const bool both = LAYOUT == kHalves && u < halves;
+    const int d0 = (LAYOUT == kHalves && !both ? u + halves : u) * VEC;
+    const bool turns = LAYOUT == kHalves ? both : d0 < 2 * a.pairs;
+    for (unsigned rb = row0; rb < all; rb += LOADS * step) {
+      const T* x[LOADS];
+      T* y[LOADS];
+      R p[LOADS], q[LAYOUT == kHalves ? LOADS : 1];
+      int cs_at[LOADS];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float2 w = cs[m + e];
-          const float f = p[e], g = q[e];
-          p[e] = f * w.x - g * w.y;
-          q[e] = g * w.x + f * w.y;
-        }
-        embed::store_vec<T, VEC>(y + m, p);
-        embed::store_vec<T, VEC>(y + a.pairs + m, q);
-      } else {
-        const int d = (u + halves) * VEC;
-        float p[VEC];
-        embed::load_vec<T, VEC>(x + d, p);
-        embed::store_vec<T, VEC>(y + d, p);
+      for (int k = 0; k < LOADS; ++k) {
+        const unsigned r = rb + k * step;
+        if (r >= all) continue;
+        const unsigned t = __umulhi(r, a.magic);
+        int h = r - t * heads;
+        const int i = h >= a.heads[0];
+        if (i) h -= a.heads[0];
+        x[k] = static_cast<const T*>(a.s[i].x) + base[t][2 * i] + h * a.s[i].xh + d0;
+        y[k] = static_cast<T*>(a.s[i].y) + base[t][2 * i + 1] + h * a.s[i].yh + d0;
+        cs_at[k] = t * a.pairs;
+        p[k].load(x[k]);
+        if constexpr (LAYOUT == kHalves)
+          if (both) q[k].load(x[k] + a.pairs);
       }
-    } else {
-      const int d0 = u * VEC;
-      float p[VEC], r[VEC];
-      embed::load_vec<T, VEC>(x + d0, p);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) r[e] = p[e];
-      if (d0 < 2 * a.pairs) {
+      for (int k = 0; k < LOADS; ++k) {
+        if (rb + k * step >= all) continue;
+        const float2* cs = turn + cs_at[k];
+        if (turns) {
+          if constexpr (LAYOUT == kHalves) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const int d = d0 + e;
-          if (d >= 2 * a.pairs) continue;
-          // the first of a pair gets a cos - b sin, the second b cos + a sin
-          bool second;
-          float other;
-          int m;
-          if constexpr (LAYOUT == kInterleaved) {
-            second = d & 1;
-            m = d >> 1;
-            other = VEC > 1 ? p[e ^ (VEC > 1)] : to_f32<T>(x[d ^ 1]);
+            for (int e = 0; e < VEC; ++e) {
+              const float2 w = cs[d0 + e];
+              const float f = p[k].get(e), g = q[k].get(e);
+              p[k].set(e, f * w.x - g * w.y);
+              q[k].set(e, g * w.x + f * w.y);
+            }
+            q[k].store(y[k] + a.pairs);
+          } else if constexpr (LAYOUT == kInterleaved && VEC > 1) {
+            // a vector holds whole pairs
+#pragma unroll
+            for (int e = 0; e < VEC; e += 2) {
+              if (d0 + e >= 2 * a.pairs) continue;
+              const float2 w = cs[(d0 + e) / 2];
+              const float f = p[k].get(e), g = p[k].get(e + 1);
+              p[k].set(e, f * w.x - g * w.y);
+              p[k].set(e + 1, g * w.x + f * w.y);
+            }
           } else {
-            second = d >= a.pairs;
-            m = second ? d - a.pairs : d;
-            other = to_f32<T>(x[second ? m : d + a.pairs]);
+            // the first of a pair gets a cos - b sin, the second b cos + a sin
+            R r = p[k];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+              const int d = d0 + e;
+              if (d >= 2 * a.pairs) continue;
+              const bool second = LAYOUT == kInterleaved ? d & 1 : d >= a.pairs;
+              const int far = LAYOUT == kInterleaved ? 1 : a.pairs;
+              const float2 w = cs[LAYOUT == kInterleaved ? d >> 1 : second ? d - a.pairs : d];
+              const float other = to_f32<T>(x[k][second ? e - far : e + far]);
+              r.set(e, p[k].get(e) * w.x + (second ? other * w.y : -(other * w.y)));
+            }
+            p[k] = r;
           }
-          const float2 w = cs[m];
-          r[e] = p[e] * w.x + (second ? other * w.y : -(other * w.y));
         }
+        p[k].store(y[k]);
       }
-      embed::store_vec<T, VEC>(y + d0, r);
     }
   }
 }

@@ -909,10 +909,14 @@ int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_
   a.freq = frequencies;
   a.amplitude = amplitude;
   a.back = back;
-  // about two angles a thread, but the tokens spread over the GPU first
-  const int64_t share = std::max<int64_t>(1, a.n / (2 * kSMs));
+  // about four angles a thread, but the tokens spread over the GPU first
+  const int64_t share = std::max<int64_t>(1, a.n / (4 * kSMs));
   a.tokens = (int)std::max<int64_t>(
-      1, std::min<int64_t>({share, rotary::MOST_TOKENS, 512 / std::max<int64_t>(pairs, 1)}));
+      1, std::min<int64_t>({share, rotary::MOST_TOKENS, 1024 / std::max<int64_t>(pairs, 1)}));
+  // row / heads by ceil(2^32 / heads) is exact while row * heads < 2^32, which the
+  // rows of one token always are (heads < 2^16)
+  if (Hq + Hk > 8192) a.tokens = 1;
+  a.magic = (unsigned)std::min<uint64_t>((1ull << 32) / (Hq + Hk) + 1, 0xffffffffu);
   const int64_t blocks = cdiv(a.n, a.tokens);
   if (blocks >= (1ll << 31)) return THERIA_ERR_UNSUPPORTED;
   const size_t smem = (size_t)a.tokens * pairs * sizeof(float2);  // 16 KB at most
@@ -1005,7 +1009,8 @@ int theria_grads_dot(const void* const* x, const void* const* u, const int64_t* 
   if (!x || !parts) return THERIA_ERR_INVALID_ARG;
   return grads_groups(x, u, nullptr, sizes, dtypes, n, [&](const grads::Table& t, int chunks) {
     const int blocks = std::min(chunks, grads::MOST_BLOCKS);
-    grads::dot_kernel<<<blocks, grads::THREADS, 0, (cudaStream_t)stream>>>(t, parts);
+    auto kern = u ? grads::dot_kernel<false> : grads::dot_kernel<true>;
+    kern<<<blocks, grads::THREADS, 0, (cudaStream_t)stream>>>(t, parts);
     parts += blocks;
     return launch_status();
   });
@@ -1043,7 +1048,7 @@ int theria_grads_clip_bwd(const void* const* x, const void* const* u, void* cons
   // the kernel's first operand is what the factor c takes
   return grads_groups(u ? u : x, u ? x : nullptr, dx, sizes, dtypes, n,
                       [&](const grads::Table& t, int chunks) {
-    return launch_chained(grads::clip_bwd_kernel, dim3(std::min(chunks, kSMs * 8)),
+    return launch_chained(u ? grads::clip_bwd_kernel<true> : grads::clip_bwd_kernel<false>, dim3(std::min(chunks, kSMs * 8)),
                           dim3(grads::THREADS), 0, (cudaStream_t)stream, t, parts, u ? np : 0,
                           stats, gnorm);
   });
