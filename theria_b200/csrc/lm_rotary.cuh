@@ -17,7 +17,7 @@
 #pragma once
 
 #include "common.cuh"
-#include "lm_embed.cuh"
+#include "tc_common.cuh"
 
 namespace theria {
 namespace rotary {
@@ -66,29 +66,67 @@ __device__ __forceinline__ int64_t position_of(const Args& a, int64_t i) {
   return i - int_at(a.offsets, a.wide, lo);
 }
 
-// VEC values as they lie in memory.
+// VEC values as they lie in memory, and as floats.
 template <typename T, int VEC>
 struct Raw {
   uint4 r;
   __device__ __forceinline__ void load(const T* p) { r = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = r; }
-  __device__ __forceinline__ float get(int e) const {
-    return to_f32<T>(reinterpret_cast<const T*>(&r)[e]);
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC == 4) v[i] = __uint_as_float(w[i]);
+      else tc::unpack2<T>(w[i], v[2 * i], v[2 * i + 1]);
+    }
   }
-  __device__ __forceinline__ void set(int e, float v) { reinterpret_cast<T*>(&r)[e] = from_f32<T>(v); }
+  __device__ __forceinline__ void set(const float (&v)[VEC]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (VEC == 4) w[i] = __float_as_uint(v[i]);
+      else w[i] = tc::pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
 };
 template <typename T>
 struct Raw<T, 1> {
   T r;
   __device__ __forceinline__ void load(const T* p) { r = *p; }
   __device__ __forceinline__ void store(T* p) const { *p = r; }
-  __device__ __forceinline__ float get(int) const { return to_f32<T>(r); }
-  __device__ __forceinline__ void set(int, float v) { r = from_f32<T>(v); }
+  __device__ __forceinline__ void get(float (&v)[1]) const { v[0] = to_f32<T>(r); }
+  __device__ __forceinline__ void set(const float (&v)[1]) { r = from_f32<T>(v[0]); }
 };
+
+// N floats of shared memory, 16 bytes at a time where N is a multiple of 4 and
+// they start on such a boundary.
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float (&v)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(p + i);
+      v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 q = *reinterpret_cast<const float2*>(p + i);
+      v[i] = q.x; v[i + 1] = q.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = p[i];
+  }
+}
 
 template <typename T, int VEC, int LAYOUT>
 __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
-  extern __shared__ float2 turn[];  // [tokens][pairs] {cos, sin} * amplitude
+  // [tokens][2][padded pairs]: all cos * amplitude of a token, then all sin
+  extern __shared__ float4 turn4[];
+  float* turn = reinterpret_cast<float*>(turn4);
+  const int padded = (a.pairs + 3) & ~3;
   __shared__ double at_pos[MOST_TOKENS];
   __shared__ int64_t base[MOST_TOKENS][4];  // where the token's q, yq, k, yk start
   constexpr int LOADS = LAYOUT == kHalves ? 2 : 4;  // heads in flight
@@ -110,7 +148,8 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
     const double turns = at_pos[t] * a.freq[m] * 0.15915494309189533577;
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    turn[i] = make_float2(c * a.amplitude, (a.back ? -s : s) * a.amplitude);
+    turn[2 * t * padded + m] = c * a.amplitude;
+    turn[(2 * t + 1) * padded + m] = (a.back ? -s : s) * a.amplitude;
   }
   __syncthreads();
   const int halves = LAYOUT == kHalves ? a.pairs / VEC : 0;  // columns of both halves at once
@@ -139,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
         if (i) h -= a.heads[0];
         x[k] = static_cast<const T*>(a.s[i].x) + base[t][2 * i] + h * a.s[i].xh + d0;
         y[k] = static_cast<T*>(a.s[i].y) + base[t][2 * i + 1] + h * a.s[i].yh + d0;
-        cs_at[k] = t * a.pairs;
+        cs_at[k] = 2 * t * padded;
         p[k].load(x[k]);
         if constexpr (LAYOUT == kHalves)
           if (both) q[k].load(x[k] + a.pairs);
@@ -147,41 +186,50 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
 #pragma unroll
       for (int k = 0; k < LOADS; ++k) {
         if (rb + k * step >= all) continue;
-        const float2* cs = turn + cs_at[k];
+        const float *cs = turn + cs_at[k], *sn = cs + padded;
         if (turns) {
+          float v[VEC];
+          p[k].get(v);
           if constexpr (LAYOUT == kHalves) {
+            float g[VEC], c[VEC], n[VEC], r[VEC];
+            q[k].get(g);
+            load_floats(cs + d0, c);
+            load_floats(sn + d0, n);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-              const float2 w = cs[d0 + e];
-              const float f = p[k].get(e), g = q[k].get(e);
-              p[k].set(e, f * w.x - g * w.y);
-              q[k].set(e, g * w.x + f * w.y);
+              r[e] = v[e] * c[e] - g[e] * n[e];
+              g[e] = g[e] * c[e] + v[e] * n[e];
             }
+            p[k].set(r);
+            q[k].set(g);
             q[k].store(y[k] + a.pairs);
           } else if constexpr (LAYOUT == kInterleaved && VEC > 1) {
-            // a vector holds whole pairs
+            // a vector holds whole pairs; the last may go past the rotated ones (the
+            // floats read there are not used)
+            float c[VEC / 2], n[VEC / 2];
+            load_floats(cs + d0 / 2, c);
+            load_floats(sn + d0 / 2, n);
 #pragma unroll
             for (int e = 0; e < VEC; e += 2) {
-              if (d0 + e >= 2 * a.pairs) continue;
-              const float2 w = cs[(d0 + e) / 2];
-              const float f = p[k].get(e), g = p[k].get(e + 1);
-              p[k].set(e, f * w.x - g * w.y);
-              p[k].set(e + 1, g * w.x + f * w.y);
+              const float f = v[e], g = v[e + 1];
+              const bool on = d0 + e < 2 * a.pairs;
+              v[e] = on ? f * c[e / 2] - g * n[e / 2] : f;
+              v[e + 1] = on ? g * c[e / 2] + f * n[e / 2] : g;
             }
+            p[k].set(v);
           } else {
             // the first of a pair gets a cos - b sin, the second b cos + a sin
-            R r = p[k];
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
               const int d = d0 + e;
               if (d >= 2 * a.pairs) continue;
               const bool second = LAYOUT == kInterleaved ? d & 1 : d >= a.pairs;
               const int far = LAYOUT == kInterleaved ? 1 : a.pairs;
-              const float2 w = cs[LAYOUT == kInterleaved ? d >> 1 : second ? d - a.pairs : d];
+              const int m = LAYOUT == kInterleaved ? d >> 1 : second ? d - a.pairs : d;
               const float other = to_f32<T>(x[k][second ? e - far : e + far]);
-              r.set(e, p[k].get(e) * w.x + (second ? other * w.y : -(other * w.y)));
+              v[e] = v[e] * cs[m] + (second ? other * sn[m] : -(other * sn[m]));
             }
-            p[k] = r;
+            p[k].set(v);
           }
         }
         p[k].store(y[k]);

@@ -919,7 +919,8 @@ int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_
   a.magic = (unsigned)std::min<uint64_t>((1ull << 32) / (Hq + Hk) + 1, 0xffffffffu);
   const int64_t blocks = cdiv(a.n, a.tokens);
   if (blocks >= (1ll << 31)) return THERIA_ERR_UNSUPPORTED;
-  const size_t smem = (size_t)a.tokens * pairs * sizeof(float2);  // 16 KB at most
+  // 16 KB of angles at most (one token: 2048 pairs), the pairs filled up to 16 bytes
+  const size_t smem = (size_t)a.tokens * 2 * up(pairs, 4) * sizeof(float);
   return by_type(dtype, [&](auto t) {
     using E = decltype(t);
     constexpr int VEC = embed::Vec<E>::n;
