@@ -1,14 +1,16 @@
 // Attention over packed sequences on the CUDA cores: float32 (always in
 // float32), and 16-bit tensors that the tensor-core kernels cannot take
-// (more than 64 query heads a key head, or rows off 16-byte boundaries).
+// (more than 128 query heads a key head, or rows off 16-byte boundaries).
 //
 // Tiles of 64 rows by 64 columns, 16 x 16 threads: a thread holds 4 x 4 of the
 // tile's scores (rows 4 ty + i, columns tx + 16 j) and, of the sums over its
 // columns, the same 4 rows of DT / 16 values.  Operands lie in shared memory as
 // float32 rows of DT + 4 values: a step of 4 along a row is one 16-byte load,
 // free of bank conflicts down the columns' 16 rows.  A score step of 4 costs 8
-// such loads for 64 products, a sums step of 4 columns 4 + 4 * DT / 64 for 16 *
-// DT / 16 * 4; the loads and the FMA pipe are about evenly used.
+// such loads (12 wavefronts a warp) for 64 products, so the FMA pipe sets the pace
+// as long as the next tile is on its way meanwhile: float32 rows come by cp.async,
+// in the forward K's while the softmax and V's sum run and V's while the next
+// scores do, in the backward into a second buffer.
 //
 // The backward is one kernel for both sides.  Its tile stays on 64 rows x1, x2
 // and walks over tiles of 64 y1, y2:
@@ -32,8 +34,21 @@ struct SimtSmem {
   static constexpr int kTile = SR * kRow;
   static constexpr int kS = SR * (SR + 4);       // a tile of scores
   static constexpr int kFwd = (3 * kTile + kS) * 4;
-  static constexpr int kBwd = (4 * kTile + 2 * kS + 2 * SR) * 4;
+  static constexpr int kBwd = (6 * kTile + kS + 4 * SR) * 4;  // x, two of y, scores, terms
 };
+
+__device__ __forceinline__ void async16(float* dst, const float* src, bool on) {
+  // on false: 16 bytes of zeros, src is not read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest `left` groups have landed (for this thread's copies).
+template <int left>
+__device__ __forceinline__ void async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(left) : "memory");
+}
 
 // 16 bytes (VEC > 1) or one value, as floats.
 template <typename T, int VEC>
@@ -49,12 +64,23 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
 }
 
 // 64 rows of a tensor into shared memory as float32, zero beyond row `n` and
-// column D.  row_at(r): the element where row r starts.
-template <typename T, int DT, typename F>
+// column D.  row_at(r): the element where row r starts.  ASYNC (float32, whole
+// rows of 16 bytes on such boundaries): by cp.async, else at once.
+template <typename T, int DT, bool ASYNC, typename F>
 __device__ __forceinline__ void load_tile(float* dst, const T* src, int n, int D, F row_at) {
-  for (int i = threadIdx.x; i < SR * DT; i += SIMT_THREADS) {
-    const int r = i / DT, d = i % DT;
-    dst[r * SimtSmem<DT>::kRow + d] = r < n && d < D ? to_f32<T>(src[row_at(r) + d]) : 0.f;
+  if constexpr (ASYNC) {
+    constexpr int CH = DT / 4;
+#pragma unroll
+    for (int i0 = 0; i0 < SR * CH; i0 += SIMT_THREADS) {
+      const int i = i0 + threadIdx.x, r = i / CH, d = (i % CH) * 4;
+      const bool on = r < n && d < D;
+      async16(dst + r * SimtSmem<DT>::kRow + d, on ? src + row_at(r) + d : src, on);
+    }
+  } else {
+    for (int i = threadIdx.x; i < SR * DT; i += SIMT_THREADS) {
+      const int r = i / DT, d = i % DT;
+      dst[r * SimtSmem<DT>::kRow + d] = r < n && d < D ? to_f32<T>(src[row_at(r) + d]) : 0.f;
+    }
   }
 }
 
@@ -90,7 +116,7 @@ __device__ __forceinline__ void tile_scores(float (&s)[4][4], const float* x, co
 template <int DT>
 struct Cols {
   static constexpr int n = DT / 16;
-  static constexpr int run = n < 4 ? n : 4;
+  static constexpr int run = n % 4 == 0 ? 4 : n % 2 == 0 ? 2 : 1;
   __device__ static int at(int c) {  // column of the thread's value c
     return (c / run) * (16 * run) + (threadIdx.x & 15) * run + c % run;
   }
@@ -141,8 +167,8 @@ __device__ __forceinline__ void put_scores(float* p, const float (&s)[4][4]) {
     for (int j = 0; j < 4; ++j) p[(4 * ty + i) * (SR + 4) + tx + 16 * j] = s[i][j];
 }
 
-template <typename T, int DT>
-__global__ void __launch_bounds__(SIMT_THREADS)
+template <typename T, int DT, bool ASYNC>
+__global__ void __launch_bounds__(SIMT_THREADS, DT <= 96 ? 2 : 1)
 simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 T* __restrict__ o, float* __restrict__ lse, const int4* items, const int* count,
                 Problem pr) {
@@ -157,10 +183,24 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   const int G = pr.G, len = it.y, first = it.z;
   const int rows = min(SR, (int)min((int64_t)len * G - first, (int64_t)SR));
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  load_tile<T, DT>(xs, q, rows, pr.D, [&](int r) {
-    const int p = first + r;
-    return (int64_t)(it.x + p / G) * pr.q_t + (int64_t)(hk * G + p % G) * pr.q_h;
+  auto load_k = [&](int j0) {
+    load_tile<T, DT, ASYNC>(ks, k, len - j0, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
+    });
+  };
+  auto load_v = [&](int j0) {
+    load_tile<T, DT, ASYNC>(vs, v, len - j0, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
+    });
+  };
+  load_tile<T, DT, ASYNC>(xs, q, rows, pr.D, [&](int r) {
+    const int p = first + r, t = p / G;
+    return (int64_t)(it.x + t) * pr.q_t + (int64_t)(hk * G + p - t * G) * pr.q_h;
   });
+  load_k(0);
+  async_commit();
+  load_v(0);
+  async_commit();
   const int last = (first + rows - 1) / G;  // the last row's token
   const int keys = pr.causal ? last + 1 : len;
   const float c = pr.scale * kLog2e;
@@ -175,17 +215,13 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     for (int x = 0; x < DT / 16; ++x) acc[i][x] = 0.f;
   }
   for (int j0 = 0; j0 < keys; j0 += SR) {
-    const int n = min(SR, len - j0);
-    __syncthreads();
-    load_tile<T, DT>(ks, k, n, pr.D, [&](int r) {
-      return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
-    });
-    load_tile<T, DT>(vs, v, n, pr.D, [&](int r) {
-      return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
-    });
+    async_wait<1>();
     __syncthreads();
     float s[4][4];
     tile_scores<DT>(s, xs, ks);
+    __syncthreads();
+    if (j0 + SR < keys) load_k(j0 + SR);
+    async_commit();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float mt = -INFINITY;
@@ -197,12 +233,12 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
       for (int x = 8; x > 0; x >>= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, x));
       const float mn = fmaxf(m[i], mt), sub = mn == -INFINITY ? 0.f : mn;
-      const float alpha = exp2f(m[i] - sub);
+      const float alpha = tc::ex2(m[i] - sub);
       m[i] = mn;
       float rs = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = exp2f(s[i][j] - sub);
+        s[i][j] = tc::ex2(s[i][j] - sub);
         rs += s[i][j];
       }
       l[i] = l[i] * alpha + rs;
@@ -210,9 +246,14 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       for (int x = 0; x < DT / 16; ++x) acc[i][x] *= alpha;
     }
     put_scores(ps, s);
+    async_wait<1>();
     __syncthreads();
     tile_sums<DT>(acc, ps, vs);
+    __syncthreads();
+    if (j0 + SR < keys) load_v(j0 + SR);
+    async_commit();
   }
+  async_wait<0>();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float sum = l[i];
@@ -263,8 +304,8 @@ terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* _
 
 // One split of a backward tile (see above).  part: NULL where there is one
 // split (results rounded to T at once), else float32 [splits][2][T * Hkv][D].
-template <typename T, int DT, bool KEYS>
-__global__ void __launch_bounds__(SIMT_THREADS)
+template <typename T, int DT, bool KEYS, bool ASYNC>
+__global__ void __launch_bounds__(SIMT_THREADS, DT <= 48 ? 2 : 1)
 simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ dout, const float2* terms, T* __restrict__ out1,
                 T* __restrict__ out2, float* part, const int4* items, const int* count,
@@ -272,9 +313,9 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   using L = SimtSmem<DT>;
   extern __shared__ float4 smem4[];
   float* x1 = reinterpret_cast<float*>(smem4);
-  float *x2 = x1 + L::kTile, *y1 = x2 + L::kTile, *y2 = y1 + L::kTile;
-  float *ps = y2 + L::kTile, *ds = ps + L::kS;
-  float2* ts = reinterpret_cast<float2*>(ds + L::kS);
+  float *x2 = x1 + L::kTile, *ybuf = x2 + L::kTile;  // y1, y2 of even and of odd tiles
+  float* ps = ybuf + 4 * L::kTile;
+  float2* ts = reinterpret_cast<float2*>(ps + L::kS);  // [2][SR]
   grid_wait();
   const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
   if (tile >= *count) return;
@@ -283,24 +324,27 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   const int64_t q_rows = (int64_t)len * G;
   const int rows = (int)min((int64_t)SR, (KEYS ? len : q_rows) - first);
-  auto q_at = [&](int64_t p, int64_t st, int64_t sh) {
-    return (it.x + p / G) * st + (hk * G + p % G) * sh;
+  auto q_at = [&](int p, int64_t st, int64_t sh) {
+    const int t = p / G;
+    return (it.x + t) * st + (int64_t)(hk * G + p - t * G) * sh;
   };
-  auto load_q = [&](float* a, float* b, int64_t p0, int n) {
-    load_tile<T, DT>(a, q, n, pr.D, [&](int r) { return q_at(p0 + r, pr.q_t, pr.q_h); });
-    load_tile<T, DT>(b, dout, n, pr.D,
-                     [&](int r) { return q_at(p0 + r, (int64_t)pr.H * pr.D, pr.D); });
+  auto load_q = [&](float* a, float* b, float2* tm, int p0, int n) {
+    load_tile<T, DT, ASYNC>(a, q, n, pr.D, [&](int r) { return q_at(p0 + r, pr.q_t, pr.q_h); });
+    load_tile<T, DT, ASYNC>(b, dout, n, pr.D,
+                            [&](int r) { return q_at(p0 + r, (int64_t)pr.H * pr.D, pr.D); });
     if (threadIdx.x < SR)
-      ts[threadIdx.x] = (int)threadIdx.x < n ? terms[q_at(p0 + threadIdx.x, pr.H, 1)]
+      tm[threadIdx.x] = (int)threadIdx.x < n ? terms[q_at(p0 + threadIdx.x, pr.H, 1)]
                                              : make_float2(-INFINITY, 0.f);
   };
   auto load_k = [&](float* a, float* b, int j0, int n) {
-    load_tile<T, DT>(a, k, n, pr.D,
-                     [&](int r) { return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h; });
-    load_tile<T, DT>(b, v, n, pr.D,
-                     [&](int r) { return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h; });
+    load_tile<T, DT, ASYNC>(a, k, n, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
+    });
+    load_tile<T, DT, ASYNC>(b, v, n, pr.D, [&](int r) {
+      return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
+    });
   };
-  if (KEYS) load_k(x1, x2, first, rows); else load_q(x1, x2, first, rows);
+  if (KEYS) load_k(x1, x2, first, rows); else load_q(x1, x2, ts, first, rows);
   // the tiles of y, and this split's share of them
   int64_t y_from = 0, y_to = KEYS ? q_rows : len;
   if (pr.causal && KEYS) y_from = (int64_t)first * G;
@@ -317,11 +361,22 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       a1[i][x] = 0.f;
       if (KEYS) a2[KEYS ? i : 0][x] = 0.f;
     }
-  for (int t = t0; t < t1; ++t) {
+  auto load_y = [&](int t) {
     const int64_t e0 = y_from + (int64_t)t * SR;
     const int n = (int)min((int64_t)SR, (KEYS ? q_rows : len) - e0);
-    __syncthreads();
-    if (KEYS) load_q(y1, y2, e0, n); else load_k(y1, y2, (int)e0, n);
+    float* y1 = ybuf + (t & 1) * 2 * L::kTile;
+    if (KEYS) load_q(y1, y1 + L::kTile, ts + (t & 1) * SR, (int)e0, n);
+    else load_k(y1, y1 + L::kTile, (int)e0, n);
+  };
+  if (t0 < t1) load_y(t0);
+  async_commit();
+  for (int t = t0; t < t1; ++t) {
+    const int64_t e0 = y_from + (int64_t)t * SR;
+    const float *y1 = ybuf + (t & 1) * 2 * L::kTile, *y2 = y1 + L::kTile;
+    const float2* tq = ts + (KEYS ? (t & 1) * SR : 0);
+    if (t + 1 < t1) load_y(t + 1);
+    async_commit();
+    async_wait<1>();
     __syncthreads();
     float s[4][4], dp[4][4];
     tile_scores<DT>(s, x1, y1);
@@ -331,20 +386,27 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * ty + i, e = tx + 16 * j;
-        const float2 tm = ts[KEYS ? e : r];
-        const int64_t qr = KEYS ? e0 + e : (int64_t)first + r;      // query row
+        const float2 tm = tq[KEYS ? e : r];
+        // key <= query token: key * G <= query row
+        const int64_t qr = KEYS ? e0 + e : (int64_t)first + r;
         const int64_t key = KEYS ? (int64_t)first + r : e0 + e;
-        const bool on = key < len && qr < q_rows && (!pr.causal || key <= qr / G);
-        const float p = on ? exp2f(fmaf(s[i][j], c, tm.x)) : 0.f;
+        const bool on = key < len && qr < q_rows && (!pr.causal || key * G <= qr);
+        const float p = on ? tc::ex2(fmaf(s[i][j], c, tm.x)) : 0.f;
         s[i][j] = p;
         dp[i][j] = on ? p * (dp[i][j] + tm.y) : 0.f;
       }
-    if (KEYS) put_scores(ps, s);
-    put_scores(ds, dp);
+    if constexpr (KEYS) {
+      put_scores(ps, s);
+      __syncthreads();
+      tile_sums<DT>(a2, ps, y2);
+      __syncthreads();
+    }
+    put_scores(ps, dp);
     __syncthreads();
-    tile_sums<DT>(a1, ds, y1);
-    if constexpr (KEYS) tile_sums<DT>(a2, ps, y2);
+    tile_sums<DT>(a1, ps, y1);
+    __syncthreads();
   }
+  async_wait<0>();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;

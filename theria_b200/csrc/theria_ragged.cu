@@ -101,12 +101,31 @@ int by_type(int dtype, F f) {
   if (dtype == THERIA_F16) return f(__half{});
   return f(__nv_bfloat16{});
 }
-template <typename F>
-int by_width(int D, F f) {
-  if (D <= 16) return f(std::integral_constant<int, 16>{});
-  if (D <= 32) return f(std::integral_constant<int, 32>{});
-  if (D <= 64) return f(std::integral_constant<int, 64>{});
-  return f(std::integral_constant<int, 128>{});
+// Calls f(DT, ASYNC): the kernels' width, and whether rows come by cp.async.
+template <typename T, typename F>
+int by_width(int D, bool async, F f) {
+  using No = std::false_type;
+  auto go = [&](auto w) {
+    if constexpr (std::is_same<T, float>::value)
+      if (async) return f(w, std::true_type{});
+    return f(w, No{});
+  };
+  if constexpr (std::is_same<T, float>::value) {
+    if (D <= 16) return go(std::integral_constant<int, 16>{});
+    if (D <= 32) return go(std::integral_constant<int, 32>{});
+  }
+  if (D <= 64) return go(std::integral_constant<int, 64>{});
+  if constexpr (std::is_same<T, float>::value)
+    if (D <= 96) return go(std::integral_constant<int, 96>{});
+  return go(std::integral_constant<int, 128>{});
+}
+// Whether the rows are whole 16-byte vectors on such boundaries.
+bool whole_rows(int dtype, const Problem& p, std::initializer_list<const void*> ptrs) {
+  const int64_t vec = 16 / elem_size(dtype);
+  bool ok = p.D % vec == 0;
+  for (const void* x : ptrs) ok = ok && tc::aligned16(x);
+  for (int64_t s : {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h}) ok = ok && s % vec == 0;
+  return ok;
 }
 
 int run_plan(const void* offsets, int wide, const Problem& p, const List& a, const List& b,
@@ -172,9 +191,9 @@ unsigned blocks(const Problem& p, int per, int step) {
 template <typename T>
 int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const FwdWs& ws,
              const Problem& p, cudaStream_t st) {
-  return by_width(p.D, [&](auto w) {
+  return by_width<T>(p.D, whole_rows(THERIA_F32, p, {q, k, v}), [&](auto w, auto async) {
     constexpr int DT = decltype(w)::value;
-    auto kern = simt_fwd_kernel<T, DT>;
+    auto kern = simt_fwd_kernel<T, DT, decltype(async)::value>;
     constexpr int smem = SimtSmem<DT>::kFwd;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
         cudaSuccess)
@@ -196,8 +215,9 @@ template <typename T>
 int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
              void* dv, const BwdWs& ws, const void* offsets, int wide, const Problem& p,
              cudaStream_t st) {
-  return by_width(p.D, [&](auto w) {
+  return by_width<T>(p.D, whole_rows(THERIA_F32, p, {q, k, v, dout}), [&](auto w, auto async) {
     constexpr int DT = decltype(w)::value;
+    constexpr bool ASYNC = decltype(async)::value;
     constexpr int smem = SimtSmem<DT>::kBwd;
     auto run = [&](auto kern, const List& l, int splits, void* o1, void* o2, float* part) {
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
@@ -209,10 +229,10 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
                             (const int*)l.count, p);
     };
     if (dq != nullptr)
-      if (int e = run(simt_bwd_kernel<T, DT, false>, ws.lq, 1, dq, nullptr, nullptr)) return e;
+      if (int e = run(simt_bwd_kernel<T, DT, false, ASYNC>, ws.lq, 1, dq, nullptr, nullptr)) return e;
     if (dk == nullptr) return (int)THERIA_OK;
     const int splits = key_splits(p, SR);
-    if (int e = run(simt_bwd_kernel<T, DT, true>, ws.lk, splits, dk, dv,
+    if (int e = run(simt_bwd_kernel<T, DT, true, ASYNC>, ws.lk, splits, dk, dv,
                     splits > 1 ? ws.part : nullptr))
       return e;
     return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : (int)THERIA_OK;
@@ -223,11 +243,10 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
 // Rows of 16 bytes on 16-byte boundaries, and a group that a tile of 64 rows
 // holds.  (Measured against the CUDA-core kernels: see ragged_tc_bwd.cuh.)
 bool use_tc(int dtype, const Problem& p, std::initializer_list<const void*> ptrs) {
-  if (dtype == THERIA_F32 || p.D % 8 || p.G > BY || tc::encode_fn() == nullptr) return false;
-  for (const void* x : ptrs)
-    if (!tc::aligned16(x)) return false;
+  if (dtype == THERIA_F32 || p.G > BY || tc::encode_fn() == nullptr) return false;
+  if (!whole_rows(dtype, p, ptrs)) return false;
   for (int64_t s : {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h})
-    if (s % 8 || s <= 0 || s >= (1ll << 38)) return false;
+    if (s <= 0 || s >= (1ll << 38)) return false;
   return true;
 }
 
