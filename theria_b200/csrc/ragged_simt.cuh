@@ -2,15 +2,21 @@
 // float32), and 16-bit tensors that the tensor-core kernels cannot take
 // (more than 128 query heads a key head, or rows off 16-byte boundaries).
 //
-// Tiles of 64 rows by 64 columns, 16 x 16 threads: a thread holds 4 x 4 of the
-// tile's scores (rows 4 ty + i, columns tx + 16 j) and, of the sums over its
-// columns, the same 4 rows of DT / 16 values.  Operands lie in shared memory as
-// float32 rows of DT + 4 values: a step of 4 along a row is one 16-byte load,
-// free of bank conflicts down the columns' 16 rows.  A score step of 4 costs 8
-// such loads (12 wavefronts a warp) for 64 products, so the FMA pipe sets the pace
-// as long as the next tile is on its way meanwhile: float32 rows come by cp.async,
-// in the forward K's while the softmax and V's sum run and V's while the next
-// scores do, in the backward into a second buffer.
+// A block is 16 warps on one tile of rows: in the forward four groups of 4 warps on
+// 32 rows, in the backward two of 8 on 64, each group taking every fourth (second)
+// tile of 64 (32) columns; their sums are put together at the end.  One block fills
+// an SM, the longest row of tiles takes a quarter (half) of the time, and the groups'
+// loads, softmax and barriers hide behind one another's products.  (One group a block
+// and two or three blocks an SM, which the hardware put on few SMs: 2395 tokens, 5
+// heads of 72, forward 148 us, queries 410, keys 254; blocks of one group alone on
+// their SM 188, 208, 301.)
+//
+// In a group a thread holds rows 4 ty + i and columns tx + 16 j of the tile's scores
+// and, of the sums over its columns, the same 4 rows of DT / 16 values.  Operands lie
+// in shared memory as float32 rows of DT + 4 values: a step of 4 along a row is one
+// 16-byte load, free of bank conflicts down the columns' 16 rows.  float32 rows come
+// by cp.async: in the forward K's while the softmax and V's sum run and V's while the
+// next scores do, in the backward into a second buffer.
 //
 // The backward is one kernel for both sides.  Its tile stays on 64 rows x1, x2
 // and walks over tiles of 64 y1, y2:
@@ -25,16 +31,27 @@
 namespace theria {
 namespace ragged {
 
-constexpr int SR = 64;             // rows and columns of a tile
-constexpr int SIMT_THREADS = 256;
+constexpr int FR = 32, FC = 64;    // rows and columns of a forward tile
+constexpr int SR = 64, SC = 32;    // ... of a backward tile
+constexpr int FWD_THREADS = FR * 4, BWD_THREADS = SR * 4;  // ... of a group
 
 template <int DT>
 struct SimtSmem {
   static constexpr int kRow = DT + 4;            // floats of an operand's row
-  static constexpr int kTile = SR * kRow;
-  static constexpr int kS = SR * (SR + 4);       // a tile of scores
-  static constexpr int kFwd = (3 * kTile + kS) * 4;
-  static constexpr int kBwd = (6 * kTile + kS + 4 * SR) * 4;  // x, two of y, scores, terms
+  // groups of a forward, of a backward block; narrow heads, of short sequences for the
+  // most part, take one (25 sequences of 64, 4 heads of 16: forward 5.7 us, with four
+  // groups 9.2)
+  static constexpr int FG = DT <= 32 ? 1 : 4, SG = DT <= 32 ? 1 : 2;
+  // a group's k, v (wide heads: tiles of half the columns), scores; a block's q
+  static constexpr int kFC = DT <= 64 ? FC : FC / 2;
+  static constexpr int kFwdGroup = 2 * kFC * kRow + FR * (kFC + 4);
+  static constexpr int kFwd = (FR * kRow + FG * kFwdGroup) * 4;
+  // a group's two of y1, y2, scores, two of terms; a block's x1, x2, terms
+  static constexpr int kBwdGroup = 4 * SC * kRow + SR * (SC + 4) + 4 * SC;
+  static constexpr int kBwd = (2 * SR * kRow + 2 * SR + SG * kBwdGroup) * 4;
+  static_assert(kFwd <= 232448 && kBwd <= 232448, "shared memory of a block");
+  // a forward group's sums go over its buffers at the end
+  static_assert(FR * kRow + 2 * FR <= kFwdGroup, "room for a group's sums");
 };
 
 __device__ __forceinline__ void async16(float* dst, const float* src, bool on) {
@@ -63,21 +80,23 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC]) {
   }
 }
 
-// 64 rows of a tensor into shared memory as float32, zero beyond row `n` and
+// N rows of a tensor into shared memory as float32, zero beyond row `n` and
 // column D.  row_at(r): the element where row r starts.  ASYNC (float32, whole
 // rows of 16 bytes on such boundaries): by cp.async, else at once.
-template <typename T, int DT, bool ASYNC, typename F>
-__device__ __forceinline__ void load_tile(float* dst, const T* src, int n, int D, F row_at) {
+template <typename T, int DT, int N, int THREADS, bool ASYNC, typename F>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int n, int D, int tid,
+                                          F row_at) {
   if constexpr (ASYNC) {
     constexpr int CH = DT / 4;
 #pragma unroll
-    for (int i0 = 0; i0 < SR * CH; i0 += SIMT_THREADS) {
-      const int i = i0 + threadIdx.x, r = i / CH, d = (i % CH) * 4;
+    for (int i0 = 0; i0 < N * CH; i0 += THREADS) {
+      const int i = i0 + tid, r = i / CH, d = (i % CH) * 4;
+      if (N * CH % THREADS != 0 && i >= N * CH) continue;
       const bool on = r < n && d < D;
       async16(dst + r * SimtSmem<DT>::kRow + d, on ? src + row_at(r) + d : src, on);
     }
   } else {
-    for (int i = threadIdx.x; i < SR * DT; i += SIMT_THREADS) {
+    for (int i = tid; i < N * DT; i += THREADS) {
       const int r = i / DT, d = i % DT;
       dst[r * SimtSmem<DT>::kRow + d] = r < n && d < D ? to_f32<T>(src[row_at(r) + d]) : 0.f;
     }
@@ -85,25 +104,26 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, int n, int D
 }
 
 // s[i][j] = x[4 ty + i] . y[tx + 16 j]
-template <int DT>
-__device__ __forceinline__ void tile_scores(float (&s)[4][4], const float* x, const float* y) {
+template <int DT, int J>
+__device__ __forceinline__ void tile_scores(float (&s)[4][J], const float* x, const float* y,
+                                            int ty) {
   constexpr int K = SimtSmem<DT>::kRow;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < J; ++j) s[i][j] = 0.f;
 #pragma unroll 4
   for (int d = 0; d < DT; d += 4) {
-    float4 a[4], b[4];
+    float4 a[4], b[J];
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(x + (4 * ty + i) * K + d);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4*>(y + (tx + 16 * j) * K + d);
+    for (int j = 0; j < J; ++j) b[j] = *reinterpret_cast<const float4*>(y + (tx + 16 * j) * K + d);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < J; ++j) {
         s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
         s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
         s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
@@ -123,13 +143,12 @@ struct Cols {
 };
 
 // acc[i][c] += sum over the tile's columns e of p[4 ty + i][e] * y[e][column c]
-template <int DT>
+template <int DT, int C>
 __device__ __forceinline__ void tile_sums(float (&acc)[4][DT / 16], const float* p,
-                                          const float* y) {
-  constexpr int K = SimtSmem<DT>::kRow, KS = SR + 4, RUN = Cols<DT>::run;
-  const int ty = threadIdx.x >> 4;
+                                          const float* y, int ty) {
+  constexpr int K = SimtSmem<DT>::kRow, KS = C + 4, RUN = Cols<DT>::run;
 #pragma unroll 2
-  for (int e = 0; e < SR; e += 4) {
+  for (int e = 0; e < C; e += 4) {
     float4 a[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(p + (4 * ty + i) * KS + e);
@@ -159,47 +178,49 @@ __device__ __forceinline__ void tile_sums(float (&acc)[4][DT / 16], const float*
   }
 }
 
-__device__ __forceinline__ void put_scores(float* p, const float (&s)[4][4]) {
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+template <int J>
+__device__ __forceinline__ void put_scores(float* p, const float (&s)[4][J], int ty) {
+  const int tx = threadIdx.x & 15;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[(4 * ty + i) * (SR + 4) + tx + 16 * j] = s[i][j];
+    for (int j = 0; j < J; ++j) p[(4 * ty + i) * (16 * J + 4) + tx + 16 * j] = s[i][j];
 }
 
 template <typename T, int DT, bool ASYNC>
-__global__ void __launch_bounds__(SIMT_THREADS, DT <= 96 ? 2 : 1)
+__global__ void __launch_bounds__(SimtSmem<DT>::FG * FWD_THREADS)
 simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 T* __restrict__ o, float* __restrict__ lse, const int4* items, const int* count,
                 Problem pr) {
   using L = SimtSmem<DT>;
   extern __shared__ float4 smem4[];
+  constexpr int C = L::kFC, FG = L::FG;
+  const int g = threadIdx.x / FWD_THREADS, tid = threadIdx.x % FWD_THREADS;
   float* xs = reinterpret_cast<float*>(smem4);
-  float *ks = xs + L::kTile, *vs = ks + L::kTile, *ps = vs + L::kTile;
+  float* mine = xs + FR * L::kRow + g * L::kFwdGroup;  // the group's
+  float *ks = mine, *vs = ks + C * L::kRow, *ps = vs + C * L::kRow;
+  auto sync = [&] { tc::named_bar(1 + g, FWD_THREADS); };
   grid_wait();
   const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
   if (tile >= *count) return;
   const int4 it = items[tile];
   const int G = pr.G, len = it.y, first = it.z;
-  const int rows = min(SR, (int)min((int64_t)len * G - first, (int64_t)SR));
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int rows = (int)min((int64_t)len * G - first, (int64_t)FR);
+  const int ty = tid >> 4, tx = tid & 15;
   auto load_k = [&](int j0) {
-    load_tile<T, DT, ASYNC>(ks, k, len - j0, pr.D, [&](int r) {
+    load_tile<T, DT, C, FWD_THREADS, ASYNC>(ks, k, len - j0, pr.D, tid, [&](int r) {
       return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
     });
   };
   auto load_v = [&](int j0) {
-    load_tile<T, DT, ASYNC>(vs, v, len - j0, pr.D, [&](int r) {
+    load_tile<T, DT, C, FWD_THREADS, ASYNC>(vs, v, len - j0, pr.D, tid, [&](int r) {
       return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
     });
   };
-  load_tile<T, DT, ASYNC>(xs, q, rows, pr.D, [&](int r) {
+  load_tile<T, DT, FR, FG * FWD_THREADS, ASYNC>(xs, q, rows, pr.D, threadIdx.x, [&](int r) {
     const int p = first + r, t = p / G;
     return (int64_t)(it.x + t) * pr.q_t + (int64_t)(hk * G + p - t * G) * pr.q_h;
   });
-  load_k(0);
-  async_commit();
-  load_v(0);
   async_commit();
   const int last = (first + rows - 1) / G;  // the last row's token
   const int keys = pr.causal ? last + 1 : len;
@@ -214,19 +235,26 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
     for (int x = 0; x < DT / 16; ++x) acc[i][x] = 0.f;
   }
-  for (int j0 = 0; j0 < keys; j0 += SR) {
+  async_wait<0>();
+  __syncthreads();  // q
+  if (g * C < keys) load_k(g * C);
+  async_commit();
+  if (g * C < keys) load_v(g * C);
+  async_commit();
+  for (int j0 = g * C; j0 < keys; j0 += FG * C) {
+    const bool more = j0 + FG * C < keys;
     async_wait<1>();
-    __syncthreads();
-    float s[4][4];
-    tile_scores<DT>(s, xs, ks);
-    __syncthreads();
-    if (j0 + SR < keys) load_k(j0 + SR);
+    sync();
+    float s[4][C / 16];
+    tile_scores<DT>(s, xs, ks, ty);
+    sync();
+    if (more) load_k(j0 + FG * C);
     async_commit();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float mt = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < C / 16; ++j) {
         s[i][j] = j0 + tx + 16 * j < lim[i] ? s[i][j] * c : -INFINITY;
         mt = fmaxf(mt, s[i][j]);
       }
@@ -237,7 +265,7 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       m[i] = mn;
       float rs = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < C / 16; ++j) {
         s[i][j] = tc::ex2(s[i][j] - sub);
         rs += s[i][j];
       }
@@ -245,20 +273,54 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
       for (int x = 0; x < DT / 16; ++x) acc[i][x] *= alpha;
     }
-    put_scores(ps, s);
+    put_scores(ps, s, ty);
     async_wait<1>();
-    __syncthreads();
-    tile_sums<DT>(acc, ps, vs);
-    __syncthreads();
-    if (j0 + SR < keys) load_v(j0 + SR);
+    sync();
+    tile_sums<DT, C>(acc, ps, vs, ty);
+    sync();
+    if (more) load_v(j0 + FG * C);
     async_commit();
   }
   async_wait<0>();
+  // the groups' sums together, in their order: each goes over the group's buffers
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+  if (g > 0) {
+    sync();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * ty + i;
+#pragma unroll
+      for (int x = 0; x < DT / 16; ++x) mine[r * L::kRow + Cols<DT>::at(x)] = acc[i][x];
+      if (tx == 0) {
+        mine[FR * L::kRow + r] = m[i];
+        mine[FR * L::kRow + FR + r] = l[i];
+      }
+    }
+  }
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll 1
+  for (int o_ = 1; o_ < FG; ++o_) {
+    const float* theirs = mine + o_ * L::kFwdGroup;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * ty + i;
+      const float m2 = theirs[FR * L::kRow + r], l2 = theirs[FR * L::kRow + FR + r];
+      const float mn = fmaxf(m[i], m2), sub = mn == -INFINITY ? 0.f : mn;
+      const float a1 = tc::ex2(m[i] - sub), a2 = tc::ex2(m2 - sub);
+      m[i] = mn;
+      l[i] = l[i] * a1 + l2 * a2;
+#pragma unroll
+      for (int x = 0; x < DT / 16; ++x)
+        acc[i][x] = acc[i][x] * a1 + theirs[r * L::kRow + Cols<DT>::at(x)] * a2;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float sum = l[i];
-#pragma unroll
-    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const float sum = l[i];
     const int r = 4 * ty + i;
     if (r >= rows) continue;
     const int p = first + r;
@@ -305,51 +367,65 @@ terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* _
 // One split of a backward tile (see above).  part: NULL where there is one
 // split (results rounded to T at once), else float32 [splits][2][T * Hkv][D].
 template <typename T, int DT, bool KEYS, bool ASYNC>
-__global__ void __launch_bounds__(SIMT_THREADS, DT <= 48 ? 2 : 1)
+__global__ void __launch_bounds__(SimtSmem<DT>::SG * BWD_THREADS)
 simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ dout, const float2* terms, T* __restrict__ out1,
                 T* __restrict__ out2, float* part, const int4* items, const int* count,
                 Problem pr) {
   using L = SimtSmem<DT>;
+  constexpr int SG = L::SG;
   extern __shared__ float4 smem4[];
+  const int g = threadIdx.x / BWD_THREADS, tid = threadIdx.x % BWD_THREADS;
   float* x1 = reinterpret_cast<float*>(smem4);
-  float *x2 = x1 + L::kTile, *ybuf = x2 + L::kTile;  // y1, y2 of even and of odd tiles
-  float* ps = ybuf + 4 * L::kTile;
-  float2* ts = reinterpret_cast<float2*>(ps + L::kS);  // [2][SR]
+  float* x2 = x1 + SR * L::kRow;
+  float2* tx_ = reinterpret_cast<float2*>(x2 + SR * L::kRow);  // queries: x's terms [SR]
+  float* mine = reinterpret_cast<float*>(tx_ + SR) + g * L::kBwdGroup;  // the group's
+  float* ps = mine + 4 * SC * L::kRow;                         // y1, y2 of even, odd tiles first
+  float2* ts = reinterpret_cast<float2*>(ps + SR * (SC + 4));  // keys: [2][SC]
+  auto sync = [&] { tc::named_bar(1 + g, BWD_THREADS); };
   grid_wait();
   const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
   if (tile >= *count) return;
   const int4 it = items[tile];
   const int G = pr.G, len = it.y, first = it.z;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const int ty = tid >> 4, tx = tid & 15;
   const int64_t q_rows = (int64_t)len * G;
   const int rows = (int)min((int64_t)SR, (KEYS ? len : q_rows) - first);
   auto q_at = [&](int p, int64_t st, int64_t sh) {
     const int t = p / G;
     return (it.x + t) * st + (int64_t)(hk * G + p - t * G) * sh;
   };
-  auto load_q = [&](float* a, float* b, float2* tm, int p0, int n) {
-    load_tile<T, DT, ASYNC>(a, q, n, pr.D, [&](int r) { return q_at(p0 + r, pr.q_t, pr.q_h); });
-    load_tile<T, DT, ASYNC>(b, dout, n, pr.D,
-                            [&](int r) { return q_at(p0 + r, (int64_t)pr.H * pr.D, pr.D); });
-    if (threadIdx.x < SR)
-      tm[threadIdx.x] = (int)threadIdx.x < n ? terms[q_at(p0 + threadIdx.x, pr.H, 1)]
-                                             : make_float2(-INFINITY, 0.f);
+  // (the numbers of rows and threads are types: integral_constant)
+  auto load_q = [&](auto rows_, auto threads_, int id, float* a, float* b, float2* tm, int p0,
+                    int n) {
+    constexpr int N = decltype(rows_)::value, TH = decltype(threads_)::value;
+    load_tile<T, DT, N, TH, ASYNC>(
+        a, q, n, pr.D, id, [&](int r) { return q_at(p0 + r, pr.q_t, pr.q_h); });
+    load_tile<T, DT, N, TH, ASYNC>(
+        b, dout, n, pr.D, id, [&](int r) { return q_at(p0 + r, (int64_t)pr.H * pr.D, pr.D); });
+    if (id < N) tm[id] = id < n ? terms[q_at(p0 + id, pr.H, 1)] : make_float2(-INFINITY, 0.f);
   };
-  auto load_k = [&](float* a, float* b, int j0, int n) {
-    load_tile<T, DT, ASYNC>(a, k, n, pr.D, [&](int r) {
+  auto load_k = [&](auto rows_, auto threads_, int id, float* a, float* b, int j0, int n) {
+    constexpr int N = decltype(rows_)::value, TH = decltype(threads_)::value;
+    load_tile<T, DT, N, TH, ASYNC>(a, k, n, pr.D, id, [&](int r) {
       return (int64_t)(it.x + j0 + r) * pr.k_t + hk * pr.k_h;
     });
-    load_tile<T, DT, ASYNC>(b, v, n, pr.D, [&](int r) {
+    load_tile<T, DT, N, TH, ASYNC>(b, v, n, pr.D, id, [&](int r) {
       return (int64_t)(it.x + j0 + r) * pr.v_t + hk * pr.v_h;
     });
   };
-  if (KEYS) load_k(x1, x2, first, rows); else load_q(x1, x2, ts, first, rows);
+  using XRows = std::integral_constant<int, SR>;
+  using YRows = std::integral_constant<int, SC>;
+  using All = std::integral_constant<int, SG * BWD_THREADS>;
+  using Group = std::integral_constant<int, BWD_THREADS>;
+  if (KEYS) load_k(XRows{}, All{}, threadIdx.x, x1, x2, first, rows);
+  else load_q(XRows{}, All{}, threadIdx.x, x1, x2, tx_, first, rows);
+  async_commit();
   // the tiles of y, and this split's share of them
   int64_t y_from = 0, y_to = KEYS ? q_rows : len;
   if (pr.causal && KEYS) y_from = (int64_t)first * G;
   if (pr.causal && !KEYS) y_to = (first + rows - 1) / G + 1;
-  const int n_y = (int)((y_to - y_from + SR - 1) / SR), splits = gridDim.y;
+  const int n_y = (int)((y_to - y_from + SC - 1) / SC), splits = gridDim.y;
   const int t0 = (int)((int64_t)n_y * blockIdx.y / splits);
   const int t1 = (int)((int64_t)n_y * (blockIdx.y + 1) / splits);
   const float c = pr.scale * kLog2e;
@@ -362,29 +438,35 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
       if (KEYS) a2[KEYS ? i : 0][x] = 0.f;
     }
   auto load_y = [&](int t) {
-    const int64_t e0 = y_from + (int64_t)t * SR;
-    const int n = (int)min((int64_t)SR, (KEYS ? q_rows : len) - e0);
-    float* y1 = ybuf + (t & 1) * 2 * L::kTile;
-    if (KEYS) load_q(y1, y1 + L::kTile, ts + (t & 1) * SR, (int)e0, n);
-    else load_k(y1, y1 + L::kTile, (int)e0, n);
+    const int64_t e0 = y_from + (int64_t)t * SC;
+    const int n = (int)min((int64_t)SC, (KEYS ? q_rows : len) - e0);
+    const int b = ((t - t0) / SG) & 1;
+    float* y1 = mine + b * 2 * SC * L::kRow;
+    if (KEYS)
+      load_q(YRows{}, Group{}, tid, y1, y1 + SC * L::kRow, ts + b * SC, (int)e0, n);
+    else
+      load_k(YRows{}, Group{}, tid, y1, y1 + SC * L::kRow, (int)e0, n);
   };
-  if (t0 < t1) load_y(t0);
+  if (t0 + g < t1) load_y(t0 + g);
   async_commit();
-  for (int t = t0; t < t1; ++t) {
-    const int64_t e0 = y_from + (int64_t)t * SR;
-    const float *y1 = ybuf + (t & 1) * 2 * L::kTile, *y2 = y1 + L::kTile;
-    const float2* tq = ts + (KEYS ? (t & 1) * SR : 0);
-    if (t + 1 < t1) load_y(t + 1);
+  async_wait<1>();
+  __syncthreads();  // x
+  for (int t = t0 + g; t < t1; t += SG) {
+    const int64_t e0 = y_from + (int64_t)t * SC;
+    const int b = ((t - t0) / SG) & 1;
+    const float *y1 = mine + b * 2 * SC * L::kRow, *y2 = y1 + SC * L::kRow;
+    const float2* tq = KEYS ? ts + b * SC : tx_;
+    if (t + SG < t1) load_y(t + SG);
     async_commit();
     async_wait<1>();
-    __syncthreads();
-    float s[4][4], dp[4][4];
-    tile_scores<DT>(s, x1, y1);
-    tile_scores<DT>(dp, x2, y2);
+    sync();
+    float s[4][SC / 16], dp[4][SC / 16];
+    tile_scores<DT>(s, x1, y1, ty);
+    tile_scores<DT>(dp, x2, y2, ty);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < SC / 16; ++j) {
         const int r = 4 * ty + i, e = tx + 16 * j;
         const float2 tm = tq[KEYS ? e : r];
         // key <= query token: key * G <= query row
@@ -396,17 +478,42 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         dp[i][j] = on ? p * (dp[i][j] + tm.y) : 0.f;
       }
     if constexpr (KEYS) {
-      put_scores(ps, s);
-      __syncthreads();
-      tile_sums<DT>(a2, ps, y2);
-      __syncthreads();
+      put_scores(ps, s, ty);
+      sync();
+      tile_sums<DT, SC>(a2, ps, y2, ty);
+      sync();
     }
-    put_scores(ps, dp);
-    __syncthreads();
-    tile_sums<DT>(a1, ps, y1);
-    __syncthreads();
+    put_scores(ps, dp, ty);
+    sync();
+    tile_sums<DT, SC>(a1, ps, y1, ty);
+    sync();
   }
   async_wait<0>();
+  if constexpr (SG > 1) {
+    // the second group's sums are added to the first's, by way of x1's and x2's place
+    float* theirs = x1;
+    __syncthreads();
+    if (g == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int x = 0; x < DT / 16; ++x) {
+          const int at = (4 * ty + i) * L::kRow + Cols<DT>::at(x);
+          theirs[at] = a1[i][x];
+          if constexpr (KEYS) theirs[SR * L::kRow + at] = a2[i][x];
+        }
+    }
+    __syncthreads();
+    if (g == 1) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int x = 0; x < DT / 16; ++x) {
+        const int at = (4 * ty + i) * L::kRow + Cols<DT>::at(x);
+        a1[i][x] += theirs[at];
+        if constexpr (KEYS) a2[i][x] += theirs[SR * L::kRow + at];
+      }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 4 * ty + i;

@@ -135,14 +135,16 @@ int run_plan(const void* offsets, int wide, const Problem& p, const List& a, con
   return launch_status();
 }
 
-// Parts that a key tile's queries are split into: until the tiles of an even
-// batch would fill the GPU twice, and no more than 32.
-int key_splits(const Problem& p, int step) {
+// Parts that a key tile's queries are split into: until the tiles of an even batch
+// would fill the GPU `waves` times, and no more than 32.  Two for the tensor-core
+// kernel; three for the CUDA cores', whose tiles take longer.
+int key_splits(const Problem& p, int step, int waves) {
   const int64_t tiles = std::max<int64_t>(1, cdiv(p.T, step) * p.Hkv);
-  return (int)std::min<int64_t>(32, std::max<int64_t>(1, 2 * kSMs / tiles));
+  return (int)std::min<int64_t>(32, std::max<int64_t>(1, waves * kSMs / tiles));
 }
+constexpr int kTcWaves = 2, kSimtWaves = 3;
 
-// Lists have room for the CUDA-core kernels' tiles of 64 packed rows; the
+// Lists have room for the CUDA-core kernels' tiles of 32 or 64 packed rows; the
 // tensor-core kernels' are larger, hence fewer (128 / G, rounded down, is at
 // least 64 / G).
 void retile(List& l, int per, int step) {
@@ -157,7 +159,7 @@ struct FwdWs {
 FwdWs fwd_ws(void* base, const Problem& p) {
   Carver c{(char*)base};
   FwdWs w{};
-  w.list = take_list(c, p, p.G, SR, 0);
+  w.list = take_list(c, p, p.G, FR, 0);
   w.bytes = c.used;
   return w;
 }
@@ -174,7 +176,7 @@ BwdWs bwd_ws(void* base, const Problem& p) {
   w.lq = take_list(c, p, p.G, SR, 0);
   w.lk = take_list(c, p, 1, SR, 1);
   w.terms = c.take<float2>((int64_t)p.T * p.H);
-  const int splits = key_splits(p, BX);
+  const int splits = std::max(key_splits(p, BX, kTcWaves), key_splits(p, SR, kSimtWaves));
   w.part = splits > 1 ? c.take<float>(2ll * splits * p.T * p.Hkv * p.D) : nullptr;
   w.bytes = c.used;
   return w;
@@ -182,7 +184,7 @@ BwdWs bwd_ws(void* base, const Problem& p) {
 
 // Blocks: the key heads of a tile side by side.
 bool grid_fits(const Problem& p) {
-  return (most_items(p.T, p.S, p.G, SR) + 1) * p.Hkv < (1ll << 31);
+  return (most_items(p.T, p.S, p.G, FR) + 1) * p.Hkv < (1ll << 31);
 }
 unsigned blocks(const Problem& p, int per, int step) {
   return (unsigned)(std::max<int64_t>(1, most_items(p.T, p.S, per, step)) * p.Hkv);
@@ -198,7 +200,7 @@ int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, c
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
         cudaSuccess)
       return (int)THERIA_ERR_LAUNCH;
-    return launch_chained(kern, dim3(blocks(p, p.G, SR)), dim3(SIMT_THREADS), smem, st, (const T*)q,
+    return launch_chained(kern, dim3(blocks(p, p.G, FR)), dim3(SimtSmem<DT>::FG * FWD_THREADS), smem, st, (const T*)q,
                           (const T*)k, (const T*)v, (T*)o, lse,
                           (const int4*)ws.list.items, (const int*)ws.list.count, p);
   });
@@ -223,7 +225,8 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
           cudaSuccess)
         return (int)THERIA_ERR_LAUNCH;
-      return launch_chained(kern, dim3(blocks(p, l.per, SR), (unsigned)splits), dim3(SIMT_THREADS),
+      return launch_chained(kern, dim3(blocks(p, l.per, SR), (unsigned)splits),
+                            dim3(SimtSmem<DT>::SG * BWD_THREADS),
                             smem, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout,
                             (const float2*)ws.terms, (T*)o1, (T*)o2, part, (const int4*)l.items,
                             (const int*)l.count, p);
@@ -231,7 +234,7 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
     if (dq != nullptr)
       if (int e = run(simt_bwd_kernel<T, DT, false, ASYNC>, ws.lq, 1, dq, nullptr, nullptr)) return e;
     if (dk == nullptr) return (int)THERIA_OK;
-    const int splits = key_splits(p, SR);
+    const int splits = key_splits(p, SR, kSimtWaves);
     if (int e = run(simt_bwd_kernel<T, DT, true, ASYNC>, ws.lk, splits, dk, dv,
                     splits > 1 ? ws.part : nullptr))
       return e;
@@ -326,7 +329,7 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
       !row_map(m + 2, q, dtype, p, p.q_t, p.q_h, BY / p.G) ||
       !row_map(m + 3, dout, dtype, p, o_t, o_h, BY / p.G))
     return THERIA_ERR_UNSUPPORTED;
-  const int splits = key_splits(p, BX);
+  const int splits = key_splits(p, BX, kTcWaves);
   if (int e = run(tc_bwd_kernel<T, HD, true, CAUSAL>, m, ws.lk, splits, dk, dv,
                   splits > 1 ? ws.part : nullptr))
     return e;
