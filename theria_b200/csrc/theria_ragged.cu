@@ -246,7 +246,7 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
 // Rows of 16 bytes on 16-byte boundaries, and a group that a tile of 64 rows
 // holds.  (Measured against the CUDA-core kernels: see ragged_tc_bwd.cuh.)
 bool use_tc(int dtype, const Problem& p, std::initializer_list<const void*> ptrs) {
-  if (dtype == THERIA_F32 || p.G > BY || tc::encode_fn() == nullptr) return false;
+  if (dtype == THERIA_F32 || p.G > KY || tc::encode_fn() == nullptr) return false;
   if (!whole_rows(dtype, p, ptrs)) return false;
   for (int64_t s : {p.q_t, p.q_h, p.k_t, p.k_h, p.v_t, p.v_h})
     if (s <= 0 || s >= (1ll << 38)) return false;
@@ -303,35 +303,39 @@ template <typename T, int HD, bool CAUSAL>
 int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* dq, void* dk,
            void* dv, const BwdWs& ws, const void* offsets, int wide, int dtype, const Problem& p,
            cudaStream_t st) {
-  constexpr int smem = BwdCfg<HD>::kAlloc;
   const int64_t o_t = (int64_t)p.H * p.D, o_h = p.D;
-  auto run = [&](auto kern, const CUtensorMap (&m)[4], const List& l, int splits, void* o1,
-                 void* o2, float* part) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-        cudaSuccess)
-      return (int)THERIA_ERR_LAUNCH;
-    return launch_chained(kern, dim3(blocks(p, l.per, l.step), (unsigned)splits), dim3(B_THREADS),
-                          smem, st, m[0], m[1], m[2], m[3], (const float2*)ws.terms, (T*)o1,
-                          (T*)o2, part, (const int4*)l.items, (const int*)l.count, p);
+  auto prepare = [&](auto kern, int smem) {
+    return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) ==
+           cudaSuccess;
   };
-  CUtensorMap m[4];
+  CUtensorMap mq, mo, mk, mv;
   if (dq != nullptr) {
-    if (!row_map(m, q, dtype, p, p.q_t, p.q_h, BX / p.G) ||
-        !row_map(m + 1, dout, dtype, p, o_t, o_h, BX / p.G) ||
-        !key_map(m + 2, k, dtype, p, p.k_t, p.k_h, BY) ||
-        !key_map(m + 3, v, dtype, p, p.v_t, p.v_h, BY))
+    using Cfg = DqCfg<HD>;
+    auto kern = tc_dq_kernel<T, HD, CAUSAL>;
+    if (!row_map(&mq, q, dtype, p, p.q_t, p.q_h, BX / p.G) ||
+        !row_map(&mo, dout, dtype, p, o_t, o_h, BX / p.G) ||
+        !key_map(&mk, k, dtype, p, p.k_t, p.k_h, QY) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, QY))
       return THERIA_ERR_UNSUPPORTED;
-    if (int e = run(tc_bwd_kernel<T, HD, false, CAUSAL>, m, ws.lq, 1, dq, nullptr, nullptr))
+    if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
+    if (int e = launch_chained(kern, dim3(blocks(p, ws.lq.per, ws.lq.step)), dim3(Cfg::kThreads),
+                               Cfg::kAlloc, st, mq, mo, mk, mv, (const float2*)ws.terms, (T*)dq,
+                               (const int4*)ws.lq.items, (const int*)ws.lq.count, p))
       return e;
   }
   if (dk == nullptr) return THERIA_OK;
-  if (!key_map(m, k, dtype, p, p.k_t, p.k_h, BX) || !key_map(m + 1, v, dtype, p, p.v_t, p.v_h, BX) ||
-      !row_map(m + 2, q, dtype, p, p.q_t, p.q_h, BY / p.G) ||
-      !row_map(m + 3, dout, dtype, p, o_t, o_h, BY / p.G))
+  using Cfg = DkvCfg<HD>;
+  auto kern = tc_dkv_kernel<T, HD, CAUSAL>;
+  if (!row_map(&mq, q, dtype, p, p.q_t, p.q_h, KY / p.G) ||
+      !row_map(&mo, dout, dtype, p, o_t, o_h, KY / p.G) ||
+      !key_map(&mk, k, dtype, p, p.k_t, p.k_h, BX) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, BX))
     return THERIA_ERR_UNSUPPORTED;
+  if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
   const int splits = key_splits(p, BX, kTcWaves);
-  if (int e = run(tc_bwd_kernel<T, HD, true, CAUSAL>, m, ws.lk, splits, dk, dv,
-                  splits > 1 ? ws.part : nullptr))
+  if (int e = launch_chained(kern, dim3(blocks(p, ws.lk.per, ws.lk.step), (unsigned)splits),
+                             dim3(Cfg::kThreads), Cfg::kAlloc, st, mk, mv, mq, mo,
+                             (const float2*)ws.terms, (T*)dk, (T*)dv,
+                             splits > 1 ? ws.part : nullptr, (const int4*)ws.lk.items,
+                             (const int*)ws.lk.count, p))
     return e;
   return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : THERIA_OK;
 }
