@@ -24,7 +24,7 @@ constexpr float kLn2 = 0.69314718055994531f;
 struct Problem {
   int T, S, H, Hkv, G, D;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;  // strides in elements
-  float scale;
+  float scale, scale_log2;  // the scores' factor; and times log2(e)
   int causal;
 };
 

@@ -224,7 +224,7 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   async_commit();
   const int last = (first + rows - 1) / G;  // the last row's token
   const int keys = pr.causal ? last + 1 : len;
-  const float c = pr.scale * kLog2e;
+  const float c = pr.scale_log2;
   float m[4], l[4], acc[4][DT / 16];
   int lim[4];
 #pragma unroll
@@ -428,7 +428,7 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   const int n_y = (int)((y_to - y_from + SC - 1) / SC), splits = gridDim.y;
   const int t0 = (int)((int64_t)n_y * blockIdx.y / splits);
   const int t1 = (int)((int64_t)n_y * (blockIdx.y + 1) / splits);
-  const float c = pr.scale * kLog2e;
+  const float c = pr.scale_log2;
   float a1[4][DT / 16], a2[KEYS ? 4 : 1][DT / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)

@@ -268,7 +268,6 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
     const float2 mine = live ? terms[row] : make_float2(-INFINITY, 0.f);  // {-lse log2 e, -z}
     const int warp_tok = first + quarter * 32 / G;  // the first token of the warp
     const int my_keys = CAUSAL ? min(len, tok + 1) : len;
-    const float scale_log2 = pr.scale * kLog2e;
     bool ok = true;
     // Waits are warp-uniform: the TMEM accesses that follow are warp-collective.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -294,7 +293,7 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
       const int hi = my_keys - y0 - cg * 32;
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
-        tc::fma2(s[e], s[e + 1], s[e], s[e + 1], scale_log2, scale_log2, mine.x, mine.x);
+        tc::fma2(s[e], s[e + 1], s[e], s[e + 1], pr.scale_log2, pr.scale_log2, mine.x, mine.x);
         s[e] = tc::ex2(s[e]);
         s[e + 1] = tc::ex2(s[e + 1]);
       }
@@ -564,7 +563,6 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const int tok = first + r;
     const bool live = tok < len;
-    const float scale_log2 = pr.scale * kLog2e;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, tc::mbar_wait(bar, parity, abort));
@@ -617,7 +615,7 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
           const float2 nl = ld_shared_f2(lse_at + e * 4);
-          tc::fma2(s[e], s[e + 1], s[e], s[e + 1], scale_log2, scale_log2, nl.x, nl.y);
+          tc::fma2(s[e], s[e + 1], s[e], s[e + 1], pr.scale_log2, pr.scale_log2, nl.x, nl.y);
           s[e] = tc::ex2(s[e]);
           s[e + 1] = tc::ex2(s[e + 1]);
           if constexpr (decltype(mk)::value) {

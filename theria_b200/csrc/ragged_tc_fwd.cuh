@@ -313,19 +313,18 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const int h = kHalves == 2 ? (idx >> 2) & 1 : 0;
     const int quarter = warp & 3;         // TMEM lanes this warp may access
     const int r = quarter * 32 + lane;    // row within the tile
-    const int tok0 = first + t * tpt, tok = tok0 + r / G;
+    const int tok0 = first + t * tpt;
     const uint32_t bar_id = 1 + t * 4 + quarter;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t t_s = tmem + t * 128 + h * CW + lane_off;
     constexpr int HO = HD / kHalves;      // O columns this warp rescales and stores
     const uint32_t t_o = tmem + 256 + t * HD + h * HO + lane_off;
     const uint32_t t_p = (kSepP ? tmem + 384 + t * 64 : tmem + t * 128 + h * 64) + lane_off;
-    const float scale_log2 = pr.scale * kLog2e;
     float* red = reinterpret_cast<float*>(smem + L::oRed);  // [2 parity][2 t][2 h][128]
     auto red_at = [&](int par, int hh) { return red + ((par * 2 + t) * 2 + hh) * FM + r; };
-    // the first token of the warp's rows: its key tiles from there on need the mask
-    const int warp_tok = tok0 + quarter * 32 / G;
-    const int my_keys = CAUSAL ? min(len, tok + 1) : len;
+    // the keys of this row, and of the warp's first: tiles beyond those need the mask
+    const int my_keys = CAUSAL ? min(len, tok0 + r / G + 1) : len;
+    const int clean = CAUSAL ? min(len, tok0 + quarter * 32 / G + 1) : len;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     // Waits are warp-uniform: the TMEM accesses that follow are warp-collective.
@@ -337,7 +336,7 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       if (!wait(s_full + t, j & 1)) { ok = false; break; }
       tc::tc_fence_after();
       const int col0 = j * FN + h * CW;
-      const bool masked = (col0 + CW > len) || (CAUSAL && col0 + CW - 1 > warp_tok);
+      const bool masked = col0 + CW > clean;
       const int lim = my_keys - col0;  // valid columns < lim
       float v[CW];
       if constexpr (CW == 128) tc::tmem_ld128(t_s, v);
@@ -365,7 +364,7 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
         tc::named_bar(bar_id, 64);
         mt = fmaxf(mt, *red_at(j & 1, h ^ 1));
       }
-      mt *= scale_log2;
+      mt *= pr.scale_log2;
       const float m_new = fmaxf(m, mt);
       float m_use = m;
       bool rescale = false;
@@ -396,46 +395,54 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       m = m_use;
       const float m_sub = m_use == -INFINITY ? 0.f : m_use;
       float rs[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // partial row sums
-      uint32_t pk[kHalves == 1 ? CW / 2 : 1];
-      // P = exp2(s - m) as 16-bit pairs, summed before they are rounded
-      auto make_p = [&](auto mk) {
-        auto pair = [&](float s0, float s1, int c) {
-          float x0, x1;
-          if constexpr (!decltype(mk)::value) {
-            tc::fma2(x0, x1, s0, s1, scale_log2, scale_log2, -m_sub, -m_sub);
-            x0 = tc::ex2(x0);
-            x1 = tc::ex2(x1);
-          } else {
-            x0 = c < lim ? tc::ex2(fmaf(s0, scale_log2, -m_sub)) : 0.f;
-            x1 = c + 1 < lim ? tc::ex2(fmaf(s1, scale_log2, -m_sub)) : 0.f;
-          }
-          const int k = 2 * ((c >> 1) & 3);  // four chains of paired sums
-          tc::add2(rs[k], rs[k + 1], rs[k], rs[k + 1], x0, x1);
-          return tc::pack2<T>(x0, x1);
-        };
-        if constexpr (kHalves == 1) {
-#pragma unroll
-          for (int i = 0; i < CW; i += 2) pk[i / 2] = pair(v[i], v[i + 1], i);
-        } else {
-          // S again from TMEM, in chunks whose P goes over columns already read
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float x[32];
-            tc::tmem_ld32(t_s + c * 32, x);
-            uint32_t px[16];
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) px[i / 2] = pair(x[i], x[i + 1], c * 32 + i);
-            tc::tmem_st16(t_p + c * 16, px);
-          }
-        }
+      // P = exp2(s - m) as 16-bit pairs, summed before they are rounded, in four
+      // chains of paired sums
+      auto plain = [&](float s0, float s1, int c) {
+        float x0, x1;
+        tc::fma2(x0, x1, s0, s1, pr.scale_log2, pr.scale_log2, -m_sub, -m_sub);
+        x0 = tc::ex2(x0);
+        x1 = tc::ex2(x1);
+        const int k = 2 * ((c >> 1) & 3);
+        tc::add2(rs[k], rs[k + 1], rs[k], rs[k + 1], x0, x1);
+        return tc::pack2<T>(x0, x1);
       };
-      if (masked) make_p(std::true_type{}); else make_p(std::false_type{});
+      auto below = [&](float s0, float s1, int c) {  // columns from lim on are masked
+        const float x0 = c < lim ? tc::ex2(fmaf(s0, pr.scale_log2, -m_sub)) : 0.f;
+        const float x1 = c + 1 < lim ? tc::ex2(fmaf(s1, pr.scale_log2, -m_sub)) : 0.f;
+        const int k = 2 * ((c >> 1) & 3);
+        tc::add2(rs[k], rs[k + 1], rs[k], rs[k + 1], x0, x1);
+        return tc::pack2<T>(x0, x1);
+      };
       if constexpr (kHalves == 1) {
+        uint32_t pk[CW / 2];
+        if (!masked) {
+#pragma unroll
+          for (int i = 0; i < CW; i += 2) pk[i / 2] = plain(v[i], v[i + 1], i);
+        } else {
+#pragma unroll
+          for (int i = 0; i < CW; i += 2) pk[i / 2] = below(v[i], v[i + 1], i);
+        }
         if (j >= 1) {
           if (!wait(pv_done + t, (j - 1) & 1)) { ok = false; break; }
           tc::tc_fence_after();
         }
         tc::tmem_st64u(t_p, pk);
+      } else {
+        // S again from TMEM, in chunks whose P goes over columns already read
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x[32];
+          tc::tmem_ld32(t_s + c * 32, x);
+          uint32_t pk[16];
+          if (!masked) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) pk[i / 2] = plain(x[i], x[i + 1], c * 32 + i);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) pk[i / 2] = below(x[i], x[i + 1], c * 32 + i);
+          }
+          tc::tmem_st16(t_p + c * 16, pk);
+        }
       }
       l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
       tc::tmem_wait_st();
@@ -455,8 +462,12 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       if (ok && wait(o_done + t, 0)) {
         tc::tc_fence_after();
         const float inv = 1.f / l;
-        const bool store = r < tpt * G && tok < len;
-        const int64_t row = (int64_t)(start + tok) * pr.H + hk * G + r % G;
+        // (read again: kept over the loop, these would not fit in registers)
+        const int4 it = items[blockIdx.x / pr.Hkv];
+        const int per = FM / pr.G, tok = it.z + t * per + r / pr.G;
+        const bool store = r < per * pr.G && tok < it.y;
+        const int64_t row =
+            (int64_t)(it.x + tok) * pr.H + (blockIdx.x % pr.Hkv) * pr.G + r % pr.G;
 #pragma unroll
         for (int c = 0; c < HO / 32; ++c) {
           float v[32];

@@ -91,6 +91,7 @@ Problem problem(const int64_t* st, int64_t T, int64_t S, int64_t H, int64_t Hkv,
     p.v_h = st[5];
   }
   p.scale = scale;
+  p.scale_log2 = scale * kLog2e;
   p.causal = causal != 0;
   return p;
 }
