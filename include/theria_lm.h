@@ -117,7 +117,8 @@ int theria_xent_bwd(const void* h, const void* w, const void* target, int wide,
  * Positions (int64 if `wide`, else int32): positions[n_positions], token i of
  * B * T taking positions[i % n_positions]; or offsets[S + 1] of S packed
  * sequences in each T, counting from its sequence's first token (0 for a token
- * of none); or neither, counting from the first of T.  D <= 4096. */
+ * of none; offsets that decrease give some of the positions, and no error); or
+ * neither, counting from the first of T.  D <= 4096. */
 int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_t* strides,
                   int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int dtype,
                   const void* positions, int64_t n_positions, const void* offsets, int64_t S,

@@ -25,7 +25,7 @@
  * Softmax statistics and sums are float32, results are rounded once, and no
  * result depends on the order in which thread blocks run.  Stream-ordered, no
  * allocation, no host synchronisation; each call returns a THERIA_* status.
- * D <= THERIA_MAX_HEAD_DIM; T, S < 2^30, T * H < 2^31, H and Hkv < 65536.
+ * scale > 0.  D <= THERIA_MAX_HEAD_DIM; T, S < 2^30, T * H < 2^31, H and Hkv < 65536.
  *
  * The reference library has no such operator: its attention takes one head
  * count and one length (theria/attention/triton_qk.py:307-369).

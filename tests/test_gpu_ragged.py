@@ -148,6 +148,30 @@ def test_rows_of_no_sequence_and_scale(dtype):
     assert sdpa_ragged(q[:0], k[:0], v[:0], _offsets([0, 0])).shape == (0, 2, 64)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_beyond_32_bits(dtype):
+    # heads in rows so long that the last sequence starts beyond 2^31 elements
+    lengths, H, Hkv, D = [70000, 300, 129], 2, 1, 64
+    T, wide = sum(lengths), 32768
+    store = torch.empty(T * wide, dtype=dtype, device="cuda").view(T, wide)
+    q, k, v, _ = _inputs(lengths[1:], H, Hkv, D, dtype)
+    for t, at in ((q, 0), (k, 1000), (v, 2000)):
+        store[lengths[0]:, at:at + t.shape[1] * D] = t.flatten(1)
+    views = [store[:, at:at + h * D].view(T, h, D) for h, at in ((H, 0), (Hkv, 1000), (Hkv, 2000))]
+    off = _offsets(lengths)[1:]  # the first 70000 tokens belong to none
+    x = [t.detach().requires_grad_(True) for t in views]
+    y = [t.requires_grad_(True) for t in (q, k, v)]
+    a, b = sdpa_ragged(*x, off), sdpa_ragged(*y, _offsets(lengths[1:]))
+    assert torch.equal(a[lengths[0]:], b) and not a[:lengths[0]].any()
+    # dk and dv are split over another number of parts, so float32 sums of terms that
+    # cancel run in another order: against the plain form, with its derived tolerances
+    do = torch.ones_like(q)
+    want, off_by = _plain(q.detach(), k.detach(), v.detach(), do, lengths[1:], 0, True, D ** -0.5)
+    for g, w, e in zip(torch.autograd.grad(a.sum(), x), want[1:], off_by[1:]):
+        assert not g[:lengths[0]].any()
+        assert ((g[lengths[0]:].double() - w).abs() <= 1.01 * e).all()
+
+
 def test_many_sequences():
     g = torch.Generator().manual_seed(3)
     lengths = torch.randint(0, 9, (1500,), generator=g).tolist()
@@ -315,6 +339,9 @@ def test_refusals():
     for args, match in bad:
         with call(match=match):
             sdpa_ragged(*args)
+    for scale in (0.0, -1.0, math.nan, math.inf):
+        with call(match="scale must"):
+            sdpa_ragged(q, k, v, off, scale=scale)
 
 
 def test_second_derivative_and_forward_mode_are_refused():

@@ -46,7 +46,7 @@ def _check(x, y, at, f, interleaved, amplitude=1.0, sign=1):
 @pytest.mark.parametrize("D,dim", [(64, 64), (128, 128), (128, 64), (80, 30), (16, 2), (9, 6), (100, 100),
                                    (72, 0), (2, 2), (1000, 998), (4096, 4096)])
 def test_rotation_and_gradient(D, dim, interleaved, dtype):
-    for T, Hq, Hk in ((1, 1, 1), (37, 5, 2), (700, 3, 1)):
+    for T, Hq, Hk in ((1, 1, 1), (37, 5, 2), (700, 3, 1), (2100, 1, 1)):
         if T * D > 400000:
             continue
         g = torch.Generator("cuda").manual_seed(T)
@@ -63,6 +63,17 @@ def test_rotation_and_gradient(D, dim, interleaved, dtype):
         _check(gk, dk, at, f, interleaved, 1.25, -1)
         alone = lm.rotary(q.detach(), None, f, at.int(), interleaved=interleaved, amplitude=1.25)
         assert torch.equal(alone, yq)
+        none = lm.rotary(q.detach()[:, :0], k.detach(), f, at, interleaved=interleaved,
+                         amplitude=1.25)
+        assert none[0].numel() == 0 and torch.equal(none[1], yk)
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 7, 64, 1000, 8192, 8193, 60000])
+def test_numbers_of_heads(heads):
+    f = lm.rotary_frequencies(8)
+    for T in (1, 5, 1500 if heads < 100 else 2):
+        x = torch.randn(T, heads, 8, device="cuda")
+        _check(x, lm.rotary(x, None, f), torch.arange(T, device="cuda"), f, False)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -18,6 +18,7 @@ count and one length (``theria/attention/triton_qk.py:307-369``).
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 
@@ -149,6 +150,8 @@ def sdpa_ragged(q, k, v, offsets, causal=True, scale=None):
     _no_tangents(_WHAT, q, k, v)
     D = q.shape[2]
     scale = default_scale(q) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise AssertionError(f"scale must be positive and finite, got {scale}")
     causal = int(bool(causal))
     if q.element_size() == 2 and D % 8:
         # zero columns up to a whole number of 16-byte rows change no score and

@@ -45,7 +45,7 @@ struct Args {
   const double* freq;    // [pairs]
   float amplitude;
   int back, tokens;      // the angle negated; tokens of a block
-  unsigned magic;        // ceil(2^32 / heads): row / heads as a product's high half
+  uint64_t magic;        // 2^32 / heads + 1: row / heads as a product's high half
 };
 
 __device__ __forceinline__ int64_t int_at(const void* p, int wide, int64_t i) {
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, 4) rotary_kernel(const Args a) {
       for (int k = 0; k < LOADS; ++k) {
         const unsigned r = rb + k * step;
         if (r >= all) continue;
-        const unsigned t = __umulhi(r, a.magic);
+        const unsigned t = (unsigned)((r * a.magic) >> 32);
         int h = r - t * heads;
         const int i = h >= a.heads[0];
         if (i) h -= a.heads[0];

@@ -913,10 +913,10 @@ int theria_rotary(const void* q, const void* k, void* yq, void* yk, const int64_
   const int64_t share = std::max<int64_t>(1, a.n / (4 * kSMs));
   a.tokens = (int)std::max<int64_t>(
       1, std::min<int64_t>({share, rotary::MOST_TOKENS, 1024 / std::max<int64_t>(pairs, 1)}));
-  // row / heads by ceil(2^32 / heads) is exact while row * heads < 2^32, which the
-  // rows of one token always are (heads < 2^16)
+  // row / heads as row * (2^32 / heads + 1) / 2^32 is exact while row * heads < 2^32,
+  // which the rows of one token always are (heads < 2^16)
   if (Hq + Hk > 8192) a.tokens = 1;
-  a.magic = (unsigned)std::min<uint64_t>((1ull << 32) / (Hq + Hk) + 1, 0xffffffffu);
+  a.magic = (1ull << 32) / (uint64_t)(Hq + Hk) + 1;
   const int64_t blocks = cdiv(a.n, a.tokens);
   if (blocks >= (1ll << 31)) return THERIA_ERR_UNSUPPORTED;
   // 16 KB of angles at most (one token: 2048 pairs), the pairs filled up to 16 bytes

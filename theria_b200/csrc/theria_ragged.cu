@@ -65,6 +65,8 @@ List take_list(Carver& c, const Problem& p, int per, int step, int by_key) {
 
 int check(const Problem& p, int64_t T, int64_t S, int64_t H, int64_t Hkv, int64_t D, int dtype) {
   if (T < 0 || S < 0 || H <= 0 || Hkv <= 0 || D <= 0 || H % Hkv) return THERIA_ERR_INVALID_ARG;
+  // (the maximum of the scores is taken before the factor)
+  if (!(p.scale > 0.f) || !(p.scale_log2 < INFINITY)) return THERIA_ERR_INVALID_ARG;
   if (dtype != THERIA_F32 && dtype != THERIA_F16 && dtype != THERIA_BF16)
     return THERIA_ERR_INVALID_ARG;
   if (D > THERIA_MAX_HEAD_DIM || T >= (1ll << 30) || S >= (1ll << 30) || H >= 65536 ||
@@ -379,7 +381,7 @@ using namespace theria::ragged;
 extern "C" {
 
 int64_t theria_ragged_fwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv) {
-  const Problem p = problem(nullptr, T, S, H, Hkv, 1, 0.f, 0);
+  const Problem p = problem(nullptr, T, S, H, Hkv, 1, 1.f, 0);
   if (check(p, T, S, H, Hkv, 1, THERIA_F32) != THERIA_OK) return 0;
   return fwd_ws(nullptr, p).bytes;
 }
@@ -417,7 +419,7 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
 
 int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv,
                                           int64_t D) {
-  const Problem p = problem(nullptr, T, S, H, Hkv, D, 0.f, 0);
+  const Problem p = problem(nullptr, T, S, H, Hkv, D, 1.f, 0);
   if (check(p, T, S, H, Hkv, D, THERIA_F32) != THERIA_OK) return 0;
   return bwd_ws(nullptr, p).bytes;
 }
