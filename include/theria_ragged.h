@@ -39,18 +39,20 @@
 extern "C" {
 #endif
 
-/* lse may be NULL. */
+/* o_rest [T, H, D] receives what o's rounding to its type left, for the backward's row
+ * term dout . o, which cancels against other terms; it and lse may be NULL. */
 int64_t theria_ragged_fwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv);
 int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, void* o, float* lse, void* workspace,
+                      const void* offsets, int wide, void* o, void* o_rest, float* lse,
+                      void* workspace,
                       int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
                       int64_t D, int dtype, float scale, int causal, void* stream);
 
-/* dq, dk, dv of <o, dout>; dq, or dk and dv together, may be NULL. */
+/* dq, dk, dv of <o, dout>; dq, or dk and dv together, may be NULL, as may o_rest. */
 int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv,
                                           int64_t D);
 int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, const void* o, const void* dout,
+                      const void* offsets, int wide, const void* o, const void* o_rest, const void* dout,
                       const float* lse, void* dq, void* dk, void* dv, void* workspace,
                       int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
                       int64_t D, int dtype, float scale, int causal, void* stream);

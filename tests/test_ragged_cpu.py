@@ -18,12 +18,12 @@ def test_ragged_arguments():
 
     def fwd(**k):
         return lib.theria_ragged_fwd(k.get("q", P), P, P, k.get("st", st), k.get("off", P), 0,
-                                     k.get("o", P), None, k.get("ws", P), k.get("size", 0),
+                                     k.get("o", P), None, None, k.get("ws", P), k.get("size", 0),
                                      k.get("T", 8), k.get("S", 2), k.get("H", 4), k.get("Hkv", 2),
                                      k.get("D", 16), k.get("dtype", 0), 1.0, 1, None)
 
     def bwd(**k):
-        return lib.theria_ragged_bwd(P, P, P, st, P, 0, P, P, k.get("lse", P), k.get("dq", P),
+        return lib.theria_ragged_bwd(P, P, P, st, P, 0, P, None, P, k.get("lse", P), k.get("dq", P),
                                      k.get("dk", P), k.get("dv", P), k.get("ws", P),
                                      k.get("size", 0), k.get("T", 8), 2, 4, 2, 16, 0, 1.0, 1, None)
 

@@ -86,9 +86,9 @@ SIGNATURES = {
     "theria_grads_clip": (_i, [_vp] * 4 + [_i64, _vp, _d, _vp, _vp, _vp]),
     "theria_grads_clip_bwd": (_i, [_vp] * 5 + [_i64] + [_vp] * 4),
     "theria_ragged_fwd_workspace_bytes": (_i64, [_i64] * 4),
-    "theria_ragged_fwd": (_i, [_vp] * 5 + [_i] + [_vp] * 3 + [_i64] * 6 + [_i, _f, _i, _vp]),
+    "theria_ragged_fwd": (_i, [_vp] * 5 + [_i] + [_vp] * 4 + [_i64] * 6 + [_i, _f, _i, _vp]),
     "theria_ragged_bwd_workspace_bytes": (_i64, [_i64] * 5),
-    "theria_ragged_bwd": (_i, [_vp] * 5 + [_i] + [_vp] * 7 + [_i64] * 6 + [_i, _f, _i, _vp]),
+    "theria_ragged_bwd": (_i, [_vp] * 5 + [_i] + [_vp] * 8 + [_i64] * 6 + [_i, _f, _i, _vp]),
     "theria_get_device_error": (_i, [ctypes.POINTER(ctypes.c_int), _vp]),
     "theria_clear_device_error": (_i, [_vp]),
     "theria_diag_bounded_wait": (_i, [_i, _vp, _vp]),

@@ -24,7 +24,7 @@ import torch
 
 from theria_b200 import _lib
 from theria_b200.attention.ops import MAX_HEAD_DIM, default_scale
-from theria_b200.lm import _call, _check, _check_ids, _no_tangents, _workspace, _DTYPES
+from theria_b200.lm import _DTYPES, _call, _check, _check_ids, _no_tangents, _ptr, _workspace
 
 _opaque = torch.compiler.disable
 _WHAT = "theria sdpa_ragged"
@@ -66,20 +66,22 @@ def _strides(q, k, v):
     return (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
 
 
-def _forward(q, k, v, offsets, causal, scale, need_lse):
+def _forward(q, k, v, offsets, causal, scale, grad):
+    """o and, for the backward, the rows' logsumexp and what o's rounding left."""
     T, H, D = q.shape
     Hkv, S = k.shape[1], offsets.shape[0] - 1
     o = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if need_lse else None
+    lse = torch.empty(T, H, dtype=torch.float32, device=q.device) if grad else None
+    rest = torch.empty_like(o) if grad and q.element_size() == 2 else None
     ws, size = _workspace("theria_ragged_fwd_workspace_bytes", q.device, T, S, H, Hkv)
     _call("theria_ragged_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _strides(q, k, v), offsets.data_ptr(), int(offsets.dtype == torch.int64), o.data_ptr(),
-          None if lse is None else lse.data_ptr(), ws.data_ptr(), size, T, S, H, Hkv, D,
+          _ptr(rest), _ptr(lse), ws.data_ptr(), size, T, S, H, Hkv, D,
           _DTYPES[q.dtype], scale, causal)
-    return o, lse
+    return o, rest, lse
 
 
-def _backward(q, k, v, offsets, o, lse, dout, causal, scale, need):
+def _backward(q, k, v, offsets, o, rest, lse, dout, causal, scale, need):
     T, H, D = q.shape
     Hkv, S = k.shape[1], offsets.shape[0] - 1
     dout = dout.contiguous()
@@ -92,9 +94,7 @@ def _backward(q, k, v, offsets, o, lse, dout, causal, scale, need):
     ws, size = _workspace("theria_ragged_bwd_workspace_bytes", q.device, T, S, H, Hkv, D)
     _call("theria_ragged_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _strides(q, k, v), offsets.data_ptr(), int(offsets.dtype == torch.int64), o.data_ptr(),
-          dout.data_ptr(), lse.data_ptr(), *(None if t is None else t.data_ptr()
-                                             for t in (dq, dk, dv)),
-          ws.data_ptr(), size, T, S, H, Hkv, D, _DTYPES[q.dtype], scale, causal)
+          _ptr(rest), dout.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), ws.data_ptr(), size, T, S, H, Hkv, D, _DTYPES[q.dtype], scale, causal)
     return dq, dk if need[1] else None, dv if need[2] else None
 
 
@@ -102,9 +102,9 @@ class _RaggedBackward(torch.autograd.Function):
     """(q, k, v, dout) -> (dq, dk, dv); a second derivative is refused."""
 
     @staticmethod
-    def forward(ctx, q, k, v, dout, rest):
-        offsets, o, lse, *more = rest
-        return _backward(q, k, v, offsets, o, lse, dout, *more)
+    def forward(ctx, q, k, v, dout, saved):
+        offsets, o, rest, lse, *more = saved
+        return _backward(q, k, v, offsets, o, rest, lse, dout, *more)
 
     @staticmethod
     def backward(ctx, *_):
@@ -115,21 +115,22 @@ class _RaggedBackward(torch.autograd.Function):
 class _Ragged(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, causal, scale):
-        o, lse = _forward(q, k, v, offsets, causal, scale, True)
-        ctx.save_for_backward(q, k, v, offsets, o, lse)
+        o, rest, lse = _forward(q, k, v, offsets, causal, scale, True)
+        ctx.save_for_backward(q, k, v, offsets, o, rest, lse)
         ctx.rest = causal, scale
         return o
 
     @staticmethod
     def backward(ctx, dout):
         _no_tangents(_WHAT, dout)
-        q, k, v, offsets, o, lse = ctx.saved_tensors
+        q, k, v, offsets, o, rest, lse = ctx.saved_tensors
         causal, scale = ctx.rest
         need = ctx.needs_input_grad[:3]
         if torch.is_grad_enabled():
-            grads = _RaggedBackward.apply(q, k, v, dout, (offsets, o, lse, causal, scale, need))
+            grads = _RaggedBackward.apply(q, k, v, dout,
+                                          (offsets, o, rest, lse, causal, scale, need))
         else:
-            grads = _backward(q, k, v, offsets, o, lse, dout, causal, scale, need)
+            grads = _backward(q, k, v, offsets, o, rest, lse, dout, causal, scale, need)
         return (*grads, None, None, None)
 
 

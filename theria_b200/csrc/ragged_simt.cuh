@@ -190,8 +190,8 @@ __device__ __forceinline__ void put_scores(float* p, const float (&s)[4][J], int
 template <typename T, int DT, bool ASYNC>
 __global__ void __launch_bounds__(SimtSmem<DT>::FG * FWD_THREADS)
 simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
-                T* __restrict__ o, float* __restrict__ lse, const int4* items, const int* count,
-                Problem pr) {
+                T* __restrict__ o, T* __restrict__ rest, float* __restrict__ lse,
+                const int4* items, const int* count, Problem pr) {
   using L = SimtSmem<DT>;
   extern __shared__ float4 smem4[];
   constexpr int C = L::kFC, FG = L::FG;
@@ -329,18 +329,23 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 #pragma unroll
     for (int x = 0; x < DT / 16; ++x) {
       const int d = Cols<DT>::at(x);
-      if (d < pr.D) o[row * pr.D + d] = from_f32<T>(acc[i][x] * inv);
+      if (d >= pr.D) continue;
+      const T value = from_f32<T>(acc[i][x] * inv);
+      o[row * pr.D + d] = value;
+      if (rest != nullptr) rest[row * pr.D + d] = from_f32<T>(acc[i][x] * inv - to_f32<T>(value));
     }
     if (lse != nullptr && tx == 0) lse[row] = (m[i] + log2f(sum)) * kLn2;
   }
 }
 
-// terms[row] = {-lse * log2(e), -rowsum(do * o)} for every row [T, H]: LANES
-// neighbouring lanes a row, each on VEC of its values at a time.  Rows of no
+// terms[row] = {-lse * log2(e), -rowsum(do * (o + rest))} for every row [T, H], rest
+// (may be NULL) being what o's rounding left: LANES neighbouring lanes a row, each on
+// VEC of its values at a time.  Rows of no
 // sequence get whatever their memory holds: no tile reads them.
 template <typename T, int VEC, int LANES>
 __global__ void __launch_bounds__(256)
-terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* __restrict__ lse,
+terms_kernel(const T* __restrict__ o, const T* __restrict__ rest, const T* __restrict__ dout,
+             const float* __restrict__ lse,
              float2* __restrict__ terms, int64_t rows, int D) {
   grid_launch();
   grid_wait();
@@ -355,6 +360,12 @@ terms_kernel(const T* __restrict__ o, const T* __restrict__ dout, const float* _
         float a[VEC], b[VEC];
         load_vec<T, VEC>(o + r * D + d, a);
         load_vec<T, VEC>(dout + r * D + d, b);
+        if (rest != nullptr) {
+          float c[VEC];
+          load_vec<T, VEC>(rest + r * D + d, c);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) a[i] += c[i];
+        }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) z = fmaf(a[i], b[i], z);
       }

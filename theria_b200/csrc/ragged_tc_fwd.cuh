@@ -78,7 +78,7 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1)
 tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, T* __restrict__ out,
-              float* __restrict__ lse, const int4* items, const int* count, const Problem pr) {
+              T* __restrict__ rest, float* __restrict__ lse, const int4* items, const int* count, const Problem pr) {
   using L = FwdCfg<HD>;
   constexpr bool kSepP = HD == 64;
   extern __shared__ uint8_t smem_raw[];
@@ -477,12 +477,25 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
           uint4* dst = reinterpret_cast<uint4*>(out + row * pr.D + d);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float* e = v + 8 * i;
-            if (d + 8 * i < pr.D)  // D is a multiple of 8
-              dst[i] = make_uint4(tc::pack2<T>(e[0] * inv, e[1] * inv),
-                                  tc::pack2<T>(e[2] * inv, e[3] * inv),
-                                  tc::pack2<T>(e[4] * inv, e[5] * inv),
-                                  tc::pack2<T>(e[6] * inv, e[7] * inv));
+            float* e = v + 8 * i;
+            if (d + 8 * i >= pr.D) continue;  // D is a multiple of 8
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              e[2 * k] *= inv;
+              e[2 * k + 1] *= inv;
+              w[k] = tc::pack2<T>(e[2 * k], e[2 * k + 1]);
+            }
+            dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            if (rest == nullptr) continue;
+            // what the rounding left
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float r0, r1;
+              tc::unpack2<T>(w[k], r0, r1);
+              w[k] = tc::pack2<T>(e[2 * k] - r0, e[2 * k + 1] - r1);
+            }
+            reinterpret_cast<uint4*>(rest + row * pr.D + d)[i] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
         if (store && h == 0 && lse != nullptr) lse[row] = (m + log2f(l)) * kLn2;

@@ -194,7 +194,7 @@ unsigned blocks(const Problem& p, int per, int step) {
 }
 
 template <typename T>
-int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const FwdWs& ws,
+int simt_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse, const FwdWs& ws,
              const Problem& p, cudaStream_t st) {
   return by_width<T>(p.D, whole_rows(THERIA_F32, p, {q, k, v}), [&](auto w, auto async) {
     constexpr int DT = decltype(w)::value;
@@ -204,7 +204,7 @@ int simt_fwd(const void* q, const void* k, const void* v, void* o, float* lse, c
         cudaSuccess)
       return (int)THERIA_ERR_LAUNCH;
     return launch_chained(kern, dim3(blocks(p, p.G, FR)), dim3(SimtSmem<DT>::FG * FWD_THREADS), smem, st, (const T*)q,
-                          (const T*)k, (const T*)v, (T*)o, lse,
+                          (const T*)k, (const T*)v, (T*)o, (T*)rest, lse,
                           (const int4*)ws.list.items, (const int*)ws.list.count, p);
   });
 }
@@ -287,8 +287,8 @@ bool row_map(CUtensorMap* m, const void* base, int dtype, const Problem& p, int6
 }
 
 template <typename T, int HD, bool CAUSAL>
-int tc_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const FwdWs& ws,
-           int dtype, const Problem& p, cudaStream_t st) {
+int tc_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
+           const FwdWs& ws, int dtype, const Problem& p, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   if (!row_map(&mq, q, dtype, p, p.q_t, p.q_h, FM / p.G) ||
       !key_map(&mk, k, dtype, p, p.k_t, p.k_h, FN) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, FN))
@@ -298,7 +298,7 @@ int tc_fwd(const void* q, const void* k, const void* v, void* o, float* lse, con
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return THERIA_ERR_LAUNCH;
   return launch_chained(kern, dim3(blocks(p, ws.list.per, ws.list.step)),
-                        dim3(FwdCfg<HD>::kThreads), smem, st, mq, mk, mv, (T*)o, lse,
+                        dim3(FwdCfg<HD>::kThreads), smem, st, mq, mk, mv, (T*)o, (T*)rest, lse,
                         (const int4*)ws.list.items, (const int*)ws.list.count, p);
 }
 
@@ -354,16 +354,16 @@ int by_tile(const Problem& p, F f) {
 }
 
 template <typename T>
-int run_terms(const void* o, const void* dout, const float* lse, const BwdWs& ws, const Problem& p,
+int run_terms(const void* o, const void* rest, const void* dout, const float* lse, const BwdWs& ws, const Problem& p,
               cudaStream_t st) {
   const int64_t rows = (int64_t)p.T * p.H;
   constexpr int VEC = 16 / sizeof(T);
-  const bool vec = p.D % VEC == 0 && tc::aligned16(o) && tc::aligned16(dout);
+  const bool vec = p.D % VEC == 0 && tc::aligned16(o) && tc::aligned16(rest) && tc::aligned16(dout);
   const int64_t units = vec ? p.D / VEC : p.D;  // a row's
   auto run = [&](auto kern, int lanes) {
     const int64_t need = cdiv(rows, 256 / lanes);
     return launch_chained(kern, dim3((unsigned)std::min<int64_t>(need, kSMs * 32)), dim3(256), 0,
-                          st, (const T*)o, (const T*)dout, lse, ws.terms, rows, p.D);
+                          st, (const T*)o, (const T*)rest, (const T*)dout, lse, ws.terms, rows, p.D);
   };
   if (!vec) return run(terms_kernel<T, 1, 32>, 32);
   if (units <= 4) return run(terms_kernel<T, VEC, 4>, 4);
@@ -387,7 +387,8 @@ int64_t theria_ragged_fwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64
 }
 
 int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, void* o, float* lse, void* workspace,
+                      const void* offsets, int wide, void* o, void* o_rest, float* lse,
+                      void* workspace,
                       int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
                       int64_t D, int dtype, float scale, int causal, void* stream) {
   const Problem p = problem(strides, T, S, H, Hkv, D, scale, causal);
@@ -399,7 +400,7 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
   cudaStream_t st = (cudaStream_t)stream;
   FwdWs ws = fwd_ws(workspace, p);
   if (!grid_fits(p)) return THERIA_ERR_UNSUPPORTED;
-  const bool on_tc = use_tc(dtype, p, {q, k, v, o});
+  const bool on_tc = use_tc(dtype, p, {q, k, v, o, o_rest});
   if (on_tc) retile(ws.list, 1, 2 * (FM / p.G));
   Blank blank{};
   blank.p[0] = o;
@@ -410,10 +411,10 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
     if constexpr (!std::is_same<E, float>::value)
       if (on_tc)
         return by_tile(p, [&](auto hd, auto causal_) {
-          return tc_fwd<E, decltype(hd)::value, decltype(causal_)::value>(q, k, v, o, lse, ws,
+          return tc_fwd<E, decltype(hd)::value, decltype(causal_)::value>(q, k, v, o, o_rest, lse, ws,
                                                                           dtype, p, st);
         });
-    return simt_fwd<E>(q, k, v, o, lse, ws, p, st);
+    return simt_fwd<E>(q, k, v, o, o_rest, lse, ws, p, st);
   });
 }
 
@@ -425,7 +426,7 @@ int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64
 }
 
 int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, const void* o, const void* dout,
+                      const void* offsets, int wide, const void* o, const void* o_rest, const void* dout,
                       const float* lse, void* dq, void* dk, void* dv, void* workspace,
                       int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
                       int64_t D, int dtype, float scale, int causal, void* stream) {
@@ -455,7 +456,7 @@ int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t
     return e;
   return by_type(dtype, [&](auto t) -> int {
     using E = decltype(t);
-    if (int e = run_terms<E>(o, dout, lse, ws, p, st)) return e;
+    if (int e = run_terms<E>(o, o_rest, dout, lse, ws, p, st)) return e;
     if constexpr (!std::is_same<E, float>::value)
       if (on_tc)
         return by_tile(p, [&](auto hd, auto causal_) {
