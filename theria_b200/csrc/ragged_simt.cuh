@@ -375,14 +375,15 @@ terms_kernel(const T* __restrict__ o, const T* __restrict__ rest, const T* __res
   }
 }
 
-// One split of a backward tile (see above).  part: NULL where there is one
-// split (results rounded to T at once), else float32 [splits][2][T * Hkv][D].
+// One split of a backward tile (see above).  part: NULL where there is one split
+// (results rounded to T at once), else float32 [splits][2][T * Hkv][D], for queries
+// [splits][T * H][D].
 template <typename T, int DT, bool KEYS, bool ASYNC>
 __global__ void __launch_bounds__(SimtSmem<DT>::SG * BWD_THREADS)
 simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                 const T* __restrict__ dout, const float2* terms, T* __restrict__ out1,
                 T* __restrict__ out2, float* part, const int4* items, const int* count,
-                Problem pr) {
+                int splits, Problem pr) {
   using L = SimtSmem<DT>;
   constexpr int SG = L::SG;
   extern __shared__ float4 smem4[];
@@ -395,7 +396,9 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   float2* ts = reinterpret_cast<float2*>(ps + SR * (SC + 4));  // keys: [2][SC]
   auto sync = [&] { tc::named_bar(1 + g, BWD_THREADS); };
   grid_wait();
-  const int tile = blockIdx.x / pr.Hkv, hk = blockIdx.x % pr.Hkv;
+  // a tile's splits side by side, so that the longest tiles' all start first
+  const int hk = blockIdx.x % pr.Hkv, sp = blockIdx.x / pr.Hkv % splits;
+  const int tile = blockIdx.x / pr.Hkv / splits;
   if (tile >= *count) return;
   const int4 it = items[tile];
   const int G = pr.G, len = it.y, first = it.z;
@@ -436,9 +439,9 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   int64_t y_from = 0, y_to = KEYS ? q_rows : len;
   if (pr.causal && KEYS) y_from = (int64_t)first * G;
   if (pr.causal && !KEYS) y_to = (first + rows - 1) / G + 1;
-  const int n_y = (int)((y_to - y_from + SC - 1) / SC), splits = gridDim.y;
-  const int t0 = (int)((int64_t)n_y * blockIdx.y / splits);
-  const int t1 = (int)((int64_t)n_y * (blockIdx.y + 1) / splits);
+  const int n_y = (int)((y_to - y_from + SC - 1) / SC);
+  const int t0 = (int)((int64_t)n_y * sp / splits);
+  const int t1 = (int)((int64_t)n_y * (sp + 1) / splits);
   const float c = pr.scale_log2;
   float a1[4][DT / 16], a2[KEYS ? 4 : 1][DT / 16];
 #pragma unroll
@@ -538,8 +541,8 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         out1[row * pr.D + d] = from_f32<T>(a1[i][x] * pr.scale);
         if constexpr (KEYS) out2[row * pr.D + d] = from_f32<T>(a2[i][x]);
       } else {
-        const int64_t plane = (int64_t)pr.T * pr.Hkv * pr.D;
-        float* to = part + 2 * plane * blockIdx.y + row * pr.D + d;
+        const int64_t plane = (int64_t)pr.T * (KEYS ? pr.Hkv : pr.H) * pr.D;
+        float* to = part + (KEYS ? 2 : 1) * plane * sp + row * pr.D + d;
         to[0] = a1[i][x] * pr.scale;
         if constexpr (KEYS) to[plane] = a2[i][x];
       }
@@ -547,25 +550,27 @@ simt_bwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
   }
 }
 
-// dk, dv from the splits' float32 sums, added in the splits' order.
+// A gradient (two, b not NULL: dk and dv) of `heads` heads from the splits' float32
+// sums, added in the splits' order.
 template <typename T>
 __global__ void __launch_bounds__(256)
 join_kernel(const float* part, int splits, const int* count, const void* offsets, int wide,
-            T* __restrict__ dk, T* __restrict__ dv, Problem pr) {
+            T* __restrict__ a, T* __restrict__ b, int heads, Problem pr) {
   grid_wait();
   if (*count == 0) return;
-  const int64_t row = (int64_t)pr.Hkv * pr.D, plane = row * pr.T;
+  const int64_t row = (int64_t)heads * pr.D, plane = row * pr.T, step = b ? 2 * plane : plane;
   const int64_t lo = offset_at(offsets, wide, 0) * row, hi = offset_at(offsets, wide, pr.S) * row;
-  const int64_t all = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += all) {
-    if (i < lo || i >= hi) continue;  // zeroed with the other rows of no sequence
-    float a = 0.f, b = 0.f;
+  // (the rows of no sequence are zeroed with the others)
+  for (int64_t i = lo + (int64_t)blockIdx.x * 256 + threadIdx.x; i < hi;
+       i += (int64_t)gridDim.x * 256) {
+    float x = 0.f, y = 0.f;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      a += part[2 * plane * s + i];
-      b += part[2 * plane * s + plane + i];
+      x += part[step * s + i];
+      if (b) y += part[step * s + plane + i];
     }
-    dk[i] = from_f32<T>(a);
-    dv[i] = from_f32<T>(b);
+    a[i] = from_f32<T>(x);
+    if (b) b[i] = from_f32<T>(y);
   }
 }
 

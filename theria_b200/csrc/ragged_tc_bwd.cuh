@@ -359,14 +359,14 @@ struct DkvCfg {
   static constexpr int kAlloc = oAbort + 4 + 1024;
 };
 
-// One split of the queries (blockIdx.y of gridDim.y).  part: NULL where there is one
-// split (results rounded to T at once), else float32 [splits][2][T * Hkv][D].
+// One split of a tile's queries.  part: NULL where there is one split (results rounded
+// to T at once), else float32 [splits][2][T * Hkv][D].
 template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(DkvCfg<HD>::kThreads, 1)
 tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
               const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
               const float2* terms, T* __restrict__ dk, T* __restrict__ dv, float* part,
-              const int4* items, const int* count, const Problem pr) {
+              const int4* items, const int* count, int splits, const Problem pr) {
   using L = DkvCfg<HD>;
   constexpr int YST = L::YST;
   constexpr bool kXT = HD == 64;  // k and v in TMEM too, as the A operands of s and dp
@@ -384,7 +384,9 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   grid_wait();
-  const int hk = blockIdx.x % pr.Hkv, at = blockIdx.x / pr.Hkv;
+  // a tile's splits side by side, so that the longest tiles' all start first
+  const int hk = blockIdx.x % pr.Hkv, sp = blockIdx.x / pr.Hkv % splits;
+  const int at = blockIdx.x / pr.Hkv / splits;
   if (at >= *count) return;
   const int4 item = items[at];
   const int start = item.x, len = item.y, first = item.z, G = pr.G;
@@ -392,8 +394,8 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
   // the queries' tokens from y_from on, and this split's share of their tiles
   const int y_from = CAUSAL ? first : 0;
   const int n_y = (len - y_from + yt - 1) / yt;
-  const int t_at = (int)((int64_t)n_y * blockIdx.y / gridDim.y);
-  const int n_iter = (int)((int64_t)n_y * (blockIdx.y + 1) / gridDim.y) - t_at;
+  const int t_at = (int)((int64_t)n_y * sp / splits);
+  const int n_iter = (int)((int64_t)n_y * (sp + 1) / splits) - t_at;
   auto tok_of = [&](int t) { return y_from + (t_at + t) * yt; };  // tile t's first token
 
   if (threadIdx.x == 0) {
@@ -667,7 +669,7 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
       for (int which = 0; which < 2; ++which) {
         const float mul = which == 0 ? pr.scale : 1.f;
         float* sums = part == nullptr ? nullptr
-                                      : part + (2 * blockIdx.y + which) * plane + row * pr.D;
+                                      : part + (2 * sp + which) * plane + row * pr.D;
 #pragma unroll 1
         for (int c = grp + 2 * set; c < HD / 32; c += 4) {
           float v[32];

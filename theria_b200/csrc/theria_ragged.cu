@@ -138,14 +138,19 @@ int run_plan(const void* offsets, int wide, const Problem& p, const List& a, con
   return launch_status();
 }
 
-// Parts that a key tile's queries are split into: until the tiles of an even batch
-// would fill the GPU `waves` times, and no more than 32.  Two for the tensor-core
-// kernel; three for the CUDA cores', whose tiles take longer.
-int key_splits(const Problem& p, int step, int waves) {
-  const int64_t tiles = std::max<int64_t>(1, cdiv(p.T, step) * p.Hkv);
-  return (int)std::min<int64_t>(32, std::max<int64_t>(1, waves * kSMs / tiles));
+// Parts that the walk of a tile is split into, of `tiles` in an even batch: until they
+// would fill the GPU `waves` times, and no more than 32.
+int parts_of(int64_t tiles, int waves) {
+  return (int)std::min<int64_t>(32, std::max<int64_t>(1, waves * kSMs / std::max<int64_t>(1, tiles)));
 }
-constexpr int kTcWaves = 2, kSimtWaves = 3;
+// dk, dv on the tensor cores: two waves (their tiles are few where the keys have few
+// heads).  On the CUDA cores, whose tiles take longer, three, and for dq two (2395
+// tokens, 5 heads of 72 on one: dq 229 us unsplit, the longest tile's own time).
+int tc_splits(const Problem& p) { return parts_of(cdiv(p.T, BX) * p.Hkv, 2); }
+int simt_splits(const Problem& p) { return parts_of(cdiv(p.T, SR) * p.Hkv, 3); }
+int simt_q_splits(const Problem& p) {
+  return parts_of(cdiv((int64_t)p.T * p.G, SR) * p.Hkv, 3);
+}
 
 // Lists have room for the CUDA-core kernels' tiles of 32 or 64 packed rows; the
 // tensor-core kernels' are larger, hence fewer (128 / G, rounded down, is at
@@ -179,8 +184,10 @@ BwdWs bwd_ws(void* base, const Problem& p) {
   w.lq = take_list(c, p, p.G, SR, 0);
   w.lk = take_list(c, p, 1, SR, 1);
   w.terms = c.take<float2>((int64_t)p.T * p.H);
-  const int splits = std::max(key_splits(p, BX, kTcWaves), key_splits(p, SR, kSimtWaves));
-  w.part = splits > 1 ? c.take<float>(2ll * splits * p.T * p.Hkv * p.D) : nullptr;
+  const int ks = std::max(tc_splits(p), simt_splits(p)), qs = simt_q_splits(p);
+  const int64_t k_row = 2ll * p.Hkv * p.D, q_row = (int64_t)p.H * p.D;
+  const int64_t part = std::max(ks > 1 ? ks * k_row : 0, qs > 1 ? qs * q_row : 0) * p.T;
+  w.part = part > 0 ? c.take<float>(part) : nullptr;
   w.bytes = c.used;
   return w;
 }
@@ -210,10 +217,10 @@ int simt_fwd(const void* q, const void* k, const void* v, void* o, void* rest, f
 }
 
 template <typename T>
-int run_join(const BwdWs& ws, int splits, const void* offsets, int wide, void* dk, void* dv,
-             const Problem& p, cudaStream_t st) {
+int run_join(const BwdWs& ws, int splits, const int* count, const void* offsets, int wide, void* a,
+             void* b, int heads, const Problem& p, cudaStream_t st) {
   return launch_chained(join_kernel<T>, dim3(kSMs * 4), dim3(256), 0, st, (const float*)ws.part,
-                        splits, (const int*)ws.lk.count, offsets, wide, (T*)dk, (T*)dv, p);
+                        splits, count, offsets, wide, (T*)a, (T*)b, heads, p);
 }
 
 template <typename T>
@@ -228,20 +235,27 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
       if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
           cudaSuccess)
         return (int)THERIA_ERR_LAUNCH;
-      return launch_chained(kern, dim3(blocks(p, l.per, SR), (unsigned)splits),
-                            dim3(SimtSmem<DT>::SG * BWD_THREADS),
-                            smem, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout,
+      return launch_chained(kern, dim3(blocks(p, l.per, SR) * (unsigned)splits),
+                            dim3(SimtSmem<DT>::SG * BWD_THREADS), smem, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout,
                             (const float2*)ws.terms, (T*)o1, (T*)o2, part, (const int4*)l.items,
-                            (const int*)l.count, p);
+                            (const int*)l.count, splits, p);
     };
-    if (dq != nullptr)
-      if (int e = run(simt_bwd_kernel<T, DT, false, ASYNC>, ws.lq, 1, dq, nullptr, nullptr)) return e;
+    if (dq != nullptr) {
+      const int splits = simt_q_splits(p);
+      if (int e = run(simt_bwd_kernel<T, DT, false, ASYNC>, ws.lq, splits, dq, nullptr,
+                      splits > 1 ? ws.part : nullptr))
+        return e;
+      if (splits > 1)
+        if (int e = run_join<T>(ws, splits, ws.lq.count, offsets, wide, dq, nullptr, p.H, p, st))
+          return e;
+    }
     if (dk == nullptr) return (int)THERIA_OK;
-    const int splits = key_splits(p, SR, kSimtWaves);
+    const int splits = simt_splits(p);
     if (int e = run(simt_bwd_kernel<T, DT, true, ASYNC>, ws.lk, splits, dk, dv,
                     splits > 1 ? ws.part : nullptr))
       return e;
-    return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : (int)THERIA_OK;
+    return splits > 1 ? run_join<T>(ws, splits, ws.lk.count, offsets, wide, dk, dv, p.Hkv, p, st)
+                      : (int)THERIA_OK;
   });
 }
 
@@ -333,14 +347,15 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
       !key_map(&mk, k, dtype, p, p.k_t, p.k_h, BX) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, BX))
     return THERIA_ERR_UNSUPPORTED;
   if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
-  const int splits = key_splits(p, BX, kTcWaves);
-  if (int e = launch_chained(kern, dim3(blocks(p, ws.lk.per, ws.lk.step), (unsigned)splits),
+  const int splits = tc_splits(p);
+  if (int e = launch_chained(kern, dim3(blocks(p, ws.lk.per, ws.lk.step) * (unsigned)splits),
                              dim3(Cfg::kThreads), Cfg::kAlloc, st, mk, mv, mq, mo,
                              (const float2*)ws.terms, (T*)dk, (T*)dv,
                              splits > 1 ? ws.part : nullptr, (const int4*)ws.lk.items,
-                             (const int*)ws.lk.count, p))
+                             (const int*)ws.lk.count, splits, p))
     return e;
-  return splits > 1 ? run_join<T>(ws, splits, offsets, wide, dk, dv, p, st) : THERIA_OK;
+  return splits > 1 ? run_join<T>(ws, splits, ws.lk.count, offsets, wide, dk, dv, p.Hkv, p, st)
+                    : THERIA_OK;
 }
 
 // Calls f(HD, CAUSAL) as integral constants.
