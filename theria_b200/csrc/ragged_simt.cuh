@@ -109,10 +109,14 @@ __device__ __forceinline__ void tile_scores(float (&s)[4][J], const float* x, co
                                             int ty) {
   constexpr int K = SimtSmem<DT>::kRow;
   const int tx = threadIdx.x & 15;
+  // even and odd values of the rows apart, two at a time (narrow rows, whose few
+  // steps leave the pairs' sums to weigh: each value in turn, 7.5 against 8.7 us for dq
+  // of 25 sequences of 64, 4 heads of 16)
+  float s2[4][J];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < J; ++j) s[i][j] = 0.f;
+    for (int j = 0; j < J; ++j) s[i][j] = s2[i][j] = 0.f;
 #pragma unroll 4
   for (int d = 0; d < DT; d += 4) {
     float4 a[4], b[J];
@@ -124,12 +128,22 @@ __device__ __forceinline__ void tile_scores(float (&s)[4][J], const float* x, co
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
-        s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
-        s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
-        s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+        if constexpr (DT >= 64) {
+          tc::fma2(s[i][j], s2[i][j], a[i].x, a[i].y, b[j].x, b[j].y, s[i][j], s2[i][j]);
+          tc::fma2(s[i][j], s2[i][j], a[i].z, a[i].w, b[j].z, b[j].w, s[i][j], s2[i][j]);
+        } else {
+          s[i][j] = fmaf(a[i].x, b[j].x, s[i][j]);
+          s[i][j] = fmaf(a[i].y, b[j].y, s[i][j]);
+          s[i][j] = fmaf(a[i].z, b[j].z, s[i][j]);
+          s[i][j] = fmaf(a[i].w, b[j].w, s[i][j]);
+        }
       }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+      if constexpr (DT >= 64) s[i][j] += s2[i][j];
 }
 
 // The columns of DT that a thread sums: DT / 16 of them, in runs of up to 4.
@@ -170,8 +184,15 @@ __device__ __forceinline__ void tile_sums(float (&acc)[4][DT / 16], const float*
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float pi = u == 0 ? a[i].x : u == 1 ? a[i].y : u == 2 ? a[i].z : a[i].w;
+          if constexpr (DT < 64) {
 #pragma unroll
-          for (int x = 0; x < RUN; ++x) acc[i][c + x] = fmaf(pi, b[x], acc[i][c + x]);
+            for (int x = 0; x < RUN; ++x) acc[i][c + x] = fmaf(pi, b[x], acc[i][c + x]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < RUN; x += 2)
+              tc::fma2(acc[i][c + x], acc[i][c + x + 1], pi, pi, b[x], b[x + 1], acc[i][c + x],
+                       acc[i][c + x + 1]);
+          }
         }
       }
     }
