@@ -226,3 +226,13 @@ def test_clipped_meta_step():
     graphed = GraphedMetaStep(ms, batch)
     graphed.step(batch)
     assert abs(ms.bucket.double().norm().item() - 1e-3) <= 1e-9
+
+
+@pytest.mark.parametrize("most", [1e6, 0.5])
+def test_some_in_place(most):
+    # the C entry writes each y, also where only the first is its x
+    x = _tensors([(100,), (9000,)], torch.float32)
+    want, _ = lm.clip_gradients(x, most)
+    out = [x[0], torch.full_like(x[1], 7.0)]
+    lm._clip(x, out, most)
+    assert all(torch.equal(a, b) for a, b in zip(out, want))

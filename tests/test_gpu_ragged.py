@@ -361,3 +361,23 @@ def test_workspace_and_arguments_at_the_c_entry():
     assert lib.theria_ragged_fwd_workspace_bytes(100, 3, 4, 3) == 0  # H not a multiple
     assert lib.theria_ragged_fwd_workspace_bytes(100, 3, 4, 2) > 0
     assert ragged._strides(*(torch.zeros(2, 2, 4),) * 3)[0] == 8
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_that_no_address_uses(dtype):
+    # a single key head, a single token: their strides may be any number
+    q, k, v, _ = _inputs([70, 9], 4, 1, 64, dtype)
+    odd = [t.as_strided(t.shape, (64, 5, 1)) for t in (k, v)]
+    off = _offsets([70, 9])
+    assert torch.equal(sdpa_ragged(q, *odd, off), sdpa_ragged(q, k, v, off))
+    one = [t[:1].as_strided((1, *t.shape[1:]), (3, 64, 1)) for t in (q, k, v)]
+    off = _offsets([1])
+    assert torch.equal(sdpa_ragged(*one, off), sdpa_ragged(q[:1], k[:1], v[:1], off))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("G", [33, 48, 63])
+def test_groups_of_one_token_a_tile(G, dtype):
+    # a tile of 64 rows holds one token, and rows that no copy fills
+    _check([90, 0, 33, 1], 2 * G, 2, 128, dtype)
+    _check([50, 7], G, 1, 72, dtype, causal=False, lead=2)

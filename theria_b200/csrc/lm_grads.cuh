@@ -40,6 +40,7 @@ struct Table {
   unsigned char dtype[MOST];
   unsigned char vec[MOST];      // its pointers are 16-byte aligned
   int n;
+  bool in_place;                // every out is its x
 };
 
 template <typename F>
@@ -241,7 +242,7 @@ clip_kernel(const __grid_constant__ Table t, const double* part, int parts, doub
     }
   }
   if (t.n == 0) return;
-  if (c == 1.0 && t.out[0] == t.x[0]) return;  // in place, nothing to clip
+  if (c == 1.0 && t.in_place) return;  // in place, nothing to clip
   combine<false>(t, (float)c, 0.f);
 }
 

@@ -35,7 +35,7 @@ struct Problem {
 struct List {
   int4* items;   // {start, n, first, 0}; NULL: no list
   int* count;    // the number of items
-  int* base;     // [S + 1] scratch
+  int* base;     // [S] scratch
   int per, step, by_key;
 };
 

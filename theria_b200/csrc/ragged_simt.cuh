@@ -1,6 +1,6 @@
 // Attention over packed sequences on the CUDA cores: float32 (always in
 // float32), and 16-bit tensors that the tensor-core kernels cannot take
-// (more than 128 query heads a key head, or rows off 16-byte boundaries).
+// (more than 64 query heads a key head, or rows off 16-byte boundaries).
 //
 // A block is 16 warps on one tile of rows: in the forward four groups of 4 warps on
 // 32 rows, in the backward two of 8 on 64, each group taking every fourth (second)
@@ -19,7 +19,7 @@
 // next scores do, in the backward into a second buffer.
 //
 // The backward is one kernel for both sides.  Its tile stays on 64 rows x1, x2
-// and walks over tiles of 64 y1, y2:
+// and walks over tiles of 32 y1, y2:
 //     queries: x = (q, do), y = (k, v):  dq += ds k
 //     keys:    x = (k, v), y = (q, do):  dk += ds^T q, dv += p^T do
 // so no sum is shared between blocks and nothing is added atomically.

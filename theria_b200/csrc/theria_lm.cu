@@ -958,12 +958,14 @@ int grads_groups(const void* const* x, const void* const* u, void* const* out,
                  const int64_t* sizes, const int* dtypes, int64_t n, F f) {
   grads::Table t;
   t.n = 0;
+  t.in_place = true;
   int64_t chunks = 0;
   auto flush = [&]() -> int {
     if (t.n == 0) return THERIA_OK;
     t.first[t.n] = (int)chunks;
     const int e = f(t, (int)chunks);
     t.n = 0;
+    t.in_place = true;
     chunks = 0;
     return e;
   };
@@ -974,6 +976,7 @@ int grads_groups(const void* const* x, const void* const* u, void* const* out,
     t.x[k] = x[i];
     t.u[k] = u ? u[i] : nullptr;
     t.out[k] = out ? out[i] : nullptr;
+    t.in_place = t.in_place && t.out[k] == t.x[k];
     t.size[k] = sizes[i];
     t.dtype[k] = (unsigned char)dtypes[i];
     t.vec[k] = tc::aligned16(x[i]) && tc::aligned16(t.u[k]) && tc::aligned16(t.out[k]);

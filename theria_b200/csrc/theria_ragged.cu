@@ -91,6 +91,13 @@ Problem problem(const int64_t* st, int64_t T, int64_t S, int64_t H, int64_t Hkv,
     p.k_h = st[3];
     p.v_t = st[4];
     p.v_h = st[5];
+    // strides that no address uses: as if contiguous, so that they rule no kernel out
+    if (T == 1) {
+      p.q_t = H * D;
+      p.k_t = p.v_t = Hkv * D;
+    }
+    if (H == 1) p.q_h = D;
+    if (Hkv == 1) p.k_h = p.v_h = D;
   }
   p.scale = scale;
   p.scale_log2 = scale * kLog2e;
