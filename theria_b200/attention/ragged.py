@@ -28,23 +28,26 @@ from theria_b200.lm import _DTYPES, _call, _check, _check_ids, _no_tangents, _pt
 
 _opaque = torch.compiler.disable
 _WHAT = "theria sdpa_ragged"
+_Strides = ctypes.c_int64 * 6
 
 
 def _check_args(q, k, v, offsets):
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check(_WHAT, name, t, q.device)
-    if q.ndim != 3 or 0 in q.shape[1:]:
+    device, dtype, shape, kv = q.device, q.dtype, tuple(q.shape), tuple(k.shape)
+    _check(_WHAT, "q", q)
+    _check(_WHAT, "k", k, device)
+    _check(_WHAT, "v", v, device)
+    if len(shape) != 3 or 0 in shape[1:]:
         raise AssertionError("q must have shape (T,H,D)")
-    T, H, D = q.shape
-    if k.ndim != 3 or k.shape[0] != T or k.shape[2] != D or k.shape[1] == 0 or H % k.shape[1]:
+    T, H, D = shape
+    if len(kv) != 3 or kv[0] != T or kv[2] != D or kv[1] == 0 or H % kv[1]:
         raise AssertionError("k must have shape (T,Hkv,D) with Hkv a divisor of H")
-    if v.shape != k.shape:
+    if tuple(v.shape) != kv:
         raise AssertionError("v must have shape (T,Hkv,D) as k")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
+    if k.dtype != dtype or v.dtype != dtype:
         raise AssertionError("q, k, v must share one dtype")
     if D > MAX_HEAD_DIM:
         raise AssertionError(f"theria_b200 supports D<={MAX_HEAD_DIM}")
-    _check_ids(_WHAT, "offsets", offsets, q.device)
+    _check_ids(_WHAT, "offsets", offsets, device)
     if offsets.ndim != 1 or offsets.shape[0] == 0:
         raise AssertionError("offsets must have shape (S+1,)")
 
@@ -53,17 +56,18 @@ def _kernel_layout(t):
     """t itself where its heads lie as the kernels read them, else a copy: the
     values of a head side by side and, for the 16-bit tensor-core kernels, every
     row on a 16-byte boundary."""
-    if t.stride(2) != 1 or (t.shape[0] > 1 and t.stride(0) <= 0) or (
-            t.shape[1] > 1 and t.stride(1) <= 0):
+    a, b, c = t.stride()
+    if c != 1 or (a <= 0 and t.shape[0] > 1) or (b <= 0 and t.shape[1] > 1):
         return t.contiguous()
-    if t.element_size() == 2 and (t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16):
+    if t.element_size() == 2 and (a % 8 or b % 8 or t.data_ptr() % 16):
         t = t.contiguous()
         return t if t.data_ptr() % 16 == 0 else t.clone()
     return t
 
 
 def _strides(q, k, v):
-    return (ctypes.c_int64 * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+    (a, b, _), (c, d, _), (e, f, _) = q.stride(), k.stride(), v.stride()
+    return _Strides(a, b, c, d, e, f)
 
 
 def _forward(q, k, v, offsets, causal, scale, grad):
@@ -94,7 +98,8 @@ def _backward(q, k, v, offsets, o, rest, lse, dout, causal, scale, need):
     ws, size = _workspace("theria_ragged_bwd_workspace_bytes", q.device, T, S, H, Hkv, D)
     _call("theria_ragged_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(),
           _strides(q, k, v), offsets.data_ptr(), int(offsets.dtype == torch.int64), o.data_ptr(),
-          _ptr(rest), dout.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), ws.data_ptr(), size, T, S, H, Hkv, D, _DTYPES[q.dtype], scale, causal)
+          _ptr(rest), dout.data_ptr(), lse.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv),
+          ws.data_ptr(), size, T, S, H, Hkv, D, _DTYPES[q.dtype], scale, causal)
     return dq, dk if need[1] else None, dv if need[2] else None
 
 

@@ -60,7 +60,7 @@ def _fn(name):
 def _call(name, device, *args):
     """One library call on `device` and torch's current stream there."""
     i = device.index
-    if i == torch.cuda.current_device():
+    if i == torch._C._cuda_getDevice():
         st = _fn(name)(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(device):
@@ -407,6 +407,7 @@ def linear_cross_entropy(hidden, weight, target, ignore_index=IGNORE_INDEX, redu
 
 # --------------------------------------------------------------------- rotary
 SCALINGS = (None, "linear", "ntk", "by_parts")
+_Strides12 = ctypes.c_int64 * 12
 
 
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original_length=None,
@@ -451,30 +452,31 @@ def _rotary_layout(t):
 
 def _rotate(q, k, frequencies, positions, offsets, interleaved, amplitude, back):
     """Rotated q and k (each may be None)."""
-    out, strides = [], []
-    for x in (q, k):
-        if x is None:
-            out.append(None)
-            strides += [0] * 6
+    out, strides, pointers, heads = [None, None], [], [], []
+    x = [None if t is None else _rotary_layout(t) for t in (q, k)]  # copies live to the launch
+    for i, xi in enumerate(x):
+        if xi is None:
+            strides += (0, 0, 0, 0, 0, 0)
+            pointers += (None, None)
+            heads.append(0)
             continue
-        x = _rotary_layout(x)
-        y = torch.empty_like(x)
-        if y.stride(-1) != 1:
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        out.append((x, y))
-        for t in (x, y):
-            strides += t.stride()[:3] if t.ndim == 4 else (0, *t.stride()[:2])
-    x = (out[0] or out[1])[0]
-    B, T, D = x.shape[0] if x.ndim == 4 else 1, x.shape[-3], x.shape[-1]
+        y, a = torch.empty_like(xi), xi.stride()
+        b, shape = y.stride(), xi.shape
+        if b[-1] != 1:
+            y = torch.empty(shape, dtype=xi.dtype, device=xi.device)
+            b = y.stride()
+        out[i], last = y, xi
+        strides += (*a[:3], *b[:3]) if len(a) == 4 else (0, a[0], a[1], 0, b[0], b[1])
+        pointers += (xi.data_ptr(), y.data_ptr())
+        heads.append(shape[-2])
     at = positions if positions is not None else offsets
-    (xq, yq), (xk, yk) = (o or (None, None) for o in out)
-    _call("theria_rotary", x.device, _ptr(xq), _ptr(xk), _ptr(yq), _ptr(yk),
-          (ctypes.c_int64 * 12)(*strides), B, T, 0 if xq is None else xq.shape[-2],
-          0 if xk is None else xk.shape[-2], D, _DTYPES[x.dtype], _ptr(positions),
+    _call("theria_rotary", last.device, pointers[0], pointers[2], pointers[1], pointers[3],
+          _Strides12(*strides), shape[0] if len(shape) == 4 else 1, shape[-3], *heads,
+          shape[-1], _DTYPES[last.dtype], _ptr(positions),
           0 if positions is None else positions.numel(), _ptr(offsets),
           0 if offsets is None else offsets.numel() - 1, 0 if at is None else _wide(at),
           frequencies.data_ptr(), frequencies.numel(), amplitude, interleaved, back)
-    return yq, yk
+    return tuple(out)
 
 
 class _Rotary(torch.autograd.Function):
@@ -518,19 +520,21 @@ def rotary(q, k, frequencies, positions=None, offsets=None, interleaved=False, a
     of packed sequences, each counted from its first token (tokens of no sequence
     stand at 0); else 0 .. T - 1.  Differentiable in q and k, any number of times.
     """
-    what = "theria rotary"
+    what, device, shape = "theria rotary", q.device, tuple(q.shape)
     _check(what, "q", q)
-    if q.ndim not in (3, 4) or q.shape[-1] == 0:
+    if len(shape) not in (3, 4) or shape[-1] == 0:
         raise AssertionError("q must have shape (T,H,D) or (B,T,H,D)")
+    tokens = shape[:-2]
     if k is not None:
-        _check(what, "k", k, q.device)
-        if k.ndim != q.ndim or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]:
+        _check(what, "k", k, device)
+        ks = tuple(k.shape)
+        if len(ks) != len(shape) or ks[:-2] != tokens or ks[-1] != shape[-1]:
             raise AssertionError("k must have q's shape up to the number of heads")
         if k.dtype != q.dtype:
             raise AssertionError("q and k must share one dtype")
-    if frequencies.dtype is not torch.float64 or frequencies.device != q.device:
+    if frequencies.dtype is not torch.float64 or frequencies.device != device:
         raise AssertionError("frequencies must be float64 on q's device")
-    if frequencies.ndim != 1 or 2 * frequencies.numel() > q.shape[-1]:
+    if frequencies.ndim != 1 or 2 * frequencies.numel() > shape[-1]:
         raise AssertionError("frequencies must have shape (pairs,) with 2 * pairs <= D")
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise AssertionError("theria rotary has no gradient for its frequencies")
@@ -538,10 +542,9 @@ def rotary(q, k, frequencies, positions=None, offsets=None, interleaved=False, a
         raise AssertionError("theria rotary takes positions or offsets, not both")
     for name, t in (("positions", positions), ("offsets", offsets)):
         if t is not None:
-            _check_ids(what, name, t, q.device)
-    tokens = q.shape[:-2]
-    if positions is not None and positions.shape not in (tokens, tokens[-1:]):
-        raise AssertionError(f"positions must have shape {tuple(tokens)} or {tuple(tokens[-1:])}")
+            _check_ids(what, name, t, device)
+    if positions is not None and tuple(positions.shape) not in (tokens, tokens[-1:]):
+        raise AssertionError(f"positions must have shape {tokens} or {tokens[-1:]}")
     if offsets is not None and (offsets.ndim != 1 or offsets.shape[0] == 0):
         raise AssertionError("offsets must have shape (S+1,)")
     _no_tangents(what, q, k)
