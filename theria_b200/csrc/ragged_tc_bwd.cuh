@@ -19,7 +19,7 @@
 // takes 150 to 300 cycles, a wait that finds its barrier passed 200, a commit 100;
 // with a few buffers the hops of the ring s -> p, ds -> sums -> s set the pace, not the
 // products (bfloat16, 8192 tokens in two sequences, 16 heads on 4 of 128, not causal:
-// dq 342 us of 160 us of products, dkv 466 of 320).  Hence one product a step and one
+// dq 335 us of 160 us of products, dkv 466 to 490 of 320).  Hence one product a step and one
 // thread a product (one issuing thread for all: dkv 640 us, two: 540), and, per side:
 //
 // tc_dq: tiles of 128 rows y, all 16 warps on one.  s, in one buffer, is free as soon
@@ -56,13 +56,16 @@ constexpr int QY = 128, KY = 64;    // rows of y: of tc_dq (keys), of tc_dkv (pa
 // (columns c .. c + 31 of D, a multiple of 8).
 template <typename T>
 __device__ __forceinline__ void put_sums(const float (&v)[32], float mul, T* to, int c, int D) {
+  const bool wide = wide_rows(to, D);  // (the same for every row)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float* e = v + 8 * i;
-    if (c + 8 * i < D)
-      reinterpret_cast<uint4*>(to + c)[i] = make_uint4(
-          tc::pack2<T>(e[0] * mul, e[1] * mul), tc::pack2<T>(e[2] * mul, e[3] * mul),
-          tc::pack2<T>(e[4] * mul, e[5] * mul), tc::pack2<T>(e[6] * mul, e[7] * mul));
+  for (int i = 0; i < 2; ++i) {
+    const float* e = v + 16 * i;
+    const int at = c + 16 * i;
+    if (at >= D) continue;
+    uint32_t w[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = tc::pack2<T>(e[2 * k] * mul, e[2 * k + 1] * mul);
+    store16(to + at, w, wide, at + 8 < D);
   }
 }
 
