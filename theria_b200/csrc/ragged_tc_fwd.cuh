@@ -24,6 +24,7 @@
 // to zero in shared memory by the producer warp, once per CTA (NaN * 0 is NaN).
 #pragma once
 
+#include "pair_exchange.cuh"
 #include "ragged_plan.cuh"
 #include "tc_common.cuh"
 
@@ -341,6 +342,8 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     const uint32_t t_p = (kSepP ? tmem + 384 + t * 64 : tmem + t * 128 + h * 64) + lane_off;
     float* red = reinterpret_cast<float*>(smem + L::oRed);  // [2 parity][2 t][2 h][128]
     auto red_at = [&](int par, int hh) { return red + ((par * 2 + t) * 2 + hh) * FM + r; };
+    auto meet = [&] { tc::named_bar(bar_id, 64); };  // the two halves' warps
+    static_assert(kHalves == 1 || !kSepP, "two halves: no wait but s_full's ends the loop");
     // the keys of this row, and of the warp's first: tiles beyond those need the mask
     const int my_keys = CAUSAL ? min(len, tok0 + r / G + 1) : len;
     const int clean = CAUSAL ? min(len, tok0 + quarter * 32 / G + 1) : len;
@@ -352,7 +355,14 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     };
     const int nt = t ? n1 : n0;
     for (int j = 0; j < nt; ++j) {
-      if (!wait(s_full + t, j & 1)) { ok = false; break; }
+      if (!wait(s_full + t, j & 1)) {
+        ok = false;
+        if constexpr (kHalves == 2) {  // tell the other half
+          float none;
+          tc::pair_exchange(red_at(j & 1, h), red_at(j & 1, h ^ 1), false, 0.f, none, meet);
+        }
+        break;
+      }
       tc::tc_fence_after();
       const int col0 = j * FN + h * CW;
       const bool masked = col0 + CW > clean;
@@ -379,9 +389,12 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
       float mt = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
                        fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
       if constexpr (kHalves == 2) {
-        *red_at(j & 1, h) = mt;
-        tc::named_bar(bar_id, 64);
-        mt = fmaxf(mt, *red_at(j & 1, h ^ 1));
+        float other;
+        if (!tc::pair_exchange(red_at(j & 1, h), red_at(j & 1, h ^ 1), true, mt, other, meet)) {
+          ok = false;
+          break;
+        }
+        mt = fmaxf(mt, other);
       }
       mt *= pr.scale_log2;
       const float m_new = fmaxf(m, mt);
@@ -472,11 +485,12 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
     // ------------------------------------------------------------ epilogue
     if (nt > 0) {
       if constexpr (kHalves == 2) {
-        // both halves come here once (same trip count; a wait that gave up makes
-        // every later one of the CTA give up)
-        *red_at(nt & 1, h) = l;
-        tc::named_bar(bar_id, 64);
-        l += *red_at(nt & 1, h ^ 1);
+        // both halves or neither (the loop above ends for both with the same `ok`)
+        if (ok) {
+          *red_at(nt & 1, h) = l;
+          meet();
+          l += *red_at(nt & 1, h ^ 1);
+        }
       }
       if (ok && wait(o_done + t, 0)) {
         tc::tc_fence_after();

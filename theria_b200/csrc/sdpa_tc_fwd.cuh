@@ -28,6 +28,7 @@
 // writes O (input dtype or fp32) and LSE = ln(2) * (m + log2 l).
 #pragma once
 
+#include "pair_exchange.cuh"
 #include "tc_common.cuh"
 
 namespace theria {
@@ -324,6 +325,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
     const uint32_t t_p = (kSepP ? tmem + 384 + t * 64 : tmem + t * 128 + h * 64) + lane_off;
     float* red = reinterpret_cast<float*>(smem + L::oRed);  // [2 parity][2 t][2 h][128]
     auto red_at = [&](int par, int hh) { return red + ((par * 2 + t) * 2 + hh) * BM + r; };
+    auto meet = [&] { tc::named_bar(bar_id, 64); };  // the two halves' warps
+    static_assert(kHalves == 1 || !kSepP, "two halves: no wait but s_full's ends the loop");
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     // Waits are warp-uniform: the TMEM accesses that follow are warp-collective.
@@ -332,7 +335,14 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
     };
     const int nt = tiles_of(t);
     for (int j = 0; j < nt; ++j) {
-      if (!wait(s_full + t, j & 1)) { ok = false; break; }
+      if (!wait(s_full + t, j & 1)) {
+        ok = false;
+        if constexpr (kHalves == 2) {  // tell the other half
+          float none;
+          tc::pair_exchange(red_at(j & 1, h), red_at(j & 1, h ^ 1), false, 0.f, none, meet);
+        }
+        break;
+      }
       tc::tc_fence_after();
       const int col0 = j * BN + h * CW;
       // Tiles that need masking (the causal diagonal, the ragged last key
@@ -363,9 +373,12 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
       float mt = fmaxf(fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])),
                        fmaxf(fmaxf(mp[4], mp[5]), fmaxf(mp[6], mp[7])));
       if constexpr (kHalves == 2) {
-        *red_at(j & 1, h) = mt;
-        tc::named_bar(bar_id, 64);
-        mt = fmaxf(mt, *red_at(j & 1, h ^ 1));
+        float other;
+        if (!tc::pair_exchange(red_at(j & 1, h), red_at(j & 1, h ^ 1), true, mt, other, meet)) {
+          ok = false;
+          break;
+        }
+        mt = fmaxf(mt, other);
       }
       mt *= scale_log2;
       const float m_new = fmaxf(m, mt);
@@ -471,12 +484,13 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
     }
     // ------------------------------------------------------------ epilogue
     if constexpr (kHalves == 2) {
-      // Both halves reach this barrier once (same trip count; a timed-out
-      // wait makes every later wait of the CTA give up, so both leave the
-      // loop), and combine their row sums here.
-      *red_at(nt & 1, h) = l;
-      tc::named_bar(bar_id, 64);
-      l += *red_at(nt & 1, h ^ 1);
+      // The halves combine their row sums, both or neither (the loop above
+      // ends for both with the same `ok`).
+      if (ok) {
+        *red_at(nt & 1, h) = l;
+        meet();
+        l += *red_at(nt & 1, h ^ 1);
+      }
     }
     if (ok && wait(o_done + t, 0)) {
       tc::tc_fence_after();
