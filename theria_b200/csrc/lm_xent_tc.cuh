@@ -579,6 +579,7 @@ tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
               for (int i = 0; i < 32; ++i)
                 if (n + i < args.D) dst[i] = from_f32<O>(v[i]);
             }
+            __syncwarp();  // the next columns' wait is warp-collective
           } else if constexpr (F32) {
             stage_free();
             stage32<float>(out_row, lane, v, 0);

@@ -676,6 +676,7 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
 #pragma unroll 1
         for (int c = grp + 2 * set; c < HD / 32; c += 4) {
           float v[32];
+          __syncwarp();  // lanes without a row left the last trip early
           if (n_iter > 0) {
             tc::tmem_ld32((which == 0 ? t_a1 : t_a2) + lane_off + c * 32, v);
           } else {

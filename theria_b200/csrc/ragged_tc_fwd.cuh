@@ -505,7 +505,8 @@ tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ 
 #pragma unroll
         for (int c = 0; c < HO / 32; ++c) {
           float v[32];
-          tc::tmem_ld32(t_o + c * 32, v);  // warp-collective: before any branch
+          __syncwarp();                    // lanes without a row left the last trip early
+          tc::tmem_ld32(t_o + c * 32, v);  // warp-collective
           if (!store) continue;
           const int d = h * HO + c * 32;
 #pragma unroll

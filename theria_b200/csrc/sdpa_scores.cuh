@@ -121,6 +121,7 @@ tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUte
 #pragma unroll 1
   for (int c = 0; c < TN / 32; ++c) {
     float v[32];
+    __syncwarp();  // lanes without a row left the last trip early
     if (ok && !skip) {
       tc::tmem_ld32(tmem + lane_off + c * 32, v);  // warp-collective
     } else {

@@ -509,6 +509,7 @@ bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
 #pragma unroll 1
         for (int c = grp * (HD / 64); c < (grp + 1) * (HD / 64); ++c) {
           float v[32];
+          __syncwarp();  // lanes without a row left the last trip early
           if (n_iter > 0) {
             tc::tmem_ld32(col + lane_off + c * 32, v);
           } else {

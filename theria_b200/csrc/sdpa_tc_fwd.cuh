@@ -500,7 +500,8 @@ fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
 #pragma unroll
       for (int c = 0; c < HO / 32; ++c) {
         float v[32];
-        tc::tmem_ld32(t_o + c * 32, v);  // warp-collective: before any branch
+        __syncwarp();                    // lanes without a row left the last trip early
+        tc::tmem_ld32(t_o + c * 32, v);  // warp-collective
         if (!store) continue;
         if (out_f32) {
           float4* dst = reinterpret_cast<float4*>(static_cast<float*>(out) + base + c * 32);

@@ -296,6 +296,7 @@ jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUt
 #pragma unroll 1
       for (int cc = grp * (HD / 64); cc < (grp + 1) * (HD / 64); ++cc) {
         float oa[32], op[32], ot[32];
+        __syncwarp();  // lanes without a row left the last trip early
         tc::tmem_ld32(tmem + C::tOA + lane_off + cc * 32, oa);
         tc::tmem_ld32(tmem + C::tOP + lane_off + cc * 32, op);
         tc::tmem_ld32(tmem + C::tOT + lane_off + cc * 32, ot);
