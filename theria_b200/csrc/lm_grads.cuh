@@ -17,8 +17,11 @@
 // sums to float64, which costs an eighth of the conversions (16 a cycle and SM:
 // at one a value they would bound 16-bit tensors).  A thread that meets very large
 // or very small values does its part of the chunk again in float64, so that norms
-// of such gradients are right.
+// of such gradients are right.  The second launch multiplies in float32, and in
+// float64 where a factor is beyond float32's normal range.
 #pragma once
+
+#include <cfloat>
 
 #include "common.cuh"
 #include "lm_embed.cuh"
@@ -227,6 +230,31 @@ __device__ __forceinline__ void combine(const Table& t, float a, float b) {
     });
 }
 
+// A factor that float32 has no normal number for: with norms near either end of
+// float32's range c, and b more so, lie beyond it while a x + b u does not.
+__device__ __forceinline__ bool beyond(double f) {
+  const double m = fabs(f);
+  return m != 0.0 && (m < (double)FLT_MIN || (m > (double)FLT_MAX && m < INFINITY));
+}
+
+// The same as combine, each value in float64: for factors beyond float32.
+template <bool TWO>
+__device__ __noinline__ void combine_wide(const Table& t, double a, double b) {
+  const int last = t.first[t.n] - 1;
+  for (int c = blockIdx.x; c <= last; c += gridDim.x)
+    chunk_at(t, last - c, [&](auto e, int i, int64_t from, int n) {
+      using T = decltype(e);
+      const T* x = static_cast<const T*>(t.x[i]) + from;
+      const T* u = static_cast<const T*>(TWO ? t.u[i] : t.x[i]) + from;
+      T* out = static_cast<T*>(t.out[i]) + from;
+      for (int k = threadIdx.x; k < n; k += THREADS) {
+        double v = a * (double)to_f32<T>(x[k]);
+        if (TWO) v = fma(b, (double)to_f32<T>(u[k]), v);
+        out[k] = from_f32<T>((float)v);
+      }
+    });
+}
+
 // out = c x (out may be x; t.n == 0: the norm alone).  stats receives {norm, c}.
 __global__ void __launch_bounds__(THREADS, 4)
 clip_kernel(const __grid_constant__ Table t, const double* part, int parts, double most,
@@ -243,7 +271,8 @@ clip_kernel(const __grid_constant__ Table t, const double* part, int parts, doub
   }
   if (t.n == 0) return;
   if (c == 1.0 && t.in_place) return;  // in place, nothing to clip
-  combine<false>(t, (float)c, 0.f);
+  if (beyond(c)) combine_wide<false>(t, c, 0.0);
+  else combine<false>(t, (float)c, 0.f);
 }
 
 // out = a u + b x (see above); u NULL: out = b x.  part: the sums of x u.
@@ -260,7 +289,10 @@ clip_bwd_kernel(const __grid_constant__ Table t, const double* part, int parts,
     if (c != 1.0) b -= c * xu / n / n;
   }
   // with u, the table has it first: combine's x is u, its u is x
-  combine<TWO>(t, TWO ? (float)c : (float)b, (float)b);
+  const double a = TWO ? c : b;
+  // (|b x| <= |b| n, which may leave float32's range where the sum does not)
+  if (beyond(a) || beyond(b) || beyond(b * n)) combine_wide<TWO>(t, a, b);
+  else combine<TWO>(t, (float)a, (float)b);
 }
 
 }  // namespace grads
