@@ -654,6 +654,74 @@ def _check_grads(what, tensors):
     return tensors
 
 
+def _reach(dims):
+    """How far behind the first address the last one lies."""
+    return sum(s * (n - 1) for s, n in dims)
+
+
+def _dims(t):
+    """(stride, size) of t's addresses in bytes, its values' own bytes among them."""
+    e = t.element_size()
+    return [(s * e, n) for s, n in zip(t.stride(), t.shape) if n > 1] + [(1, e)]
+
+
+def _folded(t):
+    """Whether two indices of t may be one address (never missed; where strides
+    interleave it may be said of a tensor without any)."""
+    dims = sorted(_dims(t))
+    return any(s <= _reach(dims[:i]) for i, (s, _) in enumerate(dims))
+
+
+def _chains(sets):
+    """The sets (address, dims) in runs whose ranges of addresses meet."""
+    runs, end = [], None
+    for one in sorted(sets, key=lambda s: s[0]):
+        if end is None or one[0] > end:
+            runs.append([])
+            end = one[0]
+        runs[-1].append(one)
+        end = max(end, one[0] + _reach(one[1]))
+    return runs
+
+
+def _apart(sets):
+    """Whether no two of the sets of addresses have one in common (never said where two
+    do).  Written as m Q + R with R < m, for m one of the strides, two addresses differ
+    where their Q or their R do: so slices of the same rows, of every second row, of
+    single heads are found to be apart."""
+    return all(len(run) == 1 or _run_apart(run) for run in _chains(sets))
+
+
+def _run_apart(run):
+    for m in sorted({s for _, dims in run for s, _ in dims if s > 1}, reverse=True):
+        parts = []  # (R's first, R's dims, Q's set)
+        for a, dims in run:
+            a -= run[0][0]
+            rest = [d for d in dims if d[0] % m]
+            if a % m + _reach(rest) >= m:
+                break
+            parts.append((a % m, rest, (a // m, [(s // m, n) for s, n in dims if s % m == 0])))
+        else:
+            if all(len(r) == 1 or _apart([p[2] for p in r]) or _apart([p[:2] for p in r])
+                   for r in _chains(parts)):
+                return True
+    return len(run) > 2 and all(_apart([x, y]) for i, x in enumerate(run) for y in run[:i])
+
+
+def _overlap(tensors):
+    """Whether two of the tensors may share an address."""
+    some = [t for t in tensors if t.numel()]
+    spans = []
+    for t in some:
+        at = t.data_ptr()
+        spans.append((at, at + (t.nbytes if t.is_contiguous() else _reach(_dims(t)) + 1)))
+    spans.sort()
+    # (most calls end here: no two ranges meet)
+    return (any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+            and not _apart([(t.data_ptr(), [(1, t.nbytes)] if t.is_contiguous() else _dims(t))
+                            for t in some]))
+
+
 def _check_max(max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0:
@@ -690,8 +758,10 @@ def clip_gradients(tensors, max_norm):
 
 @_opaque
 def clip_gradients_(tensors, max_norm):
-    """clip_gradients in place; returns the norm.  No two tensors may overlap, and
-    none may need a gradient (under ``torch.no_grad()`` they may)."""
+    """clip_gradients in place; returns the norm.  No two tensors may overlap, none
+    itself, and none may need a gradient (under ``torch.no_grad()`` they may).  Views of
+    one tensor that share no value (columns, heads, every second row) are taken; such
+    whose strides do not show it are refused."""
     what = "theria clip_gradients_"
     tensors = _check_grads(what, tensors)
     max_norm = _check_max(max_norm)
@@ -701,9 +771,9 @@ def clip_gradients_(tensors, max_norm):
     for t, c in zip(tensors, x):
         if t is not c and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
             raise AssertionError(f"{what} changes its tensors: none may be an expanded view")
-    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                   for t in x if t.numel())
-    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        if t is not c and _folded(t):
+            raise AssertionError(f"{what} changes its tensors: none may overlap itself")
+    if _overlap(tensors):
         raise AssertionError(f"{what} changes its tensors: no two may overlap")
     norm, _ = _clip(x, x, max_norm)
     for t, c in zip(tensors, x):
