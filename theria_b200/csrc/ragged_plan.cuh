@@ -45,6 +45,17 @@ struct Blank {
   int64_t row_bytes[3];  // any number
 };
 
+// The exponent of the largest size in a row of float16 cotangents as a byte that grows
+// with it: 0 for none but zeros, else 26 and more.  (2^-24 is float16's smallest number;
+// what is not finite counts as its largest.)
+__device__ __forceinline__ uint8_t fit_code(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23) - 127;
+  return most == 0.f ? 0 : (uint8_t)(min(e, 15) + 50);
+}
+// The power of two that brings that size to 2 .. 4; 1 for zeros.
+__device__ __forceinline__ int fit_power(unsigned code) { return code == 0 ? 0 : 51 - (int)code; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 constexpr int kPlanThreads = 1024;
 constexpr int kBuckets = 1024;   // of 128 keys: 131072 keys and more share one
 

@@ -31,6 +31,17 @@
 //   still made.  The two sums take 256 columns at HD = 128, which leaves no room for
 //   more.  (128 rows, one buffer: 549 us; s early, p and ds over dp: 710 and 774.)
 //
+// float16 (not bfloat16) has a short range: ds as it is would pass its largest number,
+// or lose bits below its smallest normal one, with cotangents that are not of order 1
+// (4096 keys, cotangents of 1e-3: dq off by 5 times its final rounding, so by 1.2).  So
+// ds is made of cotangents whose largest value a power of two brings to 2 .. 4, which
+// the results are divided by: for dq each row's own, added to its term in the exponent;
+// for dk and dv, whose sums run over rows, one for all rows that a CTA walks, taken
+// into (dp - z) by the multiplication-and-addition that makes it.  Neither costs an
+// instruction of the loop (2 x 4096 tokens, 16 / 4 heads of 128: row terms 21.5 -> 23 us,
+// dq 175 -> 175, dk, dv 246 -> 247 causal, 480 -> 492 not).  Large values of v can
+// still take ds past float16's range: |dp - z| is at most 8 D max|v| with such cotangents.
+//
 // Rows behind the sequence's end in a tile of y belong to others and may be
 // anything; p = 0 and ds = 0 would multiply them, so the producer warp sets them
 // to zero.
@@ -93,8 +104,8 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(DqCfg<HD>::kThreads, 1)
 tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
              const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-             const float2* terms, T* __restrict__ dq, const int4* items, const int* count,
-             const Problem pr) {
+             const float2* terms, const uint8_t* fit, T* __restrict__ dq, const int4* items,
+             const int* count, const Problem pr) {
   using L = DqCfg<HD>;
   constexpr int R1 = L::R1, R2 = L::R2;
   extern __shared__ uint8_t smem_raw[];
@@ -268,7 +279,14 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
     const int tok = first + r / G;
     const bool live = tok < len && r < xt * G;
     const int64_t row = (int64_t)(start + tok) * pr.H + hk * G + r % G;
-    const float2 mine = live ? terms[row] : make_float2(-INFINITY, 0.f);  // {-lse log2 e, -z}
+    float2 mine = live ? terms[row] : make_float2(-INFINITY, 0.f);  // {-lse log2 e, -z}
+    float mul = pr.scale;
+    if constexpr (std::is_same<T, __half>::value)
+      if (live) {  // ds of the row times 2^e
+        const int e = fit_power(fit[((int64_t)hk * pr.T + start + tok) * G + r % G]);
+        mine.x += (float)e;
+        mul *= pow2(-e);
+      }
     const int warp_tok = first + quarter * 32 / G;  // the first token of the warp
     const int my_keys = CAUSAL ? min(len, tok + 1) : len;
     bool ok = true;
@@ -329,7 +347,7 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
       if (cg < HD / 32) {
         float v[32];
         tc::tmem_ld32(t_a + lane_off + cg * 32, v);
-        if (live) put_sums<T>(v, pr.scale, dq + row * pr.D, cg * 32, pr.D);
+        if (live) put_sums<T>(v, mul, dq + row * pr.D, cg * 32, pr.D);
       }
     }
   }
@@ -359,7 +377,9 @@ struct DkvCfg {
   static constexpr int nBar = 7 + 12 + 2 * YST;
   static constexpr int oTmem = oBar + nBar * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int kAlloc = oAbort + 4 + 1024;
+  static constexpr int oFit = oAbort + 4;  // float16: each warp's largest fit_code
+  static constexpr int kAlloc = oFit + 4 * (kThreads / 32) + 1024;
+  static_assert(kAlloc <= 232448, "shared memory of a block");
 };
 
 // One split of a tile's queries.  part: NULL where there is one split (results rounded
@@ -368,8 +388,8 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(DkvCfg<HD>::kThreads, 1)
 tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
               const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-              const float2* terms, T* __restrict__ dk, T* __restrict__ dv, float* part,
-              const int4* items, const int* count, int splits, const Problem pr) {
+              const float2* terms, const uint8_t* fit, T* __restrict__ dk, T* __restrict__ dv,
+              float* part, const int4* items, const int* count, int splits, const Problem pr) {
   using L = DkvCfg<HD>;
   constexpr int YST = L::YST;
   constexpr bool kXT = HD == 64;  // k and v in TMEM too, as the A operands of s and dp
@@ -425,9 +445,41 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
   if (y_rows < KY)  // rows that no copy fills
     for (int s = warp; s < 2 * YST; s += L::kThreads / 32)
       zero_rows(smem + L::oY1 + s * L::kY, KY, HD / 64, y_rows, KY, lane);
+  constexpr bool kFit = std::is_same<T, __half>::value;
+  uint32_t* fits = reinterpret_cast<uint32_t*>(smem + L::oFit);
+  if constexpr (kFit) {  // the largest cotangent of the rows to walk: whole vectors, and ends
+    const uint8_t* from = fit + ((int64_t)hk * pr.T + start + tok_of(0)) * G;
+    const uint8_t* to = fit + ((int64_t)hk * pr.T + start + min(tok_of(n_iter), len)) * G;
+    auto up16 = [](const uint8_t* p) { return (reinterpret_cast<uintptr_t>(p) + 15) / 16; };
+    uint32_t most = 0;
+    const uint4* a = reinterpret_cast<const uint4*>(up16(from) * 16);
+    const uint4* b = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(to) / 16 * 16);
+    if (a < b) {
+      for (const uint4* p = a + threadIdx.x; p < b; p += L::kThreads) {
+        const uint4 w = *p;
+        most = __vmaxu4(most, __vmaxu4(__vmaxu4(w.x, w.y), __vmaxu4(w.z, w.w)));
+      }
+      most = __vmaxu4(most, most >> 16);
+      most = max(most & 255, most >> 8 & 255);
+      const uint8_t* head = from + threadIdx.x;
+      const uint8_t* tail = reinterpret_cast<const uint8_t*>(b) + threadIdx.x;
+      if (head < reinterpret_cast<const uint8_t*>(a)) most = max(most, (uint32_t)*head);
+      if (tail < to) most = max(most, (uint32_t)*tail);
+    } else {  // fewer than 32
+      const uint8_t* p = from + threadIdx.x;
+      if (p < to) most = *p;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) fits[warp] = most;
+  }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
+  // ds is made times 2^fitted()
+  auto fitted = [&] {
+    return fit_power(__reduce_max_sync(0xffffffffu, lane < L::kThreads / 32 ? fits[lane] : 0u));
+  };
+  const float up = kFit ? pow2(fitted()) : 1.f;
   // TMEM: buffer b of s [128 b, +64), of dp [128 b + 64, +64); the sums from 256 on;
   // HD = 64: k and v from 384 on
   const uint32_t tmem = *tmem_slot;
@@ -479,8 +531,8 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         float* rt = reinterpret_cast<float*>(smem + L::oTerm + st * KY * 8);
         rt[lane] = rv[0].x;
         rt[32 + lane] = rv[1].x;
-        rt[KY + lane] = rv[0].y;
-        rt[KY + 32 + lane] = rv[1].y;
+        rt[KY + lane] = rv[0].y * up;
+        rt[KY + 32 + lane] = rv[1].y * up;
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(y_full + st);
         if (t + 1 < n_iter) load_terms(t + 1);
@@ -646,7 +698,8 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
         for (int e = 0; e < 32; e += 2) {
           const float2 nz = ld_shared_f2(z_at + e * 4);
           float g0, g1;
-          tc::add2(g0, g1, dp[e], dp[e + 1], nz.x, nz.y);
+          if constexpr (kFit) tc::fma2(g0, g1, dp[e], dp[e + 1], up, up, nz.x, nz.y);
+          else tc::add2(g0, g1, dp[e], dp[e + 1], nz.x, nz.y);
           tc::mul2(g0, g1, s[e], s[e + 1], g0, g1);
           if constexpr (decltype(mk)::value) {
             g0 = e >= lo ? g0 : 0.f;
@@ -666,11 +719,13 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
       if (ok) tc::tc_fence_after();
     }
     if (ok) {
+      float dk_mul = pr.scale;
+      if constexpr (kFit) dk_mul *= pow2(-fitted());
       const int64_t row = (int64_t)(start + tok) * pr.Hkv + hk;
       const int64_t plane = (int64_t)pr.T * pr.Hkv * pr.D;
 #pragma unroll 1
       for (int which = 0; which < 2; ++which) {
-        const float mul = which == 0 ? pr.scale : 1.f;
+        const float mul = which == 0 ? dk_mul : 1.f;
         float* sums = part == nullptr ? nullptr
                                       : part + (2 * sp + which) * plane + row * pr.D;
 #pragma unroll 1

@@ -182,6 +182,7 @@ FwdWs fwd_ws(void* base, const Problem& p) {
 struct BwdWs {
   List lq, lk;
   float2* terms;
+  uint8_t* fit;  // [Hkv, T, G], float16 on the tensor cores
   float* part;  // room for the larger tiles' splits
   int64_t bytes;
 };
@@ -191,6 +192,7 @@ BwdWs bwd_ws(void* base, const Problem& p) {
   w.lq = take_list(c, p, p.G, SR, 0);
   w.lk = take_list(c, p, 1, SR, 1);
   w.terms = c.take<float2>((int64_t)p.T * p.H);
+  w.fit = c.take<uint8_t>((int64_t)p.T * p.H);
   const int ks = std::max(tc_splits(p), simt_splits(p)), qs = simt_q_splits(p);
   const int64_t k_row = 2ll * p.Hkv * p.D, q_row = (int64_t)p.H * p.D;
   const int64_t part = std::max(ks > 1 ? ks * k_row : 0, qs > 1 ? qs * q_row : 0) * p.T;
@@ -342,7 +344,8 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
       return THERIA_ERR_UNSUPPORTED;
     if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
     if (int e = launch_chained(kern, dim3(blocks(p, ws.lq.per, ws.lq.step)), dim3(Cfg::kThreads),
-                               Cfg::kAlloc, st, mq, mo, mk, mv, (const float2*)ws.terms, (T*)dq,
+                               Cfg::kAlloc, st, mq, mo, mk, mv, (const float2*)ws.terms,
+                               (const uint8_t*)ws.fit, (T*)dq,
                                (const int4*)ws.lq.items, (const int*)ws.lq.count, p))
       return e;
   }
@@ -357,7 +360,7 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
   const int splits = tc_splits(p);
   if (int e = launch_chained(kern, dim3(blocks(p, ws.lk.per, ws.lk.step) * (unsigned)splits),
                              dim3(Cfg::kThreads), Cfg::kAlloc, st, mk, mv, mq, mo,
-                             (const float2*)ws.terms, (T*)dk, (T*)dv,
+                             (const float2*)ws.terms, (const uint8_t*)ws.fit, (T*)dk, (T*)dv,
                              splits > 1 ? ws.part : nullptr, (const int4*)ws.lk.items,
                              (const int*)ws.lk.count, splits, p))
     return e;
@@ -376,8 +379,8 @@ int by_tile(const Problem& p, F f) {
 }
 
 template <typename T>
-int run_terms(const void* o, const void* rest, const void* dout, const float* lse, const BwdWs& ws, const Problem& p,
-              cudaStream_t st) {
+int run_terms(const void* o, const void* rest, const void* dout, const float* lse,
+              const BwdWs& ws, bool on_tc, const Problem& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.T * p.H;
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = p.D % VEC == 0 && tc::aligned16(o) && tc::aligned16(rest) && tc::aligned16(dout);
@@ -385,7 +388,8 @@ int run_terms(const void* o, const void* rest, const void* dout, const float* ls
   auto run = [&](auto kern, int lanes) {
     const int64_t need = cdiv(rows, 256 / lanes);
     return launch_chained(kern, dim3((unsigned)std::min<int64_t>(need, kSMs * 32)), dim3(256), 0,
-                          st, (const T*)o, (const T*)rest, (const T*)dout, lse, ws.terms, rows, p.D);
+                          st, (const T*)o, (const T*)rest, (const T*)dout, lse, ws.terms,
+                          on_tc ? ws.fit : (uint8_t*)nullptr, rows, p);
   };
   if (!vec) return run(terms_kernel<T, 1, 32>, 32);
   if (units <= 4) return run(terms_kernel<T, VEC, 4>, 4);
@@ -478,7 +482,7 @@ int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t
     return e;
   return by_type(dtype, [&](auto t) -> int {
     using E = decltype(t);
-    if (int e = run_terms<E>(o, o_rest, dout, lse, ws, p, st)) return e;
+    if (int e = run_terms<E>(o, o_rest, dout, lse, ws, on_tc, p, st)) return e;
     if constexpr (!std::is_same<E, float>::value)
       if (on_tc)
         return by_tile(p, [&](auto hd, auto causal_) {
