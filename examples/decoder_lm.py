@@ -150,7 +150,8 @@ def train(steps=50, dtype=torch.float32, vocab=32, d=64, heads=4, layers=2, seq_
     torch.manual_seed(seed)
     g = torch.Generator("cuda").manual_seed(seed)
     if packed:
-        model = PackedDecoderLM(vocab, d, heads, max(1, heads // 2), layers).to("cuda", dtype)
+        kv_heads = heads // 2 if heads % 2 == 0 else 1  # a divisor of the heads
+        model = PackedDecoderLM(vocab, d, heads, kv_heads, layers).to("cuda", dtype)
     else:
         model = DecoderLM(vocab, d, heads, layers, seq_len).to("cuda", dtype)
     table = torch.randperm(vocab - 1, generator=g, device="cuda")
