@@ -115,7 +115,7 @@ class PackedDecoderLM(nn.Module):
 
     def forward(self, ids, target, offsets):
         """Mean loss of the targets [T]; those that are lm.IGNORE_INDEX are not scored."""
-        if self.frequencies is None:
+        if self.frequencies is None or self.frequencies.device != ids.device:
             self.frequencies = lm.rotary_frequencies(2 * self.pairs, device=ids.device)
         x = lm.embedding(ids, self.tok, scale=self.scale)
         for block in self.blocks:

@@ -1,4 +1,5 @@
-"""examples/decoder_lm.py --packed with any number of heads."""
+"""examples/decoder_lm.py --packed with any number of heads, and a model that changes
+its device between calls."""
 
 import importlib.util
 import pathlib
@@ -9,6 +10,8 @@ import torch
 pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():
     pytest.skip("CUDA not available", allow_module_level=True)
+
+from theria_b200 import lm  # noqa: E402
 
 _path = pathlib.Path(__file__).resolve().parents[1] / "examples" / "decoder_lm.py"
 _spec = importlib.util.spec_from_file_location("decoder_lm", _path)
@@ -22,3 +25,13 @@ def test_heads(heads, d):
                                      packed=True)
     assert all(loss == loss and abs(loss) < 100 for loss in losses)
     assert heads % model.blocks[0].kv_heads == 0
+
+
+def test_frequencies_follow_the_ids():
+    model = decoder_lm.PackedDecoderLM(32, 64, 4, 2, 1).cuda()
+    ids = torch.arange(1, 31, device="cuda")
+    offsets = torch.tensor([0, 13, 30], device="cuda")
+    want = model(ids, ids, offsets)
+    model.frequencies = lm.rotary_frequencies(2 * model.pairs, device="cpu")
+    assert torch.equal(model(ids, ids, offsets), want)
+    assert model.frequencies.device == ids.device
