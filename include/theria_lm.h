@@ -138,7 +138,7 @@ int theria_grads_dot(const void* const* x, const void* const* u, const int64_t* 
 /* From the sums of x * x: norm [1] = their root (may be NULL), y = c x with c =
  * min(1, max_norm / norm), stats [2] = {norm, c} (NULL: not wanted; norm or
  * stats is).  y NULL: the norm alone.  y may be x.  With a norm that is NaN every
- * y is NaN; with an infinite one c is 0. */
+ * y is NaN; with an infinite one c is 0 (1 where max_norm is infinite too). */
 int theria_grads_clip(const void* const* x, void* const* y, const int64_t* sizes,
                       const int* dtypes, int64_t n, const double* parts, double max_norm,
                       float* norm, double* stats, void* stream);

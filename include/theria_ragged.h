@@ -18,14 +18,22 @@
  * sequence: their o and gradients are zero (lse: not written), and nothing
  * that they, or another sequence, hold reaches a result.
  *
- * Offsets that decrease or leave 0 .. T cannot be refused by the host: every
+ * (T > 0:) offsets that decrease or leave 0 .. T cannot be refused by the host: every
  * result is then zero, and THERIA_ERR_INVALID_ARG is left in the device error
  * word (theria_get_device_error).
  *
- * Softmax statistics and sums are float32, results are rounded once, and no
+ * Softmax statistics and sums are float32, and results are rounded once.  In
+ * float16 and bfloat16 the probabilities p (forward and backward) and ds = p
+ * (dp - z) (backward) are besides rounded to that type, as operands of the tensor
+ * cores: o is off by 1.2 to 1.3 times its final rounding, dq, dk, dv by 1.4.
+ * float16's short range: p loses bits below 2^-14; ds is made of cotangents
+ * brought to order 1 by powers of two, so their size does not matter (that of v
+ * does: do . v of cotangents of order 1 has to stay within float16).  float32 uses
+ * the hardware's approximate 2^x, and float32 throughout.  No
  * result depends on the order in which thread blocks run.  Stream-ordered, no
  * allocation, no host synchronisation; each call returns a THERIA_* status.
  * scale > 0.  D <= THERIA_MAX_HEAD_DIM; T, S < 2^30, T * H < 2^31, H and Hkv < 65536.
+ * With T == 0 nothing is launched, and the offsets are not looked at.
  *
  * The reference library has no such operator: its attention takes one head
  * count and one length (theria/attention/triton_qk.py:307-369).
@@ -52,10 +60,10 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
 int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64_t Hkv,
                                           int64_t D);
 int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, const void* o, const void* o_rest, const void* dout,
-                      const float* lse, void* dq, void* dk, void* dv, void* workspace,
-                      int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
-                      int64_t D, int dtype, float scale, int causal, void* stream);
+                      const void* offsets, int wide, const void* o, const void* o_rest,
+                      const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                      void* workspace, int64_t workspace_bytes, int64_t T, int64_t S, int64_t H,
+                      int64_t Hkv, int64_t D, int dtype, float scale, int causal, void* stream);
 
 #ifdef __cplusplus
 }

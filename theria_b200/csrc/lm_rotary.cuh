@@ -8,12 +8,13 @@
 // cos and sin go to shared memory first.  The angle is reduced in float64: t *
 // w in float32 would be off by t * w * 2^-24, 0.06 at position 10^6.  As whole
 // turns less their nearest integer it is exact to 2^-52 t w / 2 pi turns, and the
-// remaining half turn at most is float32's to compute (sincospi, 1 to 2 units).
+// remaining half turn at most is float32's to compute (sincospi, 1 to 2 units), as are
+// the products with the amplitude and the pair.
 //
 // A thread stays on one column of 16 bytes of the heads and has the loads of four
-// rows (token, head) in flight.  With the halves apart it moves 16 bytes of each half where a half is a whole number
-// of such vectors, else 16 bytes of the output whose partners it reads one by one
-// (from the cache: a neighbour has just loaded them).
+// rows (token, head) in flight.  With the halves apart it moves 16 bytes of each half
+// where a half is a whole number of such vectors, else 16 bytes of the output whose
+// partners it reads one by one (from the cache: a neighbour has just loaded them).
 #pragma once
 
 #include "common.cuh"

@@ -38,9 +38,11 @@ constexpr int FWD_THREADS = FR * 4, BWD_THREADS = SR * 4;  // ... of a group
 template <int DT>
 struct SimtSmem {
   static constexpr int kRow = DT + 4;            // floats of an operand's row
-  // groups of a forward, of a backward block; narrow heads, of short sequences for the
-  // most part, take one (25 sequences of 64, 4 heads of 16: forward 5.7 us, with four
-  // groups 9.2)
+  // groups of a forward, of a backward block; narrow heads take one, whose tiles are done
+  // sooner where sequences are short or many, later where they are few and long (4 heads
+  // of 16; forward, dq, dk and dv, us, with one group and with four and two: 25 x 64: 6, 8,
+  // 8 and 9, 13, 12; 200 x 64: 17, 21, 29 and 49, 34, 37; 8192: 388, 933, 854 and 397, 736,
+  // 965; 2 x 2048: 81, 239, 196 and 67, 107, 140.  The kernels do not know the lengths.)
   static constexpr int FG = DT <= 32 ? 1 : 4, SG = DT <= 32 ? 1 : 2;
   // a group's k, v (wide heads: tiles of half the columns), scores; a block's q
   static constexpr int kFC = DT <= 64 ? FC : FC / 2;
@@ -60,7 +62,9 @@ __device__ __forceinline__ void async16(float* dst, const float* src, bool on) {
                "r"(on ? 16 : 0)
                : "memory");
 }
-__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
 // All but the newest `left` groups have landed (for this thread's copies).
 template <int left>
 __device__ __forceinline__ void async_wait() {

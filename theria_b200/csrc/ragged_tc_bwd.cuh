@@ -179,7 +179,8 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
     // are masked)
     auto fetch = [&](int t, int which) {
       const int R = which ? R2 : R1, st = t % R;
-      uint64_t *full = (which ? y2_full : y1_full) + st, *empty = (which ? y2_empty : y1_empty) + st;
+      uint64_t* full = (which ? y2_full : y1_full) + st;
+      uint64_t* empty = (which ? y2_empty : y1_empty) + st;
       uint8_t* y = smem + (which ? L::oY2 : L::oY1) + st * L::kY;
       const bool ends = (t + 1) * QY > len && which == 0;
       bool ok = true;

@@ -18,6 +18,7 @@
 // O and the sum rescaled only when the maximum grows by more than 2^8.  These
 // choices, and what was measured for them, are the dense forward's
 // (sdpa_tc_fwd.cuh); what differs is where rows and keys come from and end.
+// P is rounded to 16 bits, as the tensor core's operand, after its sum was taken.
 //
 // Keys behind the sequence's end belong to the next one and may be anything.
 // Their scores are masked; their rows of V, which p = 0 would multiply, are set
@@ -98,7 +99,8 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(FwdCfg<HD>::kThreads, 1)
 tc_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, T* __restrict__ out,
-              T* __restrict__ rest, float* __restrict__ lse, const int4* items, const int* count, const Problem pr) {
+              T* __restrict__ rest, float* __restrict__ lse, const int4* items, const int* count,
+              const Problem pr) {
   using L = FwdCfg<HD>;
   constexpr bool kSepP = HD == 64;
   extern __shared__ uint8_t smem_raw[];

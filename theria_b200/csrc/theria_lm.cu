@@ -1052,9 +1052,9 @@ int theria_grads_clip_bwd(const void* const* x, const void* const* u, void* cons
   // the kernel's first operand is what the factor c takes
   return grads_groups(u ? u : x, u ? x : nullptr, dx, sizes, dtypes, n,
                       [&](const grads::Table& t, int chunks) {
-    return launch_chained(u ? grads::clip_bwd_kernel<true> : grads::clip_bwd_kernel<false>, dim3(std::min(chunks, kSMs * 8)),
-                          dim3(grads::THREADS), 0, (cudaStream_t)stream, t, parts, u ? np : 0,
-                          stats, gnorm);
+    return launch_chained(u ? grads::clip_bwd_kernel<true> : grads::clip_bwd_kernel<false>,
+                          dim3(std::min(chunks, kSMs * 8)), dim3(grads::THREADS), 0,
+                          (cudaStream_t)stream, t, parts, u ? np : 0, stats, gnorm);
   });
 }
 

@@ -148,11 +148,12 @@ int run_plan(const void* offsets, int wide, const Problem& p, const List& a, con
 // Parts that the walk of a tile is split into, of `tiles` in an even batch: until they
 // would fill the GPU `waves` times, and no more than 32.
 int parts_of(int64_t tiles, int waves) {
-  return (int)std::min<int64_t>(32, std::max<int64_t>(1, waves * kSMs / std::max<int64_t>(1, tiles)));
+  const int64_t parts = waves * kSMs / std::max<int64_t>(1, tiles);
+  return (int)std::min<int64_t>(32, std::max<int64_t>(1, parts));
 }
 // dk, dv on the tensor cores: two waves (their tiles are few where the keys have few
-// heads).  On the CUDA cores, whose tiles take longer, three, and for dq two (2395
-// tokens, 5 heads of 72 on one: dq 229 us unsplit, the longest tile's own time).
+// heads).  On the CUDA cores, whose tiles take longer, three, for dq too (2395 tokens, 5
+// heads of 72 on one: dq 137 us and 6 to join, unsplit 229, the longest tile's own time).
 int tc_splits(const Problem& p) { return parts_of(cdiv(p.T, BX) * p.Hkv, 2); }
 int simt_splits(const Problem& p) { return parts_of(cdiv(p.T, SR) * p.Hkv, 3); }
 int simt_q_splits(const Problem& p) {
@@ -210,8 +211,8 @@ unsigned blocks(const Problem& p, int per, int step) {
 }
 
 template <typename T>
-int simt_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse, const FwdWs& ws,
-             const Problem& p, cudaStream_t st) {
+int simt_fwd(const void* q, const void* k, const void* v, void* o, void* rest, float* lse,
+             const FwdWs& ws, const Problem& p, cudaStream_t st) {
   return by_width<T>(p.D, whole_rows(THERIA_F32, p, {q, k, v}), [&](auto w, auto async) {
     constexpr int DT = decltype(w)::value;
     auto kern = simt_fwd_kernel<T, DT, decltype(async)::value>;
@@ -219,8 +220,8 @@ int simt_fwd(const void* q, const void* k, const void* v, void* o, void* rest, f
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
         cudaSuccess)
       return (int)THERIA_ERR_LAUNCH;
-    return launch_chained(kern, dim3(blocks(p, p.G, FR)), dim3(SimtSmem<DT>::FG * FWD_THREADS), smem, st, (const T*)q,
-                          (const T*)k, (const T*)v, (T*)o, (T*)rest, lse,
+    return launch_chained(kern, dim3(blocks(p, p.G, FR)), dim3(SimtSmem<DT>::FG * FWD_THREADS),
+                          smem, st, (const T*)q, (const T*)k, (const T*)v, (T*)o, (T*)rest, lse,
                           (const int4*)ws.list.items, (const int*)ws.list.count, p);
   });
 }
@@ -245,8 +246,9 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
           cudaSuccess)
         return (int)THERIA_ERR_LAUNCH;
       return launch_chained(kern, dim3(blocks(p, l.per, SR) * (unsigned)splits),
-                            dim3(SimtSmem<DT>::SG * BWD_THREADS), smem, st, (const T*)q, (const T*)k, (const T*)v, (const T*)dout,
-                            (const float2*)ws.terms, (T*)o1, (T*)o2, part, (const int4*)l.items,
+                            dim3(SimtSmem<DT>::SG * BWD_THREADS), smem, st, (const T*)q,
+                            (const T*)k, (const T*)v, (const T*)dout, (const float2*)ws.terms,
+                            (T*)o1, (T*)o2, part, (const int4*)l.items,
                             (const int*)l.count, splits, p);
     };
     if (dq != nullptr) {
@@ -270,7 +272,10 @@ int simt_bwd(const void* q, const void* k, const void* v, const void* dout, void
 
 // ------------------------------------------------------ tensor-core launches
 // Rows of 16 bytes on 16-byte boundaries, and a group that a tile of 64 rows
-// holds.  (Measured against the CUDA-core kernels: see ragged_tc_bwd.cuh.)
+// holds.  Whatever the size, the CUDA-core kernels take longer (bf16; forward, dq, dk
+// and dv, us, tensor cores first): one token, 8 / 2 heads of 64: 8, 6, 7 against 10, 9, 10;
+// 25 x 64, 4 heads of 16: 8, 6, 16 against 24, 39, 38; 300 x 20, 8 / 2 heads of 64: 32, 25,
+// 67 against 130, 108, 138; 2 x 2048, 16 / 4 heads of 64: 47, 45, 62 against 761, 954, 1749.
 bool use_tc(int dtype, const Problem& p, std::initializer_list<const void*> ptrs) {
   if (dtype == THERIA_F32 || p.G > KY || tc::encode_fn() == nullptr) return false;
   if (!whole_rows(dtype, p, ptrs)) return false;
@@ -340,7 +345,8 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
     auto kern = tc_dq_kernel<T, HD, CAUSAL>;
     if (!row_map(&mq, q, dtype, p, p.q_t, p.q_h, BX / p.G) ||
         !row_map(&mo, dout, dtype, p, o_t, o_h, BX / p.G) ||
-        !key_map(&mk, k, dtype, p, p.k_t, p.k_h, QY) || !key_map(&mv, v, dtype, p, p.v_t, p.v_h, QY))
+        !key_map(&mk, k, dtype, p, p.k_t, p.k_h, QY) ||
+        !key_map(&mv, v, dtype, p, p.v_t, p.v_h, QY))
       return THERIA_ERR_UNSUPPORTED;
     if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
     if (int e = launch_chained(kern, dim3(blocks(p, ws.lq.per, ws.lq.step)), dim3(Cfg::kThreads),
@@ -437,8 +443,8 @@ int theria_ragged_fwd(const void* q, const void* k, const void* v, const int64_t
     if constexpr (!std::is_same<E, float>::value)
       if (on_tc)
         return by_tile(p, [&](auto hd, auto causal_) {
-          return tc_fwd<E, decltype(hd)::value, decltype(causal_)::value>(q, k, v, o, o_rest, lse, ws,
-                                                                          dtype, p, st);
+          return tc_fwd<E, decltype(hd)::value, decltype(causal_)::value>(
+              q, k, v, o, o_rest, lse, ws, dtype, p, st);
         });
     return simt_fwd<E>(q, k, v, o, o_rest, lse, ws, p, st);
   });
@@ -452,10 +458,10 @@ int64_t theria_ragged_bwd_workspace_bytes(int64_t T, int64_t S, int64_t H, int64
 }
 
 int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
-                      const void* offsets, int wide, const void* o, const void* o_rest, const void* dout,
-                      const float* lse, void* dq, void* dk, void* dv, void* workspace,
-                      int64_t workspace_bytes, int64_t T, int64_t S, int64_t H, int64_t Hkv,
-                      int64_t D, int dtype, float scale, int causal, void* stream) {
+                      const void* offsets, int wide, const void* o, const void* o_rest,
+                      const void* dout, const float* lse, void* dq, void* dk, void* dv,
+                      void* workspace, int64_t workspace_bytes, int64_t T, int64_t S, int64_t H,
+                      int64_t Hkv, int64_t D, int dtype, float scale, int causal, void* stream) {
   const Problem p = problem(strides, T, S, H, Hkv, D, scale, causal);
   if (int e = check(p, T, S, H, Hkv, D, dtype)) return e;
   if ((dk == nullptr) != (dv == nullptr)) return THERIA_ERR_INVALID_ARG;

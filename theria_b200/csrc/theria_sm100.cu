@@ -2,8 +2,9 @@
 //
 // The library is three translation units without relocatable device code: the
 // language-model operators of include/theria_lm.h are in theria_lm.cu, the
-// attention of include/theria_ragged.h in theria_ragged.cu, and this file includes the kernel headers and implements argument checking,
-// workspace carving and kernel selection for each entry point.
+// attention of include/theria_ragged.h in theria_ragged.cu, and this file
+// includes the kernel headers and implements argument checking, workspace
+// carving and kernel selection for each entry point.
 #include <algorithm>
 #include <cstdio>
 #include <cstring>

@@ -514,7 +514,8 @@ def rotary(q, k, frequencies, positions=None, offsets=None, interleaved=False, a
     ``position * frequencies[m]`` and is multiplied by ``amplitude``; the values
     behind pass through.  Pairs are (m, m + len(frequencies)), or with
     ``interleaved`` (2 m, 2 m + 1).  ``frequencies`` is float64 (see
-    ``rotary_frequencies``); angles are reduced in float64, so positions may be far.
+    ``rotary_frequencies``); angles are reduced in float64, so positions may be far,
+    and their cosines, sines and products are float32.
 
     Positions: ``positions`` (int64 or int32) [T] or [B, T]; or ``offsets`` [S + 1]
     of packed sequences, each counted from its first token (tokens of no sequence
@@ -745,7 +746,7 @@ def clip_gradients(tensors, max_norm):
     """``([t * c for t in tensors], norm)`` with ``norm = gradient_norm(tensors)`` and
     ``c = min(1, max_norm / norm)``; differentiable once, so that clipped steps can be
     part of an adapted model.  A norm that is NaN makes every value NaN, an
-    infinite one makes c 0."""
+    infinite one makes c 0 (1 where max_norm is infinite too)."""
     what = "theria clip_gradients"
     x = [t.contiguous() for t in _check_grads(what, tensors)]
     max_norm = _check_max(max_norm)

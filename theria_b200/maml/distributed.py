@@ -43,7 +43,8 @@ class MetaStep:
 
     ``max_norm`` clips the whole meta-gradient by its norm before Adam, after the
     exchange (``lm.clip_gradients_``: CUDA parameters); ``grad_norm`` then holds
-    the norm of the last step's gradient.
+    the norm of the last step's gradient.  The inner steps are not clipped here
+    (``inner_adapt`` and ``meta_loss_on_tasks`` clip theirs).
     """
 
     def __init__(self, model, *, meta_batch=32, inner_lr=0.4, inner_steps=5, fo=False,
