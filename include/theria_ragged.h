@@ -26,10 +26,9 @@
  * float16 and bfloat16 the probabilities p (forward and backward) and ds = p
  * (dp - z) (backward) are besides rounded to that type, as operands of the tensor
  * cores: o is off by 1.2 to 1.3 times its final rounding, dq, dk, dv by 1.4.
- * float16's short range: p loses bits below 2^-14; ds is made of cotangents
- * brought to order 1 by powers of two, so their size does not matter (that of v
- * does: do . v of cotangents of order 1 has to stay within float16).  float32 uses
- * the hardware's approximate 2^x, and float32 throughout.  No
+ * float16's short range: p loses bits below 2^-14; ds is made times a power of two
+ * by the norms of dout's and v's rows, so that their sizes do not matter.  float32
+ * uses the hardware's approximate 2^x, and float32 throughout.  No
  * result depends on the order in which thread blocks run.  Stream-ordered, no
  * allocation, no host synchronisation; each call returns a THERIA_* status.
  * scale > 0.  D <= THERIA_MAX_HEAD_DIM; T, S < 2^30, T * H < 2^31, H and Hkv < 65536.

@@ -113,3 +113,46 @@ def test_cotangents_of_zero():
     assert not any(g[:300].any() for g in got) and not got[0][:, 1].any()
     for g, w in zip(got, want):
         assert _off(g, w) <= 2 * U
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,std,std_v", [(64, 1e-2, 3e3), (40, 0.5, 1e4), (512, 1e-3, 5e3),
+                                         (4096, 1.0, 1e-3), (4096, 1e2, 1e-4), (300, 1.0, 300.0)])
+def test_sizes_of_values(n, std, std_v, causal, D):
+    lengths, H, Hkv = [n, n // 3], 4, 2
+    small = std * std_v < 1
+    for which, (std_q, std_k) in enumerate(((1 / 16, 16.0), (16.0, 1 / 16))):
+        if not small:
+            std_q = std_k = 1.0
+        q, k, v, do = _inputs(sum(lengths), H, Hkv, D, std_q, std_k)
+        do, v = ((t.float() * s).clamp(-60000, 60000).half() for t, s in ((do, std), (v, std_v)))
+        want, _ = _plain(q, k, v, do, lengths, causal)
+        assert want[which].abs().max().item() < 65504
+        got = _grads(q, k, v, do, lengths, causal)
+        assert _off(got[which], want[which]) <= 2 * U
+
+
+@pytest.mark.parametrize("H,Hkv,D", [(4, 2, 64), (4, 4, 128)])
+def test_a_single_large_row(H, Hkv, D):
+    # the tokens behind it do not see it, though they share its tile of keys
+    for what in ("cotangent", "value"):
+        q, k, v, do = _inputs(3000, H, Hkv, D, 1.0, 1.0)
+        if what == "cotangent":
+            do[10] *= 1000
+        else:
+            v[10] *= 1000
+        do = (do * 4).half()
+        want, _ = _plain(q, k, v, do, [3000], True)
+        got = _grads(q, k, v, do, [3000], True)
+        for g, w in zip(got[:2], want[:2]):
+            assert _off(g, w) <= 2 * U
+        if what == "cotangent":
+            assert _off(got[1][11:], want[1][11:]) <= 2 * U
+
+
+def test_values_of_zero():
+    q, k, v, do = _inputs(200, 4, 2, 64, 1.0, 1.0)
+    got = _grads(q, k, torch.zeros_like(v), do.half(), [200], True)
+    want, _ = _plain(q, k, torch.zeros_like(v), do.half(), [200], True)
+    assert not got[0].any() and not got[1].any() and _off(got[2], want[2]) <= 2 * U

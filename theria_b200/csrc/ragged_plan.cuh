@@ -21,8 +21,25 @@ namespace ragged {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 
+// Division of numbers below 2^31 by a constant, as a product's high half: with 2^(l - 1) <
+// d <= 2^l, m = 2^(31 + l) / d + 1 has m d - 2^(31 + l) in (0, 2^l], so the quotient is exact.
+struct Divisor {
+  uint32_t m;  // 0: by 1
+  int shift;
+  __device__ __forceinline__ unsigned quotient(unsigned n) const {
+    return m ? __umulhi(n, m) >> shift : n;
+  }
+};
+inline Divisor divisor(int d) {
+  if (d <= 1) return Divisor{0, 0};
+  int l = 1;
+  while ((1 << l) < d) ++l;
+  return Divisor{(uint32_t)((1ull << (31 + l)) / (unsigned)d + 1), l - 1};
+}
+
 struct Problem {
   int T, S, H, Hkv, G, D;
+  Divisor by_H, by_Hkv, by_G;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h;  // strides in elements
   float scale, scale_log2;  // the scores' factor; and times log2(e)
   int causal;
@@ -45,16 +62,47 @@ struct Blank {
   int64_t row_bytes[3];  // any number
 };
 
-// The exponent of the largest size in a row of float16 cotangents as a byte that grows
-// with it: 0 for none but zeros, else 26 and more.  (2^-24 is float16's smallest number;
-// what is not finite counts as its largest.)
-__device__ __forceinline__ uint8_t fit_code(float most) {
-  const int e = (int)(__float_as_uint(most) >> 23) - 127;
-  return most == 0.f ? 0 : (uint8_t)(min(e, 15) + 50);
+// A bound on the 2-norm of a row of float16 values, as a byte that grows with it: from the
+// sum of its squares, 0 for zeros, else 50 + e with the norm below 2^(e + 1), e from -24
+// (float16's smallest number) to 19 (128 of its largest, and what is not finite).
+__device__ __forceinline__ uint8_t norm_code(float squares) {
+  const int e = ((int)(__float_as_uint(squares) >> 23 & 255) - 127) >> 1;
+  return squares == 0.f ? 0 : (uint8_t)(min(e, 19) + 50);
 }
-// The power of two that brings that size to 2 .. 4; 1 for zeros.
-__device__ __forceinline__ int fit_power(unsigned code) { return code == 0 ? 0 : 51 - (int)code; }
+// The power of two that ds = p (dp - z) is multiplied by: with cotangents' norms below
+// 2^(e + 1), values' below 2^(f + 1), |dp - z| is below 2^(e + f + 3), so |ds| then
+// below 2^15 (p <= 1).
+__device__ __forceinline__ int fit_power(unsigned cotangents, unsigned values) {
+  return cotangents == 0 || values == 0 ? 0 : 112 - (int)cotangents - (int)values;
+}
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The largest of the bytes [from, to), of those that thread `id` of `threads` (32 and more,
+// which all call it) looks at: whole vectors, and the ends by bytes, none outside.
+__device__ __forceinline__ uint32_t largest_of_mine(const uint8_t* from, const uint8_t* to,
+                                                    unsigned id, unsigned threads) {
+  const uintptr_t first = (reinterpret_cast<uintptr_t>(from) + 15) & ~uintptr_t(15);
+  const uintptr_t last = reinterpret_cast<uintptr_t>(to) & ~uintptr_t(15);
+  uint32_t most = 0;
+  if (first < last) {
+    const uint4* end = reinterpret_cast<const uint4*>(last);
+    for (const uint4* p = reinterpret_cast<const uint4*>(first) + id; p < end;
+         p += threads) {
+      const uint4 w = *p;
+      most = __vmaxu4(most, __vmaxu4(__vmaxu4(w.x, w.y), __vmaxu4(w.z, w.w)));
+    }
+    most = __vmaxu4(most, most >> 16);
+    most = max(most & 255, most >> 8 & 255);
+    const uint8_t* head = from + id;
+    const uint8_t* tail = reinterpret_cast<const uint8_t*>(last) + id;
+    if (head < reinterpret_cast<const uint8_t*>(first)) most = max(most, (uint32_t)*head);
+    if (tail < to) most = max(most, (uint32_t)*tail);
+  } else {  // fewer than 32
+    const uint8_t* p = from + id;
+    if (p < to) most = *p;
+  }
+  return most;
+}
 
 constexpr int kPlanThreads = 1024;
 constexpr int kBuckets = 1024;   // of 128 keys: 131072 keys and more share one

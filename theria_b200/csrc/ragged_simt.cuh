@@ -365,25 +365,28 @@ simt_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 
 // terms[row] = {-lse * log2(e), -rowsum(do * (o + rest))} for every row [T, H], rest
 // (may be NULL) being what o's rounding left: LANES neighbouring lanes a row, each on
-// VEC of its values at a time.  fit (float16, may be NULL): fit_code of the largest size
-// in do's row, rows [Hkv, T, G] here (see ragged_tc_bwd.cuh).  Rows of no
-// sequence get whatever their memory holds: no tile reads them.
+// VEC of its values at a time.  Rows of no sequence get whatever their memory holds: no
+// tile reads them.
+// float16 (fits may be NULL): norm_code of do's rows [Hkv, T, G], and behind them of v's
+// rows [Hkv, T] (see ragged_tc_bwd.cuh).
 template <typename T, int VEC, int LANES>
 __global__ void __launch_bounds__(256)
 terms_kernel(const T* __restrict__ o, const T* __restrict__ rest, const T* __restrict__ dout,
              const float* __restrict__ lse,
-             float2* __restrict__ terms, uint8_t* __restrict__ fit, int64_t rows,
-             const Problem pr) {
+             float2* __restrict__ terms, const T* __restrict__ v, uint8_t* __restrict__ fits,
+             int64_t rows, const Problem pr) {
   const int D = pr.D;
   grid_launch();
   grid_wait();
   const int lane = threadIdx.x % LANES;
-  const int64_t all = (int64_t)gridDim.x * (256 / LANES);
+  const int64_t step = (int64_t)gridDim.x * (256 / LANES);
   const int64_t r0 = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  for (int64_t base = 0; base < rows; base += all) {  // the same trips for every lane
+  constexpr bool kFit = std::is_same<T, __half>::value;
+  const int64_t all = kFit && fits != nullptr ? rows + (int64_t)pr.T * pr.Hkv : rows;
+  for (int64_t base = 0; base < all; base += step) {  // the same trips for every lane
     const int64_t r = base + r0;
-    float z = 0.f, most = 0.f;
-    if (r < rows)
+    float z = 0.f, squares = 0.f;
+    if (r < rows) {
       for (int d = lane * VEC; d < D; d += LANES * VEC) {
         float a[VEC], b[VEC];
         load_vec<T, VEC>(o + r * D + d, a);
@@ -396,21 +399,34 @@ terms_kernel(const T* __restrict__ o, const T* __restrict__ rest, const T* __res
         }
 #pragma unroll
         for (int i = 0; i < VEC; ++i) z = fmaf(a[i], b[i], z);
-        if constexpr (std::is_same<T, __half>::value)
+        if constexpr (kFit)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) most = fmaxf(most, fabsf(b[i]));
+          for (int i = 0; i < VEC; ++i) squares = fmaf(b[i], b[i], squares);
       }
+    } else if (kFit && r < all) {
+      const unsigned vr = (unsigned)(r - rows), t = pr.by_Hkv.quotient(vr), hk = vr - t * pr.Hkv;
+      for (int d = lane * VEC; d < D; d += LANES * VEC) {
+        float b[VEC];
+        load_vec<T, VEC>(v + t * pr.v_t + hk * pr.v_h + d, b);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) squares = fmaf(b[i], b[i], squares);
+      }
+    }
 #pragma unroll
     for (int x = LANES / 2; x > 0; x >>= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
     if (r < rows && lane == 0) terms[r] = make_float2(-lse[r] * kLog2e, -z);
-    if constexpr (std::is_same<T, __half>::value) {
-      if (fit == nullptr) continue;
+    if constexpr (kFit) {
+      if (fits == nullptr) continue;
 #pragma unroll
-      for (int x = LANES / 2; x > 0; x >>= 1)
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
-      if (r < rows && lane == 0) {
-        const unsigned t = (unsigned)r / pr.H, h = (unsigned)r - t * pr.H, hk = h / pr.G;
-        fit[((int64_t)hk * pr.T + t) * pr.G + (h - hk * pr.G)] = fit_code(most);
+      for (int x = LANES / 2; x > 0; x >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, x);
+      if (r >= all || lane != 0) continue;
+      if (r < rows) {
+        const unsigned t = pr.by_H.quotient((unsigned)r), h = (unsigned)r - t * pr.H;
+        const unsigned hk = pr.by_G.quotient(h);
+        fits[((int64_t)hk * pr.T + t) * pr.G + (h - hk * pr.G)] = norm_code(squares);
+      } else {
+        const unsigned vr = (unsigned)(r - rows), t = pr.by_Hkv.quotient(vr);
+        fits[rows + (int64_t)(vr - t * pr.Hkv) * pr.T + t] = norm_code(squares);
       }
     }
   }

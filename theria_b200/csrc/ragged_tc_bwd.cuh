@@ -32,15 +32,15 @@
 //   more.  (128 rows, one buffer: 549 us; s early, p and ds over dp: 710 and 774.)
 //
 // float16 (not bfloat16) has a short range: ds as it is would pass its largest number,
-// or lose bits below its smallest normal one, with cotangents that are not of order 1
-// (4096 keys, cotangents of 1e-3: dq off by 5 times its final rounding, so by 1.2).  So
-// ds is made of cotangents whose largest value a power of two brings to 2 .. 4, which
-// the results are divided by: for dq each row's own, added to its term in the exponent;
-// for dk and dv, whose sums run over rows, one for all rows that a CTA walks, taken
-// into (dp - z) by the multiplication-and-addition that makes it.  Neither costs an
-// instruction of the loop (2 x 4096 tokens, 16 / 4 heads of 128: row terms 21.5 -> 23 us,
-// dq 175 -> 175, dk, dv 246 -> 247 causal, 480 -> 492 not).  Large values of v can
-// still take ds past float16's range: |dp - z| is at most 8 D max|v| with such cotangents.
+// or lose bits below its smallest normal one, with cotangents and values that are not of
+// order 1 (4096 keys, cotangents of 1e-3: dq off by 5 times its final rounding, so by
+// 1.2).  So ds is made times a power of two that takes the largest it can be to 2^15, by
+// the norms of the cotangents and of v, and the results are divided by it: for dq each
+// row's own, added to its term in the exponent; for dk and dv, whose sums run over rows,
+// one for all rows that a CTA walks, taken into (dp - z) by the multiplication-and-
+// addition that makes it.  Neither costs an instruction of the loop (2 x 4096 tokens, 16 / 4
+// heads of 128: row terms 21 -> 28 us, dq 177 -> 181, dk, dv 249 -> 248 causal, 476 -> 497
+// not; of 64: 11.6 -> 16.4, 137 -> 134, 196 -> 199).
 //
 // Rows behind the sequence's end in a tile of y belong to others and may be
 // anything; p = 0 and ds = 0 would multiply them, so the producer warp sets them
@@ -96,7 +96,8 @@ struct DqCfg {
   static constexpr int nBar = 13 + 2 * R1 + 2 * R2;
   static constexpr int oTmem = oBar + nBar * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int kAlloc = oAbort + 4 + 1024;  // slack to align the base to 1024
+  static constexpr int oFit = oAbort + 4;  // float16: each warp's largest norm_code
+  static constexpr int kAlloc = oFit + 4 * (kThreads / 32) + 1024;  // slack to align the base
   static_assert(kAlloc <= 232448, "shared memory of a block");
 };
 
@@ -104,7 +105,7 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(DqCfg<HD>::kThreads, 1)
 tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
              const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-             const float2* terms, const uint8_t* fit, T* __restrict__ dq, const int4* items,
+             const float2* terms, const uint8_t* fits, T* __restrict__ dq, const int4* items,
              const int* count, const Problem pr) {
   using L = DqCfg<HD>;
   constexpr int R1 = L::R1, R2 = L::R2;
@@ -282,12 +283,21 @@ tc_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ C
     const int64_t row = (int64_t)(start + tok) * pr.H + hk * G + r % G;
     float2 mine = live ? terms[row] : make_float2(-INFINITY, 0.f);  // {-lse log2 e, -z}
     float mul = pr.scale;
-    if constexpr (std::is_same<T, __half>::value)
-      if (live) {  // ds of the row times 2^e
-        const int e = fit_power(fit[((int64_t)hk * pr.T + start + tok) * G + r % G]);
-        mine.x += (float)e;
-        mul *= pow2(-e);
-      }
+    if constexpr (std::is_same<T, __half>::value) {  // ds of the row times 2^e
+      // the largest of the values that the tile's rows see
+      uint32_t* largest = reinterpret_cast<uint32_t*>(smem + L::oFit);
+      const uint8_t* values = fits + (int64_t)pr.T * pr.H + (int64_t)hk * pr.T + start;
+      const uint32_t code = live ? fits[((int64_t)hk * pr.T + start + tok) * G + r % G] : 0u;
+      const uint32_t of_mine = __reduce_max_sync(
+          0xffffffffu, largest_of_mine(values, values + keys, threadIdx.x - 32 * L::kCtl,
+                                       32 * L::kWarps));
+      if (lane == 0) largest[warp - L::kCtl] = of_mine;
+      tc::named_bar(1, 32 * L::kWarps);  // (before any wait that may give up)
+      const int e = fit_power(
+          code, __reduce_max_sync(0xffffffffu, lane < L::kWarps ? largest[lane] : 0u));
+      mine.x += (float)e;
+      mul *= pow2(-e);
+    }
     const int warp_tok = first + quarter * 32 / G;  // the first token of the warp
     const int my_keys = CAUSAL ? min(len, tok + 1) : len;
     bool ok = true;
@@ -378,7 +388,7 @@ struct DkvCfg {
   static constexpr int nBar = 7 + 12 + 2 * YST;
   static constexpr int oTmem = oBar + nBar * 8;
   static constexpr int oAbort = oTmem + 4;
-  static constexpr int oFit = oAbort + 4;  // float16: each warp's largest fit_code
+  static constexpr int oFit = oAbort + 4;  // float16: each warp's largest norm_codes
   static constexpr int kAlloc = oFit + 4 * (kThreads / 32) + 1024;
   static_assert(kAlloc <= 232448, "shared memory of a block");
 };
@@ -389,7 +399,7 @@ template <typename T, int HD, bool CAUSAL>
 __global__ void __launch_bounds__(DkvCfg<HD>::kThreads, 1)
 tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
               const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
-              const float2* terms, const uint8_t* fit, T* __restrict__ dk, T* __restrict__ dv,
+              const float2* terms, const uint8_t* fits, T* __restrict__ dk, T* __restrict__ dv,
               float* part, const int4* items, const int* count, int splits, const Problem pr) {
   using L = DkvCfg<HD>;
   constexpr int YST = L::YST;
@@ -447,40 +457,29 @@ tc_dkv_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ 
     for (int s = warp; s < 2 * YST; s += L::kThreads / 32)
       zero_rows(smem + L::oY1 + s * L::kY, KY, HD / 64, y_rows, KY, lane);
   constexpr bool kFit = std::is_same<T, __half>::value;
-  uint32_t* fits = reinterpret_cast<uint32_t*>(smem + L::oFit);
-  if constexpr (kFit) {  // the largest cotangent of the rows to walk: whole vectors, and ends
-    const uint8_t* from = fit + ((int64_t)hk * pr.T + start + tok_of(0)) * G;
-    const uint8_t* to = fit + ((int64_t)hk * pr.T + start + min(tok_of(n_iter), len)) * G;
-    auto up16 = [](const uint8_t* p) { return (reinterpret_cast<uintptr_t>(p) + 15) / 16; };
-    uint32_t most = 0;
-    const uint4* a = reinterpret_cast<const uint4*>(up16(from) * 16);
-    const uint4* b = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(to) / 16 * 16);
-    if (a < b) {
-      for (const uint4* p = a + threadIdx.x; p < b; p += L::kThreads) {
-        const uint4 w = *p;
-        most = __vmaxu4(most, __vmaxu4(__vmaxu4(w.x, w.y), __vmaxu4(w.z, w.w)));
-      }
-      most = __vmaxu4(most, most >> 16);
-      most = max(most & 255, most >> 8 & 255);
-      const uint8_t* head = from + threadIdx.x;
-      const uint8_t* tail = reinterpret_cast<const uint8_t*>(b) + threadIdx.x;
-      if (head < reinterpret_cast<const uint8_t*>(a)) most = max(most, (uint32_t)*head);
-      if (tail < to) most = max(most, (uint32_t)*tail);
-    } else {  // fewer than 32
-      const uint8_t* p = from + threadIdx.x;
-      if (p < to) most = *p;
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) fits[warp] = most;
+  uint32_t* largest = reinterpret_cast<uint32_t*>(smem + L::oFit);
+  if constexpr (kFit) {  // of the rows to walk, and of the values that their z may hold
+    const uint8_t* rows = fits + ((int64_t)hk * pr.T + start) * G;
+    const uint8_t* values = fits + (int64_t)pr.T * pr.H + (int64_t)hk * pr.T + start;
+    const uint32_t a = __reduce_max_sync(
+        0xffffffffu, largest_of_mine(rows + (int64_t)tok_of(0) * G,
+                                     rows + (int64_t)min(tok_of(n_iter), len) * G,
+                                     threadIdx.x, L::kThreads));
+    const uint32_t b = __reduce_max_sync(
+        0xffffffffu, largest_of_mine(values, values + len, threadIdx.x, L::kThreads));
+    if (lane == 0) largest[warp] = a << 8 | b;
   }
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  // ds is made times 2^fitted()
+  // ds is made times 2^fitted() (a whole warp calls it)
   auto fitted = [&] {
-    return fit_power(__reduce_max_sync(0xffffffffu, lane < L::kThreads / 32 ? fits[lane] : 0u));
+    const uint32_t w = lane < L::kThreads / 32 ? largest[lane] : 0u;
+    return fit_power(__reduce_max_sync(0xffffffffu, w >> 8),
+                     __reduce_max_sync(0xffffffffu, w & 255));
   };
-  const float up = kFit ? pow2(fitted()) : 1.f;
+  float up = 1.f;
+  if constexpr (kFit) up = pow2(fitted());
   // TMEM: buffer b of s [128 b, +64), of dp [128 b + 64, +64); the sums from 256 on;
   // HD = 64: k and v from 384 on
   const uint32_t tmem = *tmem_slot;

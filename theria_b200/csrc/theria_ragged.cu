@@ -84,6 +84,9 @@ Problem problem(const int64_t* st, int64_t T, int64_t S, int64_t H, int64_t Hkv,
   p.Hkv = (int)Hkv;
   p.G = Hkv > 0 ? (int)(H / Hkv) : 0;
   p.D = (int)D;
+  p.by_H = divisor(p.H);
+  p.by_Hkv = divisor(p.Hkv);
+  p.by_G = divisor(p.G);
   if (st != nullptr) {
     p.q_t = st[0];
     p.q_h = st[1];
@@ -183,7 +186,7 @@ FwdWs fwd_ws(void* base, const Problem& p) {
 struct BwdWs {
   List lq, lk;
   float2* terms;
-  uint8_t* fit;  // [Hkv, T, G], float16 on the tensor cores
+  uint8_t* fits;  // [Hkv, T, G] and [Hkv, T], float16 on the tensor cores
   float* part;  // room for the larger tiles' splits
   int64_t bytes;
 };
@@ -193,7 +196,7 @@ BwdWs bwd_ws(void* base, const Problem& p) {
   w.lq = take_list(c, p, p.G, SR, 0);
   w.lk = take_list(c, p, 1, SR, 1);
   w.terms = c.take<float2>((int64_t)p.T * p.H);
-  w.fit = c.take<uint8_t>((int64_t)p.T * p.H);
+  w.fits = c.take<uint8_t>((int64_t)p.T * (p.H + p.Hkv));
   const int ks = std::max(tc_splits(p), simt_splits(p)), qs = simt_q_splits(p);
   const int64_t k_row = 2ll * p.Hkv * p.D, q_row = (int64_t)p.H * p.D;
   const int64_t part = std::max(ks > 1 ? ks * k_row : 0, qs > 1 ? qs * q_row : 0) * p.T;
@@ -351,7 +354,7 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
     if (!prepare(kern, Cfg::kAlloc)) return THERIA_ERR_LAUNCH;
     if (int e = launch_chained(kern, dim3(blocks(p, ws.lq.per, ws.lq.step)), dim3(Cfg::kThreads),
                                Cfg::kAlloc, st, mq, mo, mk, mv, (const float2*)ws.terms,
-                               (const uint8_t*)ws.fit, (T*)dq,
+                               (const uint8_t*)ws.fits, (T*)dq,
                                (const int4*)ws.lq.items, (const int*)ws.lq.count, p))
       return e;
   }
@@ -366,7 +369,7 @@ int tc_bwd(const void* q, const void* k, const void* v, const void* dout, void* 
   const int splits = tc_splits(p);
   if (int e = launch_chained(kern, dim3(blocks(p, ws.lk.per, ws.lk.step) * (unsigned)splits),
                              dim3(Cfg::kThreads), Cfg::kAlloc, st, mk, mv, mq, mo,
-                             (const float2*)ws.terms, (const uint8_t*)ws.fit, (T*)dk, (T*)dv,
+                             (const float2*)ws.terms, (const uint8_t*)ws.fits, (T*)dk, (T*)dv,
                              splits > 1 ? ws.part : nullptr, (const int4*)ws.lk.items,
                              (const int*)ws.lk.count, splits, p))
     return e;
@@ -385,17 +388,18 @@ int by_tile(const Problem& p, F f) {
 }
 
 template <typename T>
-int run_terms(const void* o, const void* rest, const void* dout, const float* lse,
-              const BwdWs& ws, bool on_tc, const Problem& p, cudaStream_t st) {
+int run_terms(const void* o, const void* rest, const void* dout, const void* v,
+              const float* lse, const BwdWs& ws, bool on_tc, const Problem& p, cudaStream_t st) {
   const int64_t rows = (int64_t)p.T * p.H;
+  uint8_t* fits = on_tc && std::is_same<T, __half>::value ? ws.fits : nullptr;
   constexpr int VEC = 16 / sizeof(T);
   const bool vec = p.D % VEC == 0 && tc::aligned16(o) && tc::aligned16(rest) && tc::aligned16(dout);
   const int64_t units = vec ? p.D / VEC : p.D;  // a row's
   auto run = [&](auto kern, int lanes) {
-    const int64_t need = cdiv(rows, 256 / lanes);
+    const int64_t need = cdiv(rows + (fits ? (int64_t)p.T * p.Hkv : 0), 256 / lanes);
     return launch_chained(kern, dim3((unsigned)std::min<int64_t>(need, kSMs * 32)), dim3(256), 0,
                           st, (const T*)o, (const T*)rest, (const T*)dout, lse, ws.terms,
-                          on_tc ? ws.fit : (uint8_t*)nullptr, rows, p);
+                          (const T*)v, fits, rows, p);
   };
   if (!vec) return run(terms_kernel<T, 1, 32>, 32);
   if (units <= 4) return run(terms_kernel<T, VEC, 4>, 4);
@@ -488,7 +492,7 @@ int theria_ragged_bwd(const void* q, const void* k, const void* v, const int64_t
     return e;
   return by_type(dtype, [&](auto t) -> int {
     using E = decltype(t);
-    if (int e = run_terms<E>(o, o_rest, dout, lse, ws, on_tc, p, st)) return e;
+    if (int e = run_terms<E>(o, o_rest, dout, v, lse, ws, on_tc, p, st)) return e;
     if constexpr (!std::is_same<E, float>::value)
       if (on_tc)
         return by_tile(p, [&](auto hd, auto causal_) {
