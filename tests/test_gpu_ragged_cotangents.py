@@ -156,3 +156,18 @@ def test_values_of_zero():
     got = _grads(q, k, torch.zeros_like(v), do.half(), [200], True)
     want, _ = _plain(q, k, torch.zeros_like(v), do.half(), [200], True)
     assert not got[0].any() and not got[1].any() and _off(got[2], want[2]) <= 2 * U
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_a_cotangent_that_is_not_finite_leaves_the_others_their_bits(value):
+    # a small sequence of cotangents of 1e-3; the keys behind row 5 share its tile
+    q, k, v, do = _inputs(700, 4, 2, 64, 16.0, 1 / 16)
+    do = (do * 1e-3).half()
+    want = _grads(q, k, v, do, [700], True)
+    do[5] = value
+    got = _grads(q, k, v, do, [700], True)
+    assert torch.equal(got[0][:5], want[0][:5]) and torch.equal(got[0][6:], want[0][6:])
+    without = do.clone()
+    without[5] = 0
+    exact, _ = _plain(q, k, v, without, [700], True)
+    assert _off(got[1][6:], exact[1][6:]) <= 2 * U

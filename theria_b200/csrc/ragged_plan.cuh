@@ -63,11 +63,12 @@ struct Blank {
 };
 
 // A bound on the 2-norm of a row of float16 values, as a byte that grows with it: from the
-// sum of its squares, 0 for zeros, else 50 + e with the norm below 2^(e + 1), e from -24
-// (float16's smallest number) to 19 (128 of its largest, and what is not finite).
+// sum of its squares, 50 + e with the norm below 2^(e + 1), e from -24 (float16's smallest
+// number) to 19 (128 of its largest); 0 for zeros, and for a row that is not finite, whose
+// gradients are not either: it leaves the others theirs.
 __device__ __forceinline__ uint8_t norm_code(float squares) {
-  const int e = ((int)(__float_as_uint(squares) >> 23 & 255) - 127) >> 1;
-  return squares == 0.f ? 0 : (uint8_t)(min(e, 19) + 50);
+  const int e = (int)(__float_as_uint(squares) >> 23 & 255);
+  return squares == 0.f || e == 255 ? 0 : (uint8_t)(((e - 127) >> 1) + 50);
 }
 // The power of two that ds = p (dp - z) is multiplied by: with cotangents' norms below
 // 2^(e + 1), values' below 2^(f + 1), |dp - z| is below 2^(e + f + 3), so |ds| then
