@@ -1,5 +1,5 @@
-"""sdpa_ragged in float16 with cotangents that are not of order 1: its gradients are
-linear in them, and float16's range is short.
+"""sdpa_ragged in float16 with cotangents and values that are not of order 1: its
+gradients are linear in both, and float16's range is short.
 
 Tolerance on the 2-norm of dq, dk: each is rounded once, and is a sum of as many
 products of ds, rounded once too.  With independent values the sum of the products'
